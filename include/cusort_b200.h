@@ -277,6 +277,108 @@ cudaError_t cusort_mgpu_wait(void* comm, cudaStream_t stream);
 int cusort_mgpu_set_timing(int enable);
 int cusort_mgpu_get_phase_times(float* ms, const char** names, int capacity);
 
+/* ---- token routing and cache placement (no counterpart in the reference) --
+ * Keys to positions below a sparse (mixture-of-experts) language model: which
+ * experts a token goes to, its rows grouped by expert and back, and where a
+ * serving step's new tokens lie in a paged cache.  Device pointers, naturally
+ * aligned; asynchronous on `stream`, no host synchronisation, no device
+ * allocation.  Arguments out of range return cudaErrorInvalidValue before any
+ * launch.  Sums are held in 32 bits and rounded once to the element type. */
+typedef enum cusort_float_type { CUSORT_FLOAT_F32 = 0, CUSORT_FLOAT_F16 = 1, CUSORT_FLOAT_BF16 = 2 } cusort_float_type;
+typedef enum cusort_score { CUSORT_SCORE_SOFTMAX = 0, CUSORT_SCORE_SIGMOID = 1 } cusort_score;
+typedef enum cusort_group_score { CUSORT_GROUP_MAX = 0, CUSORT_GROUP_TOP2 = 1 } cusort_group_score;
+
+/* Routing of num_tokens rows of num_experts logits (row_stride elements
+ * apart) to the k best experts each.
+ *   - An expert is available where its logit is above -inf (NaN is not) and
+ *     so is its bias (d_bias: num_experts floats, or NULL).
+ *   - Its score is the softmax over the available experts, or the sigmoid.
+ *     Experts are ordered by the logit (both scores grow with it), or with a
+ *     bias by score + bias; the bias takes no part in the weights.  Equal ones
+ *     go to the lower expert; -0 equals +0.
+ *   - The experts form `groups` equal contiguous groups, of which the best
+ *     groups_kept stay.  A group's value is its best expert's order value
+ *     (CUSORT_GROUP_MAX) or the sum of its two best (CUSORT_GROUP_TOP2; of the
+ *     scores where there is no bias, those of a softmax up to its divisor).
+ *   - d_experts[t*k+j], d_weights[t*k+j]: the j-th best expert and its score
+ *     (divided by the sum of the chosen ones' with `renormalize`) times scale.
+ *     Where fewer than k are available, expert -1 and weight 0 follow.
+ * num_experts <= 1024, k <= 32, groups <= 32. */
+cudaError_t cusort_route(cusort_float_type type, const void* d_logits, int64_t row_stride, const float* d_bias,
+                         float* d_weights, int32_t* d_experts, int64_t num_tokens, int num_experts, int k,
+                         int groups, int groups_kept, cusort_score score, cusort_group_score group_score,
+                         int renormalize, float scale, cudaStream_t stream);
+
+/* Gradient of the logits (num_tokens rows of num_experts, contiguous, of the
+ * logits' type) from the weights' gradient, with the experts that cusort_route
+ * chose.  The choice itself has no gradient, nor has the bias. */
+cudaError_t cusort_route_backward(cusort_float_type type, const float* d_grad_weights, const void* d_logits,
+                                  int64_t row_stride, const float* d_bias, const int32_t* d_experts,
+                                  void* d_grad_logits, int64_t num_tokens, int num_experts, int k,
+                                  cusort_score score, int renormalize, float scale, cudaStream_t stream);
+
+/* Groups pairs by expert, stably: d_experts[i] (expert_bytes 4 or 8: int32 or
+ * int64) is the expert of pair i; pairs outside [0, num_experts) are dropped.
+ *   d_counts[e]: pairs of expert e; d_offsets[e]: the first row of its
+ *   segment, a multiple of `align`, d_offsets[num_experts] the end of the last
+ *   one; d_positions[i]: the row of pair i, -1 if dropped; d_sources[r], r <
+ *   capacity: the pair at row r, -1 where there is none.
+ * capacity >= num_pairs + min(num_experts, num_pairs) * (align - 1), below
+ * 2^31; num_experts <= 1024.  Two-phase temp protocol. */
+cudaError_t cusort_plan_dispatch(void* d_temp_storage, size_t* temp_storage_bytes, int expert_bytes,
+                                 const void* d_experts, int64_t num_pairs, int num_experts, int align,
+                                 int64_t capacity, int32_t* d_counts, int32_t* d_offsets, int32_t* d_sources,
+                                 int32_t* d_positions, cudaStream_t stream);
+
+/* d_rows[r] = row d_sources[r] / k of d_x (rows of row_bytes bytes,
+ * row_stride_bytes apart; d_rows contiguous), zeros where d_sources[r] < 0.
+ * d_sources and d_positions (num_tokens x k) as cusort_plan_dispatch gives
+ * them.  k <= 32. */
+cudaError_t cusort_dispatch_rows(const void* d_x, int64_t row_stride_bytes, size_t row_bytes,
+                                 const int32_t* d_sources, const int32_t* d_positions, void* d_rows,
+                                 int64_t num_tokens, int k, int64_t capacity, cudaStream_t stream);
+
+/* d_out[t] = d_residual[t] + sum over j of d_weights[t*k+j] * d_rows[d_positions[t*k+j]];
+ * positions outside [0, capacity) add nothing.  d_residual may be NULL (rows
+ * residual_stride elements apart), and d_weights too (ones: the gradient of
+ * cusort_dispatch_rows). */
+cudaError_t cusort_combine_rows(cusort_float_type type, const void* d_rows, const float* d_weights,
+                                const int32_t* d_positions, const void* d_residual, int64_t residual_stride,
+                                void* d_out, int64_t num_tokens, int k, int64_t capacity, int64_t hidden,
+                                cudaStream_t stream);
+
+/* Gradients of cusort_combine_rows (its residual's is d_grad_out itself):
+ * d_grad_rows[r] = d_weights[s] * d_grad_out[s / k], s = d_sources[r], zeros where s < 0;
+ * d_grad_weights[i] = d_grad_out[i / k] . d_rows[d_positions[i]], 0 where there is none. */
+cudaError_t cusort_combine_rows_backward(cusort_float_type type, const void* d_grad_out, int64_t grad_stride,
+                                         const void* d_rows, const float* d_weights, const int32_t* d_sources,
+                                         const int32_t* d_positions, void* d_grad_rows, float* d_grad_weights,
+                                         int64_t num_tokens, int k, int64_t capacity, int64_t hidden,
+                                         cudaStream_t stream);
+
+/* Placement of one serving step in a paged cache of blocks of block_size
+ * tokens.  Request r has d_cached_lens[r] tokens there and brings
+ * d_new_lens[r] (below 0: 0); row r of d_block_tables (table_width entries,
+ * rows table_stride entries apart) names its blocks.
+ *   - The blocks that its new tokens need are taken from the end of
+ *     d_free_blocks[0 .. *d_num_free) (room for num_blocks), in the requests'
+ *     order, and written into its table.  A request is served if its blocks
+ *     fit its table and there were free ones for it and all before it;
+ *     d_served[r] says so.  One that is not keeps its table.
+ *     *d_num_free_out: the free blocks that are left.
+ *   - d_free_blocks and d_num_free NULL: the tables hold all blocks already.
+ *   - d_starts[r]: the first new token of request r; d_starts[num_requests]:
+ *     their number.  Token i < num_tokens: its position in its request and its
+ *     slot, block * block_size + position % block_size; slot -1 where the
+ *     request is not served or the table's entry is negative, both -1 beyond
+ *     the last token.
+ * num_requests <= 16384, block_size <= 2^20, num_blocks <= 2^30. */
+cudaError_t cusort_page_plan(const int32_t* d_cached_lens, const int32_t* d_new_lens, int num_requests,
+                             int block_size, int32_t* d_block_tables, int64_t table_stride, int table_width,
+                             const int32_t* d_free_blocks, int num_blocks, const int32_t* d_num_free,
+                             int64_t num_tokens, int64_t* d_slots, int32_t* d_positions, int32_t* d_starts,
+                             uint8_t* d_served, int32_t* d_num_free_out, cudaStream_t stream);
+
 /* ---- library state, status and diagnostics (no reference counterpart;
  *      the reference has compile-time macros only, libcusort.cuh:119-148) -- */
 
