@@ -10,7 +10,8 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kFewRequests = 512;
+constexpr int64_t kFewTokens = 148 * 1024;
 constexpr int kMaxRequests = 16384;  // two 32-bit scans of them fit in shared memory
 constexpr uint32_t kAll = 0xffffffffu;
 constexpr uint32_t kMost = 0x7fffffffu;
@@ -48,22 +49,31 @@ __device__ __forceinline__ Request request_of(const PageArgs& a, int r) {
 }
 
 // Every CTA scans all requests (they are few), then takes its share of the
-// tokens: a search for the token's request, and its block from the table or,
-// for a block of this step, straight from the free list, so that no CTA waits
-// for another's table entries.  A block's first token writes its entry.
-__global__ void __launch_bounds__(kThreads) page_plan_kernel(PageArgs a) {
+// tokens, N consecutive ones to a thread: a search for the first one's request
+// and a walk from there, the blocks from the table or, for blocks of this
+// step, straight from the free list, so that no CTA waits for another's table
+// entries.  A block's first token writes its entry.
+template <int THREADS, int N>
+__global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
+  constexpr int W = THREADS / 32;
   extern __shared__ uint32_t s_scan[];  // [R + 1] token starts, [R + 1] blocks taken before
-  __shared__ uint32_t s_sums[2][kThreads / 32];
+  __shared__ uint32_t s_sums[2][W];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = a.num_requests;
   uint32_t *s_start = s_scan, *s_taken = s_scan + R + 1;
-  const int each = (R + kThreads - 1) / kThreads, r0 = threadIdx.x * each, r1 = min(r0 + each, R);
+  for (int r = threadIdx.x; r < R; r += THREADS) {
+    const Request q = request_of(a, r);
+    s_start[r] = q.fresh;
+    s_taken[r] = q.need;
+  }
+  __syncthreads();
+  const int each = (R + THREADS - 1) / THREADS, r0 = min((int)threadIdx.x * each, R), r1 = min(r0 + each, R);
   uint32_t tokens = 0, blocks = 0;
   for (int r = r0; r < r1; ++r) {
-    const Request q = request_of(a, r);
+    const uint32_t n = s_start[r], b = s_taken[r];
     s_start[r] = tokens;
     s_taken[r] = blocks;
-    tokens = add_sat(tokens, q.fresh);
-    blocks = add_sat(blocks, q.need);
+    tokens = add_sat(tokens, n);
+    blocks = add_sat(blocks, b);
   }
   uint32_t in_t = tokens, in_b = blocks;
 #pragma unroll
@@ -80,7 +90,7 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(PageArgs a) {
     s_start[r] = add_sat(s_start[r], before_t);
     s_taken[r] = add_sat(s_taken[r], before_b);
   }
-  if (threadIdx.x == kThreads - 1) {
+  if (threadIdx.x == THREADS - 1) {
     s_start[R] = add_sat(before_t, tokens);
     s_taken[R] = add_sat(before_b, blocks);
   }
@@ -88,53 +98,99 @@ __global__ void __launch_bounds__(kThreads) page_plan_kernel(PageArgs a) {
   const uint32_t left = a.num_free == nullptr ? 0u : (uint32_t)min(max(*a.num_free, 0), a.num_blocks);
   if (blockIdx.x == 0) {
     uint32_t used = 0;
-    for (int r = threadIdx.x; r < R; r += kThreads) {
+    for (int r = threadIdx.x; r < R; r += THREADS) {
       const Request q = request_of(a, r);
       const uint32_t upto = s_taken[r + 1];
       a.served[r] = q.fits && (q.need == 0 || upto <= left);
       if (upto <= left) used = max(used, upto);
     }
-    for (int r = threadIdx.x; r <= R; r += kThreads) a.starts[r] = (int32_t)s_start[r];
+    for (int r = threadIdx.x; r <= R; r += THREADS) a.starts[r] = (int32_t)s_start[r];
     used = __reduce_max_sync(kAll, used);
     __syncthreads();
     if (lane == 0) s_sums[0][warp] = used;
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int w = 1; w < kThreads / 32; ++w) used = max(used, s_sums[0][w]);
+      for (int w = 1; w < W; ++w) used = max(used, s_sums[0][w]);
       if (a.num_free_out != nullptr) *a.num_free_out = (int32_t)(left - used);
     }
   }
   const int64_t total = s_start[R], most = max(total, a.num_tokens);
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < most; i += (int64_t)gridDim.x * kThreads) {
-    int64_t slot = -1;
-    int32_t position = -1;
-    if (i < total) {
-      int lo = 0, hi = R;  // the last request that starts at or before i
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (s_start[mid] <= i) lo = mid; else hi = mid;
-      }
-      const Request q = request_of(a, lo);
-      const uint32_t pos = min(q.cached + (uint32_t)(i - s_start[lo]), kMost);
-      position = (int32_t)pos;
-      if (q.fits && (q.need == 0 || s_taken[lo + 1] <= left)) {
-        const uint32_t b = a.block_size, page = pos / b, in = pos - page * b, held = (q.cached + b - 1) / b;
-        int32_t* entry = a.tables + lo * a.table_stride + page;
-        int32_t id;
-        if (a.num_free != nullptr && page >= held) {
-          id = a.free_blocks[left - 1 - (s_taken[lo] + page - held)];
-          if (in == 0) *entry = id;
-        } else {
-          id = *entry;
-        }
-        if (id >= 0) slot = (int64_t)id * b + in;
+  const uint32_t size = a.block_size;
+  for (int64_t i0 = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * N; i0 < most; i0 += (int64_t)gridDim.x * THREADS * N) {
+    int64_t slot[N];
+    int32_t position[N];
+    int r = 0;  // the last request that starts at or before i0
+    if (i0 < total) {
+      int hi = R;
+      while (hi - r > 1) {
+        const int mid = (r + hi) >> 1;
+        if (s_start[mid] <= i0) r = mid; else hi = mid;
       }
     }
-    if (i < a.num_tokens) {
-      a.slots[i] = slot;
-      a.positions[i] = position;
+    uint32_t next = 0, pos = 0, page = 0, in = 0, held = 0, taken = 0;
+    int32_t* table = nullptr;
+    int32_t id = -1;
+    bool served = false, fetch = true;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int64_t i = i0 + n;
+      slot[n] = position[n] = -1;
+      if (i >= total) continue;
+      if (n == 0 || i >= next) {
+        while (n > 0 && s_start[r + 1] <= i) ++r;
+        const Request q = request_of(a, r);
+        next = s_start[r + 1];
+        taken = s_taken[r];
+        pos = min(q.cached + (uint32_t)(i - s_start[r]), kMost);
+        page = pos / size;
+        in = pos - page * size;
+        held = a.num_free != nullptr ? (q.cached + size - 1) / size : (uint32_t)a.table_width;
+        served = q.fits && (q.need == 0 || s_taken[r + 1] <= left);
+        table = a.tables + r * a.table_stride;
+        fetch = true;
+      } else {
+        pos = min(pos + 1, kMost);
+        if (++in == size) in = 0, ++page, fetch = true;
+      }
+      position[n] = (int32_t)pos;
+      if (!served) continue;
+      if (fetch) {
+        id = page < held ? table[page] : a.free_blocks[left - 1 - (taken + page - held)];
+        if (page >= held && in == 0) table[page] = id;
+        fetch = false;
+      }
+      if (id >= 0) slot[n] = (int64_t)id * size + in;
+    }
+    if (N == 4 && i0 + N <= a.num_tokens) {
+      longlong2* out = reinterpret_cast<longlong2*>(a.slots + i0);
+      out[0] = make_longlong2(slot[0], slot[1 % N]);
+      out[1] = make_longlong2(slot[2 % N], slot[3 % N]);
+      *reinterpret_cast<int4*>(a.positions + i0) =
+          make_int4(position[0], position[1 % N], position[2 % N], position[3 % N]);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (i0 + n < a.num_tokens) {
+          a.slots[i0 + n] = slot[n];
+          a.positions[i0 + n] = position[n];
+        }
+      }
     }
   }
+}
+
+template <int THREADS, int N>
+cudaError_t run(const PageArgs& a, cudaStream_t stream) {
+  const size_t smem = sizeof(uint32_t) * 2 * (a.num_requests + 1);
+  if (smem > 47 * 1024) {  // beside the sums
+    const cudaError_t e = cudaFuncSetAttribute(page_plan_kernel<THREADS, N>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e) return e;
+  }
+  const int64_t per_cta = THREADS * N;
+  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(148, (a.num_tokens + per_cta - 1) / per_cta));
+  page_plan_kernel<THREADS, N><<<grid, THREADS, smem, stream>>>(a);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -158,13 +214,9 @@ extern "C" cudaError_t cusort_page_plan(const int32_t* d_cached_lens, const int3
   const PageArgs a{d_cached_lens, d_new_lens, num_requests, block_size, num_blocks, num_tokens, d_block_tables,
                    table_stride, table_width, d_free_blocks, d_num_free, d_slots, d_positions, d_starts, d_served,
                    d_num_free_out};
-  const size_t smem = sizeof(uint32_t) * 2 * (num_requests + 1);
-  if (smem > 48 * 1024 - 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)(sizeof(uint32_t) * 2 * (kMaxRequests + 1)));
-    if (e) return e;
-  }
-  const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(148, (num_tokens + kThreads - 1) / kThreads));
-  page_plan_kernel<<<grid, kThreads, smem, stream>>>(a);
-  return cudaGetLastError();
+  // Four tokens to a thread need one search instead of four and whole-vector stores, but a longer chain; a large CTA
+  // scans many requests faster.
+  const bool aligned = ((reinterpret_cast<uintptr_t>(d_slots) | reinterpret_cast<uintptr_t>(d_positions)) & 15) == 0;
+  if (num_tokens > kFewTokens && aligned) return run<1024, 4>(a, stream);
+  return num_requests > kFewRequests ? run<1024, 1>(a, stream) : run<256, 1>(a, stream);
 }
