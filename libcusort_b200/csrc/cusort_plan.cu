@@ -14,15 +14,17 @@ namespace {
 using namespace cusort_b200;
 
 constexpr int kMaxExperts = 1024;
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
-constexpr int kMaxTiles = 148;      // one CTA per SM
-constexpr int kMinTileItems = 2048;  // below this a tile's fixed cost exceeds its items'
+constexpr int kThreads = 1024;     // per CTA; kSmallThreads where all pairs are few
+constexpr int kSmallThreads = 256;
+constexpr int64_t kSmallItems = 1024;
+constexpr int64_t kOneTileItems = 8192;   // up to here one CTA does it all, in one launch
+constexpr int64_t kMinTileItems = 2048;
+constexpr int kMaxTiles = 148;            // one CTA per SM
 constexpr uint32_t kAll = 0xffffffffu;
 
 struct PlanArgs {
   const void* experts;
-  int64_t items, capacity, tile_items;  // tile_items: a multiple of 32 * kWarps
+  int64_t items, capacity, tile_items;
   int num_experts, align;
   uint32_t* tile_counts;  // [tiles][num_experts]; null: one tile, counted in place
   int32_t *counts, *offsets, *sources, *positions;
@@ -39,9 +41,11 @@ __device__ __forceinline__ int expert_of(const PlanArgs& a, int64_t i, int64_t e
 template <typename I>
 __global__ void __launch_bounds__(kThreads) plan_count_kernel(PlanArgs a) {
   __shared__ uint32_t s_count[kMaxExperts];
+  dev::pdl_launch_dependents();
   for (int e = threadIdx.x; e < a.num_experts; e += kThreads) s_count[e] = 0;
   __syncthreads();
   const int64_t begin = blockIdx.x * a.tile_items, end = min(begin + a.tile_items, a.items);
+#pragma unroll 2
   for (int64_t i = begin + threadIdx.x; i < end; i += kThreads) {
     const int e = expert_of<I>(a, i, end);
     if (e < a.num_experts) atomicAdd(&s_count[e], 1u);
@@ -51,51 +55,65 @@ __global__ void __launch_bounds__(kThreads) plan_count_kernel(PlanArgs a) {
   for (int e = threadIdx.x; e < a.num_experts; e += kThreads) out[e] = s_count[e];
 }
 
-// Every CTA adds up the tiles before its own and all of them, scans the
-// aligned totals, and gives its items their rows: warp by warp over
-// contiguous runs, in each 32 items the peers of an expert by their lanes.
-template <typename I>
-__global__ void __launch_bounds__(kThreads) plan_place_kernel(PlanArgs a) {
-  extern __shared__ uint32_t s_warp[];  // [kWarps][num_experts]: the next row of an expert in a warp's run
-  __shared__ uint32_t s_total[kMaxExperts], s_offset[kMaxExperts + 1], s_sums[kWarps];
+// Every CTA counts its tile warp by warp (a warp's items are one run), adds up
+// the tiles before its own and all of them, scans the aligned totals, and
+// gives its items their rows: in each 32 items the peers of an expert by their
+// lanes.
+template <typename I, int THREADS>
+__global__ void __launch_bounds__(THREADS) plan_place_kernel(PlanArgs a) {
+  constexpr int W = THREADS / 32;
+  extern __shared__ uint32_t s_warp[];  // [W][num_experts]: the next item of an expert in a warp's run
+  __shared__ uint32_t s_before[kMaxExperts], s_total[kMaxExperts], s_offset[kMaxExperts + 1], s_sums[W];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = a.num_experts;
   const int64_t begin = blockIdx.x * a.tile_items, end = min(begin + a.tile_items, a.items);
-  const int64_t run = a.tile_items / kWarps;
+  const int64_t run = (a.tile_items + 32 * W - 1) / (32 * W) * 32;
   const int64_t wbegin = min(begin + warp * run, end), wend = min(wbegin + run, end);
-  for (int i = threadIdx.x; i < kWarps * E; i += kThreads) s_warp[i] = 0;
+  for (int i = threadIdx.x; i < W * E; i += THREADS) s_warp[i] = 0;
+  for (int e = threadIdx.x; e < E; e += THREADS) s_before[e] = s_total[e] = 0;
   __syncthreads();
   uint32_t* mine = s_warp + warp * E;
+#pragma unroll 4
   for (int64_t i = wbegin + lane; i < wend; i += 32) {
     const int e = expert_of<I>(a, i, wend);
     if (e < E) atomicAdd(&mine[e], 1u);
   }
-  __syncthreads();
-  // each expert: items before this tile, its total
-  for (int e = threadIdx.x; e < E; e += kThreads) {
-    uint32_t before = 0, total = 0;
-    if (a.tile_counts != nullptr) {
-      for (int t = 0; t < gridDim.x; ++t) {
+  if (a.tile_counts != nullptr) {
+    // columns of the tiles' counts: as many threads to an expert as there are
+    dev::pdl_wait();
+    const int parts = max(1, THREADS / E), tiles = gridDim.x;
+    for (int i = threadIdx.x; i < parts * E; i += THREADS) {
+      const int e = i % E;
+      uint32_t before = 0, total = 0;
+#pragma unroll 8
+      for (int t = i / E; t < tiles; t += parts) {
         const uint32_t c = a.tile_counts[(int64_t)t * E + e];
         if (t < blockIdx.x) before += c;
         total += c;
       }
+      atomicAdd(&s_before[e], before);
+      atomicAdd(&s_total[e], total);
     }
-    uint32_t at = before;
-    for (int w = 0; w < kWarps; ++w) {
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += THREADS) {
+    uint32_t at = s_before[e];
+#pragma unroll 8
+    for (int w = 0; w < W; ++w) {
       const uint32_t c = s_warp[w * E + e];
       s_warp[w * E + e] = at;
       at += c;
     }
-    s_total[e] = a.tile_counts != nullptr ? total : at;
+    if (a.tile_counts == nullptr) s_total[e] = at;
   }
   __syncthreads();
-  // exclusive scan of the aligned totals: four experts to a thread
+  // exclusive scan of the aligned totals, P experts to a thread
   {
+    constexpr int P = kMaxExperts / THREADS;
     const uint32_t al = a.align;
-    uint32_t v[4], sum = 0;
+    uint32_t v[P], sum = 0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int e = threadIdx.x * 4 + j;
+    for (int j = 0; j < P; ++j) {
+      const int e = threadIdx.x * P + j;
       v[j] = sum;
       sum += e < E ? (s_total[e] + al - 1) / al * al : 0;
     }
@@ -107,21 +125,22 @@ __global__ void __launch_bounds__(kThreads) plan_place_kernel(PlanArgs a) {
     }
     if (lane == 31) s_sums[warp] = in;
     __syncthreads();
-    uint32_t before = in - sum;
-    for (int w = 0; w < warp; ++w) before += s_sums[w];
+    uint32_t before = lane < warp ? s_sums[lane] : 0;  // W <= 32
+    before = __reduce_add_sync(kAll, before) + in - sum;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (threadIdx.x * 4 + j < E) s_offset[threadIdx.x * 4 + j] = before + v[j];
-    if (threadIdx.x == kThreads - 1) s_offset[E] = before + sum;
+    for (int j = 0; j < P; ++j)
+      if (threadIdx.x * P + j < E) s_offset[threadIdx.x * P + j] = before + v[j];
+    if (threadIdx.x == THREADS - 1) s_offset[E] = before + sum;
   }
   __syncthreads();
   if (blockIdx.x == 0) {
-    for (int e = threadIdx.x; e < E; e += kThreads) {
+    for (int e = threadIdx.x; e < E; e += THREADS) {
       a.counts[e] = (int32_t)s_total[e];
       a.offsets[e] = (int32_t)s_offset[e];
     }
     if (threadIdx.x == 0) a.offsets[E] = (int32_t)s_offset[E];
   }
+#pragma unroll 4
   for (int64_t base = wbegin; base < wend; base += 32) {
     const int64_t i = base + lane;
     const int e = expert_of<I>(a, i, wend);
@@ -139,12 +158,12 @@ __global__ void __launch_bounds__(kThreads) plan_place_kernel(PlanArgs a) {
   }
   // rows that hold no pair: the ends of the segments, and what follows the last
   if (a.align > 1) {
-    for (int e = blockIdx.x * kWarps + warp; e < E; e += gridDim.x * kWarps)
+    for (int e = blockIdx.x * W + warp; e < E; e += gridDim.x * W)
       for (int64_t r = (int64_t)s_offset[e] + s_total[e] + lane; r < min((int64_t)s_offset[e + 1], a.capacity); r += 32)
         a.sources[r] = -1;
   }
-  for (int64_t r = (int64_t)s_offset[E] + blockIdx.x * kThreads + threadIdx.x; r < a.capacity;
-       r += (int64_t)gridDim.x * kThreads)
+  for (int64_t r = (int64_t)s_offset[E] + blockIdx.x * THREADS + threadIdx.x; r < a.capacity;
+       r += (int64_t)gridDim.x * THREADS)
     a.sources[r] = -1;
 }
 
@@ -154,21 +173,41 @@ struct PlanShape {
 };
 
 PlanShape shape_of(int64_t items) {
-  const int64_t step = 32 * kWarps;
+  if (items <= kOneTileItems) return {1, std::max<int64_t>(items, 1)};
   int64_t tile = std::max<int64_t>(kMinTileItems, (items + kMaxTiles - 1) / kMaxTiles);
-  tile = (tile + step - 1) / step * step;
-  return {(int)std::max<int64_t>(1, (items + tile - 1) / tile), tile};
+  tile = (tile + kThreads - 1) / kThreads * kThreads;
+  return {(int)((items + tile - 1) / tile), tile};
+}
+
+template <typename I, int THREADS>
+cudaError_t place(const PlanArgs& a, int tiles, cudaStream_t stream) {
+  const size_t smem = sizeof(uint32_t) * (THREADS / 32) * a.num_experts;
+  if (smem > 32 * 1024) {  // beside the static arrays
+    const cudaError_t e = cudaFuncSetAttribute(plan_place_kernel<I, THREADS>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e) return e;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(tiles);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = tiles > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, plan_place_kernel<I, THREADS>, a);
 }
 
 template <typename I>
 cudaError_t run(const PlanArgs& a, int tiles, cudaStream_t stream) {
-  const size_t smem = sizeof(uint32_t) * kWarps * a.num_experts;
+  if (tiles == 1 && a.items <= kSmallItems) return place<I, kSmallThreads>(a, 1, stream);
   if (tiles > 1) {
     plan_count_kernel<I><<<tiles, kThreads, 0, stream>>>(a);
     if (const cudaError_t e = cudaGetLastError()) return e;
   }
-  plan_place_kernel<I><<<tiles, kThreads, smem, stream>>>(a);
-  return cudaGetLastError();
+  return place<I, kThreads>(a, tiles, stream);
 }
 
 }  // namespace
