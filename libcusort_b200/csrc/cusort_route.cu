@@ -8,6 +8,7 @@
 #include <type_traits>
 
 #include "../../include/cusort_b200.h"
+#include "cusort_device.cuh"
 #include "cusort_float.cuh"
 
 namespace {
@@ -17,7 +18,8 @@ using namespace cusort_b200;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxChosen = 32;  // one lane per chosen expert
 constexpr int kMaxGroups = 32;  // one lane per group
-constexpr int kWarps = 4;       // tokens per CTA
+constexpr int kWarps = 4;       // per CTA
+constexpr int64_t kBusyWarps = 148 * 4 * 6;
 constexpr uint32_t kAll = 0xffffffffu;
 
 struct RouteArgs {
@@ -28,6 +30,7 @@ struct RouteArgs {
   int32_t* experts;
   int64_t tokens;
   int num_experts, k, k_lanes;  // k_lanes: the power of two from k on
+  int per_warp;                 // tokens to a warp, at most 32 / k_lanes
   int groups, groups_kept, per_group, group_lanes;  // group_lanes: lanes to a group, 0 where groups end inside a lane
   bool wide;                                        // rows and their addresses are whole vectors
   bool softmax, renormalize, top2;
@@ -42,7 +45,7 @@ struct RouteBackwardArgs {
   const int32_t* experts;
   void* grad_logits;
   int64_t tokens;
-  int num_experts, k, k_lanes;
+  int num_experts, k, k_lanes, per_warp;
   bool wide;
   bool softmax, renormalize;
   float scale;
@@ -69,9 +72,9 @@ __device__ __forceinline__ float sum_over(float x, int lanes) {
   return x;
 }
 __device__ __forceinline__ float warp_max(float x) {
-#pragma unroll
-  for (int d = 16; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(kAll, x, d));
-  return x;
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
 }
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
@@ -100,35 +103,150 @@ template <typename T, int V> constexpr int vector_length() {
   return V * sizeof(T) <= 16 ? V : 16 / (int)sizeof(T);
 }
 
-// The lane's V consecutive logits, from expert lane * V on; -inf beyond the
-// last.
+// The lane's V consecutive values of a row, from expert lane * V on; -inf
+// beyond the last.
 template <typename T, int V>
-__device__ __forceinline__ void load_logits(float (&x)[V], const T* row, int lane, int num_experts, bool wide) {
+__device__ __forceinline__ void load_row(T (&x)[V], const T* row, int lane, int num_experts, bool wide) {
   constexpr int N = vector_length<T, V>();
+  const T none = dev::from_float<T>(neg_inf());
   if (wide) {
 #pragma unroll
     for (int c = 0; c < V; c += N) {
       if (lane * V + c < num_experts) {
         const auto p = *reinterpret_cast<const dev::Pack<T, N>*>(row + lane * V + c);
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[c + i] = logit(p.v[i]);
+        for (int i = 0; i < N; ++i) x[c + i] = p.v[i];
       } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[c + i] = neg_inf();
+        for (int i = 0; i < N; ++i) x[c + i] = none;
       }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = lane * V + i < num_experts ? logit(row[lane * V + i]) : neg_inf();
+    for (int i = 0; i < V; ++i) x[i] = lane * V + i < num_experts ? row[lane * V + i] : none;
   }
+}
+
+// The k largest keys (0: none) of a warp whose lanes hold V consecutive
+// experts each, in order, equal ones by their expert; lane base + j gets the
+// j-th key and its expert.  UNIQUE: no two keys but 0 are equal.
+//
+// Few experts to a lane: k rounds over all keys.  More: the k-th largest of
+// the lanes' own maxima is below no more than k - 1 keys in other lanes, so
+// the k largest are among the keys from it on, seldom more than a few beyond
+// k; these are gathered one to a lane, and the rounds are over one key each.
+// Instructions to a token at k = 8: 8 keys to a lane 400 -> 200, 4 about equal.
+template <int V, bool UNIQUE>
+__device__ __forceinline__ void choose(uint32_t (&key)[V], int k, int lane, int base, uint2* scratch, uint32_t& mine,
+                                       int& chosen) {
+  if constexpr (V >= (UNIQUE ? 16 : 8)) {
+    uint32_t m = key[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) m = max(m, key[i]);
+    uint32_t low = 1;
+    for (int n = 0; n < k;) {
+      const uint32_t most = __reduce_max_sync(kAll, m);
+      if (most == 0) {
+        low = 1;
+        break;
+      }
+      low = most;
+      n += __popc(__ballot_sync(kAll, m == most));
+      m = m == most ? 0u : m;
+    }
+    uint32_t mask = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) mask |= (key[i] >= low ? 1u : 0u) << i;
+    const int count = __popc(mask);
+    const uint32_t b0 = __ballot_sync(kAll, count & 1), b1 = __ballot_sync(kAll, count & 2),
+                   b2 = __ballot_sync(kAll, count & 4), b3 = __ballot_sync(kAll, count & ~7);
+    const int total = __popc(b0) + 2 * __popc(b1) + 4 * __popc(b2);
+    if (b3 == 0 && total <= 32) {
+      const uint32_t below = dev::lanemask_lt();
+      int at = __popc(b0 & below) + 2 * __popc(b1 & below) + 4 * __popc(b2 & below);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (mask >> i & 1u) scratch[at++] = make_uint2(key[i], lane * V + i);
+      __syncwarp();
+      uint2 c = lane < total ? scratch[lane] : make_uint2(0u, 0u);
+      __syncwarp();
+      int from = 0;
+      const int n = min(k, total);
+      for (int j = 0; j < n; ++j) {
+        const uint32_t most = __reduce_max_sync(kAll, c.x);
+        const int owner = __ffs(__ballot_sync(kAll, c.x == most)) - 1;
+        if (lane == owner) c.x = 0;
+        if (lane == base + j) mine = most, from = owner;
+      }
+      const int e = __shfl_sync(kAll, (int)c.y, from);
+      if (lane >= base && lane < base + n) chosen = e;
+      return;
+    }
+  }
+  if constexpr (UNIQUE) {
+    // The next largest key is the one with the largest key - last, modulo 2^32: what is not below `last` comes out
+    // smaller than what is, so nothing has to be taken out.
+    uint32_t last = 0;
+    for (int j = 0; j < k; ++j) {
+      uint32_t best = key[0] - last;
+#pragma unroll
+      for (int i = 1; i < V; ++i) best = max(best, key[i] - last);
+      last += __reduce_max_sync(kAll, best);
+      if (last == 0) break;
+      if (lane == base + j) mine = last;
+    }
+    if (lane >= base && mine != 0) chosen = 0xffff - (mine & 0xffffu);
+  } else {
+    for (int j = 0; j < k; ++j) {
+      uint32_t best = key[0];
+#pragma unroll
+      for (int i = 1; i < V; ++i) best = max(best, key[i]);
+      const uint32_t most = __reduce_max_sync(kAll, best);
+      if (most == 0) break;
+      const int owner = __ffs(__ballot_sync(kAll, best == most)) - 1;  // equal ones: the lower lane
+      uint32_t hits = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) hits |= (key[i] == most ? 1u : 0u) << i;
+      hits = lane == owner ? hits & (0u - hits) : 0u;
+#pragma unroll
+      for (int i = 0; i < V; ++i) key[i] = hits >> i & 1u ? 0u : key[i];
+      const int e = __shfl_sync(kAll, __ffs(hits) - 1, owner) + owner * V;
+      if (lane == base + j) mine = most, chosen = e;
+    }
+  }
+}
+
+// Order keys of 16-bit logits, unique: the logit's order above, the expert
+// below (lower experts larger); 0 where the logit is -inf or NaN.  The signed
+// order of two halves at once: negative ones inverted, the others with the
+// sign bit set.
+template <typename T, int V>
+__device__ __forceinline__ void narrow_keys(uint32_t (&key)[V], const T (&x)[V], int lane) {
+  using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+  constexpr uint32_t kInf = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
+  constexpr uint32_t kLeast = (0x8000u - kInf) << 16;             // from the first above -inf
+  constexpr uint32_t kSpan = (2 * kInf - 1) << 16 | 0xffffu;  // to +inf
+#pragma unroll
+  for (int i = 0; i < V; i += 2) {
+    T2 pair;
+    pair.x = x[i];
+    pair.y = x[i + 1 < V ? i + 1 : i];
+    T2 zero;
+    zero.x = zero.y = dev::from_float<T>(0.f);
+    pair = __hadd2(pair, zero);  // -0 becomes +0
+    uint32_t w = *reinterpret_cast<uint32_t*>(&pair);
+    w ^= ((w & 0x80008000u) >> 15) * 0xffffu | 0x80008000u;
+    key[i] = w << 16 | (0xffffu - (lane * V + i));
+    if (i + 1 < V) key[i + 1] = (w & 0xffff0000u) | (0xffffu - (lane * V + i + 1));
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) key[i] = key[i] - kLeast <= kSpan ? key[i] : 0u;
 }
 
 // Which groups stay: lane's mask of its V experts (bit i: expert lane * V + i).
 // value: what groups go by, -inf where not available.
 template <int V>
 __device__ uint32_t kept_experts(const RouteArgs& a, const float (&value)[V], int lane) {
-  float mine = neg_inf();  // the value of the group that this lane stands for
-  int group = lane;
   if (a.group_lanes != 0) {
     // a group is group_lanes whole lanes: its two best by exchange among them
     float b1 = value[0], b2 = neg_inf();
@@ -142,16 +260,18 @@ __device__ uint32_t kept_experts(const RouteArgs& a, const float (&value)[V], in
       b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
       b1 = fmaxf(b1, o1);
     }
-    mine = a.top2 && b2 > neg_inf() ? b1 + b2 : b1;
-    group = lane / a.group_lanes;
-    int ahead = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      const float v = __shfl_sync(kAll, mine, g * a.group_lanes);
-      ahead += v > mine || (v == mine && g < group);
+    const int shift = __ffs(a.group_lanes) - 1, group = lane >> shift;
+    // groups_kept rounds: the largest, the lower lane among equals.  -inf has a key above 0, so that every round
+    // takes one group.
+    uint32_t key = group < a.groups ? order_key((a.top2 && b2 > neg_inf() ? b1 + b2 : b1) + 0.f) : 0u, kept = 0;
+    for (int n = 0; n < a.groups_kept; ++n) {
+      const uint32_t most = __reduce_max_sync(kAll, key);
+      if (group == (__ffs(__ballot_sync(kAll, key == most)) - 1) >> shift) key = 0, kept = kAll;
     }
-    return ahead < a.groups_kept ? kAll : 0u;
+    return kept;
   }
   // groups of any length: one after the other, lane g keeps group g's
+  float mine = neg_inf();
   for (int g = 0; g < a.groups; ++g) {
     float b1 = neg_inf(), b2 = neg_inf();
 #pragma unroll
@@ -184,126 +304,116 @@ __device__ uint32_t kept_experts(const RouteArgs& a, const float (&value)[V], in
   return mask;
 }
 
-// One warp per token; a lane holds V consecutive experts, so that a lower lane
-// means a lower expert and groups are runs of lanes.  k rounds choose the
-// largest order key; lane j keeps the j-th.
+// A warp takes per_warp tokens one after the other; a lane holds V consecutive
+// experts, so that a lower lane means a lower expert and groups are runs of
+// lanes.  The chosen experts of its tokens lie k_lanes lanes apart, and their
+// weights are computed for all tokens at once.
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kWarps) route_kernel(RouteArgs a) {
+  __shared__ uint2 s_scratch[kWarps][32];
   const int lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (t >= a.tokens) return;
-  const T* row = static_cast<const T*>(a.logits) + t * a.stride;
-
-  float x[V];
-  load_logits<T, V>(x, row, lane, a.num_experts, a.wide);
+  const int64_t t0 = ((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * a.per_warp;
+  if (t0 >= a.tokens) return;
+  const int tokens = (int)min((int64_t)a.per_warp, a.tokens - t0);
+  const T* row = static_cast<const T*>(a.logits) + t0 * a.stride;
   const bool biased = a.bias != nullptr, grouped = a.groups_kept < a.groups;
-  uint32_t mask = kAll;  // experts of the lane that may be chosen
-  float top = neg_inf(), total = 0.f;
-  float c[V];  // what experts are ordered by: the logit (both scores grow with it), or the score plus the bias
-#pragma unroll
-  for (int i = 0; i < V; ++i) c[i] = x[i];
   const bool need_total = a.softmax && (biased || !a.renormalize);
-  if (need_total || biased || (grouped && a.top2)) {
-    float b[V], s[V];
-    if (biased) {
+  const bool need_score = need_total || biased || (grouped && a.top2);
+
+  float b[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = lane * V + i;
-        b[i] = e < a.num_experts ? a.bias[e] : 0.f;
-        if (!(b[i] > neg_inf())) x[i] = neg_inf();
-      }
-    }
-    if (a.softmax) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) top = fmaxf(top, x[i]);
-      top = warp_max(top);
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        s[i] = x[i] > neg_inf() ? exp_below(x[i], top) : 0.f;
-        total += s[i];
-      }
-      total = warp_sum(total);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = sigmoid(x[i]);  // 0 at -inf
-    }
-    if (biased) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) c[i] = x[i] > neg_inf() ? (a.softmax ? s[i] / total : s[i]) + b[i] : neg_inf();
-    }
-    if (grouped && a.top2 && !biased) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = x[i] > neg_inf() ? s[i] : neg_inf();
-      mask = kept_experts<V>(a, s, lane);
-    } else if (grouped) {
-      mask = kept_experts<V>(a, c, lane);
-    }
-  } else if (grouped) {
-    mask = kept_experts<V>(a, c, lane);
-  }
+  for (int i = 0; i < V; ++i) b[i] = biased && lane * V + i < a.num_experts ? a.bias[lane * V + i] : 0.f;
 
   int chosen = -1;
+  uint32_t mine = 0;
+  float top = neg_inf(), total = 0.f;  // of the token whose chosen expert the lane holds
+  T raw[V];
+  load_row<T, V>(raw, row, lane, a.num_experts, a.wide);
+  for (int n = 0; n < tokens; ++n) {
+    const int base = n * a.k_lanes;
+    T now[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) now[i] = raw[i];
+    row += a.stride;
+    if (n + 1 < tokens) load_row<T, V>(raw, row, lane, a.num_experts, a.wide);
+    uint32_t mask = kAll;  // experts of the lane that may be chosen
+    float c[V];  // what experts are ordered by: the logit (both scores grow with it), or the score plus the bias
+    if (sizeof(T) == 4 || need_score || grouped) {
+      float x[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) c[i] = x[i] = b[i] > neg_inf() ? logit(now[i]) : neg_inf();
+      if (need_score) {
+        float s[V];
+        if (a.softmax) {
+          float m = x[0], sum = 0.f;
+#pragma unroll
+          for (int i = 1; i < V; ++i) m = fmaxf(m, x[i]);
+          m = warp_max(m);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            s[i] = x[i] > neg_inf() ? exp_below(x[i], m) : 0.f;
+            sum += s[i];
+          }
+          sum = warp_sum(sum);
+          if (lane >= base) top = m, total = sum;  // later tokens' lanes are set again
+          if (biased) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) c[i] = s[i] / sum;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) s[i] = sigmoid(x[i]);
+          if (biased) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) c[i] = s[i];
+          }
+        }
+        if (biased) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) c[i] = x[i] > neg_inf() ? c[i] + b[i] : neg_inf();
+        }
+        if (grouped && a.top2 && !biased) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) s[i] = x[i] > neg_inf() ? s[i] : neg_inf();
+          mask = kept_experts<V>(a, s, lane);
+        } else if (grouped) {
+          mask = kept_experts<V>(a, c, lane);
+        }
+      } else if (grouped) {
+        mask = kept_experts<V>(a, c, lane);
+      }
+    }
+    uint32_t key[V];
+    if (sizeof(T) == 2 && !biased) {
+      if constexpr (sizeof(T) == 2) narrow_keys<T, V>(key, now, lane);
+      if (grouped) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = mask >> i & 1u ? key[i] : 0u;
+      }
+      choose<V, true>(key, a.k, lane, base, s_scratch[threadIdx.x >> 5], mine, chosen);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) key[i] = c[i] > neg_inf() && (mask >> i & 1u) ? order_key(c[i]) : 0u;
+      choose<V, false>(key, a.k, lane, base, s_scratch[threadIdx.x >> 5], mine, chosen);
+    }
+  }
+
+  const int n = lane / a.k_lanes, j = lane - n * a.k_lanes;
+  const int64_t t = t0 + n;
+  const bool has = chosen >= 0;
   float xc = neg_inf();  // the chosen expert's logit
-  if (sizeof(T) == 2 && !biased) {
-    // a 16-bit logit's order and its expert fit one word, lower experts above higher ones
-    uint32_t key[V], mine = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      // of the widened value the low 16 bits are zero (bf16), or the low 13 and the exponent's range is short (f16):
-      // the narrow value's own bits are ordered
-      const uint32_t bits = __float_as_uint(x[i]);
-      uint32_t narrow;
-      if constexpr (std::is_same_v<T, __nv_bfloat16>) narrow = bits >> 16;
-      else narrow = __half_as_ushort(__float2half_rn(x[i]));
-      narrow = (narrow ^ (narrow & 0x8000u ? 0xffffu : 0x8000u)) << 16;
-      key[i] = x[i] > neg_inf() && (mask >> i & 1u) ? narrow | (0xffffu - (lane * V + i)) : 0u;
-    }
-    for (int j = 0; j < a.k; ++j) {
-      uint32_t best = key[0];
-#pragma unroll
-      for (int i = 1; i < V; ++i) best = max(best, key[i]);
-      best = __reduce_max_sync(kAll, best);
-      if (best == 0) break;
-      if (lane == j) mine = best;
-#pragma unroll
-      for (int i = 0; i < V; ++i) key[i] = key[i] == best ? 0u : key[i];
-    }
-    if (mine != 0) {
-      chosen = 0xffff - (mine & 0xffffu);
+  if (has) {
+    if (biased) {
+      xc = logit(static_cast<const T*>(a.logits)[t * a.stride + chosen]);
+    } else if constexpr (std::is_same_v<T, float>) {
+      xc = from_order_key(mine);
+    } else {
       uint32_t narrow = mine >> 16;
       narrow ^= narrow & 0x8000u ? 0x8000u : 0xffffu;
       if constexpr (std::is_same_v<T, __nv_bfloat16>) xc = __uint_as_float(narrow << 16);
       else xc = __half2float(__ushort_as_half((unsigned short)narrow));
     }
-  } else {
-    uint32_t key[V], mine = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = c[i] > neg_inf() && (mask >> i & 1u) ? order_key(c[i]) : 0u;
-    for (int j = 0; j < a.k; ++j) {
-      uint32_t best = key[0];
-#pragma unroll
-      for (int i = 1; i < V; ++i) best = max(best, key[i]);
-      const uint32_t most = __reduce_max_sync(kAll, best);
-      if (most == 0) break;
-      const int owner = __ffs(__ballot_sync(kAll, best == most)) - 1;  // equal ones: the lower lane
-      int at = 0;
-      if (lane == owner) {
-        bool open = true;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if (open && key[i] == most) {
-            at = i;
-            key[i] = 0;
-            open = false;
-          }
-        }
-      }
-      at = __shfl_sync(kAll, at, owner) + owner * V;
-      if (lane == j) chosen = at, mine = most;
-    }
-    if (chosen >= 0) xc = biased ? logit(row[chosen]) : from_order_key(mine);
   }
-  const bool has = chosen >= 0;
   float w;
   if (a.softmax && a.renormalize) {
     const float m = max_over(xc, a.k_lanes);
@@ -315,99 +425,116 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(RouteArgs a) {
     const float sum = sum_over(w, a.k_lanes);
     w = sum > 0.f ? w / sum : 0.f;
   }
-  if (lane < a.k) {
-    a.experts[t * a.k + lane] = chosen;
-    a.weights[t * a.k + lane] = w * a.scale;
+  if (n < tokens && j < a.k) {
+    a.experts[t * a.k + j] = chosen;
+    a.weights[t * a.k + j] = w * a.scale;
   }
 }
 
-// One warp per token; the row of the gradient is put together in shared
-// memory.
+// A warp takes per_warp tokens: first the gradients at all their chosen
+// experts, k_lanes lanes to a token, then row after row, put together in
+// shared memory.
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwardArgs a) {
   __shared__ alignas(16) float s_row[kWarps][32 * V];
   const int lane = threadIdx.x & 31;
-  const int64_t t = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (t >= a.tokens) return;
-  const T* row = static_cast<const T*>(a.logits) + t * a.stride;
-  T* out = static_cast<T*>(a.grad_logits) + t * a.num_experts;
+  const int64_t t0 = ((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * a.per_warp;
+  if (t0 >= a.tokens) return;
+  const int tokens = (int)min((int64_t)a.per_warp, a.tokens - t0);
+  const int mine = lane / a.k_lanes, j = lane - mine * a.k_lanes;
+  const T* row = static_cast<const T*>(a.logits) + t0 * a.stride;
+  T* out = static_cast<T*>(a.grad_logits) + t0 * a.num_experts;
   float* buf = s_row[threadIdx.x >> 5];
 
-  const int id = lane < a.k ? a.experts[t * a.k + lane] : -1;
-  float xc = neg_inf();
-  if (id >= 0 && id < a.num_experts) xc = logit_at(row, a.bias, id);
+  int id = -1;
+  float xc = neg_inf(), g = 0.f;
+  if (mine < tokens && j < a.k) {
+    id = a.experts[(t0 + mine) * a.k + j];
+    g = a.grad_weights[(t0 + mine) * a.k + j];
+    if (id >= 0 && id < a.num_experts) xc = logit_at(row + mine * a.stride, a.bias, id);
+  }
   const bool has = xc > neg_inf();
-  const float g = has ? a.grad_weights[t * a.k + lane] : 0.f;
+  if (!has) g = 0.f;
 
   const bool dense = a.softmax && !a.renormalize;
-  float x[V], top = neg_inf(), total = 0.f;
-  if (dense) {
-    load_logits<T, V>(x, row, lane, a.num_experts, a.wide);
-    if (a.bias != nullptr) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const int e = lane * V + i;
-        if (e < a.num_experts && !(a.bias[e] > neg_inf())) x[i] = neg_inf();
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) top = fmaxf(top, x[i]);
-    top = warp_max(top);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      x[i] = x[i] > neg_inf() ? exp_below(x[i], top) : 0.f;
-      total += x[i];
-    }
-    total = warp_sum(total);
-  }
-  float at;          // the chosen experts' own part
-  float used = 0.f;  // sum over the chosen of g w (w without the scale)
-  if (a.softmax) {
-    float p;
-    if (a.renormalize) {
-      const float m = max_over(xc, a.k_lanes);
-      p = has ? exp_below(xc, m) : 0.f;
-      const float sum = sum_over(p, a.k_lanes);
-      p = sum > 0.f ? p / sum : 0.f;
-    } else {
-      p = has ? exp_below(xc, top) / total : 0.f;
-    }
-    used = __shfl_sync(kAll, sum_over(g * p, a.k_lanes), 0);
-    at = a.scale * p * (a.renormalize ? g - used : g);
-  } else {
+  float at = 0.f;  // the chosen experts' own part
+  if (a.softmax && a.renormalize) {
+    const float m = max_over(xc, a.k_lanes);
+    float p = has ? exp_below(xc, m) : 0.f;
+    const float sum = sum_over(p, a.k_lanes);
+    p = sum > 0.f ? p / sum : 0.f;
+    at = a.scale * p * (g - sum_over(g * p, a.k_lanes));
+  } else if (!a.softmax) {
     const float e = expf(-fabsf(xc));
     const float slope = has ? e / ((1.f + e) * (1.f + e)) : 0.f;  // s (1 - s), without the difference
     at = g;
     if (a.renormalize) {
       const float s = has ? sigmoid(xc) : 0.f;
       const float sum = sum_over(s, a.k_lanes);
-      used = sum_over(sum > 0.f ? g * (s / sum) : 0.f, a.k_lanes);
+      const float used = sum_over(sum > 0.f ? g * (s / sum) : 0.f, a.k_lanes);
       at = sum > 0.f ? (g - used) / sum : 0.f;
     }
     at *= a.scale * slope;
   }
-  const float each = dense && total > 0.f ? -(a.scale * used) / total : 0.f;
+  T raw[V];
+  if (dense) load_row<T, V>(raw, row, lane, a.num_experts, a.wide);
+  for (int n = 0; n < tokens; ++n, out += a.num_experts) {
+    float x[V];
+    if (dense) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) buf[lane * V + i] = dense ? each * x[i] : 0.f;
-  __syncwarp();
-  if (has) atomicAdd(&buf[id], at);  // ids of one token are distinct: no two lanes meet
-  __syncwarp();
-  constexpr int N = vector_length<T, V>();
-  if (a.wide) {
+      for (int i = 0; i < V; ++i) x[i] = logit(raw[i]);
+      row += a.stride;
+      if (n + 1 < tokens) load_row<T, V>(raw, row, lane, a.num_experts, a.wide);
+      if (a.bias != nullptr) {
 #pragma unroll
-    for (int c = 0; c < V; c += N) {
-      const int e = lane * V + c;
-      dev::Pack<T, N> p;
+        for (int i = 0; i < V; ++i) {
+          const int e = lane * V + i;
+          if (e < a.num_experts && !(a.bias[e] > neg_inf())) x[i] = neg_inf();
+        }
+      }
+      float top = x[0], total = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) p.v[i] = dev::from_float<T>(buf[e + i]);
-      if (e < a.num_experts) *reinterpret_cast<dev::Pack<T, N>*>(out + e) = p;
+      for (int i = 1; i < V; ++i) top = fmaxf(top, x[i]);
+      top = warp_max(top);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        x[i] = x[i] > neg_inf() ? exp_below(x[i], top) : 0.f;
+        total += x[i];
+      }
+      total = warp_sum(total);
+      const float p = has && mine == n ? exp_below(xc, top) / total : 0.f;
+      const float used = warp_sum(g * p);
+      if (mine == n) at = a.scale * p * g;
+      const float each = total > 0.f ? -(a.scale * used) / total : 0.f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] *= each;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) x[i] = 0.f;
     }
-  } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = i * 32 + lane;
-      if (e < a.num_experts) out[e] = dev::from_float<T>(buf[e]);
+    for (int i = 0; i < V; ++i) buf[lane * V + i] = x[i];
+    __syncwarp();
+    if (has && mine == n) atomicAdd(&buf[id], at);  // ids of one token are distinct: no two lanes meet
+    __syncwarp();
+    constexpr int N = vector_length<T, V>();
+    if (a.wide) {
+#pragma unroll
+      for (int c = 0; c < V; c += N) {
+        const int e = lane * V + c;
+        dev::Pack<T, N> p;
+#pragma unroll
+        for (int i = 0; i < N; ++i) p.v[i] = dev::from_float<T>(buf[e + i]);
+        if (e < a.num_experts) *reinterpret_cast<dev::Pack<T, N>*>(out + e) = p;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int e = i * 32 + lane;
+        if (e < a.num_experts) out[e] = dev::from_float<T>(buf[e]);
+      }
     }
+    __syncwarp();
   }
 }
 
@@ -436,9 +563,18 @@ int lanes_per_group(int num_experts, int per_group) {
   return per_group % v == 0 && (n & (n - 1)) == 0 ? n : 0;
 }
 
+// Tokens to a warp: what a warp does once for its tokens is the cheaper the
+// more they are, as long as kBusyWarps warps are left (about six to each of
+// the 592 schedulers).
+int tokens_per_warp(int64_t tokens, int k) {
+  int n = 32 / lanes_for(k);
+  while (n > 1 && tokens / n < kBusyWarps) n /= 2;
+  return n;
+}
+
 template <template <typename, int> class K, typename Args>
 cudaError_t launch(int type, int num_experts, int64_t tokens, const Args& a, cudaStream_t stream) {
-  const int64_t grid = (tokens + kWarps - 1) / kWarps;
+  const int64_t per_cta = (int64_t)kWarps * a.per_warp, grid = (tokens + per_cta - 1) / per_cta;
   if (grid > INT32_MAX) return cudaErrorInvalidValue;
   const bool known = with_float_type(type, [&](auto zero) {
     using T = decltype(zero);
@@ -484,8 +620,8 @@ extern "C" cudaError_t cusort_route(cusort_float_type type, const void* d_logits
   if (num_tokens == 0) return cudaSuccess;
   if (d_logits == nullptr || d_weights == nullptr || d_experts == nullptr) return cudaErrorInvalidValue;
   const int per_group = num_experts / groups;
-  const RouteArgs a{d_logits, row_stride, d_bias, d_weights, d_experts, num_tokens, num_experts, k, lanes_for(k), groups,
-                    groups_kept, per_group, lanes_per_group(num_experts, per_group),
+  const RouteArgs a{d_logits, row_stride, d_bias, d_weights, d_experts, num_tokens, num_experts, k, lanes_for(k),
+                    tokens_per_warp(num_tokens, k), groups, groups_kept, per_group, lanes_per_group(num_experts, per_group),
                     whole_vectors(type, num_experts, {d_logits}, row_stride), score == CUSORT_SCORE_SOFTMAX,
                     renormalize != 0, group_score == CUSORT_GROUP_TOP2, scale};
   return launch<Forward>(type, num_experts, num_tokens, a, stream);
@@ -501,7 +637,7 @@ extern "C" cudaError_t cusort_route_backward(cusort_float_type type, const float
   if (d_grad_weights == nullptr || d_logits == nullptr || d_experts == nullptr || d_grad_logits == nullptr)
     return cudaErrorInvalidValue;
   const RouteBackwardArgs a{d_grad_weights, d_logits, row_stride, d_bias, d_experts, d_grad_logits, num_tokens,
-                            num_experts, k, lanes_for(k),
+                            num_experts, k, lanes_for(k), tokens_per_warp(num_tokens, k),
                             whole_vectors(type, num_experts, {d_logits, d_grad_logits}, row_stride),
                             score == CUSORT_SCORE_SOFTMAX, renormalize != 0, scale};
   return launch<Backward>(type, num_experts, num_tokens, a, stream);
