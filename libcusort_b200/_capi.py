@@ -6,9 +6,12 @@ Loading fails loudly when it is missing: there is no fallback path.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libcusort_b200.so"
+NATIVE_PATH = LIB_PATH.with_name("_cusort_torch.so")
 
 # cusort_key_type (include/cusort_b200.h)
 KEY_TYPES = {
@@ -82,6 +85,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_native = None
 
 
 class CusortError(RuntimeError):
@@ -106,6 +110,24 @@ def load() -> C.CDLL:
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+def native():
+    """The native half of the PyTorch functions in routing.py and paging.py (raises if it has not been built)."""
+    global _native
+    if _native is None:
+        if not NATIVE_PATH.exists():
+            raise RuntimeError(
+                f"{NATIVE_PATH} is missing: build it with `python -m libcusort_b200.build` "
+                "(there is no CPU or library fallback for this path)")
+        import torch  # noqa: F401  (its libraries have to be there first)
+        load()
+        loader = importlib.machinery.ExtensionFileLoader("_cusort_torch", str(NATIVE_PATH))
+        spec = importlib.util.spec_from_loader("_cusort_torch", loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        _native = module
+    return _native
 
 
 def check(code: int, what: str) -> None:

@@ -3,6 +3,9 @@
 Every .cu under csrc/ is compiled for sm_100a only
 (-gencode arch=compute_100a,code=sm_100a) in parallel, then linked into one
 shared library with the CUDA runtime linked statically and NCCL dynamically.
+Where PyTorch is installed, csrc/torch_binding.cpp is compiled beside it
+(libcusort_b200/_lib/_cusort_torch.so): the native half of the routing and
+placement operators' Python functions, over the same C ABI.
 Run as ``python -m libcusort_b200.build`` or through ``__graft_entry__.build()``.
 
 Environment CUSORT_NVCC_DEFINES adds preprocessor definitions to every
@@ -13,10 +16,12 @@ kept beside the library, so a change of them forces a rebuild.
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -24,6 +29,7 @@ CSRC = PKG / "csrc"
 OUT_DIR = PKG / "_lib"
 OBJ_DIR = PKG / "_build"
 LIB = OUT_DIR / "libcusort_b200.so"
+BINDING = OUT_DIR / "_cusort_torch.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall",
@@ -65,12 +71,37 @@ def _compile(src: Path, verbose: bool) -> tuple[Path, str]:
     return obj, r.stderr
 
 
+def torch_dir() -> Path | None:
+    """Where PyTorch's headers and libraries lie (found without importing it)."""
+    spec = importlib.util.find_spec("torch")
+    return Path(list(spec.submodule_search_locations)[0]) if spec else None
+
+
+def _build_binding() -> None:
+    t = torch_dir()
+    if t is None:
+        print("PyTorch is not installed: the PyTorch binding is not built", file=sys.stderr)
+        return
+    cuda = Path(nvcc()).resolve().parents[1]
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-sign-compare",
+           "-I" + sysconfig.get_paths()["include"], "-isystem", str(t / "include"), "-isystem",
+           str(t / "include" / "torch" / "csrc" / "api" / "include"), "-isystem", str(cuda / "include"),
+           str(CSRC / "torch_binding.cpp"), "-o", str(tmp), "-L" + str(t / "lib"), "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-L" + str(OUT_DIR), "-l:" + LIB.name,
+           "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed for torch_binding.cpp:\n{r.stderr}")
+    os.replace(tmp, BINDING)
+
+
 def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
 def up_to_date() -> bool:
-    if not LIB.exists():
+    if not LIB.exists() or (torch_dir() is not None and not BINDING.exists()):
         return False
     if (STAMP.read_text() if STAMP.exists() else "") != " ".join(extra_defines()):
         return False
@@ -98,6 +129,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
+    _build_binding()
     STAMP.write_text(" ".join(extra_defines()))
     if verbose:
         print("".join(logs))
