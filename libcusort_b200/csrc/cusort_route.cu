@@ -246,7 +246,7 @@ __device__ __forceinline__ void narrow_keys(uint32_t (&key)[V], const T (&x)[V],
 // Which groups stay: lane's mask of its V experts (bit i: expert lane * V + i).
 // value: what groups go by, -inf where not available.
 template <int V>
-__device__ uint32_t kept_experts(const RouteArgs& a, const float (&value)[V], int lane) {
+__device__ __forceinline__ uint32_t kept_experts(const RouteArgs& a, const float (&value)[V], int lane) {
   if (a.group_lanes != 0) {
     // a group is group_lanes whole lanes: its two best by exchange among them
     float b1 = value[0], b2 = neg_inf();
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(RouteArgs a) {
     uint32_t mask = kAll;  // experts of the lane that may be chosen
     float c[V];  // what experts are ordered by: the logit (both scores grow with it), or the score plus the bias
     if (sizeof(T) == 4 || need_score || grouped) {
-      float x[V];
+      float x[V], value[V];  // value: what groups go by
 #pragma unroll
       for (int i = 0; i < V; ++i) c[i] = x[i] = b[i] > neg_inf() ? logit(now[i]) : neg_inf();
       if (need_score) {
@@ -372,16 +372,16 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(RouteArgs a) {
 #pragma unroll
           for (int i = 0; i < V; ++i) c[i] = x[i] > neg_inf() ? c[i] + b[i] : neg_inf();
         }
-        if (grouped && a.top2 && !biased) {
+        if (a.top2 && !biased) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) s[i] = x[i] > neg_inf() ? s[i] : neg_inf();
-          mask = kept_experts<V>(a, s, lane);
-        } else if (grouped) {
-          mask = kept_experts<V>(a, c, lane);
+          for (int i = 0; i < V; ++i) value[i] = x[i] > neg_inf() ? s[i] : neg_inf();
         }
-      } else if (grouped) {
-        mask = kept_experts<V>(a, c, lane);
       }
+      if (biased || !a.top2) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) value[i] = c[i];
+      }
+      if (grouped) mask = kept_experts<V>(a, value, lane);
     }
     uint32_t key[V];
     if (sizeof(T) == 2 && !biased) {

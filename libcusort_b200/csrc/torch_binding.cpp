@@ -253,9 +253,10 @@ PyObject* plan_dispatch(PyObject* const* p) {
     return cusort_plan_dispatch(nullptr, &bytes, wide ? 8 : 4, nullptr, pairs, (int)num, (int)align, capacity, nullptr,
                                 nullptr, nullptr, nullptr, s);
   });
-  at::Tensor temp = empty({(int64_t)bytes}, at::kByte, device);
   at::Tensor counts = empty({num}, at::kInt, device), offsets = empty({num + 1}, at::kInt, device);
   at::Tensor sources = empty({capacity}, at::kInt, device), positions = empty(experts.sizes(), at::kInt, device);
+  // one byte is asked for where nothing is needed: any address does
+  const at::Tensor temp = bytes > 1 ? empty({(int64_t)bytes}, at::kByte, device) : counts;
   launch("cusort_plan_dispatch", device, [&](cudaStream_t s) {
     return cusort_plan_dispatch(temp.data_ptr(), &bytes, wide ? 8 : 4, experts.data_ptr(), pairs, (int)num, (int)align,
                                 capacity, ptr<int32_t>(counts), ptr<int32_t>(offsets), ptr<int32_t>(sources),
