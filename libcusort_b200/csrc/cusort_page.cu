@@ -19,6 +19,8 @@ constexpr uint32_t kMost = 0x7fffffffu;
 struct PageArgs {
   const int32_t *cached, *fresh;  // tokens in the cache, tokens of this step
   int num_requests, block_size, num_blocks;  // num_blocks: length of the free list
+  unsigned long long inverse;                // of the block size, see blocks_of
+  bool whole_lengths;                        // the lengths can be read four at a time
   int64_t num_tokens;
   int32_t* tables;
   int64_t table_stride;
@@ -33,19 +35,48 @@ struct PageArgs {
 // Sums stop at 2^31 - 1, so that lengths of any size keep their order.
 __device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) { return min(a + b, kMost); }
 
+// n / a.block_size for n < 2^32: the high word of n * (2^64 / size rounded up), which errs by less than n * size / 2^64.
+__device__ __forceinline__ uint32_t blocks_of(const PageArgs& a, uint32_t n) {
+  return a.block_size == 1 ? n : (uint32_t)__umul64hi(n, a.inverse);
+}
+
+// The sum of 32 lanes' values, each at most 2^31 - 1, up to that.
+__device__ __forceinline__ uint32_t sum_sat(uint32_t v) {
+  const uint64_t high = __reduce_add_sync(kAll, v >> 16), low = __reduce_add_sync(kAll, v & 0xffffu);
+  return (uint32_t)min((high << 16) + low, (uint64_t)kMost);
+}
+
 struct Request {
-  uint32_t cached, fresh, need;  // need: blocks to be taken from the free list
+  uint32_t cached, fresh, held, need;  // held: blocks before this step; need: blocks to be taken from the free list
   bool fits;
 };
 
-__device__ __forceinline__ Request request_of(const PageArgs& a, int r) {
+__device__ __forceinline__ Request request_of(const PageArgs& a, int32_t cached, int32_t fresh) {
   Request q;
-  q.cached = (uint32_t)max(a.cached[r], 0);
-  q.fresh = (uint32_t)max(a.fresh[r], 0);
-  const uint32_t b = a.block_size, held = (q.cached + b - 1) / b, end = (q.cached + q.fresh + b - 1) / b;
+  q.cached = (uint32_t)max(cached, 0);
+  q.fresh = (uint32_t)max(fresh, 0);
+  const uint32_t up = a.block_size - 1;
+  q.held = blocks_of(a, q.cached + up);
+  const uint32_t end = blocks_of(a, q.cached + q.fresh + up);  // of no use beyond 2^31, where the request does not fit
   q.fits = q.cached + q.fresh <= kMost && end <= (uint32_t)a.table_width;
-  q.need = q.fits && a.num_free != nullptr ? end - held : 0;
+  q.need = q.fits && a.num_free != nullptr ? end - q.held : 0;
   return q;
+}
+__device__ __forceinline__ Request request_of(const PageArgs& a, int r) {
+  return request_of(a, a.cached[r], a.fresh[r]);
+}
+
+// The last of starts[0 .. n) that is at most i (starts[0] is), found by the
+// whole warp.
+__device__ __forceinline__ int warp_search(const uint32_t* starts, int n, int64_t i, int lane) {
+  int at = 0;
+  while (n > 1) {
+    const int step = (n + 31) >> 5, probe = lane * step;
+    const int below = __popc(__ballot_sync(kAll, probe < n && starts[at + (probe < n ? probe : 0)] <= i));
+    at += (below - 1) * step;
+    n = min(step, n - (below - 1) * step);
+  }
+  return at;
 }
 
 // Every CTA scans all requests (they are few), then takes its share of the
@@ -60,68 +91,78 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
   __shared__ uint32_t s_sums[2][W];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = a.num_requests;
   uint32_t *s_start = s_scan, *s_taken = s_scan + R + 1;
-  for (int r = threadIdx.x; r < R; r += THREADS) {
-    const Request q = request_of(a, r);
-    s_start[r] = q.fresh;
-    s_taken[r] = q.need;
-  }
-  __syncthreads();
-  const int each = (R + THREADS - 1) / THREADS, r0 = min((int)threadIdx.x * each, R), r1 = min(r0 + each, R);
-  uint32_t tokens = 0, blocks = 0;
-  for (int r = r0; r < r1; ++r) {
-    const uint32_t n = s_start[r], b = s_taken[r];
-    s_start[r] = tokens;
-    s_taken[r] = blocks;
-    tokens = add_sat(tokens, n);
-    blocks = add_sat(blocks, b);
-  }
-  uint32_t in_t = tokens, in_b = blocks;
+  uint32_t sum_t = 0, sum_b = 0;  // of the requests so far
+  for (int base = 0; base < R; base += THREADS * 4) {
+    const int r0 = base + threadIdx.x * 4;
+    int32_t cached[4], fresh[4];
+    if (a.whole_lengths && r0 + 4 <= R) {
+      *reinterpret_cast<int4*>(cached) = *reinterpret_cast<const int4*>(a.cached + r0);
+      *reinterpret_cast<int4*>(fresh) = *reinterpret_cast<const int4*>(a.fresh + r0);
+    } else {
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const uint32_t t = __shfl_up_sync(kAll, in_t, d), b = __shfl_up_sync(kAll, in_b, d);
-    if (lane >= d) in_t = add_sat(in_t, t), in_b = add_sat(in_b, b);
+      for (int j = 0; j < 4; ++j) {
+        cached[j] = r0 + j < R ? a.cached[r0 + j] : 0;
+        fresh[j] = r0 + j < R ? a.fresh[r0 + j] : 0;
+      }
+    }
+    uint32_t tokens[4], blocks[4], in_t = 0, in_b = 0;  // before each of the four, then of all
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const Request q = request_of(a, cached[j], fresh[j]);
+      tokens[j] = in_t;
+      blocks[j] = in_b;
+      in_t = add_sat(in_t, q.fresh);
+      in_b = add_sat(in_b, q.need);
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t t = __shfl_up_sync(kAll, in_t, d), b = __shfl_up_sync(kAll, in_b, d);
+      if (lane >= d) in_t = add_sat(in_t, t), in_b = add_sat(in_b, b);
+    }
+    if (lane == 31) s_sums[0][warp] = in_t, s_sums[1][warp] = in_b;
+    uint32_t before_t = __shfl_up_sync(kAll, in_t, 1), before_b = __shfl_up_sync(kAll, in_b, 1);
+    if (lane == 0) before_t = before_b = 0;
+    __syncthreads();
+    const uint32_t warp_t = lane < W ? s_sums[0][lane] : 0, warp_b = lane < W ? s_sums[1][lane] : 0;
+    before_t = add_sat(add_sat(before_t, sum_t), sum_sat(lane < warp ? warp_t : 0));
+    before_b = add_sat(add_sat(before_b, sum_b), sum_sat(lane < warp ? warp_b : 0));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (r0 + j < R) {
+        s_start[r0 + j] = add_sat(before_t, tokens[j]);
+        s_taken[r0 + j] = add_sat(before_b, blocks[j]);
+      }
+    }
+    sum_t = add_sat(sum_t, sum_sat(warp_t));
+    sum_b = add_sat(sum_b, sum_sat(warp_b));
+    __syncthreads();
   }
-  uint32_t before_t = __shfl_up_sync(kAll, in_t, 1), before_b = __shfl_up_sync(kAll, in_b, 1);
-  if (lane == 0) before_t = before_b = 0;
-  if (lane == 31) s_sums[0][warp] = in_t, s_sums[1][warp] = in_b;
-  __syncthreads();
-  for (int w = 0; w < warp; ++w) before_t = add_sat(before_t, s_sums[0][w]), before_b = add_sat(before_b, s_sums[1][w]);
-  for (int r = r0; r < r1; ++r) {
-    s_start[r] = add_sat(s_start[r], before_t);
-    s_taken[r] = add_sat(s_taken[r], before_b);
-  }
-  if (threadIdx.x == THREADS - 1) {
-    s_start[R] = add_sat(before_t, tokens);
-    s_taken[R] = add_sat(before_b, blocks);
-  }
+  if (threadIdx.x == 0) s_start[R] = sum_t, s_taken[R] = sum_b;
   __syncthreads();
   const uint32_t left = a.num_free == nullptr ? 0u : (uint32_t)min(max(*a.num_free, 0), a.num_blocks);
-  if (blockIdx.x == 0) {
-    uint32_t used = 0;
-    for (int r = threadIdx.x; r < R; r += THREADS) {
+  for (int r = blockIdx.x * THREADS + threadIdx.x; r <= R; r += gridDim.x * THREADS) {
+    a.starts[r] = (int32_t)s_start[r];
+    const uint32_t taken = s_taken[r];
+    // the requests before r got their blocks, and r is the first that did not
+    if (a.num_free_out != nullptr && taken <= left && (r == R || s_taken[r + 1] > left))
+      *a.num_free_out = (int32_t)(left - taken);
+    if (r < R) {
       const Request q = request_of(a, r);
-      const uint32_t upto = s_taken[r + 1];
-      a.served[r] = q.fits && (q.need == 0 || upto <= left);
-      if (upto <= left) used = max(used, upto);
-    }
-    for (int r = threadIdx.x; r <= R; r += THREADS) a.starts[r] = (int32_t)s_start[r];
-    used = __reduce_max_sync(kAll, used);
-    __syncthreads();
-    if (lane == 0) s_sums[0][warp] = used;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < W; ++w) used = max(used, s_sums[0][w]);
-      if (a.num_free_out != nullptr) *a.num_free_out = (int32_t)(left - used);
+      a.served[r] = q.fits && (q.need == 0 || s_taken[r + 1] <= left);
     }
   }
   const int64_t total = s_start[R], most = max(total, a.num_tokens);
   const uint32_t size = a.block_size;
-  for (int64_t i0 = ((int64_t)blockIdx.x * THREADS + threadIdx.x) * N; i0 < most; i0 += (int64_t)gridDim.x * THREADS * N) {
+  for (int64_t w0 = ((int64_t)blockIdx.x * THREADS + warp * 32) * N; w0 < most; w0 += (int64_t)gridDim.x * THREADS * N) {
+    const int64_t i0 = w0 + lane * N;
     int64_t slot[N];
     int32_t position[N];
-    int r = 0;  // the last request that starts at or before i0
-    if (i0 < total) {
-      int hi = R;
+    // the last request that starts at or before i0: the warp's first one by all of its lanes, then each lane from
+    // there to the warp's last one
+    int r = 0;
+    if (w0 < total) {
+      r = warp_search(s_start, R, w0, lane);
+      int hi = r + 1 + warp_search(s_start + r, R - r, min(w0 + 32 * N, total) - 1, lane);
       while (hi - r > 1) {
         const int mid = (r + hi) >> 1;
         if (s_start[mid] <= i0) r = mid; else hi = mid;
@@ -142,9 +183,9 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
         next = s_start[r + 1];
         taken = s_taken[r];
         pos = min(q.cached + (uint32_t)(i - s_start[r]), kMost);
-        page = pos / size;
+        page = blocks_of(a, pos);
         in = pos - page * size;
-        held = a.num_free != nullptr ? (q.cached + size - 1) / size : (uint32_t)a.table_width;
+        held = a.num_free != nullptr ? q.held : (uint32_t)a.table_width;
         served = q.fits && (q.need == 0 || s_taken[r + 1] <= left);
         table = a.tables + r * a.table_stride;
         fetch = true;
@@ -211,7 +252,10 @@ extern "C" cudaError_t cusort_page_plan(const int32_t* d_cached_lens, const int3
                             (table_width > 0 && d_block_tables == nullptr))) ||
       (num_tokens > 0 && (d_slots == nullptr || d_positions == nullptr)))
     return cudaErrorInvalidValue;
-  const PageArgs a{d_cached_lens, d_new_lens, num_requests, block_size, num_blocks, num_tokens, d_block_tables,
+  const bool whole =
+      ((reinterpret_cast<uintptr_t>(d_cached_lens) | reinterpret_cast<uintptr_t>(d_new_lens)) & 15) == 0;
+  const unsigned long long inverse = block_size == 1 ? 0 : ~0ull / block_size + 1;
+  const PageArgs a{d_cached_lens, d_new_lens, num_requests, block_size, num_blocks, inverse, whole, num_tokens, d_block_tables,
                    table_stride, table_width, d_free_blocks, d_num_free, d_slots, d_positions, d_starts, d_served,
                    d_num_free_out};
   // Four tokens to a thread need one search instead of four and whole-vector stores, but a longer chain; a large CTA
