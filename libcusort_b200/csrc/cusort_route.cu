@@ -308,17 +308,22 @@ __device__ __forceinline__ uint32_t kept_experts(const RouteArgs& a, const float
 // experts, so that a lower lane means a lower expert and groups are runs of
 // lanes.  The chosen experts of its tokens lie k_lanes lanes apart, and their
 // weights are computed for all tokens at once.
-template <typename T, int V>
-__global__ void __launch_bounds__(32 * kWarps) route_kernel(RouteArgs a) {
+//
+// SCORED: scores of all experts are needed (a softmax's sum, a bias, groups by
+// their scores); GROUPED: groups_kept < groups.  A kernel of its own for what
+// needs neither holds half the registers.
+// Seven CTAs to an SM instead of the four that the scored kernels would take
+// (8192 x 256 logits, us: softmax 9.5 -> 8.0, sigmoid, bias and groups 14.7 ->
+// 13.2, in spite of 48 bytes spilled; ten CTAs 14.8).
+template <typename T, int V, bool SCORED, bool GROUPED>
+__global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 7 : 1) route_kernel(RouteArgs a) {
   __shared__ uint2 s_scratch[kWarps][32];
   const int lane = threadIdx.x & 31;
   const int64_t t0 = ((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * a.per_warp;
   if (t0 >= a.tokens) return;
   const int tokens = (int)min((int64_t)a.per_warp, a.tokens - t0);
   const T* row = static_cast<const T*>(a.logits) + t0 * a.stride;
-  const bool biased = a.bias != nullptr, grouped = a.groups_kept < a.groups;
-  const bool need_total = a.softmax && (biased || !a.renormalize);
-  const bool need_score = need_total || biased || (grouped && a.top2);
+  const bool biased = SCORED && a.bias != nullptr;
 
   float b[V];
 #pragma unroll
@@ -338,11 +343,11 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(RouteArgs a) {
     if (n + 1 < tokens) load_row<T, V>(raw, row, lane, a.num_experts, a.wide);
     uint32_t mask = kAll;  // experts of the lane that may be chosen
     float c[V];  // what experts are ordered by: the logit (both scores grow with it), or the score plus the bias
-    if (sizeof(T) == 4 || need_score || grouped) {
+    if constexpr (sizeof(T) == 4 || SCORED || GROUPED) {
       float x[V], value[V];  // value: what groups go by
 #pragma unroll
       for (int i = 0; i < V; ++i) c[i] = x[i] = b[i] > neg_inf() ? logit(now[i]) : neg_inf();
-      if (need_score) {
+      if constexpr (SCORED) {
         float s[V];
         if (a.softmax) {
           float m = x[0], sum = 0.f;
@@ -381,12 +386,12 @@ __global__ void __launch_bounds__(32 * kWarps) route_kernel(RouteArgs a) {
 #pragma unroll
         for (int i = 0; i < V; ++i) value[i] = c[i];
       }
-      if (grouped) mask = kept_experts<V>(a, value, lane);
+      if constexpr (GROUPED) mask = kept_experts<V>(a, value, lane);
     }
     uint32_t key[V];
     if (sizeof(T) == 2 && !biased) {
       if constexpr (sizeof(T) == 2) narrow_keys<T, V>(key, now, lane);
-      if (grouped) {
+      if constexpr (GROUPED) {
 #pragma unroll
         for (int i = 0; i < V; ++i) key[i] = mask >> i & 1u ? key[i] : 0u;
       }
@@ -591,7 +596,13 @@ cudaError_t launch(int type, int num_experts, int64_t tokens, const Args& a, cud
 }
 
 template <typename T, int V> struct Forward {
-  static void run(int grid, const RouteArgs& a, cudaStream_t s) { route_kernel<T, V><<<grid, 32 * kWarps, 0, s>>>(a); }
+  static void run(int grid, const RouteArgs& a, cudaStream_t s) {
+    const bool grouped = a.groups_kept < a.groups;
+    const bool scored = a.bias != nullptr || (a.softmax && !a.renormalize) || (grouped && a.top2);
+    if (grouped) route_kernel<T, V, true, true><<<grid, 32 * kWarps, 0, s>>>(a);
+    else if (scored) route_kernel<T, V, true, false><<<grid, 32 * kWarps, 0, s>>>(a);
+    else route_kernel<T, V, false, false><<<grid, 32 * kWarps, 0, s>>>(a);
+  }
 };
 template <typename T, int V> struct Backward {
   static void run(int grid, const RouteBackwardArgs& a, cudaStream_t s) {
