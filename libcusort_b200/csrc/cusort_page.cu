@@ -7,6 +7,7 @@
 #include <cstdint>
 
 #include "../../include/cusort_b200.h"
+#include "cusort_overlap.cuh"
 
 namespace {
 
@@ -91,6 +92,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
   __shared__ uint32_t s_sums[2][W];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = a.num_requests;
   uint32_t *s_start = s_scan, *s_taken = s_scan + R + 1;
+  cusort_b200::dev::wait_for_previous();
   uint32_t sum_t = 0, sum_b = 0;  // of the requests so far
   for (int base = 0; base < R; base += THREADS * 4) {
     const int r0 = base + threadIdx.x * 4;
@@ -230,8 +232,7 @@ cudaError_t run(const PageArgs& a, cudaStream_t stream) {
   }
   const int64_t per_cta = THREADS * N;
   const int grid = (int)std::max<int64_t>(1, std::min<int64_t>(148, (a.num_tokens + per_cta - 1) / per_cta));
-  page_plan_kernel<THREADS, N><<<grid, THREADS, smem, stream>>>(a);
-  return cudaGetLastError();
+  return cusort_b200::launch_after_previous(page_plan_kernel<THREADS, N>, grid, THREADS, smem, a, stream);
 }
 
 }  // namespace

@@ -7,7 +7,7 @@
 #include <cstdint>
 
 #include "../../include/cusort_b200.h"
-#include "cusort_device.cuh"
+#include "cusort_overlap.cuh"
 
 namespace {
 
@@ -51,7 +51,7 @@ __device__ __forceinline__ int expert_of(const PlanArgs& a, int64_t i, int64_t e
 template <typename I>
 __global__ void __launch_bounds__(kThreads) plan_count_kernel(PlanArgs a) {
   __shared__ uint32_t s_count[kMaxExperts];
-  dev::pdl_launch_dependents();
+  dev::wait_for_previous();
   clear_sources(a, (int64_t)blockIdx.x * kThreads + threadIdx.x, (int64_t)gridDim.x * kThreads);
   for (int e = threadIdx.x; e < a.num_experts; e += kThreads) s_count[e] = 0;
   __syncthreads();
@@ -114,6 +114,7 @@ __global__ void __launch_bounds__(THREADS) plan_place_kernel(PlanArgs a) {
   const bool alone = a.tile_counts == nullptr;
   const int bits = 32 - __clz(E);  // E itself stands for no expert
   uint16_t* mine = s_warp + warp * E;
+  dev::wait_for_previous();
   if (alone) clear_sources(a, threadIdx.x, THREADS);  // else the count kernel's part
   for (int e = threadIdx.x; e < E; e += THREADS) s_before[e] = s_total[e] = 0;
 
@@ -145,7 +146,6 @@ __global__ void __launch_bounds__(THREADS) plan_place_kernel(PlanArgs a) {
   if (!alone) {
     // columns of the tiles' counts: as many threads to an expert as there are
     __syncthreads();
-    dev::pdl_wait();
     const int parts = max(1, THREADS / E), tiles = gridDim.x;
     for (int i = threadIdx.x; i < parts * E; i += THREADS) {
       const int e = i % E;
@@ -258,25 +258,14 @@ cudaError_t place(const PlanArgs& a, int tiles, cudaStream_t stream) {
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     if (e) return e;
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(tiles);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = tiles > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, plan_place_kernel<I, THREADS>, a);
+  return launch_after_previous(plan_place_kernel<I, THREADS>, tiles, THREADS, smem, a, stream);
 }
 
 template <typename I>
 cudaError_t run(const PlanArgs& a, int tiles, cudaStream_t stream) {
   if (tiles == 1 && a.items <= kSmallItems) return place<I, kSmallThreads>(a, 1, stream);
   if (tiles > 1) {
-    plan_count_kernel<I><<<tiles, kThreads, 0, stream>>>(a);
-    if (const cudaError_t e = cudaGetLastError()) return e;
+    if (const cudaError_t e = launch_after_previous(plan_count_kernel<I>, tiles, kThreads, 0, a, stream)) return e;
   }
   return place<I, kThreads>(a, tiles, stream);
 }

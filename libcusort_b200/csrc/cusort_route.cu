@@ -8,8 +8,8 @@
 #include <type_traits>
 
 #include "../../include/cusort_b200.h"
-#include "cusort_device.cuh"
 #include "cusort_float.cuh"
+#include "cusort_overlap.cuh"
 
 namespace {
 
@@ -317,6 +317,7 @@ __device__ __forceinline__ uint32_t kept_experts(const RouteArgs& a, const float
 // 13.2, in spite of 48 bytes spilled; ten CTAs 14.8).
 template <typename T, int V, bool SCORED, bool GROUPED>
 __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 7 : 1) route_kernel(RouteArgs a) {
+  dev::wait_for_previous();
   __shared__ uint2 s_scratch[kWarps][32];
   const int lane = threadIdx.x & 31;
   const int64_t t0 = ((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * a.per_warp;
@@ -441,6 +442,7 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 7 : 1) route_kernel(Rout
 // shared memory.
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwardArgs a) {
+  dev::wait_for_previous();
   __shared__ alignas(16) float s_row[kWarps][32 * V];
   const int lane = threadIdx.x & 31;
   const int64_t t0 = ((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * a.per_warp;
@@ -580,33 +582,34 @@ int tokens_per_warp(int64_t tokens, int k) {
 template <template <typename, int> class K, typename Args>
 cudaError_t launch(int type, int num_experts, int64_t tokens, const Args& a, cudaStream_t stream) {
   const int64_t per_cta = (int64_t)kWarps * a.per_warp, grid = (tokens + per_cta - 1) / per_cta;
-  if (grid > INT32_MAX) return cudaErrorInvalidValue;
-  const bool known = with_float_type(type, [&](auto zero) {
+  cudaError_t err = cudaErrorInvalidValue;
+  with_float_type(type, [&](auto zero) {
     using T = decltype(zero);
     switch (experts_per_lane(num_experts)) {
-      case 1: K<T, 1>::run((int)grid, a, stream); break;
-      case 2: K<T, 2>::run((int)grid, a, stream); break;
-      case 4: K<T, 4>::run((int)grid, a, stream); break;
-      case 8: K<T, 8>::run((int)grid, a, stream); break;
-      case 16: K<T, 16>::run((int)grid, a, stream); break;
-      default: K<T, 32>::run((int)grid, a, stream); break;
+      case 1: err = K<T, 1>::run(grid, a, stream); break;
+      case 2: err = K<T, 2>::run(grid, a, stream); break;
+      case 4: err = K<T, 4>::run(grid, a, stream); break;
+      case 8: err = K<T, 8>::run(grid, a, stream); break;
+      case 16: err = K<T, 16>::run(grid, a, stream); break;
+      default: err = K<T, 32>::run(grid, a, stream); break;
     }
   });
-  return known ? cudaGetLastError() : cudaErrorInvalidValue;
+  return err;
 }
 
 template <typename T, int V> struct Forward {
-  static void run(int grid, const RouteArgs& a, cudaStream_t s) {
+  static cudaError_t run(int64_t grid, const RouteArgs& a, cudaStream_t s) {
     const bool grouped = a.groups_kept < a.groups;
     const bool scored = a.bias != nullptr || (a.softmax && !a.renormalize) || (grouped && a.top2);
-    if (grouped) route_kernel<T, V, true, true><<<grid, 32 * kWarps, 0, s>>>(a);
-    else if (scored) route_kernel<T, V, true, false><<<grid, 32 * kWarps, 0, s>>>(a);
-    else route_kernel<T, V, false, false><<<grid, 32 * kWarps, 0, s>>>(a);
+    return launch_after_previous(grouped  ? route_kernel<T, V, true, true>
+                                 : scored ? route_kernel<T, V, true, false>
+                                          : route_kernel<T, V, false, false>,
+                                 grid, 32 * kWarps, 0, a, s);
   }
 };
 template <typename T, int V> struct Backward {
-  static void run(int grid, const RouteBackwardArgs& a, cudaStream_t s) {
-    route_backward_kernel<T, V><<<grid, 32 * kWarps, 0, s>>>(a);
+  static cudaError_t run(int64_t grid, const RouteBackwardArgs& a, cudaStream_t s) {
+    return launch_after_previous(route_backward_kernel<T, V>, grid, 32 * kWarps, 0, a, s);
   }
 };
 

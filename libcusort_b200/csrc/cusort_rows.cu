@@ -10,6 +10,7 @@
 
 #include "../../include/cusort_b200.h"
 #include "cusort_float.cuh"
+#include "cusort_overlap.cuh"
 
 namespace {
 
@@ -19,7 +20,7 @@ constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBackwardThreads = 256;
 constexpr int kMaxChosen = 32;
-constexpr int kEmptyRows = 4;           // rows that a warp looks at to clear those without a pair
+constexpr int kEmptyRows = 8;           // rows that a warp looks at to clear those without a pair
 constexpr int64_t kBusyWarps = 148 * 16;
 constexpr uint32_t kAll = 0xffffffffu;
 
@@ -62,6 +63,7 @@ struct DispatchArgs {
 // 93 % (8192 tokens, k = 8, rows of 8 KB).
 template <typename V, int U>
 __global__ void __launch_bounds__(kThreads) dispatch_kernel(DispatchArgs a) {
+  dev::wait_for_previous();
   const int lane = threadIdx.x & 31;
   int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   const V* x = static_cast<const V*>(a.x);
@@ -104,6 +106,7 @@ struct CombineArgs {
 // of 8 KB: K x U = 4 x 1 85 % of the copy rate, 4 x 2 91 %, 4 x 4 99 %).
 template <typename T, int N, int U>
 __global__ void __launch_bounds__(kThreads) combine_kernel(CombineArgs a) {
+  dev::wait_for_previous();
   using B = dev::Bits<T, N>;
   constexpr int K = 4;
   const int lane = threadIdx.x & 31;
@@ -186,6 +189,7 @@ struct CombineBackwardArgs {
 // that hold no pair.
 template <typename T, int N, int U>
 __global__ void __launch_bounds__(kBackwardThreads) combine_backward_kernel(CombineBackwardArgs a) {
+  dev::wait_for_previous();
   using B = dev::Bits<T, N>;
   const int lane = threadIdx.x & 31;
   int64_t w = (int64_t)blockIdx.x * (kBackwardThreads / 32) + (threadIdx.x >> 5);
@@ -261,20 +265,15 @@ cudaError_t dispatch(DispatchArgs a, size_t row_bytes, int64_t stride_bytes, cud
   a.stride = stride_bytes / (int64_t)sizeof(V);
   a.chunks = div_up(a.vectors, 32 * U);
   a.empty_warps = div_up(a.capacity, kEmptyRows);
-  const int64_t grid = div_up(a.empty_warps + a.tokens * a.chunks, kWarps);
-  if (grid > INT32_MAX) return cudaErrorInvalidValue;
-  dispatch_kernel<V, U><<<(int)grid, kThreads, 0, stream>>>(a);
-  return cudaGetLastError();
+  return launch_after_previous(dispatch_kernel<V, U>, div_up(a.empty_warps + a.tokens * a.chunks, kWarps), kThreads, 0,
+                               a, stream);
 }
 
 template <typename T, int BYTES, int U>
 cudaError_t combine(CombineArgs a, cudaStream_t stream) {
   constexpr int N = BYTES / (int)sizeof(T);
   a.chunks = div_up(a.hidden, 32 * N * U);
-  const int64_t grid = div_up(a.tokens * a.chunks, kWarps);
-  if (grid > INT32_MAX) return cudaErrorInvalidValue;
-  combine_kernel<T, N, U><<<(int)grid, kThreads, 0, stream>>>(a);
-  return cudaGetLastError();
+  return launch_after_previous(combine_kernel<T, N, U>, div_up(a.tokens * a.chunks, kWarps), kThreads, 0, a, stream);
 }
 
 template <typename T, int BYTES, int U>
@@ -282,9 +281,8 @@ cudaError_t combine_backward(CombineBackwardArgs a, cudaStream_t stream) {
   a.empty_warps = div_up(a.capacity, kEmptyRows);
   const int64_t grid = div_up(a.empty_warps + a.pairs, kBackwardThreads / 32);
   if (grid == 0) return cudaSuccess;
-  if (grid > INT32_MAX) return cudaErrorInvalidValue;
-  combine_backward_kernel<T, BYTES / (int)sizeof(T), U><<<(int)grid, kBackwardThreads, 0, stream>>>(a);
-  return cudaGetLastError();
+  return launch_after_previous(combine_backward_kernel<T, BYTES / (int)sizeof(T), U>, grid, kBackwardThreads, 0, a,
+                               stream);
 }
 
 }  // namespace
