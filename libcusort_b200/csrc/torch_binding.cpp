@@ -11,6 +11,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/TensorImpl.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -125,6 +126,70 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, at::Device device) 
   return at::Tensor(at::detail::empty_cuda(shape, type, device, std::nullopt));
 }
 
+// The outputs of one call: each an allocation of its own, or all of them parts
+// of one (five allocations took as long as the launch).
+class Outputs {
+ public:
+  Outputs(at::Device device, bool separate) : device_(device), separate_(separate) {}
+
+  // Asks for an output; its number.
+  int add(at::IntArrayRef shape, at::ScalarType type) {
+    Output& o = outputs_[count_];
+    o.type = type;
+    o.shape.assign(shape.begin(), shape.end());
+    int64_t bytes = (int64_t)c10::elementSize(type);
+    for (const int64_t n : shape) bytes *= n;
+    o.offset = bytes_;
+    bytes_ += (bytes + 15) & ~int64_t(15);
+    return count_++;
+  }
+
+  void allocate() {
+    if (separate_) {
+      for (int i = 0; i < count_; ++i) outputs_[i].tensor = empty(outputs_[i].shape, outputs_[i].type, device_);
+      return;
+    }
+    const at::Tensor all = empty({bytes_}, at::kByte, device_);
+    for (int i = 0; i < count_; ++i) {
+      Output& o = outputs_[i];
+      o.tensor = at::detail::make_tensor<c10::TensorImpl>(
+          c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(o.type));
+      o.tensor.unsafeGetTensorImpl()->set_storage_offset(o.offset / (int64_t)c10::elementSize(o.type));
+      o.tensor.unsafeGetTensorImpl()->set_sizes_contiguous(o.shape);
+    }
+  }
+
+  template <typename T>
+  T* ptr(int i) const {
+    return static_cast<T*>(outputs_[i].tensor.data_ptr());
+  }
+
+  // The outputs as a tuple; extra None: one more element.
+  PyObject* tuple(bool extra_none = false) {
+    PyObject* t = PyTuple_New(count_ + extra_none);
+    if (t == nullptr) throw Refused{nullptr, {}};
+    for (int i = 0; i < count_; ++i) PyTuple_SET_ITEM(t, i, THPVariable_Wrap(std::move(outputs_[i].tensor)));
+    if (extra_none) {
+      Py_INCREF(Py_None);
+      PyTuple_SET_ITEM(t, count_, Py_None);
+    }
+    return t;
+  }
+
+ private:
+  struct Output {
+    at::ScalarType type;
+    c10::SmallVector<int64_t, 4> shape;
+    int64_t offset;
+    at::Tensor tensor;
+  };
+  at::Device device_;
+  bool separate_;
+  int count_ = 0;
+  int64_t bytes_ = 0;
+  Output outputs_[5];
+};
+
 template <typename T>
 T* ptr(const at::Tensor& t) {
   return static_cast<T*>(t.data_ptr());
@@ -231,7 +296,7 @@ PyObject* route_backward(PyObject* const* p) {
   return wrap(std::move(out));
 }
 
-// experts, num_experts, align
+// experts, num_experts, align, separate
 PyObject* plan_dispatch(PyObject* const* p) {
   const at::Tensor& experts = tensor(p[0], "experts");
   const int64_t num = whole(p[1]), align = whole(p[2]);
@@ -253,16 +318,18 @@ PyObject* plan_dispatch(PyObject* const* p) {
     return cusort_plan_dispatch(nullptr, &bytes, wide ? 8 : 4, nullptr, pairs, (int)num, (int)align, capacity, nullptr,
                                 nullptr, nullptr, nullptr, s);
   });
-  at::Tensor counts = empty({num}, at::kInt, device), offsets = empty({num + 1}, at::kInt, device);
-  at::Tensor sources = empty({capacity}, at::kInt, device), positions = empty(experts.sizes(), at::kInt, device);
+  Outputs out(device, truth(p[3]));
+  const int counts = out.add({num}, at::kInt), offsets = out.add({num + 1}, at::kInt);
+  const int sources = out.add({capacity}, at::kInt), positions = out.add(experts.sizes(), at::kInt);
+  out.allocate();
   // one byte is asked for where nothing is needed: any address does
-  const at::Tensor temp = bytes > 1 ? empty({(int64_t)bytes}, at::kByte, device) : counts;
+  const at::Tensor temp = bytes > 1 ? empty({(int64_t)bytes}, at::kByte, device) : at::Tensor();
   launch("cusort_plan_dispatch", device, [&](cudaStream_t s) {
-    return cusort_plan_dispatch(temp.data_ptr(), &bytes, wide ? 8 : 4, experts.data_ptr(), pairs, (int)num, (int)align,
-                                capacity, ptr<int32_t>(counts), ptr<int32_t>(offsets), ptr<int32_t>(sources),
-                                ptr<int32_t>(positions), s);
+    return cusort_plan_dispatch(bytes > 1 ? temp.data_ptr() : out.ptr<void>(counts), &bytes, wide ? 8 : 4,
+                                experts.data_ptr(), pairs, (int)num, (int)align, capacity, out.ptr<int32_t>(counts),
+                                out.ptr<int32_t>(offsets), out.ptr<int32_t>(sources), out.ptr<int32_t>(positions), s);
   });
-  return tuple(wrap(std::move(counts)), wrap(std::move(offsets)), wrap(std::move(sources)), wrap(std::move(positions)));
+  return out.tuple();
 }
 
 // A plan's positions [tokens, k], and its sources where they are given.
@@ -338,7 +405,7 @@ PyObject* combine_backward(PyObject* const* p) {
   return tuple(wrap(std::move(grad_rows)), wrap(std::move(grad_weights)));
 }
 
-// cached_lens, new_lens, block_tables, block_size, num_tokens, free_blocks, num_free
+// cached_lens, new_lens, block_tables, block_size, num_tokens, free_blocks, num_free, separate
 PyObject* page_plan(PyObject* const* p) {
   const at::Tensor &cached = tensor(p[0], "cached_lens"), &fresh = tensor(p[1], "new_lens"),
                    &tables = tensor(p[2], "block_tables");
@@ -371,21 +438,19 @@ PyObject* page_plan(PyObject* const* p) {
     check(*num_free, "num_free", at::kInt, device, {1});
   }
   check_cuda(cached, "cached_lens");
-  at::Tensor slots = empty({tokens}, at::kLong, device), positions = empty({tokens}, at::kInt, device);
-  at::Tensor starts = empty({requests + 1}, at::kInt, device), served = empty({requests}, at::kBool, device), left;
-  if (num_free != nullptr) left = empty({1}, at::kInt, device);
+  Outputs out(device, truth(p[7]));
+  const int slots = out.add({tokens}, at::kLong), positions = out.add({tokens}, at::kInt);
+  const int starts = out.add({requests + 1}, at::kInt), served = out.add({requests}, at::kBool);
+  const int left = num_free == nullptr ? -1 : out.add({1}, at::kInt);
+  out.allocate();
   launch("cusort_page_plan", device, [&](cudaStream_t s) {
     return cusort_page_plan(ptr<int32_t>(cached), ptr<int32_t>(fresh), (int)requests, (int)block, ptr<int32_t>(tables),
                             std::max(tables.stride(0), width), (int)width, ptr<int32_t>(blocks),
                             blocks == nullptr ? 0 : (int)blocks->numel(), ptr<int32_t>(num_free), tokens,
-                            ptr<int64_t>(slots), ptr<int32_t>(positions), ptr<int32_t>(starts),
-                            ptr<uint8_t>(served), num_free == nullptr ? nullptr : ptr<int32_t>(left), s);
+                            out.ptr<int64_t>(slots), out.ptr<int32_t>(positions), out.ptr<int32_t>(starts),
+                            out.ptr<uint8_t>(served), left < 0 ? nullptr : out.ptr<int32_t>(left), s);
   });
-  PyObject* rest = Py_None;
-  if (num_free != nullptr) rest = wrap(std::move(left));
-  else Py_INCREF(rest);
-  return tuple(wrap(std::move(slots)), wrap(std::move(positions)), wrap(std::move(starts)), wrap(std::move(served)),
-               rest);
+  return out.tuple(left < 0);
 }
 
 // The boundary: no C++ exception leaves through it.
@@ -408,9 +473,9 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
 
 #define ENTRY(name, n) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<name, n>)), METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {ENTRY(route, 9),   ENTRY(route_backward, 7), ENTRY(plan_dispatch, 3),
+PyMethodDef kMethods[] = {ENTRY(route, 9),   ENTRY(route_backward, 7), ENTRY(plan_dispatch, 4),
                           ENTRY(dispatch, 3), ENTRY(combine, 5),       ENTRY(combine_backward, 5),
-                          ENTRY(page_plan, 7), {nullptr, nullptr, 0, nullptr}};
+                          ENTRY(page_plan, 8), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_cusort_torch", nullptr, -1, kMethods};
 

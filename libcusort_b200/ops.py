@@ -157,7 +157,7 @@ route.register_autograd(_route_grad, setup_context=_route_setup)
 @torch.library.custom_op("cusort::plan_dispatch", mutates_args=())
 def plan_dispatch(experts: torch.Tensor, num_experts: int,
                   align: int = 1) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return tuple(routing.plan_dispatch(experts, num_experts, align=align))
+    return tuple(routing.plan_dispatch(experts, num_experts, align=align, separate=True))
 
 
 @plan_dispatch.register_fake
@@ -245,7 +245,7 @@ def page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
               num_tokens: int, free_blocks: torch.Tensor, num_free: torch.Tensor
               ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     return tuple(paging.page_plan(cached_lens, new_lens, block_tables, block_size, num_tokens,
-                                  free_blocks=free_blocks, num_free=num_free))
+                                  free_blocks=free_blocks, num_free=num_free, separate=True))
 
 
 @page_plan.register_fake

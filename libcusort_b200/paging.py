@@ -27,7 +27,7 @@ class PagePlan(NamedTuple):
 
 def page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor, block_size: int,
               num_tokens: int, *, free_blocks: torch.Tensor | None = None,
-              num_free: torch.Tensor | None = None) -> PagePlan:
+              num_free: torch.Tensor | None = None, separate: bool = False) -> PagePlan:
     """Request r has ``cached_lens[r]`` tokens in the cache and brings ``new_lens[r]``; row r of
     ``block_tables`` (int32 [requests, width], written in place) names its blocks of ``block_size``
     tokens.  New blocks come from the end of ``free_blocks[:num_free]`` in the requests' order; a
@@ -35,6 +35,7 @@ def page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     slots are -1 and its table stays.  ``free_blocks`` and ``num_free`` are only read, so a step can
     be planned again; its caller goes on with the returned ``num_free``.  Without a free list the
     tables hold all blocks already.  ``num_tokens``: the length of the slot map, which may be more
-    or less than there are new tokens."""
+    or less than there are new tokens.  The plan's tensors are parts of one allocation, unless
+    ``separate``."""
     return PagePlan._make(_capi.native().page_plan(cached_lens, new_lens, block_tables, block_size, num_tokens,
-                                                   free_blocks, num_free))
+                                                   free_blocks, num_free, separate))

@@ -80,11 +80,13 @@ def dispatch_capacity(num_pairs: int, num_experts: int, align: int = 1) -> int:
     return num_pairs + min(num_experts, num_pairs) * (align - 1)
 
 
-def plan_dispatch(experts: torch.Tensor, num_experts: int, *, align: int = 1) -> DispatchPlan:
+def plan_dispatch(experts: torch.Tensor, num_experts: int, *, align: int = 1,
+                  separate: bool = False) -> DispatchPlan:
     """Groups (token, expert) pairs by expert, stably.  ``experts``: contiguous int32 or int64,
     [tokens, k] or of any shape; values outside [0, num_experts) (such as -1) are dropped.  Every
-    expert's segment starts at a multiple of ``align`` rows; rows between hold no pair."""
-    return DispatchPlan._make(_capi.native().plan_dispatch(experts, num_experts, align))
+    expert's segment starts at a multiple of ``align`` rows; rows between hold no pair.  The plan's
+    tensors are parts of one allocation, unless ``separate``."""
+    return DispatchPlan._make(_capi.native().plan_dispatch(experts, num_experts, align, separate))
 
 
 def dispatch(x: torch.Tensor, sources: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:

@@ -326,3 +326,23 @@ def test_same_inputs_same_bits():
         b = (routing.route(logits, 6)[0], routing.route_backward(g, logits, ids), routing.combine(y, w, plan.positions),
              *routing.combine_backward(gout, y, w, plan.sources, plan.positions))
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("separate", [False, True])
+def test_plan_tensors_do_not_overlap(separate):
+    for T, k, E, align in ((0, 2, 3, 1), (5, 3, 7, 4), (2000, 5, 33, 16)):
+        ids = torch.randint(0, E, (T, k), device="cuda", dtype=torch.int32)
+        plan = routing.plan_dispatch(ids, E, align=align, separate=separate)
+        expect = R.plan(ids.cpu().numpy(), E, align, plan.sources.numel())
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * 4) for t in plan if t.numel())
+        assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:]))
+        assert all(t.data_ptr() % 16 == 0 and t.is_contiguous() for t in plan)
+        assert len({t.untyped_storage().data_ptr() for t in plan if t.numel()}) == (len(spans) if separate else 1)
+        for t in plan:  # each can be written without the others' noticing
+            kept = [u.clone() for u in plan]
+            t.fill_(77)
+            for u, was in zip(plan, kept):
+                assert u is t or torch.equal(u, was)
+            t.copy_(kept[[u is t for u in plan].index(True)])
+        for got, ref in zip(plan, expect):
+            np.testing.assert_array_equal(got.cpu().numpy(), ref)
