@@ -69,7 +69,7 @@ __device__ __forceinline__ Request request_of(const PageArgs& a, int r) {
 
 // The last of starts[0 .. n) that is at most i (starts[0] is), found by the
 // whole warp.
-__device__ __forceinline__ int warp_search(const uint32_t* starts, int n, int64_t i, int lane) {
+__device__ __forceinline__ int warp_search(const uint32_t* starts, int n, uint32_t i, int lane) {
   int at = 0;
   while (n > 1) {
     const int step = (n + 31) >> 5, probe = lane * step;
@@ -142,6 +142,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
   if (threadIdx.x == 0) s_start[R] = sum_t, s_taken[R] = sum_b;
   __syncthreads();
   const uint32_t left = a.num_free == nullptr ? 0u : (uint32_t)min(max(*a.num_free, 0), a.num_blocks);
+  const uint32_t room = (uint32_t)a.num_tokens;  // below 2^31, and a step of the grid fits beside it
   for (int r = blockIdx.x * THREADS + threadIdx.x; r <= R; r += gridDim.x * THREADS) {
     a.starts[r] = (int32_t)s_start[r];
     const uint32_t taken = s_taken[r];
@@ -150,13 +151,20 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
       *a.num_free_out = (int32_t)(left - taken);
     if (r < R) {
       const Request q = request_of(a, r);
-      a.served[r] = q.fits && (q.need == 0 || s_taken[r + 1] <= left);
+      const bool served = q.fits && (q.need == 0 || s_taken[r + 1] <= left);
+      a.served[r] = served;
+      // blocks whose first token lies beyond the slot map, where no token's thread comes by
+      if (served && s_start[r + 1] > room) {
+        for (uint32_t n = 0; n < q.need; ++n)
+          if (s_start[r] + ((q.held + n) * a.block_size - q.cached) >= room)
+            a.tables[r * a.table_stride + q.held + n] = a.free_blocks[left - 1 - (taken + n)];
+      }
     }
   }
-  const int64_t total = s_start[R], most = max(total, a.num_tokens);
+  const uint32_t total = s_start[R];
   const uint32_t size = a.block_size;
-  for (int64_t w0 = ((int64_t)blockIdx.x * THREADS + warp * 32) * N; w0 < most; w0 += (int64_t)gridDim.x * THREADS * N) {
-    const int64_t i0 = w0 + lane * N;
+  for (uint32_t w0 = (blockIdx.x * THREADS + warp * 32) * N; w0 < room; w0 += gridDim.x * THREADS * N) {
+    const uint32_t i0 = w0 + lane * N;
     int64_t slot[N];
     int32_t position[N];
     // the last request that starts at or before i0: the warp's first one by all of its lanes, then each lane from
@@ -176,7 +184,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
     bool served = false, fetch = true;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int64_t i = i0 + n;
+      const uint32_t i = i0 + n;
       slot[n] = position[n] = -1;
       if (i >= total) continue;
       if (n == 0 || i >= next) {
@@ -184,7 +192,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
         const Request q = request_of(a, r);
         next = s_start[r + 1];
         taken = s_taken[r];
-        pos = min(q.cached + (uint32_t)(i - s_start[r]), kMost);
+        pos = min(q.cached + (i - s_start[r]), kMost);
         page = blocks_of(a, pos);
         in = pos - page * size;
         held = a.num_free != nullptr ? q.held : (uint32_t)a.table_width;
@@ -204,7 +212,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
       }
       if (id >= 0) slot[n] = (int64_t)id * size + in;
     }
-    if (N == 4 && i0 + N <= a.num_tokens) {
+    if (N == 4 && i0 + N <= room) {
       longlong2* out = reinterpret_cast<longlong2*>(a.slots + i0);
       out[0] = make_longlong2(slot[0], slot[1 % N]);
       out[1] = make_longlong2(slot[2 % N], slot[3 % N]);
@@ -213,7 +221,7 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
     } else {
 #pragma unroll
       for (int n = 0; n < N; ++n) {
-        if (i0 + n < a.num_tokens) {
+        if (i0 + n < room) {
           a.slots[i0 + n] = slot[n];
           a.positions[i0 + n] = position[n];
         }
