@@ -135,52 +135,56 @@ __device__ __forceinline__ void load_row(T (&x)[V], const T* row, int lane, int 
 // the lanes' own maxima is below no more than k - 1 keys in other lanes, so
 // the k largest are among the keys from it on, seldom more than a few beyond
 // k; these are gathered one to a lane, and the rounds are over one key each.
-// Instructions to a token at k = 8: 8 keys to a lane 400 -> 200, 4 about equal.
+// Measured (us, all keys -> gathered, k = 8, 32-bit logits unless said): 32768
+// tokens of 128 experts 20.2 -> 17.1 (at k = 4 12.6 -> 12.8, so not there);
+// 16-bit logits, whose rounds are shorter, 256 experts 14.1 -> 20.6 (not there).
 template <int V, bool UNIQUE>
 __device__ __forceinline__ void choose(uint32_t (&key)[V], int k, int lane, int base, uint2* scratch, uint32_t& mine,
                                        int& chosen) {
-  if constexpr (V >= (UNIQUE ? 16 : 8)) {
-    uint32_t m = key[0];
+  if constexpr (V >= (UNIQUE ? 16 : 4)) {
+    if (V > 4 || k > 4) {
+      uint32_t m = key[0];
 #pragma unroll
-    for (int i = 1; i < V; ++i) m = max(m, key[i]);
-    uint32_t low = 1;
-    for (int n = 0; n < k;) {
-      const uint32_t most = __reduce_max_sync(kAll, m);
-      if (most == 0) {
-        low = 1;
-        break;
+      for (int i = 1; i < V; ++i) m = max(m, key[i]);
+      uint32_t low = 1;
+      for (int n = 0; n < k;) {
+        const uint32_t most = __reduce_max_sync(kAll, m);
+        if (most == 0) {
+          low = 1;
+          break;
+        }
+        low = most;
+        n += __popc(__ballot_sync(kAll, m == most));
+        m = m == most ? 0u : m;
       }
-      low = most;
-      n += __popc(__ballot_sync(kAll, m == most));
-      m = m == most ? 0u : m;
-    }
-    uint32_t mask = 0;
+      uint32_t mask = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) mask |= (key[i] >= low ? 1u : 0u) << i;
-    const int count = __popc(mask);
-    const uint32_t b0 = __ballot_sync(kAll, count & 1), b1 = __ballot_sync(kAll, count & 2),
-                   b2 = __ballot_sync(kAll, count & 4), b3 = __ballot_sync(kAll, count & ~7);
-    const int total = __popc(b0) + 2 * __popc(b1) + 4 * __popc(b2);
-    if (b3 == 0 && total <= 32) {
-      const uint32_t below = dev::lanemask_lt();
-      int at = __popc(b0 & below) + 2 * __popc(b1 & below) + 4 * __popc(b2 & below);
+      for (int i = 0; i < V; ++i) mask |= (key[i] >= low ? 1u : 0u) << i;
+      const int count = __popc(mask);
+      const uint32_t b0 = __ballot_sync(kAll, count & 1), b1 = __ballot_sync(kAll, count & 2),
+                     b2 = __ballot_sync(kAll, count & 4), b3 = __ballot_sync(kAll, count & ~7);
+      const int total = __popc(b0) + 2 * __popc(b1) + 4 * __popc(b2);
+      if (b3 == 0 && total <= 32) {
+        const uint32_t below = dev::lanemask_lt();
+        int at = __popc(b0 & below) + 2 * __popc(b1 & below) + 4 * __popc(b2 & below);
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (mask >> i & 1u) scratch[at++] = make_uint2(key[i], lane * V + i);
-      __syncwarp();
-      uint2 c = lane < total ? scratch[lane] : make_uint2(0u, 0u);
-      __syncwarp();
-      int from = 0;
-      const int n = min(k, total);
-      for (int j = 0; j < n; ++j) {
-        const uint32_t most = __reduce_max_sync(kAll, c.x);
-        const int owner = __ffs(__ballot_sync(kAll, c.x == most)) - 1;
-        if (lane == owner) c.x = 0;
-        if (lane == base + j) mine = most, from = owner;
+        for (int i = 0; i < V; ++i)
+          if (mask >> i & 1u) scratch[at++] = make_uint2(key[i], lane * V + i);
+        __syncwarp();
+        uint2 c = lane < total ? scratch[lane] : make_uint2(0u, 0u);
+        __syncwarp();
+        int from = 0;
+        const int n = min(k, total);
+        for (int j = 0; j < n; ++j) {
+          const uint32_t most = __reduce_max_sync(kAll, c.x);
+          const int owner = __ffs(__ballot_sync(kAll, c.x == most)) - 1;
+          if (lane == owner) c.x = 0;
+          if (lane == base + j) mine = most, from = owner;
+        }
+        const int e = __shfl_sync(kAll, (int)c.y, from);
+        if (lane >= base && lane < base + n) chosen = e;
+        return;
       }
-      const int e = __shfl_sync(kAll, (int)c.y, from);
-      if (lane >= base && lane < base + n) chosen = e;
-      return;
     }
   }
   if constexpr (UNIQUE) {
@@ -314,9 +318,10 @@ __device__ __forceinline__ uint32_t kept_experts(const RouteArgs& a, const float
 // needs neither holds half the registers.
 // Seven CTAs to an SM instead of the four that the scored kernels would take
 // (8192 x 256 logits, us: softmax 9.5 -> 8.0, sigmoid, bias and groups 14.7 ->
-// 13.2, in spite of 48 bytes spilled; ten CTAs 14.8).
+// 13.2, in spite of 48 bytes spilled; ten CTAs 14.8), and four instead of two
+// from 257 experts on (8192 x 512, softmax: 20.6 -> 15.8).
 template <typename T, int V, bool SCORED, bool GROUPED>
-__global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 7 : 1) route_kernel(RouteArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 7 : V == 16 ? 4 : 1) route_kernel(RouteArgs a) {
   dev::wait_for_previous();
   __shared__ uint2 s_scratch[kWarps][32];
   const int lane = threadIdx.x & 31;
