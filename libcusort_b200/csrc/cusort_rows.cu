@@ -18,7 +18,7 @@ using namespace cusort_b200;
 
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
-constexpr int kBackwardThreads = 256;
+constexpr int kBackwardThreads = 128;  // 256: 187 us where it takes 181 (see combine_backward_kernel)
 constexpr int kMaxChosen = 32;
 constexpr int kEmptyRows = 8;           // rows that a warp looks at to clear those without a pair
 constexpr int64_t kBusyWarps = 148 * 16;
@@ -187,8 +187,8 @@ struct CombineBackwardArgs {
 // One warp per pair: its row's gradient, and its weight's as a dot product.
 // The pairs of a token lie side by side, so that its gradient comes from
 // memory once and from the caches k - 1 times.  The first warps clear the rows
-// that hold no pair.  Bound by memory: 8192 tokens, k = 8, rows of 8 KB 187 us
-// (93 % of the copy rate); 4099 tokens, k = 6, rows of 4 KB 40 us (86 %).
+// that hold no pair.  Bound by memory: 8192 tokens, k = 8, rows of 8 KB 181 us
+// (97 % of the copy rate); 4099 tokens, k = 6, rows of 4 KB 39 us (87 %).
 template <typename T, int N, int U>
 __global__ void __launch_bounds__(kBackwardThreads) combine_backward_kernel(CombineBackwardArgs a) {
   dev::wait_for_previous();
