@@ -134,10 +134,12 @@ __device__ __forceinline__ void load_row(T (&x)[V], const T* row, int lane, int 
 // Few experts to a lane: k rounds over all keys.  More: the k-th largest of
 // the lanes' own maxima is below no more than k - 1 keys in other lanes, so
 // the k largest are among the keys from it on, seldom more than a few beyond
-// k; these are gathered one to a lane, and the rounds are over one key each.
-// Measured (us, all keys -> gathered, k = 8, 32-bit logits unless said): 32768
-// tokens of 128 experts 20.2 -> 17.1 (at k = 4 12.6 -> 12.8, so not there);
-// 16-bit logits, whose rounds are shorter, 256 experts 14.1 -> 20.6 (not there).
+// k; these are gathered one to a lane and take the place that the number of
+// those before them says.  Counting takes more exchanges than rounds would,
+// but none waits for another (8192 x 256 f32, k = 8: 7.1 us in rounds, 6.4).
+// Measured (us, all keys -> gathered): 32768 tokens of 128 experts, 32-bit
+// logits, k = 8 20.2 -> 15.5, k = 4 12.6 -> 14.0 (not there); 16-bit logits,
+// whose rounds are shorter, 256 experts, k = 8 14.1 -> 18.6 (not there).
 template <int V, bool UNIQUE>
 __device__ __forceinline__ void choose(uint32_t (&key)[V], int k, int lane, int base, uint2* scratch, uint32_t& mine,
                                        int& chosen) {
@@ -146,17 +148,11 @@ __device__ __forceinline__ void choose(uint32_t (&key)[V], int k, int lane, int 
       uint32_t m = key[0];
 #pragma unroll
       for (int i = 1; i < V; ++i) m = max(m, key[i]);
-      uint32_t low = 1;
-      for (int n = 0; n < k;) {
-        const uint32_t most = __reduce_max_sync(kAll, m);
-        if (most == 0) {
-          low = 1;
-          break;
-        }
-        low = most;
-        n += __popc(__ballot_sync(kAll, m == most));
-        m = m == most ? 0u : m;
-      }
+      int above = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) above += __shfl_sync(kAll, m, i) > m;
+      // lanes whose maximum has fewer than k above it hold the k largest; the smallest of them
+      const uint32_t low = max(1u, __reduce_min_sync(kAll, above < k ? m : 0xffffffffu));
       uint32_t mask = 0;
 #pragma unroll
       for (int i = 0; i < V; ++i) mask |= (key[i] >= low ? 1u : 0u) << i;
@@ -173,16 +169,21 @@ __device__ __forceinline__ void choose(uint32_t (&key)[V], int k, int lane, int 
         __syncwarp();
         uint2 c = lane < total ? scratch[lane] : make_uint2(0u, 0u);
         __syncwarp();
-        int from = 0;
-        const int n = min(k, total);
-        for (int j = 0; j < n; ++j) {
-          const uint32_t most = __reduce_max_sync(kAll, c.x);
-          const int owner = __ffs(__ballot_sync(kAll, c.x == most)) - 1;
-          if (lane == owner) c.x = 0;
-          if (lane == base + j) mine = most, from = owner;
+        // a candidate's place is the number of those before it
+        int place = 0;
+#pragma unroll 4
+        for (int i = 0; i < total; ++i) {
+          const uint32_t other = __shfl_sync(kAll, c.x, i);
+          place += other > c.x || (other == c.x && i < lane);
         }
-        const int e = __shfl_sync(kAll, (int)c.y, from);
-        if (lane >= base && lane < base + n) chosen = e;
+        if (lane < total) scratch[place] = c;
+        __syncwarp();
+        if (lane >= base && lane - base < min(k, total)) {
+          c = scratch[lane - base];
+          mine = c.x;
+          chosen = (int)c.y;
+        }
+        __syncwarp();
         return;
       }
     }
@@ -315,7 +316,7 @@ __device__ __forceinline__ uint32_t kept_experts(const RouteArgs& a, const float
 //
 // Bound by instruction issue and, within a token, by the chain of its rounds
 // (ncu: 53-60 % of the issue slots, 6-8 % of the DRAM rate).  Measured: 8192 x
-// 256 f32, sigmoid with a bias, 4 of 8 groups, k = 8: 12.9 us; 32768 x 128
+// 256 f32, sigmoid with a bias, 4 of 8 groups, k = 8: 12.2 us; 32768 x 128
 // bf16, renormalised softmax, k = 4: 7.9 us (1.2 TB/s); 16 x 64: 2.0 us.
 //
 // SCORED: scores of all experts are needed (a softmax's sum, a bias, groups by
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 7 : V == 16 ? 4 : 1) rou
 //   sigmoid                 dl = ds s (1 - s), ds = scale g, or
 //                           (scale g - u) / S renormalised
 // Bound by latency (ncu: 46 % of the issue slots).  Measured, 32768 x 128 bf16,
-// k = 4: 4.4 us where only the chosen have a gradient (2.1 TB/s), 12.3 us where
+// k = 4: 4.0 us where only the chosen have a gradient (2.1 TB/s), 11.0 us where
 // all do.
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwardArgs a) {
@@ -479,6 +480,12 @@ __global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwa
   }
   const bool has = xc > neg_inf();
   if (!has) g = 0.f;
+
+  // Experts that route chose are distinct, so that no two lanes meet in a row; an atomic add (half a microsecond over
+  // 32768 tokens) is kept for callers' own.
+  bool twice = false;
+  for (int d = 1; d < a.k_lanes; ++d) twice |= __shfl_xor_sync(kAll, id, d) == id && has;
+  const bool distinct = !__any_sync(kAll, twice);
 
   const bool dense = a.softmax && !a.renormalize;
   float at = 0.f;  // the chosen experts' own part
@@ -525,11 +532,11 @@ __global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwa
         x[i] = x[i] > neg_inf() ? exp_below(x[i], top) : 0.f;
         total += x[i];
       }
-      total = warp_sum(total);
-      const float p = has && mine == n ? exp_below(xc, top) / total : 0.f;
-      const float used = warp_sum(g * p);
-      if (mine == n) at = a.scale * p * g;
-      const float each = total > 0.f ? -(a.scale * used) / total : 0.f;
+      const float e = has && mine == n ? exp_below(xc, top) : 0.f;
+      const float sum = warp_sum(total), used = warp_sum(g * e);
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      if (mine == n) at = a.scale * g * (e * inv);
+      const float each = -(a.scale * inv) * (used * inv);
 #pragma unroll
       for (int i = 0; i < V; ++i) x[i] *= each;
     } else {
@@ -539,7 +546,10 @@ __global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwa
 #pragma unroll
     for (int i = 0; i < V; ++i) buf[lane * V + i] = x[i];
     __syncwarp();
-    if (has && mine == n) atomicAdd(&buf[id], at);  // ids of one token are distinct: no two lanes meet
+    if (has && mine == n) {
+      if (distinct) buf[id] += at;
+      else atomicAdd(&buf[id], at);
+    }
     __syncwarp();
     constexpr int N = vector_length<T, V>();
     if (a.wide) {

@@ -346,3 +346,20 @@ def test_plan_tensors_do_not_overlap(separate):
             t.copy_(kept[[u is t for u in plan].index(True)])
         for got, ref in zip(plan, expect):
             np.testing.assert_array_equal(got.cpu().numpy(), ref)
+
+
+@pytest.mark.parametrize("score,renormalize", [("softmax", False), ("sigmoid", False)])
+def test_route_gradient_adds_up_repeated_experts(score, renormalize):
+    """Experts that a caller repeats within a token: their parts add up."""
+    rng = _rng("repeated", score)
+    logits, x = _logits(rng, 70, 24, "f32", masks=False)
+    ids = rng.integers(0, 24, (70, 6))
+    ids[:, 3] = ids[:, 0]
+    ids[::2, 4] = ids[::2, 0]
+    grad = rng.normal(size=(70, 6)).astype(np.float32)
+    g = routing.route_backward(_cuda(grad), logits, _cuda(ids.astype(np.int32)), score=score, renormalize=renormalize)
+    # the reference adds each pair's part by itself
+    ref = np.zeros((70, 24))
+    for j in range(6):
+        ref += R.route_backward(grad[:, j:j + 1], x, ids[:, j:j + 1], None, score, renormalize)
+    np.testing.assert_allclose(g.double().cpu().numpy(), ref, rtol=1e-5, atol=2e-6 * np.abs(grad).max())
