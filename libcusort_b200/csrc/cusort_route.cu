@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 7 : V == 16 ? 4 : 1) rou
 //   sigmoid                 dl = ds s (1 - s), ds = scale g, or
 //                           (scale g - u) / S renormalised
 // Bound by latency (ncu: 46 % of the issue slots).  Measured, 32768 x 128 bf16,
-// k = 4: 4.0 us where only the chosen have a gradient (2.1 TB/s), 11.0 us where
+// k = 4: 4.4 us where only the chosen have a gradient (1.9 TB/s), 11.7 us where
 // all do.
 template <typename T, int V>
 __global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwardArgs a) {
@@ -480,12 +480,6 @@ __global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwa
   }
   const bool has = xc > neg_inf();
   if (!has) g = 0.f;
-
-  // Experts that route chose are distinct, so that no two lanes meet in a row; an atomic add (half a microsecond over
-  // 32768 tokens) is kept for callers' own.
-  bool twice = false;
-  for (int d = 1; d < a.k_lanes; ++d) twice |= __shfl_xor_sync(kAll, id, d) == id && has;
-  const bool distinct = !__any_sync(kAll, twice);
 
   const bool dense = a.softmax && !a.renormalize;
   float at = 0.f;  // the chosen experts' own part
@@ -546,10 +540,7 @@ __global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwa
 #pragma unroll
     for (int i = 0; i < V; ++i) buf[lane * V + i] = x[i];
     __syncwarp();
-    if (has && mine == n) {
-      if (distinct) buf[id] += at;
-      else atomicAdd(&buf[id], at);
-    }
+    if (has && mine == n) atomicAdd(&buf[id], at);  // lanes meet only where a caller repeats an expert
     __syncwarp();
     constexpr int N = vector_length<T, V>();
     if (a.wide) {
