@@ -40,10 +40,17 @@ __device__ __forceinline__ void clear_empty_rows(V* rows, const int32_t* sources
   const int64_t r = r0 + lane;
   uint32_t empty = __ballot_sync(kAll, lane < kEmptyRows && r < capacity && sources[r < capacity ? r : 0] < 0);
   const V zero{};
+  constexpr int kPer16 = 16 / (int)sizeof(V);
   for (; empty; empty &= empty - 1) {
+    // whole 16-byte words between what lies before the first and after the last of them
     V* row = rows + (r0 + __ffs(empty) - 1) * vectors;
+    const int64_t before = (16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / sizeof(V), head = min(before, vectors);
+    const int64_t words = (vectors - head) / kPer16, rest = vectors - head - words * kPer16;
+    uint4* body = reinterpret_cast<uint4*>(row + head);
+    if (lane < head) row[lane] = zero;
 #pragma unroll 4
-    for (int64_t i = lane; i < vectors; i += 32) row[i] = zero;
+    for (int64_t i = lane; i < words; i += 32) body[i] = make_uint4(0, 0, 0, 0);
+    if (lane < rest) row[head + words * kPer16 + lane] = zero;
   }
 }
 
