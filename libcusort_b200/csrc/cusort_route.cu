@@ -448,6 +448,16 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 7 : V == 16 ? 4 : 1) rou
   }
 }
 
+// Where an expert's value lies in a warp's row in shared memory: the lanes'
+// 16-byte words side by side, so that none of them share a bank (as V values
+// a lane in a run, 32768 x 1024 gradients took 81 us).
+template <int V>
+__device__ __forceinline__ int place_of(int expert) {
+  if constexpr (V <= 4) return expert;
+  const int lane = expert / V, i = expert % V;
+  return (i / 4 * 32 + lane) * 4 + i % 4;
+}
+
 // A warp takes per_warp tokens: first the gradients at all their chosen
 // experts, k_lanes lanes to a token, then row after row, put together in
 // shared memory.  With w the weights, u = sum of g w, S the chosen scores' sum:
@@ -457,9 +467,10 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 7 : V == 16 ? 4 : 1) rou
 //                           (scale g - u) / S renormalised
 // Bound by latency (ncu: 46 % of the issue slots).  Measured, 32768 x 128 bf16,
 // k = 4: 4.4 us where only the chosen have a gradient (1.9 TB/s), 11.7 us where
-// all do.
+// all do.  Many experts: as many CTAs to an SM as keep all values in registers
+// (32768 x 512 bf16, k = 8: 18.1 -> 12.4 and 38.5 -> 25.5 us).
 template <typename T, int V>
-__global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwardArgs a) {
+__global__ void __launch_bounds__(32 * kWarps, V <= 4 ? 1 : V == 8 ? 10 : V == 16 ? 8 : 4) route_backward_kernel(RouteBackwardArgs a) {
   dev::wait_for_previous();
   __shared__ alignas(16) float s_row[kWarps][32 * V];
   const int lane = threadIdx.x & 31;
@@ -538,9 +549,9 @@ __global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwa
       for (int i = 0; i < V; ++i) x[i] = 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) buf[lane * V + i] = x[i];
+    for (int i = 0; i < V; ++i) buf[place_of<V>(lane * V + i)] = x[i];
     __syncwarp();
-    if (has && mine == n) atomicAdd(&buf[id], at);  // lanes meet only where a caller repeats an expert
+    if (has && mine == n) atomicAdd(&buf[place_of<V>(id)], at);  // lanes meet only where a caller repeats an expert
     __syncwarp();
     constexpr int N = vector_length<T, V>();
     if (a.wide) {
@@ -549,14 +560,14 @@ __global__ void __launch_bounds__(32 * kWarps) route_backward_kernel(RouteBackwa
         const int e = lane * V + c;
         dev::Pack<T, N> p;
 #pragma unroll
-        for (int i = 0; i < N; ++i) p.v[i] = dev::from_float<T>(buf[e + i]);
+        for (int i = 0; i < N; ++i) p.v[i] = dev::from_float<T>(buf[place_of<V>(e + i)]);
         if (e < a.num_experts) *reinterpret_cast<dev::Pack<T, N>*>(out + e) = p;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int e = i * 32 + lane;
-        if (e < a.num_experts) out[e] = dev::from_float<T>(buf[e]);
+        if (e < a.num_experts) out[e] = dev::from_float<T>(buf[place_of<V>(e)]);
       }
     }
     __syncwarp();
