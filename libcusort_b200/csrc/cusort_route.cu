@@ -229,8 +229,8 @@ template <typename T, int V>
 __device__ __forceinline__ void narrow_keys(uint32_t (&key)[V], const T (&x)[V], int lane) {
   using T2 = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
   constexpr uint32_t kInf = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
-  constexpr uint32_t kLeast = (0x8000u - kInf) << 16;             // from the first above -inf
-  constexpr uint32_t kSpan = (2 * kInf - 1) << 16 | 0xffffu;  // to +inf
+  constexpr uint32_t kLeast = (0x8000u - kInf) << 16;           // from the first above -inf
+  constexpr uint32_t kSpan = (2 * kInf) << 16 | 0xffffu;        // to +inf itself; NaN lies beyond, on either side
 #pragma unroll
   for (int i = 0; i < V; i += 2) {
     T2 pair;

@@ -363,3 +363,32 @@ def test_route_gradient_adds_up_repeated_experts(score, renormalize):
     for j in range(6):
         ref += R.route_backward(grad[:, j:j + 1], x, ids[:, j:j + 1], None, score, renormalize)
     np.testing.assert_allclose(g.double().cpu().numpy(), ref, rtol=1e-5, atol=2e-6 * np.abs(grad).max())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("score,renormalize", [("softmax", False), ("softmax", True), ("sigmoid", False),
+                                               ("sigmoid", True)])
+@pytest.mark.parametrize("shape", [(40, 8, 3, 1, 1), (40, 60, 4, 1, 1), (40, 64, 6, 8, 3), (40, 128, 4, 1, 1),
+                                   (40, 256, 8, 8, 4), (40, 512, 8, 1, 1), (40, 1000, 5, 4, 2), (7105, 64, 4, 1, 1)],
+                         ids=str)
+def test_route_infinite_logits_of_all_types(shape, score, renormalize, dtype):
+    """Positive infinity is the best logit there is, for any type (f16 logits reach it from 65520 on)."""
+    T, E, k, groups, kept = shape
+    rng = _rng("infinite", shape, score, renormalize, dtype)
+    x = rng.normal(size=(T, E))
+    x[rng.random((T, E)) < 1.5 / E] = np.inf
+    x[rng.random((T, E)) < 0.1] = -np.inf
+    x[rng.random((T, E)) < 0.1] = np.nan
+    x[rng.random((T, E)) < 0.1] = torch.finfo(TYPES[dtype]).max
+    logits = _cuda(x).to(TYPES[dtype])
+    x = logits.double().cpu().numpy()
+    how = dict(score=score, groups=groups, groups_kept=kept, renormalize=renormalize)
+    w, ids = routing.route(logits, k, **how)
+    rw, rids, _ = R.route(x, k, **how)  # logits alone decide: no rounding takes part
+    np.testing.assert_array_equal(ids.cpu().numpy(), rids)
+    np.testing.assert_allclose(w.cpu().numpy(), rw, rtol=1e-5, atol=1e-37)
+    grad = rng.normal(size=(T, k)).astype(np.float32)
+    g = routing.route_backward(_cuda(grad), logits, ids, score=score, renormalize=renormalize)
+    rg = R.route_backward(grad, x, rids, None, score, renormalize)
+    np.testing.assert_allclose(g.double().cpu().numpy(), rg, rtol=RTOL[dtype] * 4,
+                               atol=max(ATOL[dtype], 2e-6 * np.abs(grad).max()))
