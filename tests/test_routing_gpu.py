@@ -392,3 +392,18 @@ def test_route_infinite_logits_of_all_types(shape, score, renormalize, dtype):
     rg = R.route_backward(grad, x, rids, None, score, renormalize)
     np.testing.assert_allclose(g.double().cpu().numpy(), rg, rtol=RTOL[dtype] * 4,
                                atol=max(ATOL[dtype], 2e-6 * np.abs(grad).max()))
+
+
+def test_route_gradient_of_tiny_scores():
+    """Renormalised sigmoids that are subnormal in 32 bits: their quotient by their sum is an ordinary number, and so is
+    the gradient, w (1 - s) (g - u).  The scores are multiples of 2^-149 above 3e-39, off by 3e-7 of themselves and by
+    expf's 2 units, 2.4e-7; their quotients and differences of those, g = +-20, add up to less than 3e-6 of 20."""
+    x = np.array([[-88.5, -88.5], [-88.0, -88.25], [-87.5, -88.5], [-88.6, -30.0]], np.float32)
+    grad = np.array([[20, -20]] * 4, np.float32)
+    w, ids = routing.route(_cuda(x), 2, score="sigmoid", renormalize=True)
+    rw, rids, _ = R.route(x, 2, score="sigmoid", renormalize=True)
+    np.testing.assert_array_equal(ids.cpu().numpy(), rids)
+    np.testing.assert_allclose(w.cpu().numpy(), rw, rtol=3e-6, atol=1e-37)
+    g = routing.route_backward(_cuda(grad), _cuda(x), ids, score="sigmoid", renormalize=True)
+    rg = R.route_backward(grad, x, rids, None, "sigmoid", True)
+    np.testing.assert_allclose(g.cpu().numpy(), rg, rtol=3e-6, atol=20 * 3e-6)
