@@ -236,10 +236,11 @@ __global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
 
 template <int THREADS, int N>
 cudaError_t run(const PageArgs& a, cudaStream_t stream) {
-  const size_t smem = sizeof(uint32_t) * 2 * (a.num_requests + 1);
+  const size_t smem = sizeof(uint32_t) * 2 * (a.num_requests + 1), most = sizeof(uint32_t) * 2 * (kMaxRequests + 1);
   if (smem > 47 * 1024) {  // beside the sums
+    // the limit is the kernel's, not the call's: the same one from every host thread
     const cudaError_t e = cudaFuncSetAttribute(page_plan_kernel<THREADS, N>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     if (e) return e;
   }
   const int64_t per_cta = THREADS * N;

@@ -121,3 +121,36 @@ def test_planned_again():
     was = t.clone()
     b = paging.page_plan(_cuda(cached), _cuda(new), t, 16, int(new.sum()), free_blocks=f, num_free=n)
     assert torch.equal(t, was) and all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+def test_c_abi_from_two_threads():
+    """Steps of different numbers of requests, planned from two host threads at once: the C ABI is called without the
+    interpreter's lock.  Each thread has tensors and a stream of its own."""
+    import threading
+
+    from libcusort_b200 import _capi
+    lib = _capi.load()
+    refused = []
+
+    def plan(requests, stream):
+        with torch.cuda.stream(stream):
+            lens, new = torch.zeros(requests, dtype=torch.int32, device="cuda"), _cuda(np.ones(requests))
+            tables, free = torch.zeros(requests, 1, dtype=torch.int32, device="cuda"), _cuda(np.arange(requests))
+            left, rest = _cuda([requests]), _cuda([0])
+            slots = torch.zeros(requests, dtype=torch.int64, device="cuda")
+            positions, starts = torch.zeros_like(lens), torch.zeros(requests + 1, dtype=torch.int32, device="cuda")
+            served = torch.zeros(requests, dtype=torch.uint8, device="cuda")
+            stream.synchronize()
+            args = (lens.data_ptr(), new.data_ptr(), requests, 16, tables.data_ptr(), 1, 1, free.data_ptr(), requests,
+                    left.data_ptr(), requests, slots.data_ptr(), positions.data_ptr(), starts.data_ptr(),
+                    served.data_ptr(), rest.data_ptr(), stream.cuda_stream)
+            refused.extend(rc for rc in (lib.cusort_page_plan(*args) for _ in range(4000)) if rc != 0)
+            stream.synchronize()
+            assert bool(served.all()) and int(rest) == 0 and int(starts[-1]) == requests
+
+    threads = [threading.Thread(target=plan, args=(n, torch.cuda.Stream())) for n in (16384, 7000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not refused, f"{len(refused)} calls refused, with {set(refused)}"
