@@ -365,7 +365,8 @@ cudaError_t cusort_combine_rows_backward(cusort_float_type type, const void* d_g
  *     order, and written into its table.  A request is served if its blocks
  *     fit its table and there were free ones for it and all before it;
  *     d_served[r] says so.  One that is not keeps its table.
- *     *d_num_free_out: the free blocks that are left.
+ *     *d_num_free_out: the free blocks that are left (not d_num_free itself,
+ *     which is read while it is written: refused).
  *   - d_free_blocks and d_num_free NULL: the tables hold all blocks already.
  *   - d_starts[r]: the first new token of request r; d_starts[num_requests]:
  *     their number.  Token i < num_tokens: its position in its request and its

@@ -266,6 +266,8 @@ extern "C" cudaError_t cusort_page_plan(const int32_t* d_cached_lens, const int3
                             (table_width > 0 && d_block_tables == nullptr))) ||
       (num_tokens > 0 && (d_slots == nullptr || d_positions == nullptr)))
     return cudaErrorInvalidValue;
+  // every CTA reads the count, whenever it comes to run, and one writes what is left
+  if (d_num_free != nullptr && d_num_free == d_num_free_out) return cudaErrorInvalidValue;
   const bool whole =
       ((reinterpret_cast<uintptr_t>(d_cached_lens) | reinterpret_cast<uintptr_t>(d_new_lens)) & 15) == 0;
   const unsigned long long inverse = block_size == 1 ? 0 : ~0ull / block_size + 1;

@@ -183,3 +183,11 @@ def test_page_arguments():
                 dict(blocks=(1 << 30) + 1), dict(left=None), dict(tokens=-1), dict(tokens=1 << 31), dict(slots=None),
                 dict(positions=None), dict(starts=None), dict(served=None), dict(rest=None)):
         assert call(**bad) == INVALID, bad
+
+
+def test_page_plan_counts_apart():
+    """The count of free blocks may not be updated in place: it is read by every CTA, and written by one."""
+    lens, starts = C.c_void_p(0x20000), C.c_void_p(0x30000)
+    rc = _capi.load().cusort_page_plan(lens, lens, 4, 16, P, 8, 8, P, 32, C.c_void_p(0x40000), 9, P, P, starts, P,
+                                       C.c_void_p(0x40000), None)
+    assert rc == INVALID
