@@ -49,7 +49,11 @@ template <typename... A>
 
 const at::Tensor& tensor(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) refuse(PyExc_TypeError, name, " must be a tensor");
-  return THPVariable_Unpack(o);
+  const at::Tensor& t = THPVariable_Unpack(o);
+  // memory that does not hold the values: the kernels would read it as it is
+  if (t.is_conj() || t.is_neg() || t._is_zerotensor())
+    refuse(PyExc_ValueError, name, " must not be a lazy view (call resolve_conj() or resolve_neg(), or clone it, first)");
+  return t;
 }
 
 const at::Tensor* maybe(PyObject* o, const char* name) { return o == Py_None ? nullptr : &tensor(o, name); }

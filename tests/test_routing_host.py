@@ -191,3 +191,19 @@ def test_page_plan_counts_apart():
     rc = _capi.load().cusort_page_plan(lens, lens, 4, 16, P, 8, 8, P, 32, C.c_void_p(0x40000), 9, P, P, starts, P,
                                        C.c_void_p(0x40000), None)
     assert rc == INVALID
+
+
+@pytest.mark.parametrize("call", [
+    lambda: routing.dispatch(_t(4, 16, dtype=torch.complex64).conj(), _i(8), _i(4, 2)),
+    lambda: routing.dispatch(torch._neg_view(_t(4, 16)), _i(8), _i(4, 2)),
+    lambda: routing.route(torch._neg_view(_t(4, 8)), 2),
+    lambda: routing.route(_t(4, 8), 2, bias=torch._neg_view(_t(8))),
+    lambda: routing.combine(torch._neg_view(_t(8, 16)), _t(4, 2), _i(4, 2)),
+    lambda: routing.combine(_t(8, 16), torch._neg_view(_t(4, 2)), _i(4, 2)),
+    lambda: routing.combine(_t(8, 16), torch._efficientzerotensor((4, 2), device=M), _i(4, 2)),
+    lambda: paging.page_plan(torch._neg_view(_i(3)), _i(3), _i(3, 4), 16, 9),
+])
+def test_lazy_views_are_refused(call):
+    """Tensors whose memory does not hold their values yet."""
+    with pytest.raises(ValueError, match="resolve"):
+        call()
