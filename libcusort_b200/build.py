@@ -3,19 +3,21 @@
 Every .cu under csrc/ is compiled for sm_100a only
 (-gencode arch=compute_100a,code=sm_100a) in parallel, then linked into one
 shared library with the CUDA runtime linked statically and NCCL dynamically.
-Where PyTorch is installed, csrc/torch_binding.cpp is compiled beside it
+Where a PyTorch with CUDA is installed, csrc/torch_binding.cpp is compiled beside it
 (libcusort_b200/_lib/_cusort_torch.so): the native half of the routing and
 placement operators' Python functions, over the same C ABI.
 Run as ``python -m libcusort_b200.build`` or through ``__graft_entry__.build()``.
 
 Environment CUSORT_NVCC_DEFINES adds preprocessor definitions to every
 compile (e.g. ``-DCUSORT_LOOKBACK_TIMER=1`` for the lookback-timer build that
-``bench.py --lookback-stall`` reads); the definitions of the last build are
-kept beside the library, so a change of them forces a rebuild.
+``bench.py --lookback-stall`` reads); the definitions of the last build
+and the version of PyTorch are kept beside the library, so a change of them
+forces a rebuild.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.metadata
 import importlib.util
 import os
 import shutil
@@ -77,11 +79,24 @@ def torch_dir() -> Path | None:
     return Path(list(spec.submodule_search_locations)[0]) if spec else None
 
 
-def _build_binding() -> None:
+def torch_version() -> str:
+    try:
+        return importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError:
+        return ""
+
+
+def binding_possible() -> bool:
+    """Whether a PyTorch with CUDA is there to build the binding against."""
     t = torch_dir()
-    if t is None:
-        print("PyTorch is not installed: the PyTorch binding is not built", file=sys.stderr)
+    return t is not None and (t / "lib" / "libc10_cuda.so").exists()
+
+
+def _build_binding() -> None:
+    if not binding_possible():
+        print("no PyTorch with CUDA is installed: the PyTorch binding is not built", file=sys.stderr)
         return
+    t = torch_dir()
     cuda = Path(nvcc()).resolve().parents[1]
     tmp = BINDING.with_suffix(".so.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-sign-compare",
@@ -100,12 +115,18 @@ def sources() -> list[Path]:
     return sorted(CSRC.glob("*.cu"))
 
 
+def stamp() -> str:
+    """What else than the sources a build depends on."""
+    return "\n".join([" ".join(extra_defines()), "torch " + torch_version() if binding_possible() else "no binding"])
+
+
 def up_to_date() -> bool:
-    if not LIB.exists() or (torch_dir() is not None and not BINDING.exists()):
-        return False
-    if (STAMP.read_text() if STAMP.exists() else "") != " ".join(extra_defines()):
+    if not LIB.exists() or (STAMP.read_text() if STAMP.exists() else "") != stamp():
         return False
     t = LIB.stat().st_mtime
+    # the binding is compiled after the library is linked: an older one is left over from before a failure
+    if binding_possible() and not (BINDING.exists() and BINDING.stat().st_mtime >= t):
+        return False
     deps = list(CSRC.glob("*")) + [PKG.parent / "include" / "cusort_b200.h", Path(__file__)]
     return all(p.stat().st_mtime <= t for p in deps if p.exists())
 
@@ -130,7 +151,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         raise RuntimeError(f"link failed:\n{r.stderr}")
     os.replace(tmp, LIB)
     _build_binding()
-    STAMP.write_text(" ".join(extra_defines()))
+    STAMP.write_text(stamp())
     if verbose:
         print("".join(logs))
     return LIB
