@@ -20,9 +20,6 @@ KEY_TYPES = {
 }
 KEY_BYTES = {"u8": 1, "i8": 1, "u16": 2, "i16": 2, "u32": 4, "i32": 4, "u64": 8, "i64": 8, "f32": 4, "f64": 8}
 
-# cusort_float_type
-FLOAT_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
-
 CUDA_SUCCESS = 0
 CUDA_ERROR_INVALID_VALUE = 1
 CUDA_ERROR_TIMEOUT = 909  # cudaErrorTimeout
