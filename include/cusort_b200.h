@@ -303,6 +303,8 @@ typedef enum cusort_group_score { CUSORT_GROUP_MAX = 0, CUSORT_GROUP_TOP2 = 1 } 
  *   - d_experts[t*k+j], d_weights[t*k+j]: the j-th best expert and its score
  *     (divided by the sum of the chosen ones' with `renormalize`) times scale.
  *     Where fewer than k are available, expert -1 and weight 0 follow.
+ *     Sigmoids are taken in 32 bits: they are 0 for logits below about -88.7,
+ *     and where all chosen ones are, so are the renormalised weights.
  * num_experts <= 1024, k <= 32, groups <= 32. */
 cudaError_t cusort_route(cusort_float_type type, const void* d_logits, int64_t row_stride, const float* d_bias,
                          float* d_weights, int32_t* d_experts, int64_t num_tokens, int num_experts, int k,
@@ -311,7 +313,8 @@ cudaError_t cusort_route(cusort_float_type type, const void* d_logits, int64_t r
 
 /* Gradient of the logits (num_tokens rows of num_experts, contiguous, of the
  * logits' type) from the weights' gradient, with the experts that cusort_route
- * chose.  The choice itself has no gradient, nor has the bias. */
+ * chose.  The choice itself has no gradient, nor has the bias.  Experts that a
+ * caller repeats in a token add their parts up, in no fixed order. */
 cudaError_t cusort_route_backward(cusort_float_type type, const float* d_grad_weights, const void* d_logits,
                                   int64_t row_stride, const float* d_bias, const int32_t* d_experts,
                                   void* d_grad_logits, int64_t num_tokens, int num_experts, int k,

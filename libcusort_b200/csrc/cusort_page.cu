@@ -86,9 +86,9 @@ __device__ __forceinline__ int warp_search(const uint32_t* starts, int n, uint32
 // step, straight from the free list, so that no CTA waits for another's table
 // entries.  A block's first token writes its entry.
 //
-// Bound by latency where there are few tokens (256 requests of one: 3.2 us),
+// Bound by latency where there are few tokens (256 requests of one: 3.3 us),
 // by instruction issue where there are many (1.05M tokens of 4096 requests:
-// 10.3 us; 3.5 us of it are the launch and the scan; 51 % of the issue slots).
+// 10.6 us; 3.5 us of it are the launch and the scan; 51 % of the issue slots).
 template <int THREADS, int N>
 __global__ void __launch_bounds__(THREADS) page_plan_kernel(PageArgs a) {
   constexpr int W = THREADS / 32;

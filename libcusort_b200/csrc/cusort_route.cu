@@ -315,17 +315,21 @@ __device__ __forceinline__ uint32_t kept_experts(const RouteArgs& a, const float
 // weights are computed for all tokens at once.
 //
 // Bound by instruction issue and, within a token, by the chain of its rounds
-// (ncu: 53-60 % of the issue slots, 6-8 % of the DRAM rate).  Measured: 8192 x
-// 256 f32, sigmoid with a bias, 4 of 8 groups, k = 8: 12.2 us; 32768 x 128
-// bf16, renormalised softmax, k = 4: 7.9 us (1.2 TB/s); 16 x 64: 2.0 us.
+// (ncu: 54-61 % of the issue slots, 34-37 % of the warps, 6-8 % of the DRAM
+// rate).  Measured: 8192 x 256 f32, sigmoid with a bias, 4 of 8 groups, k = 8:
+// 12.2 us; 32768 x 128 bf16, renormalised softmax, k = 4: 7.8 us (1.2 TB/s);
+// 16 x 64: 2.0 us.
 //
 // SCORED: scores of all experts are needed (a softmax's sum, a bias, groups by
 // their scores); GROUPED: groups_kept < groups.  A kernel of its own for what
 // needs neither holds half the registers.
 // Seven CTAs to an SM instead of the four that the scored kernels would take
-// (8192 x 256 logits, us: softmax 9.5 -> 8.0, sigmoid, bias and groups 14.7 ->
-// 13.2, in spite of 48 bytes spilled; ten CTAs 14.8), and four instead of two
-// from 257 experts on (8192 x 512, softmax: 20.6 -> 15.8).
+// (8192 x 256 f32 logits, us: softmax 9.5 -> 8.0, sigmoid, bias and groups 14.7
+// -> 13.2, in spite of 44 bytes spilled; ten CTAs 14.8), and four instead of two
+// from 257 experts on (8192 x 512, softmax: 20.6 -> 15.8).  Measured for 32-bit
+// logits.  Of 8 and 16 experts to a lane the scored kernels of all types spill,
+// up to 36 bytes, with groups 36 to 92; those of 32 with groups, at the 255
+// registers that there are, 32 to 92.
 template <typename T, int V, bool SCORED, bool GROUPED>
 __global__ void __launch_bounds__(32 * kWarps, V <= 8 ? 7 : V == 16 ? 4 : 1) route_kernel(RouteArgs a) {
   dev::wait_for_previous();
@@ -465,8 +469,8 @@ __device__ __forceinline__ int place_of(int expert) {
 //   softmax                 dl = scale p g at the chosen, - p u everywhere
 //   sigmoid                 dl = scale g s (1 - s), or
 //                           (scale g - u) (s / S) (1 - s) renormalised
-// Bound by latency (ncu: 46 % of the issue slots).  Measured, 32768 x 128 bf16,
-// k = 4: 4.4 us where only the chosen have a gradient (1.9 TB/s), 11.7 us where
+// Bound by latency (ncu: 45 % of the issue slots).  Measured, 32768 x 128 bf16,
+// k = 4: 4.2 us where only the chosen have a gradient (2.0 TB/s), 11.4 us where
 // all do.  Many experts: as many CTAs to an SM as keep all values in registers
 // (32768 x 512 bf16, k = 8: 18.1 -> 12.4 and 38.5 -> 25.5 us).
 template <typename T, int V>
@@ -553,7 +557,7 @@ __global__ void __launch_bounds__(32 * kWarps, V <= 4 ? 1 : V == 8 ? 10 : V == 1
 #pragma unroll
     for (int i = 0; i < V; ++i) buf[place_of<V>(lane * V + i)] = x[i];
     __syncwarp();
-    if (has && mine == n) atomicAdd(&buf[place_of<V>(id)], at);  // lanes meet only where a caller repeats an expert
+    if (has && mine == n) atomicAdd(&buf[place_of<V>(id)], at);  // lanes meet, in any order, only where a caller repeats an expert
     __syncwarp();
     constexpr int N = vector_length<T, V>();
     if (a.wide) {

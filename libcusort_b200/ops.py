@@ -28,8 +28,8 @@ others are gathered by the sorted permutation).  The segmented operators sort ev
 outside every segment keep their input.
 
 The routing operators are those of ``libcusort_b200.routing`` (its docstrings have the details), with
-gradients through autograd: ``route`` to the logits, ``dispatch`` to the rows, ``combine`` to the rows, the
-weights and the residual.  ``page_plan`` is that of ``libcusort_b200.paging`` with a free list.
+gradients through autograd: ``route`` to the logits, ``dispatch`` to the rows (float32, float16 or bfloat16
+ones), ``combine`` to the rows, the weights and the residual.  ``page_plan`` is that of ``libcusort_b200.paging`` with a free list.
 
 All of them are stable, allocate fresh outputs (the inputs are never written, except ``page_plan``'s block tables), run on torch's current
 CUDA stream through the C ABI (``cusort_sort_keys``, ``cusort_sort_pairs``, ``cusort_route`` and so on) and have

@@ -35,7 +35,8 @@ def page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     slots are -1 and its table stays.  ``free_blocks`` and ``num_free`` are only read, so a step can
     be planned again; its caller goes on with the returned ``num_free``.  Without a free list the
     tables hold all blocks already.  ``num_tokens``: the length of the slot map, which may be more
-    or less than there are new tokens.  The plan's tensors are parts of one allocation, unless
+    or less than there are new tokens; blocks that begin beyond it are written one after the other,
+    so a map that leaves out most of a long prompt makes the call slow.  The plan's tensors are parts of one allocation, unless
     ``separate``."""
     return PagePlan._make(_capi.native().page_plan(cached_lens, new_lens, block_tables, block_size, num_tokens,
                                                    free_blocks, num_free, separate))

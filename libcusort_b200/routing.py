@@ -7,7 +7,8 @@ token goes to, its rows grouped by expert, and back.
 experts' rows up again.  Each has its gradient as a function of its own
 (``route_backward``, ``dispatch_backward``, ``combine_backward``);
 ``torch.ops.cusort.route / dispatch / combine`` (``libcusort_b200.ops``) tie
-them to autograd.
+them to autograd; the functions here take tensors that require a gradient and
+return ones that do not.
 
     weights, experts = route(logits, k, renormalize=True)
     plan = plan_dispatch(experts, num_experts)
@@ -70,7 +71,8 @@ def route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, experts: to
                    bias: torch.Tensor | None = None, score: str = "softmax", renormalize: bool = False,
                    scale: float = 1.0) -> torch.Tensor:
     """Gradient of ``route``'s logits (their type, contiguous) from that of its weights
-    (float32 [tokens, k]), with the experts it chose and the same arguments."""
+    (float32 [tokens, k]), with the experts it chose and the same arguments.  Where a caller repeats
+    an expert in a token, its parts are added up in no fixed order."""
     return _capi.native().route_backward(grad_weights, logits, experts, bias, _choice("score", score, _SCORES),
                                          renormalize, scale)
 
@@ -91,7 +93,8 @@ def plan_dispatch(experts: torch.Tensor, num_experts: int, *, align: int = 1,
 
 def dispatch(x: torch.Tensor, sources: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
     """rows[r] = x[sources[r] // k], zeros where sources[r] is -1: the tokens' rows ([tokens, hidden]
-    of any type, rows any distance apart) in the order of a plan."""
+    of any type, rows any distance apart) in the order of a plan.  Its gradient is there for
+    float32, float16 and bfloat16 rows."""
     return _capi.native().dispatch(x, sources, positions)
 
 
