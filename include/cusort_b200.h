@@ -359,6 +359,43 @@ cudaError_t cusort_combine_rows_backward(cusort_float_type type, const void* d_g
                                          int64_t num_tokens, int k, int64_t capacity, int64_t hidden,
                                          cudaStream_t stream);
 
+/* The experts' matrix products: for every row r of expert e's segment
+ * (d_offsets[e] <= r < d_offsets[e] + d_counts[e], as cusort_plan_dispatch
+ * gives them)
+ *   d_out[r] = d_rows[r] x weights[e],
+ * zeros for rows of no segment.  float16 or bfloat16 alone; sums in 32 bits,
+ * rounded once.  d_rows: `capacity` rows of `in` contiguous elements,
+ * row_stride elements apart; weights[e][i][o] at d_weights + e * expert_stride
+ * + i * in_stride + o * out_stride, one of the last two strides 1; d_out:
+ * capacity x out, contiguous, on a 16-byte boundary.  With weights and widths
+ * the other way round it is the gradient of the rows.
+ * Segments beyond the capacity are cut there; they must not overlap.
+ * 1 <= in, out <= 2^20, capacity < 2^31, num_experts <= 1024.
+ * Two-phase temp protocol, with the same arguments in both calls: operands
+ * whose addresses and strides are all multiples of 16 bytes need none, others
+ * are laid out anew there (at a 16-byte boundary). */
+cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp_storage_bytes, cusort_float_type type,
+                                   const void* d_rows, int64_t row_stride, const void* d_weights,
+                                   int64_t expert_stride, int64_t in_stride, int64_t out_stride,
+                                   const int32_t* d_counts, const int32_t* d_offsets, void* d_out, int64_t capacity,
+                                   int64_t in, int64_t out, int num_experts, cudaStream_t stream);
+
+/* Gradient of the weights: d_grad_weights[e] = sum over the rows r of e's
+ * segment of d_rows[r]^T x d_grad_out[r], zeros for experts without rows;
+ * contiguous [num_experts][in][out], or with in_contiguous
+ * [num_experts][out][in], on a 16-byte boundary.  The rest as above. */
+cudaError_t cusort_expert_products_grad_weights(void* d_temp_storage, size_t* temp_storage_bytes,
+                                                cusort_float_type type, const void* d_rows, int64_t row_stride,
+                                                const void* d_grad_out, int64_t grad_stride, const int32_t* d_counts,
+                                                const int32_t* d_offsets, void* d_grad_weights, int in_contiguous,
+                                                int64_t capacity, int64_t in, int64_t out, int num_experts,
+                                                cudaStream_t stream);
+
+/* Whether a wait inside one of these products ran out on the current device
+ * since the last call (cusort_set_wait_limit_ns): 0, or 1 and their results
+ * are not to be used.  Synchronises `stream`. */
+cudaError_t cusort_read_product_status(uint32_t* status, cudaStream_t stream);
+
 /* Placement of one serving step in a paged cache of blocks of block_size
  * tokens.  Request r has d_cached_lens[r] tokens there and brings
  * d_new_lens[r] (below 0: 0); row r of d_block_tables (table_width entries,

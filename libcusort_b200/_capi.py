@@ -69,6 +69,11 @@ SIGNATURES = {
     "cusort_dispatch_rows": (_i, [_vp, _i64, _sz, _vp, _vp, _vp, _i64, _i, _i64, _vp]),
     "cusort_combine_rows": (_i, [_i, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i, _i64, _i64, _vp]),
     "cusort_combine_rows_backward": (_i, [_i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i, _i64, _i64, _vp]),
+    "cusort_expert_products": (_i, [_vp, _P_SZ, _i, _vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _i64,
+                                    _i, _vp]),
+    "cusort_expert_products_grad_weights": (_i, [_vp, _P_SZ, _i, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i, _i64, _i64,
+                                                 _i64, _i, _vp]),
+    "cusort_read_product_status": (_i, [C.POINTER(_u32), _vp]),
     "cusort_page_plan": (_i, [_vp, _vp, _i, _i, _vp, _i64, _i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
     "cusort_version": (C.c_char_p, []),
     "cusort_set_launch_mode": (_i, [_i]),
@@ -110,7 +115,7 @@ def load() -> C.CDLL:
 
 
 def native():
-    """The native half of the PyTorch functions in routing.py and paging.py (raises if it has not been built)."""
+    """The native half of the PyTorch functions in routing.py, experts.py and paging.py (raises if it has not been built)."""
     global _native
     if _native is None:
         if not NATIVE_PATH.exists():

@@ -1,0 +1,755 @@
+// cusort_experts.cu -- the experts' matrix products: every row of a segment
+// times its expert's weights, and the gradient of the weights.  (The gradient
+// of the rows is the product with the weights' other order.)
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+
+#include "../../include/cusort_b200.h"
+#include "cusort_dispatch.h"
+#include "cusort_float.cuh"
+#include "cusort_overlap.cuh"
+#include "cusort_tensor.cuh"
+
+namespace cusort_b200 {
+
+cudaError_t encode_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                       const uint32_t* box) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<Encode> known{nullptr};
+  Encode encode = known.load();
+  if (encode == nullptr) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q);
+    if (e != cudaSuccess || q != cudaDriverEntryPointSuccess || f == nullptr)
+      return e != cudaSuccess ? e : cudaErrorNotSupported;
+    known = encode = reinterpret_cast<Encode>(f);
+  }
+  cuuint64_t d[3], s[2];
+  cuuint32_t b[3], one[3] = {1, 1, 1};
+  for (int i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i];
+  for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i];
+  // both types have 16 bits, and nothing but zeros outside depends on which it is
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d, s, b, one,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+}  // namespace cusort_b200
+
+namespace {
+
+using namespace cusort_b200;
+
+constexpr int kMaxExperts = 1024;
+constexpr int kThreads = 256;  // warp 0 brings tiles, 1 multiplies, 2 and 3 clear rows, 4 to 7 store
+constexpr int kSms = 148;
+constexpr int kBlockK = 64;              // contracted elements to a stage: one swizzle row
+constexpr int kTileM = 128;              // lanes of tensor memory
+constexpr uint32_t kBytesA = kTileM * kBlockK * 2;
+constexpr uint32_t kAll = 0xffffffffu;
+
+// Products that gave up waiting (a bounded wait ran out): 1.
+__device__ uint32_t g_product_status;
+
+// Expert segments as the CTA keeps them in shared memory.
+struct Segments {
+  int32_t* first;  // [experts] rows: clamped into [0, capacity]
+  int32_t* count;
+  int32_t* tiles;  // [experts + 1] sums of the tiles before each expert
+};
+
+struct SegmentArgs {
+  const int32_t *counts, *offsets;
+  int experts, capacity;
+};
+
+// First row and number of rows of an expert's segment, within the rows there are.
+__device__ __forceinline__ int2 segment(const SegmentArgs& a, int e) {
+  const int first = min(max(a.offsets[e], 0), a.capacity);
+  return make_int2(first, min(max(a.counts[e], 0), a.capacity - first));
+}
+
+// All threads: fills s; tiles(count) is the number of tiles of an expert with that many rows.
+template <typename F>
+__device__ __forceinline__ void load_segments(const SegmentArgs& a, const Segments& s, uint32_t* sums, F&& tiles) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int kEach = kMaxExperts / kThreads;
+  const int per = (a.experts + kThreads - 1) / kThreads;  // consecutive experts to a thread
+  int mine[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = threadIdx.x * per + i;
+    mine[i] = 0;
+    if (i < per && e < a.experts) {
+      const int2 seg = segment(a, e);
+      s.first[e] = seg.x;
+      s.count[e] = seg.y;
+      mine[i] = tiles(seg.y);
+    }
+    sum += mine[i];
+  }
+  int scan = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(kAll, scan, d);
+    if (lane >= d) scan += v;
+  }
+  if (lane == 31) sums[warp] = scan;
+  __syncthreads();
+  int before = scan - sum;
+  for (int w = 0; w < warp; ++w) before += sums[w];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = threadIdx.x * per + i;
+    if (i < per && e < a.experts) {
+      s.tiles[e] = before;
+      before += mine[i];
+      if (e == a.experts - 1) s.tiles[a.experts] = before;
+    }
+  }
+  __syncthreads();
+}
+
+// The expert whose tiles hold tile t.
+__device__ __forceinline__ int find(const int32_t* tiles, int experts, int t) {
+  int low = 0, high = experts;  // tiles[low] <= t < tiles[high]
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (tiles[mid] <= t) low = mid;
+    else high = mid;
+  }
+  return low;
+}
+
+// Barriers and flags of one CTA.
+template <int STAGES> struct Pipe {
+  uint64_t full[STAGES], empty[STAGES], sum_full[2], sum_empty[2];
+  uint32_t tmem, gave_up, sums[8];
+};
+
+template <int STAGES>
+__device__ __forceinline__ void init_pipe(Pipe<STAGES>& p, uint32_t columns) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) dev::mbar_init(&p.full[i], 1), dev::mbar_init(&p.empty[i], 1);
+    for (int i = 0; i < 2; ++i) dev::mbar_init(&p.sum_full[i], 1), dev::mbar_init(&p.sum_empty[i], 4);
+    p.gave_up = 0;
+    dev::fence_mbar_init();
+  }
+  if (threadIdx.x / 32 == 1) dev::tmem_alloc(&p.tmem, columns);
+  dev::tmem_fence_before();
+  __syncthreads();
+  dev::tmem_fence_after();
+}
+
+// The end of every warp's work: tensor memory is given back.
+template <int STAGES>
+__device__ __forceinline__ void close_pipe(Pipe<STAGES>& p, uint32_t columns) {
+  dev::tmem_fence_before();
+  __syncthreads();
+  if (threadIdx.x == 0 && p.gave_up) atomicOr(&g_product_status, 1u);
+  if (threadIdx.x / 32 == 1) {
+    dev::tmem_fence_after();
+    dev::tmem_free(p.tmem, columns);
+  }
+}
+
+// The producer's place in the ring of stages.
+template <int STAGES> struct Ring {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == STAGES) stage = 0, parity ^= 1;
+  }
+};
+
+// After a wait ran out: no copy of this CTA is left in flight.  `issued`
+// stages were filled, the last one before ring's place.
+template <int STAGES>
+__device__ __forceinline__ void drain(Pipe<STAGES>& p, Ring<STAGES> ring, int64_t issued, uint64_t limit_ns) {
+  const int64_t last = issued < STAGES ? issued : STAGES;
+  for (int64_t i = 0; i < last; ++i) {
+    if (ring.stage == 0) ring.stage = STAGES, ring.parity ^= 1;
+    --ring.stage;
+    dev::mbar_wait(&p.full[ring.stage], ring.parity, nullptr, limit_ns);
+  }
+}
+
+// A wait of a whole warp, whose lanes go on alike.
+template <int STAGES>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Pipe<STAGES>& p, uint64_t limit_ns) {
+  return __all_sync(kAll, dev::mbar_wait(bar, parity, &p.gave_up, limit_ns));
+}
+
+__device__ __forceinline__ uint32_t align_up(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
+
+// Zeros in 16-bit elements [begin, end) of x, by `threads` threads.
+__device__ __forceinline__ void clear(uint16_t* x, int64_t begin, int64_t end, int thread, int threads) {
+  if (begin >= end) return;
+  const int64_t head = min(end, begin + (int64_t)((16 - (reinterpret_cast<uintptr_t>(x + begin) & 15)) % 16) / 2);
+  const int64_t words = (end - head) / 8;
+  uint4* body = reinterpret_cast<uint4*>(x + head);
+  if (begin + thread < head) x[begin + thread] = 0;
+#pragma unroll 4
+  for (int64_t i = thread; i < words; i += threads) body[i] = make_uint4(0, 0, 0, 0);
+  if (head + words * 8 + thread < end) x[head + words * 8 + thread] = 0;
+}
+
+// ---------------------------------------------------------------- the products
+
+struct ProductArgs {
+  CUtensorMap weights, rows;
+  SegmentArgs segments;
+  void* out;
+  int in, width;      // of a row, and of a row of the result
+  int width_tiles;    // tiles of kTileM of the result's width
+  uint64_t limit_ns;  // bound on every wait
+};
+
+template <int BN, int STAGES> struct ProductShape {
+  static constexpr uint32_t kBytesB = BN * kBlockK * 2, kStage = kBytesA + kBytesB;
+  static constexpr int kBoxRows = BN / 4;  // a tile of few rows brings few boxes
+  static constexpr uint32_t kColumns = 2 * BN;
+  static constexpr uint32_t kStaging = 4 * 2048;  // 32 x 32 16-bit elements for each storing warp
+  static size_t bytes(int experts) {
+    return 1024 + STAGES * kStage + kStaging + sizeof(Pipe<STAGES>) + 4 * (3 * (size_t)experts + 1);
+  }
+};
+
+struct ProductTile {
+  int expert, row, rows, column;  // first row and number of rows; first column of the result
+};
+
+template <int BN>
+__device__ __forceinline__ ProductTile product_tile(const ProductArgs& a, const Segments& s, uint32_t t) {
+  ProductTile p;
+  p.expert = find(s.tiles, a.segments.experts, t / a.width_tiles);
+  const uint32_t before = s.tiles[p.expert], tiles = s.tiles[p.expert + 1] - before;
+  const uint32_t local = t - before * a.width_tiles, count = s.count[p.expert];
+  // the rows in equal tiles, whole steps of the instruction's width
+  const uint32_t per = align_up((count + tiles - 1) / tiles, 16), tile = local % tiles;
+  p.row = s.first[p.expert] + tile * per;
+  p.rows = min(per, count - tile * per);
+  p.column = local / tiles * kTileM;
+  return p;
+}
+
+// out^T = weights^T x rows^T by tiles of 128 of the result's columns (the
+// lanes of tensor memory) and up to BN rows of one segment.  So the
+// instruction's width is the number of rows, in steps of 16: an expert with
+// three rows costs a width of 16, and its weights stream through the 128
+// lanes.
+template <typename T, int BN, int STAGES, bool IN_ORDER>
+__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
+  using Shape = ProductShape<BN, STAGES>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* base = raw + (align_up(dev::smem_u32(raw), 1024) - dev::smem_u32(raw));
+  uint8_t* staging = base + STAGES * Shape::kStage;
+  Pipe<STAGES>& p = *reinterpret_cast<Pipe<STAGES>*>(staging + Shape::kStaging);
+  const int experts = a.segments.experts;
+  Segments s;
+  s.first = reinterpret_cast<int32_t*>(&p + 1);
+  s.count = s.first + experts;
+  s.tiles = s.count + experts;
+
+  init_pipe(p, Shape::kColumns);
+  dev::wait_for_previous();
+  load_segments(a.segments, s, p.sums, [](int count) { return (count + BN - 1) / BN; });
+  const uint32_t tiles = (uint32_t)s.tiles[experts] * a.width_tiles;
+  const int steps = (a.in + kBlockK - 1) / kBlockK;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t stages = dev::smem_u32(base);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      Ring<STAGES> ring;
+      int64_t issued = 0;
+      bool ok = true;
+      for (uint32_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        const ProductTile tile = product_tile<BN>(a, s, t);
+        const int boxes = (tile.rows + Shape::kBoxRows - 1) / Shape::kBoxRows;
+        for (int k = 0; k < steps; ++k) {
+          if (!dev::mbar_wait(&p.empty[ring.stage], ring.parity ^ 1, &p.gave_up, a.limit_ns)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = dev::smem_u32(&p.full[ring.stage]), at = stages + ring.stage * Shape::kStage;
+          dev::mbar_arrive_expect_tx(&p.full[ring.stage], kBytesA + boxes * Shape::kBoxRows * dev::kBoxRowBytes);
+          if (IN_ORDER) {
+            dev::tma_load_3d(at, &a.weights, bar, k * kBlockK, tile.column, tile.expert);
+          } else {
+            dev::tma_load_3d(at, &a.weights, bar, tile.column, k * kBlockK, tile.expert);
+            dev::tma_load_3d(at + kBytesA / 2, &a.weights, bar, tile.column + kBlockK, k * kBlockK, tile.expert);
+          }
+          for (int b = 0; b < boxes; ++b)
+            dev::tma_load_2d(at + kBytesA + b * Shape::kBoxRows * dev::kBoxRowBytes, &a.rows, bar, k * kBlockK,
+                             tile.row + b * Shape::kBoxRows);
+          ring.next();
+          ++issued;
+        }
+      }
+      if (!ok) drain(p, ring, issued, a.limit_ns);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      Ring<STAGES> ring;
+      Ring<2> sums;
+      bool ok = true;
+      for (uint32_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        const ProductTile tile = product_tile<BN>(a, s, t);
+        const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, !IN_ORDER, false, kTileM,
+                                                          align_up(tile.rows, 16));
+        if (!dev::mbar_wait(&p.sum_empty[sums.stage], sums.parity ^ 1, &p.gave_up, a.limit_ns)) break;
+        dev::tmem_fence_after();
+        const uint32_t sum = p.tmem + sums.stage * BN;
+        for (int k = 0; k < steps; ++k) {
+          if (!dev::mbar_wait(&p.full[ring.stage], ring.parity, &p.gave_up, a.limit_ns)) {
+            ok = false;
+            break;
+          }
+          dev::tmem_fence_after();
+          const uint32_t at = stages + ring.stage * Shape::kStage;
+          const uint64_t da = dev::operand_descriptor(at, IN_ORDER ? 16 : kBytesA / 2, 1024);
+          const uint64_t db = dev::operand_descriptor(at + kBytesA, 16, 1024);
+#pragma unroll
+          for (int i = 0; i < kBlockK / 16; ++i)
+            dev::mma_issue(sum, da + i * (IN_ORDER ? 32 : 2048) / 16, db + i * 32 / 16, instruction, k + i > 0);
+          dev::mma_commit(dev::smem_u32(&p.empty[ring.stage]));
+          ring.next();
+        }
+        dev::mma_commit(dev::smem_u32(&p.sum_full[sums.stage]));
+        sums.next();
+      }
+    }
+  } else if (warp < 4) {
+    // rows that hold no pair: those between the segments by the expert before, those behind the last in equal parts
+    uint16_t* out = static_cast<uint16_t*>(a.out);
+    const int thread = threadIdx.x - 64;
+    for (int e = blockIdx.x; e < experts; e += gridDim.x) {
+      const int end = s.first[e] + s.count[e];
+      if (e + 1 < experts) clear(out, (int64_t)end * a.width, (int64_t)s.first[e + 1] * a.width, thread, 64);
+      if (e == 0) clear(out, 0, (int64_t)s.first[0] * a.width, thread, 64);
+    }
+    const int end = s.first[experts - 1] + s.count[experts - 1], left = a.segments.capacity - end;
+    const int per = (left + gridDim.x - 1) / gridDim.x;
+    const int64_t r0 = end + (int64_t)min((int64_t)left, (int64_t)blockIdx.x * per);
+    clear(out, r0 * a.width, min(r0 + per, (int64_t)a.segments.capacity) * a.width, thread, 64);
+  } else {
+    // the sums to 16 bits, through shared memory from a column of the result to a lane to a row's piece to a lane
+    Ring<2> sums;
+    const int quarter = warp & 3;
+    uint8_t* mine = staging + quarter * 2048;
+    T* out = static_cast<T*>(a.out);
+    const bool whole = a.width % 8 == 0;  // the result's first byte lies on a 16-byte boundary
+    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+      const ProductTile tile = product_tile<BN>(a, s, t);
+      if (!warp_wait(&p.sum_full[sums.stage], sums.parity, p, a.limit_ns)) break;
+      dev::tmem_fence_after();
+      const int column = tile.column + quarter * 32;
+      for (int c = 0; c < tile.rows; c += 32) {
+        uint32_t v[32];
+        dev::tmem_load32(p.tmem + sums.stage * BN + c + ((uint32_t)quarter << 21), v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const uint32_t both = dev::from_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), T{});
+          const uint32_t other = __shfl_xor_sync(kAll, both, 1);
+          // even lanes: row 2j, odd ones: row 2j + 1, each of this column and its neighbour
+          const uint32_t word = lane & 1 ? __byte_perm(other, both, 0x7632) : __byte_perm(both, other, 0x5410);
+          *reinterpret_cast<uint32_t*>(mine + (2 * j + (lane & 1)) * 64 + (lane >> 1) * 4) = word;
+        }
+        __syncwarp();
+        const int rows = min(32, tile.rows - c);
+        const int64_t first = (int64_t)(tile.row + c);
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + lane / 4, at = column + lane % 4 * 8;
+            if (row < rows && at < a.width)
+              *reinterpret_cast<uint4*>(out + (first + row) * a.width + at) =
+                  *reinterpret_cast<const uint4*>(mine + row * 64 + lane % 4 * 16);
+          }
+        } else if (column + lane < a.width) {
+          for (int row = 0; row < rows; ++row)
+            out[(first + row) * a.width + column + lane] = *reinterpret_cast<const T*>(mine + row * 64 + lane * 2);
+        }
+        __syncwarp();
+      }
+      dev::tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) dev::mbar_arrive(&p.sum_empty[sums.stage]);
+      sums.next();
+    }
+  }
+  __syncwarp();
+  close_pipe(p, Shape::kColumns);
+}
+
+// ---------------------------------------------------- the gradient of the weights
+
+struct GradArgs {
+  CUtensorMap slow, fast;  // the rows whose width is the gradient's slower dimension, and those of the contiguous one
+  SegmentArgs segments;
+  void* out;  // [experts][slow_width][fast_width]
+  int slow_width, fast_width, slow_tiles, fast_tiles;
+  uint64_t limit_ns;
+};
+
+constexpr int kGradN = 256;
+constexpr int kGradStages = 4;
+constexpr uint32_t kGradStage = kBytesA + kGradN * kBlockK * 2;
+constexpr uint32_t kGradPitch = 80;  // bytes between the staged rows of 64: 8 lanes' 16-byte pieces fall on all banks
+constexpr uint32_t kGradStaging = 4 * 32 * kGradPitch;
+
+size_t grad_bytes(int experts) {
+  return 1024 + kGradStages * kGradStage + kGradStaging + sizeof(Pipe<kGradStages>) + 4 * (3 * (size_t)experts + 1);
+}
+
+// gradient[e] = slow_e^T x fast_e, contracted over the rows of e's segment: both operands lie with the contracted
+// dimension across.  Rows behind the segment's end that the last step brings along are cleared in shared memory: they
+// are another expert's, or anything at all.
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) grad_weights_kernel(const __grid_constant__ GradArgs a) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* base = raw + (align_up(dev::smem_u32(raw), 1024) - dev::smem_u32(raw));
+  uint8_t* staging = base + kGradStages * kGradStage;
+  Pipe<kGradStages>& p = *reinterpret_cast<Pipe<kGradStages>*>(staging + kGradStaging);
+  const int experts = a.segments.experts;
+
+  init_pipe(p, 512);
+  dev::wait_for_previous();
+  const uint32_t per_expert = (uint32_t)a.slow_tiles * a.fast_tiles, tiles = per_expert * experts;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t stages = dev::smem_u32(base);
+  constexpr int kChunks = kGradN / kBlockK;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      Ring<kGradStages> ring;
+      int64_t issued = 0;
+      bool ok = true;
+      for (uint32_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        const uint32_t local = t % per_expert;
+        const int2 seg = segment(a.segments, t / per_expert);
+        const int m = local % a.slow_tiles * kTileM, n = local / a.slow_tiles * kGradN;
+        const int chunks = min(kChunks, (a.fast_width - n + kBlockK - 1) / kBlockK);
+        for (int k = 0; k < seg.y; k += kBlockK) {
+          if (!dev::mbar_wait(&p.empty[ring.stage], ring.parity ^ 1, &p.gave_up, a.limit_ns)) {
+            ok = false;
+            break;
+          }
+          const uint32_t bar = dev::smem_u32(&p.full[ring.stage]), at = stages + ring.stage * kGradStage;
+          dev::mbar_arrive_expect_tx(&p.full[ring.stage], kBytesA + chunks * (kBytesA / 2));
+          dev::tma_load_2d(at, &a.slow, bar, m, seg.x + k);
+          dev::tma_load_2d(at + kBytesA / 2, &a.slow, bar, m + kBlockK, seg.x + k);
+          for (int c = 0; c < chunks; ++c)
+            dev::tma_load_2d(at + kBytesA + c * (kBytesA / 2), &a.fast, bar, n + c * kBlockK, seg.x + k);
+          ring.next();
+          ++issued;
+        }
+      }
+      if (!ok) drain(p, ring, issued, a.limit_ns);
+    }
+  } else if (warp == 1) {
+    Ring<kGradStages> ring;
+    Ring<2> sums;
+    bool ok = true;
+    for (uint32_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+      const uint32_t local = t % per_expert;
+      const int count = segment(a.segments, t / per_expert).y;
+      if (count == 0) continue;
+      const int n = local / a.slow_tiles * kGradN;
+      const int chunks = min(kChunks, (a.fast_width - n + kBlockK - 1) / kBlockK);
+      const uint32_t instruction =
+          dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, true, true, kTileM, chunks * kBlockK);
+      if (!warp_wait(&p.sum_empty[sums.stage], sums.parity ^ 1, p, a.limit_ns)) break;
+      dev::tmem_fence_after();
+      const uint32_t sum = p.tmem + sums.stage * kGradN;
+      for (int k = 0; k < count; k += kBlockK) {
+        if (!warp_wait(&p.full[ring.stage], ring.parity, p, a.limit_ns)) {
+          ok = false;
+          break;
+        }
+        const int valid = min(kBlockK, count - k), depth = (valid + 15) / 16;
+        if (valid < depth * 16) {
+          const int pieces = (depth * 16 - valid) * 8 * (2 + chunks);  // 16 bytes each
+          for (int i = lane; i < pieces; i += 32) {
+            const int column = i / ((depth * 16 - valid) * 8), within = i % ((depth * 16 - valid) * 8);
+            *reinterpret_cast<uint4*>(base + ring.stage * kGradStage + column * (kBytesA / 2) + valid * 128 +
+                                      within * 16) = make_uint4(0, 0, 0, 0);
+          }
+          dev::fence_proxy_async_smem();
+          __syncwarp();
+        }
+        if (lane == 0) {
+          dev::tmem_fence_after();
+          const uint32_t at = stages + ring.stage * kGradStage;
+          const uint64_t da = dev::operand_descriptor(at, kBytesA / 2, 1024);
+          const uint64_t db = dev::operand_descriptor(at + kBytesA, kBytesA / 2, 1024);
+          for (int i = 0; i < depth; ++i)
+            dev::mma_issue(sum, da + i * 2048 / 16, db + i * 2048 / 16, instruction, k + i > 0);
+          dev::mma_commit(dev::smem_u32(&p.empty[ring.stage]));
+        }
+        ring.next();
+        __syncwarp();
+      }
+      if (lane == 0) dev::mma_commit(dev::smem_u32(&p.sum_full[sums.stage]));
+      sums.next();
+    }
+  } else if (warp >= 4) {
+    Ring<2> sums;
+    const int quarter = warp & 3;
+    uint8_t* mine = staging + quarter * 32 * kGradPitch;
+    const bool whole = a.fast_width % 8 == 0;
+    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+      const uint32_t local = t % per_expert;
+      const int expert = t / per_expert, m = local % a.slow_tiles * kTileM + quarter * 32,
+                n = local / a.slow_tiles * kGradN;
+      const int columns = min(kGradN, a.fast_width - n), rows = min(32, a.slow_width - m);
+      const bool empty = segment(a.segments, expert).y == 0;
+      T* out = static_cast<T*>(a.out) + ((int64_t)expert * a.slow_width + m) * a.fast_width + n;
+      if (!empty) {
+        if (!warp_wait(&p.sum_full[sums.stage], sums.parity, p, a.limit_ns)) break;
+        dev::tmem_fence_after();
+      }
+      for (int c = 0; c < columns; c += 32) {
+        if (!empty) {
+          uint32_t v[32];
+          dev::tmem_load32(p.tmem + sums.stage * kGradN + c + ((uint32_t)quarter << 21), v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint4 w;
+            w.x = dev::from_float2(__uint_as_float(v[8 * j]), __uint_as_float(v[8 * j + 1]), T{});
+            w.y = dev::from_float2(__uint_as_float(v[8 * j + 2]), __uint_as_float(v[8 * j + 3]), T{});
+            w.z = dev::from_float2(__uint_as_float(v[8 * j + 4]), __uint_as_float(v[8 * j + 5]), T{});
+            w.w = dev::from_float2(__uint_as_float(v[8 * j + 6]), __uint_as_float(v[8 * j + 7]), T{});
+            *reinterpret_cast<uint4*>(mine + lane * kGradPitch + j * 16) = w;
+          }
+          __syncwarp();
+        }
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + lane / 4, at = c + lane % 4 * 8;
+            if (row < rows && at < columns)
+              *reinterpret_cast<uint4*>(out + (int64_t)row * a.fast_width + at) =
+                  empty ? make_uint4(0, 0, 0, 0)
+                        : *reinterpret_cast<const uint4*>(mine + row * kGradPitch + lane % 4 * 16);
+          }
+        } else if (c + lane < columns) {
+          for (int row = 0; row < rows; ++row)
+            out[(int64_t)row * a.fast_width + c + lane] =
+                empty ? dev::from_float<T>(0.f) : *reinterpret_cast<const T*>(mine + row * kGradPitch + lane * 2);
+        }
+        __syncwarp();
+      }
+      if (!empty) {
+        dev::tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) dev::mbar_arrive(&p.sum_empty[sums.stage]);
+        sums.next();
+      }
+    }
+  }
+  __syncwarp();
+  close_pipe(p, 512);
+}
+
+// --------------------------------------------------------- operands laid out anew
+
+struct RepackArgs {
+  const uint16_t* x;
+  uint16_t* y;
+  int64_t outer_stride, row_stride, pitch;  // elements
+  int64_t rows;                             // of all outer parts together
+  int per_outer, width;
+  const int32_t* counts;  // where it is given: outer parts with none are left out
+};
+
+// Rows of a width or at an address that the tiled copies do not take (they want 16-byte steps), copied to where they
+// do: y[r] = x's row r, `pitch` elements apart.  One warp to a row; bound by the narrow loads.
+__global__ void __launch_bounds__(256) repack_kernel(const __grid_constant__ RepackArgs a) {
+  dev::wait_for_previous();
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5); r < a.rows; r += gridDim.x * 8ll) {
+    const int64_t outer = r / a.per_outer;
+    if (a.counts != nullptr && a.counts[outer] <= 0) continue;
+    const uint16_t* x = a.x + outer * a.outer_stride + (r - outer * a.per_outer) * a.row_stride;
+    uint16_t* y = a.y + r * a.pitch;
+#pragma unroll 8
+    for (int i = lane; i < a.width; i += 32) y[i] = x[i];
+  }
+}
+
+// ------------------------------------------------------------------- the host side
+
+// An operand: `outer` matrices of `rows` rows of `width` contiguous elements.
+struct Operand {
+  const void* data;
+  int64_t outer, rows, width, outer_stride, row_stride;
+
+  bool ready() const {
+    return ((reinterpret_cast<uintptr_t>(data) | (uintptr_t)(rows > 1 ? row_stride * 2 : 0) |
+             (uintptr_t)(outer > 1 ? outer_stride * 2 : 0)) & 15) == 0 &&
+           (rows <= 1 || row_stride >= width) && (outer <= 1 || outer_stride > 0);
+  }
+  int64_t pitch() const { return (width + 7) / 8 * 8; }
+  size_t bytes() const { return ready() ? 0 : ((size_t)(outer * rows * pitch()) * 2 + 255) / 256 * 256; }
+
+  // Copies it to `temp`, if need be.
+  cudaError_t prepare(uint8_t*& temp, const int32_t* counts, cudaStream_t stream) {
+    if (ready()) return cudaSuccess;
+    const size_t size = bytes();
+    RepackArgs a{static_cast<const uint16_t*>(data), reinterpret_cast<uint16_t*>(temp), outer_stride, row_stride,
+                 pitch(), outer * rows, (int)rows, (int)width, counts};
+    data = temp;
+    row_stride = pitch();
+    outer_stride = rows * pitch();
+    temp += size;
+    return launch_after_previous(repack_kernel, std::min<int64_t>(kSms * 8, (a.rows + 7) / 8), 256, 0, a, stream);
+  }
+
+  cudaError_t map(CUtensorMap* m, bool matrix, uint32_t box_rows) const {
+    // strides of dimensions of one element are never used, but have to be in order
+    const uint64_t row = (uint64_t)(rows > 1 ? row_stride : pitch()) * 2;
+    const uint64_t dims[3] = {(uint64_t)width, (uint64_t)rows, (uint64_t)outer};
+    const uint64_t strides[2] = {row, outer > 1 ? (uint64_t)outer_stride * 2 : row * rows};
+    const uint32_t box[3] = {kBlockK, box_rows, 1};
+    return encode_map(m, data, matrix ? 2 : 3, dims, strides, box);
+  }
+};
+
+template <typename Kernel, typename Args>
+cudaError_t run(Kernel kernel, const Args& a, int64_t tiles, size_t smem, cudaStream_t stream) {
+  // the limit is the kernel's, not the call's: the same one from every host thread
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e) return e;
+  return launch_after_previous(kernel, std::max<int64_t>(1, std::min<int64_t>(kSms, tiles)), kThreads, smem, a, stream);
+}
+
+template <typename T, int BN, int STAGES>
+cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order, int64_t tiles, cudaStream_t stream) {
+  using Shape = ProductShape<BN, STAGES>;
+  cudaError_t e = weights.map(&a.weights, false, in_order ? kTileM : kBlockK);
+  if (!e) e = rows.map(&a.rows, true, Shape::kBoxRows);
+  if (e) return e;
+  const size_t smem = Shape::bytes(a.segments.experts);
+  return in_order ? run(product_kernel<T, BN, STAGES, true>, a, tiles, smem, stream)
+                  : run(product_kernel<T, BN, STAGES, false>, a, tiles, smem, stream);
+}
+
+bool half_type(int type) { return type == CUSORT_FLOAT_F16 || type == CUSORT_FLOAT_BF16; }
+
+// Rows of a tile where experts have few rows on average, and where they have many.
+constexpr int kFewRows = 64, kManyRows = 256;
+
+bool sizes_fit(int64_t capacity, int64_t in, int64_t out, int experts) {
+  return capacity >= 0 && capacity <= INT32_MAX && in >= 1 && in <= (1 << 20) && out >= 1 && out <= (1 << 20) &&
+         experts >= 1 && experts <= kMaxExperts;
+}
+
+}  // namespace
+
+extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp_storage_bytes, cusort_float_type type,
+                                              const void* d_rows, int64_t row_stride, const void* d_weights,
+                                              int64_t expert_stride, int64_t in_stride, int64_t out_stride,
+                                              const int32_t* d_counts, const int32_t* d_offsets, void* d_out,
+                                              int64_t capacity, int64_t in, int64_t out, int num_experts,
+                                              cudaStream_t stream) {
+  if (temp_storage_bytes == nullptr || !half_type(type) || !sizes_fit(capacity, in, out, num_experts) ||
+      row_stride < 0 || expert_stride < 0 || in_stride < 0 || out_stride < 0)
+    return cudaErrorInvalidValue;
+  const bool in_order = !(out_stride == 1 || out == 1);
+  if (in_order && in_stride != 1 && in != 1) return cudaErrorInvalidValue;
+  Operand rows{d_rows, 1, capacity, in, 0, row_stride};
+  Operand weights{d_weights, num_experts, in_order ? out : in, in_order ? in : out, expert_stride,
+                  in_order ? out_stride : in_stride};
+  const size_t need = std::max<size_t>(1, capacity == 0 ? 0 : rows.bytes() + weights.bytes());
+  if (d_temp_storage == nullptr) {
+    *temp_storage_bytes = need;
+    return cudaSuccess;
+  }
+  if (*temp_storage_bytes < need) return cudaErrorInvalidValue;
+  if (capacity == 0) return cudaSuccess;
+  if (d_rows == nullptr || d_weights == nullptr || d_counts == nullptr || d_offsets == nullptr || d_out == nullptr ||
+      (reinterpret_cast<uintptr_t>(d_out) & 15) != 0 || (need > 1 && (reinterpret_cast<uintptr_t>(d_temp_storage) & 15) != 0))
+    return cudaErrorInvalidValue;
+  const bool few = capacity <= (int64_t)kFewRows * num_experts;
+  ProductArgs a;
+  a.segments = {d_counts, d_offsets, num_experts, (int)capacity};
+  a.out = d_out;
+  a.in = (int)in;
+  a.width = (int)out;
+  a.width_tiles = (int)((out + kTileM - 1) / kTileM);
+  a.limit_ns = wait_limit_ns();
+  // at most one part-filled tile to an expert, and no expert without a row
+  const int64_t tiles = (capacity / (few ? kFewRows : kManyRows) + std::min<int64_t>(num_experts, capacity)) * a.width_tiles;
+  if (tiles > INT32_MAX) return cudaErrorInvalidValue;
+  uint8_t* temp = static_cast<uint8_t*>(d_temp_storage);
+  cudaError_t e = rows.prepare(temp, nullptr, stream);
+  if (!e) e = weights.prepare(temp, d_counts, stream);
+  if (e) return e;
+  const auto go = [&](auto t) {
+    using T = decltype(t);
+    return few ? product<T, kFewRows, 8>(a, weights, rows, in_order, tiles, stream)
+               : product<T, kManyRows, 4>(a, weights, rows, in_order, tiles, stream);
+  };
+  return type == CUSORT_FLOAT_F16 ? go(__half{}) : go(__nv_bfloat16{});
+}
+
+extern "C" cudaError_t cusort_expert_products_grad_weights(
+    void* d_temp_storage, size_t* temp_storage_bytes, cusort_float_type type, const void* d_rows, int64_t row_stride,
+    const void* d_grad_out, int64_t grad_stride, const int32_t* d_counts, const int32_t* d_offsets,
+    void* d_grad_weights, int in_contiguous, int64_t capacity, int64_t in, int64_t out, int num_experts,
+    cudaStream_t stream) {
+  if (temp_storage_bytes == nullptr || !half_type(type) || !sizes_fit(capacity, in, out, num_experts) ||
+      row_stride < 0 || grad_stride < 0)
+    return cudaErrorInvalidValue;
+  Operand slow{d_rows, 1, capacity, in, 0, row_stride}, fast{d_grad_out, 1, capacity, out, 0, grad_stride};
+  if (in_contiguous) std::swap(slow, fast);
+  const size_t need = std::max<size_t>(1, capacity == 0 ? 0 : slow.bytes() + fast.bytes());
+  if (d_temp_storage == nullptr) {
+    *temp_storage_bytes = need;
+    return cudaSuccess;
+  }
+  if (*temp_storage_bytes < need) return cudaErrorInvalidValue;
+  if (d_grad_weights == nullptr || (reinterpret_cast<uintptr_t>(d_grad_weights) & 15) != 0) return cudaErrorInvalidValue;
+  if (capacity == 0) return cudaMemsetAsync(d_grad_weights, 0, (size_t)num_experts * in * out * 2, stream);
+  if (d_rows == nullptr || d_grad_out == nullptr || d_counts == nullptr || d_offsets == nullptr ||
+      (need > 1 && (reinterpret_cast<uintptr_t>(d_temp_storage) & 15) != 0))
+    return cudaErrorInvalidValue;
+  GradArgs a;
+  a.segments = {d_counts, d_offsets, num_experts, (int)capacity};
+  a.out = d_grad_weights;
+  a.slow_width = (int)slow.width;
+  a.fast_width = (int)fast.width;
+  a.slow_tiles = (int)((slow.width + kTileM - 1) / kTileM);
+  a.fast_tiles = (int)((fast.width + kGradN - 1) / kGradN);
+  a.limit_ns = wait_limit_ns();
+  const int64_t tiles = (int64_t)a.slow_tiles * a.fast_tiles * num_experts;
+  if (tiles > INT32_MAX) return cudaErrorInvalidValue;
+  uint8_t* temp = static_cast<uint8_t*>(d_temp_storage);
+  cudaError_t e = slow.prepare(temp, nullptr, stream);
+  if (!e) e = fast.prepare(temp, nullptr, stream);
+  if (!e) e = slow.map(&a.slow, true, kBlockK);
+  if (!e) e = fast.map(&a.fast, true, kBlockK);
+  if (e) return e;
+  return type == CUSORT_FLOAT_F16 ? run(grad_weights_kernel<__half>, a, tiles, grad_bytes(num_experts), stream)
+                                  : run(grad_weights_kernel<__nv_bfloat16>, a, tiles, grad_bytes(num_experts), stream);
+}
+
+extern "C" cudaError_t cusort_read_product_status(uint32_t* status, cudaStream_t stream) {
+  if (status == nullptr) return cudaErrorInvalidValue;
+  void* word = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&word, g_product_status);
+  if (!e) e = cudaMemcpyAsync(status, word, sizeof(uint32_t), cudaMemcpyDeviceToHost, stream);
+  if (!e) e = cudaMemsetAsync(word, 0, sizeof(uint32_t), stream);
+  return e ? e : cudaStreamSynchronize(stream);
+}

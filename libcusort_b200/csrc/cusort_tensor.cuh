@@ -1,0 +1,120 @@
+// cusort_tensor.cuh -- what the matrix products need of the tensor cores and
+// of the tiled copies: bounded barrier waits, tensor maps, shared-memory and
+// instruction descriptors, accumulators in tensor memory.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "cusort_device.cuh"
+
+namespace cusort_b200 {
+namespace dev {
+
+// A tile of 64 16-bit elements (128 bytes) along the contiguous dimension: the
+// width of every box that the tiled copies bring, whose 16-byte pieces they
+// permute within each 8 rows (128-byte swizzle).
+constexpr int kBoxElements = 64;
+constexpr int kBoxRowBytes = 128;
+
+__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          dst),
+      "l"(map), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+      "[%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+// Shared-memory matrix descriptor of a 128-byte-swizzled operand.  `leading`
+// and `stride` in bytes:
+//   contracted dimension contiguous: `stride` from one group of 8 rows to the
+//   next (1024), `leading` unused; 16 elements on: 32 bytes on;
+//   other dimension contiguous: `leading` from one 64-element column of boxes
+//   to the next, `stride` from one group of 8 contracted rows to the next
+//   (1024); 16 contracted elements on: 2048 bytes on.
+__device__ __forceinline__ uint64_t operand_descriptor(uint32_t address, uint32_t leading, uint32_t stride) {
+  return (uint64_t)((address & 0x3ffff) >> 4) | (uint64_t)(leading >> 4) << 16 | (uint64_t)(stride >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// Instruction descriptor: 16-bit operands of one type, 32-bit sums.
+__host__ __device__ constexpr uint32_t mma_instruction(bool bf16, bool a_transposed, bool b_transposed, int m, int n) {
+  return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (a_transposed ? 1u << 15 : 0u) | (b_transposed ? 1u << 16 : 0u) |
+         (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
+}
+
+// One thread: accumulator (at the tensor-memory address) (+)= A x B.
+__device__ __forceinline__ void mma_issue(uint32_t accumulator, uint64_t a, uint64_t b, uint32_t instruction,
+                                          bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(accumulator),
+      "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add)
+      : "memory");
+}
+// The barrier gets one arrival when the products issued so far are done.
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(columns)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t address, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns) : "memory");
+}
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 columns of this warp's 32 lanes of tensor memory: v[i] = column i of this thread's lane.
+__device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(address));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Waits for a phase of a barrier, `limit_ns` at most and no longer than until
+// another thread of the CTA has given up (*gave_up, in shared memory).
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t* gave_up, uint64_t limit_ns) {
+  if (mbar_try_wait(bar, parity)) return true;
+  SpinGuard guard;
+  while (!mbar_try_wait(bar, parity)) {
+    if (guard.expired(gave_up, limit_ns)) {
+      if (gave_up != nullptr) *(volatile uint32_t*)gave_up = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+}  // namespace dev
+
+// Tensor map of 16-bit elements with 128-byte swizzle, zeros outside.  dims
+// and box from the contiguous dimension on; strides in bytes, of the
+// dimensions after it.
+cudaError_t encode_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                       const uint32_t* box);
+
+}  // namespace cusort_b200

@@ -4,8 +4,8 @@
 // decode step, so what the host spends on a call is what the call costs: from
 // Python through ctypes it was 16 us for cusort_route, from here it is 5.
 //
-// Plain CPython functions of positional arguments; libcusort_b200/routing.py
-// and paging.py give them their names, defaults and documentation.
+// Plain CPython functions of positional arguments; libcusort_b200/routing.py,
+// experts.py and paging.py give them their names, defaults and documentation.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -24,6 +24,7 @@
 namespace {
 
 constexpr int kMaxExperts = 1024, kMaxChosen = 32, kMaxGroups = 32, kMaxRequests = 16384;
+constexpr int64_t kMaxWidth = 1 << 20;
 
 // A Python exception on its way to the entry point.
 struct Refused {
@@ -409,6 +410,110 @@ PyObject* combine_backward(PyObject* const* p) {
   return tuple(wrap(std::move(grad_rows)), wrap(std::move(grad_weights)));
 }
 
+cusort_float_type half_type(const at::Tensor& t, const char* name) {
+  if (t.scalar_type() != at::kHalf && t.scalar_type() != at::kBFloat16)
+    refuse(PyExc_TypeError, name, " must be float16 or bfloat16 (got ", name_of(t.scalar_type()), ")");
+  return float_type(t, name);
+}
+
+// A plan's segments over the rows of t.
+void check_segments(const at::Tensor& counts, const at::Tensor& offsets, const at::Tensor& t) {
+  if (counts.dim() != 1 || counts.numel() < 1 || counts.numel() > kMaxExperts)
+    refuse(PyExc_ValueError, "counts must be [experts], 1 to ", kMaxExperts, " of them (got shape ", shape_of(counts),
+           ")");
+  check(counts, "counts", at::kInt, t.device(), {counts.numel()});
+  check(offsets, "offsets", at::kInt, t.device(), {counts.numel() + 1});
+  if (t.size(0) > INT32_MAX) refuse(PyExc_ValueError, "2^31 rows and more are not supported (got ", t.size(0), ")");
+}
+
+void check_width(const char* name, int64_t width) {
+  if (width < 1 || width > kMaxWidth)
+    refuse(PyExc_ValueError, "rows of 1 to ", kMaxWidth, " elements are supported (got ", name, " of ", width, ")");
+}
+
+// Whether the last dimension but one is the contiguous one of the experts' matrices.
+bool in_contiguous(const at::Tensor& weights) {
+  const bool out = weights.stride(2) == 1 || weights.size(2) == 1, in = weights.stride(1) == 1 || weights.size(1) == 1;
+  if (!out && !in && weights.numel() > 0)
+    refuse(PyExc_ValueError, "weights must be contiguous along one of their last two dimensions (got strides ",
+           weights.strides(), ")");
+  return !out;
+}
+
+// The workspace of a call: f(its address, its size) is the call itself.
+template <typename F>
+void launch_with_temp(const char* what, at::Device device, F&& f) {
+  size_t bytes = 0;
+  launch(what, device, [&](cudaStream_t s) { return f(nullptr, &bytes, s); });
+  // one byte is asked for where nothing is needed: any address does
+  const at::Tensor temp = bytes > 1 ? empty({(int64_t)bytes}, at::kByte, device) : at::Tensor();
+  launch(what, device, [&](cudaStream_t s) { return f(bytes > 1 ? temp.data_ptr() : (void*)&bytes, &bytes, s); });
+}
+
+// rows, weights, counts, offsets, whether the weights are taken the other way round, the rows' name
+PyObject* expert_products(PyObject* const* p) {
+  const char* name = PyUnicode_AsUTF8(p[5]);
+  const at::Tensor &rows = tensor(p[0], name), &weights = tensor(p[1], "weights"), &counts = tensor(p[2], "counts"),
+                   &offsets = tensor(p[3], "offsets");
+  const bool back = truth(p[4]);
+  const cusort_float_type type = half_type(rows, name);
+  check_rows(rows, name);
+  check_segments(counts, offsets, rows);
+  const int64_t experts = counts.numel(), capacity = rows.size(0);
+  if (weights.dim() != 3 || weights.size(0) != experts || weights.size(back ? 2 : 1) != rows.size(1) ||
+      weights.scalar_type() != rows.scalar_type() || weights.device() != rows.device())
+    refuse(PyExc_ValueError, "weights must be ", name_of(rows.scalar_type()), " of shape (", experts, ", ",
+           back ? "in, " + text(rows.size(1)) : text(rows.size(1)) + ", out", ") on ", rows.device(), " (got ",
+           name_of(weights.scalar_type()), ", ", shape_of(weights), ", ", weights.device(), ")");
+  const int64_t in = rows.size(1), out = weights.size(back ? 1 : 2);
+  check_width(name, in);
+  check_width("the result", out);
+  in_contiguous(weights);
+  check_cuda(rows, name);
+  at::Tensor result = empty({capacity, out}, rows.scalar_type(), rows.device());
+  launch_with_temp("cusort_expert_products", rows.device(), [&](void* temp, size_t* bytes, cudaStream_t s) {
+    return cusort_expert_products(temp, bytes, type, rows.data_ptr(), rows.stride(0), weights.data_ptr(),
+                                  weights.stride(0), weights.stride(back ? 2 : 1), weights.stride(back ? 1 : 2),
+                                  ptr<int32_t>(counts), ptr<int32_t>(offsets), result.data_ptr(), capacity, in, out,
+                                  (int)experts, s);
+  });
+  return wrap(std::move(result));
+}
+
+// grad_out, rows, counts, offsets, whether the gradient lies with its second dimension contiguous
+PyObject* expert_products_grad_weights(PyObject* const* p) {
+  const at::Tensor &grad = tensor(p[0], "grad_out"), &rows = tensor(p[1], "rows"), &counts = tensor(p[2], "counts"),
+                   &offsets = tensor(p[3], "offsets");
+  const bool in_last = truth(p[4]);
+  const cusort_float_type type = half_type(rows, "rows");
+  check_rows(rows, "rows");
+  check_segments(counts, offsets, rows);
+  const int64_t experts = counts.numel(), capacity = rows.size(0), in = rows.size(1);
+  if (grad.dim() != 2) refuse(PyExc_ValueError, "grad_out must be [capacity, out] (got shape ", shape_of(grad), ")");
+  const int64_t out = grad.size(1);
+  check_like(grad, "grad_out", rows, capacity, out);
+  check_width("rows", in);
+  check_width("grad_out", out);
+  check_cuda(rows, "rows");
+  at::Tensor result = empty({experts, in_last ? out : in, in_last ? in : out}, rows.scalar_type(), rows.device());
+  launch_with_temp("cusort_expert_products_grad_weights", rows.device(),
+                   [&](void* temp, size_t* bytes, cudaStream_t s) {
+                     return cusort_expert_products_grad_weights(
+                         temp, bytes, type, rows.data_ptr(), rows.stride(0), grad.data_ptr(), grad.stride(0),
+                         ptr<int32_t>(counts), ptr<int32_t>(offsets), result.data_ptr(), in_last, capacity, in, out,
+                         (int)experts, s);
+                   });
+  return wrap(in_last ? result.transpose(1, 2) : std::move(result));
+}
+
+// weights
+PyObject* weights_in_contiguous(PyObject* const* p) {
+  const at::Tensor& weights = tensor(p[0], "weights");
+  if (weights.dim() != 3)
+    refuse(PyExc_ValueError, "weights must be [experts, in, out] (got shape ", shape_of(weights), ")");
+  return PyBool_FromLong(in_contiguous(weights));
+}
+
 // cached_lens, new_lens, block_tables, block_size, num_tokens, free_blocks, num_free, separate
 PyObject* page_plan(PyObject* const* p) {
   const at::Tensor &cached = tensor(p[0], "cached_lens"), &fresh = tensor(p[1], "new_lens"),
@@ -479,7 +584,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {ENTRY(route, 9),   ENTRY(route_backward, 7), ENTRY(plan_dispatch, 4),
                           ENTRY(dispatch, 3), ENTRY(combine, 5),       ENTRY(combine_backward, 5),
-                          ENTRY(page_plan, 8), {nullptr, nullptr, 0, nullptr}};
+                          ENTRY(expert_products, 6), ENTRY(expert_products_grad_weights, 5),
+                          ENTRY(weights_in_contiguous, 1), ENTRY(page_plan, 8), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_cusort_torch", nullptr, -1, kMethods};
 

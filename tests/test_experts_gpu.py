@@ -1,0 +1,183 @@
+"""The experts' products and their gradients against a plain implementation in 64 bits."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from libcusort_b200 import experts as X  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    assert X.product_status() == 0
+
+
+def plan(counts, align=1, tail=0):
+    """counts, offsets, capacity and which rows belong to an expert."""
+    offsets, at = [0], 0
+    for c in counts:
+        at += -(-c // align) * align
+        offsets.append(at)
+    there = torch.zeros(at + tail, dtype=torch.bool, device="cuda")
+    for o, c in zip(offsets, counts):
+        there[o:o + c] = True
+    return (torch.tensor(counts, dtype=torch.int32, device="cuda"),
+            torch.tensor(offsets, dtype=torch.int32, device="cuda"), at + tail, there)
+
+
+def matrix(rows, width, dtype, there=None, pitch=None, shift=0, seed=0):
+    """Random rows, NaN and infinities where ``there`` is false; rows `pitch` elements apart, `shift` behind a start."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    pitch = pitch or width
+    x = torch.randn(rows * pitch + shift + 8, generator=gen, device="cuda").to(dtype)[shift:].as_strided(
+        (rows, width), (pitch, 1))
+    if there is not None:
+        x[~there] = torch.tensor([float("nan"), float("inf")], device="cuda").repeat(width)[:width].to(dtype)
+    return x
+
+
+def weights_of(experts, fin, fout, dtype, order, seed=1):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    shape = (experts, fin, fout) if order == "in_out" else (experts, fout, fin)
+    w = torch.randn(*shape, generator=gen, device="cuda").to(dtype)
+    return w if order == "in_out" else w.transpose(1, 2)
+
+
+def close(got, want, size, depth):
+    """One rounding of the result (half a step: eps / 2 of it, and half the smallest subnormal), and `depth` 32-bit
+    additions, each off by a step (2^-23) of at most the sum of all products' sizes."""
+    info = torch.finfo(got.dtype)
+    tiny = 2.0 ** -25 if got.dtype == torch.float16 else 2.0 ** -134
+    bound = info.eps / 2 * want.abs() + (1 + info.eps) * depth * 2.0 ** -23 * size + tiny
+    bad = ~((got.double() - want).abs() <= bound)
+    assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), got[bad][:4], want[bad][:4])
+
+
+def check(counts, fin, fout, dtype="bf16", order="in_out", align=1, tail=0, pitch=None, shift=0, grad_pitch=None):
+    dtype = TYPES[dtype]
+    c, o, capacity, there = plan(counts, align, tail)
+    x = matrix(capacity, fin, dtype, there, pitch, shift)
+    g = matrix(capacity, fout, dtype, there, grad_pitch, seed=2)
+    w = weights_of(len(counts), fin, fout, dtype, order)
+    out = X.expert_products(x, w, c, o)
+    grad_rows, grad_weights = X.expert_products_backward(g, x, w, c, o)
+    assert out.shape == (capacity, fout) and out.dtype == dtype and out.is_contiguous()
+    assert grad_rows.shape == x.shape and grad_weights.shape == w.shape
+    assert grad_weights.stride() == w.stride() or min(fin, fout) == 1
+    assert not out[~there].any() and not grad_rows[~there].any()
+    for e, (first, count) in enumerate(zip(o.tolist(), counts)):
+        at = slice(first, first + count)
+        xe, ge, we = x[at].double(), g[at].double(), w[e].double()
+        close(out[at], xe @ we, xe.abs() @ we.abs(), fin)
+        close(grad_rows[at], ge @ we.T, ge.abs() @ we.T.abs(), fout)
+        close(grad_weights[e], xe.T @ ge, xe.T.abs() @ ge.abs(), max(count, 1))
+
+
+@pytest.mark.parametrize("order", ["in_out", "out_in"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("fin,fout", [(64, 128), (128, 64), (72, 200), (8, 8), (512, 264), (200, 1032)])
+def test_few_rows_an_expert(fin, fout, dtype, order):
+    check([0, 1, 3, 0, 16, 17, 33, 64, 0, 40], fin, fout, dtype, order)
+
+
+@pytest.mark.parametrize("order", ["in_out", "out_in"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("fin,fout", [(64, 128), (264, 136), (136, 520)])
+def test_many_rows_an_expert(fin, fout, dtype, order):
+    check([0, 255, 1, 256, 257, 0, 300, 1000, 63, 65], fin, fout, dtype, order)
+
+
+@pytest.mark.parametrize("align,tail", [(16, 0), (128, 70), (7, 1000), (1, 333)])
+@pytest.mark.parametrize("fin,fout", [(64, 136), (40, 33)])
+def test_rows_of_no_segment_are_zeros_and_not_read(fin, fout, align, tail):
+    check([5, 0, 128, 130, 0, 1, 0], fin, fout, "bf16", align=align, tail=tail)
+
+
+@pytest.mark.parametrize("order", ["in_out", "out_in"])
+@pytest.mark.parametrize("fin,fout", [(1, 1), (7, 5), (1, 64), (64, 1), (33, 130), (771, 257), (66, 72), (72, 66)])
+def test_widths_of_no_16_bytes(fin, fout, order):
+    check([3, 0, 70, 1, 20], fin, fout, "f16", order)
+
+
+@pytest.mark.parametrize("pitch,shift,grad_pitch", [(80, 0, 72), (72, 4, 64), (65, 0, 67), (64, 8, 64), (64, 1, 71)])
+def test_rows_apart_and_off_16_bytes(pitch, shift, grad_pitch):
+    check([9, 130, 0, 31], 64, 64, "bf16", pitch=pitch, shift=shift, grad_pitch=grad_pitch)
+
+
+def test_one_expert_and_the_most():
+    check([700], 136, 72)
+    check([1], 64, 64)
+    check([i % 3 for i in range(1024)], 64, 72)
+
+
+def test_nothing_to_do():
+    check([0, 0, 0], 64, 72)
+    check([0, 0, 0], 64, 72, tail=50)
+    check([0], 33, 5, "f16")
+
+
+def test_expanded_rows_and_weights():
+    c, o, capacity, _ = plan([3, 5])
+    x = matrix(1, 64, torch.bfloat16).expand(capacity, 64)
+    w = weights_of(1, 64, 72, torch.bfloat16, "in_out").expand(2, 64, 72)
+    close(X.expert_products(x, w, c, o), x.double() @ w[0].double(), x.double().abs() @ w[0].double().abs(), 64)
+
+
+def test_weights_apart():
+    c, o, capacity, _ = plan([30, 70])
+    whole = weights_of(2, 80, 96, torch.bfloat16, "in_out")
+    for w in (whole[:, :64, :72], whole[:, 3:67, 8:80], whole[:, :64, 1:73], whole.transpose(1, 2)[:, :64, 5:77]):
+        x = matrix(capacity, 64, torch.bfloat16)
+        out = X.expert_products(x, w, c, o)
+        for e, at in enumerate((slice(0, 30), slice(30, 100))):
+            close(out[at], x[at].double() @ w[e].double(), x[at].double().abs() @ w[e].double().abs(), 64)
+
+
+def test_infinities_and_nan_stay_in_their_rows():
+    c, o, capacity, _ = plan([40, 40])
+    x = matrix(capacity, 128, torch.bfloat16)
+    w = weights_of(2, 128, 128, torch.bfloat16, "in_out")
+    clean = X.expert_products(x, w, c, o)
+    x[7, 3], x[50, 100], x[39, 0] = float("nan"), float("inf"), float("-inf")
+    out = X.expert_products(x, w, c, o)
+    hit = torch.zeros(capacity, dtype=torch.bool, device="cuda")
+    hit[[7, 39, 50]] = True
+    assert torch.equal(out[~hit], clean[~hit]) and not torch.isfinite(out[hit]).any()
+
+
+def test_overflow_of_the_type():
+    c, o, _, _ = plan([2])
+    x = torch.full((2, 64), 200.0, device="cuda", dtype=torch.float16)
+    w = torch.full((1, 64, 8), 200.0, device="cuda", dtype=torch.float16)
+    assert torch.isposinf(X.expert_products(x, w, c, o)).all()
+
+
+def test_same_result_again_and_on_another_stream():
+    c, o, capacity, _ = plan([100, 0, 333, 7], 16)
+    x, w, g = matrix(capacity, 264, torch.bfloat16), weights_of(4, 264, 520, torch.bfloat16, "in_out"), None
+    g = matrix(capacity, 520, torch.bfloat16, seed=3)
+    first = (X.expert_products(x, w, c, o), *X.expert_products_backward(g, x, w, c, o))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        again = (X.expert_products(x, w, c, o), *X.expert_products_backward(g, x, w, c, o))
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_segments_that_are_no_plan_stay_inside():
+    """Counts and offsets beyond the rows are cut there; nothing outside the tensors is touched."""
+    x = matrix(40, 64, torch.bfloat16)
+    w = weights_of(3, 64, 72, torch.bfloat16, "in_out")
+    c = torch.tensor([10, 1 << 30, -5], dtype=torch.int32, device="cuda")
+    o = torch.tensor([0, 10, 1 << 30, 2000], dtype=torch.int32, device="cuda")
+    out = X.expert_products(x, w, c, o)
+    close(out[10:], x[10:].double() @ w[1].double(), x[10:].double().abs() @ w[1].double().abs(), 64)
+    grad = X.expert_products_grad_weights(matrix(40, 72, torch.bfloat16, seed=5), x, c, o)
+    assert torch.isfinite(grad).all() and not grad[2].any()
