@@ -53,7 +53,7 @@ constexpr int kMaxExperts = 1024;
 constexpr int kThreads = 256;  // warp 0 brings tiles, 1 multiplies, 2 and 3 clear rows, 4 to 7 store
 constexpr int kSms = 148;
 constexpr int kBlockK = 64;              // contracted elements to a stage: one swizzle row
-constexpr int kTileM = 128;              // lanes of tensor memory
+constexpr int kTileM = 128;              // lanes of a CTA's tensor memory
 constexpr uint32_t kBytesA = kTileM * kBlockK * 2;
 constexpr uint32_t kAll = 0xffffffffu;
 
@@ -130,35 +130,46 @@ __device__ __forceinline__ int find(const int32_t* tiles, int experts, int t) {
   return low;
 }
 
-// Barriers and flags of one CTA.
-template <int STAGES> struct Pipe {
-  uint64_t full[STAGES], empty[STAGES], sum_full[2], sum_empty[2];
+// Barriers and flags of one CTA.  PAIR: two CTAs work on one tile, each with
+// half of either operand; the first one multiplies.
+template <int STAGES, bool PAIR> struct Pipe {
+  uint64_t full[STAGES];   // a stage's copies are there; those of both CTAs count on the first one's barrier
+  uint64_t empty[STAGES];  // a stage was multiplied
+  uint64_t end[STAGES];    // in the first of two CTAs: the other's end of a segment is ready
+  uint64_t sum_full[2], sum_empty[2];
   uint32_t tmem, gave_up, sums[8];
 };
 
-template <int STAGES>
-__device__ __forceinline__ void init_pipe(Pipe<STAGES>& p, uint32_t columns) {
+template <int STAGES, bool PAIR>
+__device__ __forceinline__ void init_pipe(Pipe<STAGES, PAIR>& p, uint32_t columns) {
   if (threadIdx.x == 0) {
-    for (int i = 0; i < STAGES; ++i) dev::mbar_init(&p.full[i], 1), dev::mbar_init(&p.empty[i], 1);
-    for (int i = 0; i < 2; ++i) dev::mbar_init(&p.sum_full[i], 1), dev::mbar_init(&p.sum_empty[i], 4);
+    for (int i = 0; i < STAGES; ++i) {
+      dev::mbar_init(&p.full[i], 1);
+      dev::mbar_init(&p.empty[i], 1);
+      dev::mbar_init(&p.end[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) dev::mbar_init(&p.sum_full[i], 1), dev::mbar_init(&p.sum_empty[i], PAIR ? 8 : 4);
     p.gave_up = 0;
     dev::fence_mbar_init();
   }
-  if (threadIdx.x / 32 == 1) dev::tmem_alloc(&p.tmem, columns);
+  __syncwarp();
+  if (threadIdx.x / 32 == 1) dev::tmem_alloc<PAIR>(&p.tmem, columns);
   dev::tmem_fence_before();
-  __syncthreads();
+  if (PAIR) dev::cluster_sync();
+  else __syncthreads();
   dev::tmem_fence_after();
 }
 
 // The end of every warp's work: tensor memory is given back.
-template <int STAGES>
-__device__ __forceinline__ void close_pipe(Pipe<STAGES>& p, uint32_t columns) {
+template <int STAGES, bool PAIR>
+__device__ __forceinline__ void close_pipe(Pipe<STAGES, PAIR>& p, uint32_t columns) {
   dev::tmem_fence_before();
-  __syncthreads();
+  if (PAIR) dev::cluster_sync();
+  else __syncthreads();
   if (threadIdx.x == 0 && p.gave_up) atomicOr(&g_product_status, 1u);
   if (threadIdx.x / 32 == 1) {
     dev::tmem_fence_after();
-    dev::tmem_free(p.tmem, columns);
+    dev::tmem_free<PAIR>(p.tmem, columns);
   }
 }
 
@@ -171,22 +182,27 @@ template <int STAGES> struct Ring {
   }
 };
 
-// After a wait ran out: no copy of this CTA is left in flight.  `issued`
-// stages were filled, the last one before ring's place.
-template <int STAGES>
-__device__ __forceinline__ void drain(Pipe<STAGES>& p, Ring<STAGES> ring, int64_t issued, uint64_t limit_ns) {
-  const int64_t last = issued < STAGES ? issued : STAGES;
-  for (int64_t i = 0; i < last; ++i) {
-    if (ring.stage == 0) ring.stage = STAGES, ring.parity ^= 1;
-    --ring.stage;
-    dev::mbar_wait(&p.full[ring.stage], ring.parity, nullptr, limit_ns);
-  }
+// After a wait ran out: copies in flight, which take microseconds, are given a
+// millisecond before the CTA ends.
+__device__ __forceinline__ void settle() {
+  const uint64_t t0 = dev::globaltimer_ns();
+  while (dev::globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
 }
 
-// A wait of a whole warp, whose lanes go on alike.
-template <int STAGES>
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Pipe<STAGES>& p, uint64_t limit_ns) {
-  return __all_sync(kAll, dev::mbar_wait(bar, parity, &p.gave_up, limit_ns));
+// A wait of a whole warp.  One lane asks: 32 of them keep shared memory busy, which the copies and products need (a
+// third of the products' rate was lost to the storing warps' waits).
+template <bool CLUSTER = false, int STAGES, bool PAIR>
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Pipe<STAGES, PAIR>& p, uint64_t limit_ns) {
+  bool ok = true;
+  if ((threadIdx.x & 31) == 0) ok = dev::mbar_wait<CLUSTER>(bar, parity, &p.gave_up, limit_ns);
+  return __shfl_sync(kAll, ok, 0);
+}
+
+// The storing warps have read a sum: one lane says so.
+template <int STAGES, bool PAIR>
+__device__ __forceinline__ void release_sum(Pipe<STAGES, PAIR>& p, int sum) {
+  if (PAIR) dev::mbar_arrive_first(&p.sum_empty[sum]);
+  else dev::mbar_arrive(&p.sum_empty[sum]);
 }
 
 __device__ __forceinline__ uint32_t align_up(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
@@ -214,13 +230,17 @@ struct ProductArgs {
   uint64_t limit_ns;  // bound on every wait
 };
 
-template <int BN, int STAGES> struct ProductShape {
-  static constexpr uint32_t kBytesB = BN * kBlockK * 2, kStage = kBytesA + kBytesB;
-  static constexpr int kBoxRows = BN / 4;  // a tile of few rows brings few boxes
+// PAIR: tiles of 256 columns of the result, 128 in each of two CTAs, and half of the rows in each.
+template <int BN, int STAGES, bool PAIR> struct ProductShape {
+  static constexpr int kCtas = PAIR ? 2 : 1, kTile = kTileM * kCtas;
+  static constexpr int kRowStep = 16 * kCtas;       // the instruction's width comes in such steps
+  static constexpr int kBoxRows = BN / kCtas / 4;   // a tile of few rows brings few boxes
+  static constexpr uint32_t kBytesB = BN / kCtas * kBlockK * 2, kStage = kBytesA + kBytesB;
+  static constexpr uint32_t kBoxBytes = kBoxRows * dev::kBoxRowBytes;
   static constexpr uint32_t kColumns = 2 * BN;
   static constexpr uint32_t kStaging = 4 * 2048;  // 32 x 32 16-bit elements for each storing warp
   static size_t bytes(int experts) {
-    return 1024 + STAGES * kStage + kStaging + sizeof(Pipe<STAGES>) + 4 * (3 * (size_t)experts + 1);
+    return 1024 + STAGES * kStage + kStaging + sizeof(Pipe<STAGES, PAIR>) + 4 * (3 * (size_t)experts + 1);
   }
 };
 
@@ -228,32 +248,33 @@ struct ProductTile {
   int expert, row, rows, column;  // first row and number of rows; first column of the result
 };
 
-template <int BN>
+template <typename Shape>
 __device__ __forceinline__ ProductTile product_tile(const ProductArgs& a, const Segments& s, uint32_t t) {
   ProductTile p;
   p.expert = find(s.tiles, a.segments.experts, t / a.width_tiles);
   const uint32_t before = s.tiles[p.expert], tiles = s.tiles[p.expert + 1] - before;
   const uint32_t local = t - before * a.width_tiles, count = s.count[p.expert];
   // the rows in equal tiles, whole steps of the instruction's width
-  const uint32_t per = align_up((count + tiles - 1) / tiles, 16), tile = local % tiles;
+  const uint32_t per = align_up((count + tiles - 1) / tiles, Shape::kRowStep), tile = local % tiles;
   p.row = s.first[p.expert] + tile * per;
   p.rows = min(per, count - tile * per);
-  p.column = local / tiles * kTileM;
+  p.column = local / tiles * Shape::kTile;
   return p;
 }
 
-// out^T = weights^T x rows^T by tiles of 128 of the result's columns (the
-// lanes of tensor memory) and up to BN rows of one segment.  So the
-// instruction's width is the number of rows, in steps of 16: an expert with
-// three rows costs a width of 16, and its weights stream through the 128
+// out^T = weights^T x rows^T by tiles of 128 (PAIR: 256) of the result's
+// columns (the lanes of tensor memory) and up to BN rows of one segment.  So
+// the instruction's width is the number of rows, in steps of 16: an expert
+// with three rows costs a width of 16, and its weights stream through the
 // lanes.
-template <typename T, int BN, int STAGES, bool IN_ORDER>
-__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
-  using Shape = ProductShape<BN, STAGES>;
+template <typename T, int BN, int STAGES, bool PAIR, bool IN_ORDER>
+__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads, 1)
+    product_kernel(const __grid_constant__ ProductArgs a) {
+  using Shape = ProductShape<BN, STAGES, PAIR>;
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (align_up(dev::smem_u32(raw), 1024) - dev::smem_u32(raw));
   uint8_t* staging = base + STAGES * Shape::kStage;
-  Pipe<STAGES>& p = *reinterpret_cast<Pipe<STAGES>*>(staging + Shape::kStaging);
+  Pipe<STAGES, PAIR>& p = *reinterpret_cast<Pipe<STAGES, PAIR>*>(staging + Shape::kStaging);
   const int experts = a.segments.experts;
   Segments s;
   s.first = reinterpret_cast<int32_t*>(&p + 1);
@@ -265,49 +286,53 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   load_segments(a.segments, s, p.sums, [](int count) { return (count + BN - 1) / BN; });
   const uint32_t tiles = (uint32_t)s.tiles[experts] * a.width_tiles;
   const int steps = (a.in + kBlockK - 1) / kBlockK;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = PAIR ? dev::cluster_rank() : 0;
+  const uint32_t t0 = blockIdx.x / Shape::kCtas, t_step = gridDim.x / Shape::kCtas;
   const uint32_t stages = dev::smem_u32(base);
 
   if (warp == 0) {
     if (lane == 0) {
       Ring<STAGES> ring;
-      int64_t issued = 0;
       bool ok = true;
-      for (uint32_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-        const ProductTile tile = product_tile<BN>(a, s, t);
-        const int boxes = (tile.rows + Shape::kBoxRows - 1) / Shape::kBoxRows;
+      for (uint32_t t = t0; ok && t < tiles; t += t_step) {
+        const ProductTile tile = product_tile<Shape>(a, s, t);
+        const int column = tile.column + rank * kTileM;
+        const int mine = align_up(tile.rows, Shape::kRowStep) / Shape::kCtas, row = tile.row + rank * mine;
+        const int boxes = (mine + Shape::kBoxRows - 1) / Shape::kBoxRows;
         for (int k = 0; k < steps; ++k) {
           if (!dev::mbar_wait(&p.empty[ring.stage], ring.parity ^ 1, &p.gave_up, a.limit_ns)) {
             ok = false;
             break;
           }
-          const uint32_t bar = dev::smem_u32(&p.full[ring.stage]), at = stages + ring.stage * Shape::kStage;
-          dev::mbar_arrive_expect_tx(&p.full[ring.stage], kBytesA + boxes * Shape::kBoxRows * dev::kBoxRowBytes);
+          const uint32_t at = stages + ring.stage * Shape::kStage;
+          const uint32_t own = dev::smem_u32(&p.full[ring.stage]), bar = PAIR ? dev::in_first(own) : own;
+          // the first CTA's barrier counts the copies of both
+          if (rank == 0)
+            dev::mbar_arrive_expect_tx(&p.full[ring.stage], Shape::kCtas * (kBytesA + boxes * Shape::kBoxBytes));
           if (IN_ORDER) {
-            dev::tma_load_3d(at, &a.weights, bar, k * kBlockK, tile.column, tile.expert);
+            dev::tma_load_3d<PAIR>(at, &a.weights, bar, k * kBlockK, column, tile.expert);
           } else {
-            dev::tma_load_3d(at, &a.weights, bar, tile.column, k * kBlockK, tile.expert);
-            dev::tma_load_3d(at + kBytesA / 2, &a.weights, bar, tile.column + kBlockK, k * kBlockK, tile.expert);
+            dev::tma_load_3d<PAIR>(at, &a.weights, bar, column, k * kBlockK, tile.expert);
+            dev::tma_load_3d<PAIR>(at + kBytesA / 2, &a.weights, bar, column + kBlockK, k * kBlockK, tile.expert);
           }
           for (int b = 0; b < boxes; ++b)
-            dev::tma_load_2d(at + kBytesA + b * Shape::kBoxRows * dev::kBoxRowBytes, &a.rows, bar, k * kBlockK,
-                             tile.row + b * Shape::kBoxRows);
+            dev::tma_load_2d<PAIR>(at + kBytesA + b * Shape::kBoxBytes, &a.rows, bar, k * kBlockK,
+                                   row + b * Shape::kBoxRows);
           ring.next();
-          ++issued;
         }
       }
-      if (!ok) drain(p, ring, issued, a.limit_ns);
+      if (!ok) settle();
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 && rank == 0) {
     if (lane == 0) {
       Ring<STAGES> ring;
       Ring<2> sums;
       bool ok = true;
-      for (uint32_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-        const ProductTile tile = product_tile<BN>(a, s, t);
-        const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, !IN_ORDER, false, kTileM,
-                                                          align_up(tile.rows, 16));
-        if (!dev::mbar_wait(&p.sum_empty[sums.stage], sums.parity ^ 1, &p.gave_up, a.limit_ns)) break;
+      for (uint32_t t = t0; ok && t < tiles; t += t_step) {
+        const ProductTile tile = product_tile<Shape>(a, s, t);
+        const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, !IN_ORDER, false,
+                                                          Shape::kTile, align_up(tile.rows, Shape::kRowStep));
+        if (!dev::mbar_wait<PAIR>(&p.sum_empty[sums.stage], sums.parity ^ 1, &p.gave_up, a.limit_ns)) break;
         dev::tmem_fence_after();
         const uint32_t sum = p.tmem + sums.stage * BN;
         for (int k = 0; k < steps; ++k) {
@@ -321,15 +346,15 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           const uint64_t db = dev::operand_descriptor(at + kBytesA, 16, 1024);
 #pragma unroll
           for (int i = 0; i < kBlockK / 16; ++i)
-            dev::mma_issue(sum, da + i * (IN_ORDER ? 32 : 2048) / 16, db + i * 32 / 16, instruction, k + i > 0);
-          dev::mma_commit(dev::smem_u32(&p.empty[ring.stage]));
+            dev::mma_issue<PAIR>(sum, da + i * (IN_ORDER ? 32 : 2048) / 16, db + i * 32 / 16, instruction, k + i > 0);
+          dev::mma_commit<PAIR>(&p.empty[ring.stage]);
           ring.next();
         }
-        dev::mma_commit(dev::smem_u32(&p.sum_full[sums.stage]));
+        dev::mma_commit<PAIR>(&p.sum_full[sums.stage]);
         sums.next();
       }
     }
-  } else if (warp < 4) {
+  } else if (warp == 2 || warp == 3) {
     // rows that hold no pair: those between the segments by the expert before, those behind the last in equal parts
     uint16_t* out = static_cast<uint16_t*>(a.out);
     const int thread = threadIdx.x - 64;
@@ -342,18 +367,18 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     const int per = (left + gridDim.x - 1) / gridDim.x;
     const int64_t r0 = end + (int64_t)min((int64_t)left, (int64_t)blockIdx.x * per);
     clear(out, r0 * a.width, min(r0 + per, (int64_t)a.segments.capacity) * a.width, thread, 64);
-  } else {
+  } else if (warp >= 4) {
     // the sums to 16 bits, through shared memory from a column of the result to a lane to a row's piece to a lane
     Ring<2> sums;
     const int quarter = warp & 3;
     uint8_t* mine = staging + quarter * 2048;
     T* out = static_cast<T*>(a.out);
     const bool whole = a.width % 8 == 0;  // the result's first byte lies on a 16-byte boundary
-    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-      const ProductTile tile = product_tile<BN>(a, s, t);
+    for (uint32_t t = t0; t < tiles; t += t_step) {
+      const ProductTile tile = product_tile<Shape>(a, s, t);
       if (!warp_wait(&p.sum_full[sums.stage], sums.parity, p, a.limit_ns)) break;
       dev::tmem_fence_after();
-      const int column = tile.column + quarter * 32;
+      const int column = tile.column + rank * kTileM + quarter * 32;
       for (int c = 0; c < tile.rows; c += 32) {
         uint32_t v[32];
         dev::tmem_load32(p.tmem + sums.stage * BN + c + ((uint32_t)quarter << 21), v);
@@ -384,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       }
       dev::tmem_fence_before();
       __syncwarp();
-      if (lane == 0) dev::mbar_arrive(&p.sum_empty[sums.stage]);
+      if (lane == 0) release_sum(p, sums.stage);
       sums.next();
     }
   }
@@ -403,104 +428,132 @@ struct GradArgs {
 };
 
 constexpr int kGradN = 256;
-constexpr int kGradStages = 4;
-constexpr uint32_t kGradStage = kBytesA + kGradN * kBlockK * 2;
+constexpr int kGradStages = 6;
+constexpr uint32_t kGradStage = kBytesA + kGradN / 2 * kBlockK * 2;
 constexpr uint32_t kGradPitch = 80;  // bytes between the staged rows of 64: 8 lanes' 16-byte pieces fall on all banks
 constexpr uint32_t kGradStaging = 4 * 32 * kGradPitch;
+constexpr int kChunkBytes = kBytesA / 2;  // 64 contracted rows of 64 elements
 
-size_t grad_bytes(int experts) {
-  return 1024 + kGradStages * kGradStage + kGradStaging + sizeof(Pipe<kGradStages>) + 4 * (3 * (size_t)experts + 1);
+size_t grad_bytes() {
+  return 1024 + kGradStages * kGradStage + kGradStaging + sizeof(Pipe<kGradStages, true>);
 }
+
+struct GradTile {
+  int expert, slow, fast, chunks;  // first elements; 64-element chunks of the contiguous dimension in each of the CTAs
+  int2 segment;
+};
+
+__device__ __forceinline__ GradTile grad_tile(const GradArgs& a, uint32_t t) {
+  const uint32_t per_expert = (uint32_t)a.slow_tiles * a.fast_tiles, local = t % per_expert;
+  GradTile g;
+  g.expert = t / per_expert;
+  g.slow = local % a.slow_tiles * (2 * kTileM);
+  g.fast = local / a.slow_tiles * kGradN;
+  g.chunks = min(kGradN / 2, (a.fast_width - g.fast + 1) / 2 + kBlockK - 1) / kBlockK;
+  g.segment = segment(a.segments, g.expert);
+  return g;
+}
+
+// Whether the step from row k of a segment on ends inside one of the instruction's 16 contracted rows.
+__device__ __forceinline__ bool has_end(int count, int k) { return count - k < kBlockK && count % 16 != 0; }
 
 // gradient[e] = slow_e^T x fast_e, contracted over the rows of e's segment: both operands lie with the contracted
 // dimension across.  Rows behind the segment's end that the last step brings along are cleared in shared memory: they
 // are another expert's, or anything at all.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) grad_weights_kernel(const __grid_constant__ GradArgs a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    grad_weights_kernel(const __grid_constant__ GradArgs a) {
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (align_up(dev::smem_u32(raw), 1024) - dev::smem_u32(raw));
   uint8_t* staging = base + kGradStages * kGradStage;
-  Pipe<kGradStages>& p = *reinterpret_cast<Pipe<kGradStages>*>(staging + kGradStaging);
-  const int experts = a.segments.experts;
+  Pipe<kGradStages, true>& p = *reinterpret_cast<Pipe<kGradStages, true>*>(staging + kGradStaging);
 
   init_pipe(p, 512);
   dev::wait_for_previous();
-  const uint32_t per_expert = (uint32_t)a.slow_tiles * a.fast_tiles, tiles = per_expert * experts;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t tiles = (uint32_t)a.slow_tiles * a.fast_tiles * a.segments.experts;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = dev::cluster_rank();
+  const uint32_t t0 = blockIdx.x / 2, t_step = gridDim.x / 2;
   const uint32_t stages = dev::smem_u32(base);
-  constexpr int kChunks = kGradN / kBlockK;
 
   if (warp == 0) {
     if (lane == 0) {
       Ring<kGradStages> ring;
-      int64_t issued = 0;
       bool ok = true;
-      for (uint32_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-        const uint32_t local = t % per_expert;
-        const int2 seg = segment(a.segments, t / per_expert);
-        const int m = local % a.slow_tiles * kTileM, n = local / a.slow_tiles * kGradN;
-        const int chunks = min(kChunks, (a.fast_width - n + kBlockK - 1) / kBlockK);
-        for (int k = 0; k < seg.y; k += kBlockK) {
+      for (uint32_t t = t0; ok && t < tiles; t += t_step) {
+        const GradTile g = grad_tile(a, t);
+        const int slow = g.slow + rank * kTileM, fast = g.fast + rank * g.chunks * kBlockK;
+        for (int k = 0; k < g.segment.y; k += kBlockK) {
           if (!dev::mbar_wait(&p.empty[ring.stage], ring.parity ^ 1, &p.gave_up, a.limit_ns)) {
             ok = false;
             break;
           }
-          const uint32_t bar = dev::smem_u32(&p.full[ring.stage]), at = stages + ring.stage * kGradStage;
-          dev::mbar_arrive_expect_tx(&p.full[ring.stage], kBytesA + chunks * (kBytesA / 2));
-          dev::tma_load_2d(at, &a.slow, bar, m, seg.x + k);
-          dev::tma_load_2d(at + kBytesA / 2, &a.slow, bar, m + kBlockK, seg.x + k);
-          for (int c = 0; c < chunks; ++c)
-            dev::tma_load_2d(at + kBytesA + c * (kBytesA / 2), &a.fast, bar, n + c * kBlockK, seg.x + k);
+          const uint32_t at = stages + ring.stage * kGradStage, bytes = (2 + g.chunks) * kChunkBytes;
+          const uint32_t own = dev::smem_u32(&p.full[ring.stage]);
+          const int row = g.segment.x + k;
+          // copies that the other CTA has to clear the end of count on its own barrier
+          const bool end = has_end(g.segment.y, k);
+          if (rank == 0) dev::mbar_arrive_expect_tx(&p.full[ring.stage], end ? bytes : 2 * bytes);
+          else if (end) dev::mbar_arrive_expect_tx(&p.full[ring.stage], bytes);
+          const uint32_t bar = end ? own : dev::in_first(own);
+          dev::tma_load_2d<true>(at, &a.slow, bar, slow, row);
+          dev::tma_load_2d<true>(at + kChunkBytes, &a.slow, bar, slow + kBlockK, row);
+          for (int c = 0; c < g.chunks; ++c)
+            dev::tma_load_2d<true>(at + kBytesA + c * kChunkBytes, &a.fast, bar, fast + c * kBlockK, row);
           ring.next();
-          ++issued;
         }
       }
-      if (!ok) drain(p, ring, issued, a.limit_ns);
+      if (!ok) settle();
     }
   } else if (warp == 1) {
+    // the first CTA multiplies; both look after the ends of segments in their own copies
     Ring<kGradStages> ring;
     Ring<2> sums;
+    uint32_t ends = 0;  // a bit for each stage: parity of its barrier of ends, or the other CTA's own barrier
     bool ok = true;
-    for (uint32_t t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
-      const uint32_t local = t % per_expert;
-      const int count = segment(a.segments, t / per_expert).y;
+    for (uint32_t t = t0; ok && t < tiles; t += t_step) {
+      const GradTile g = grad_tile(a, t);
+      const int count = g.segment.y;
       if (count == 0) continue;
-      const int n = local / a.slow_tiles * kGradN;
-      const int chunks = min(kChunks, (a.fast_width - n + kBlockK - 1) / kBlockK);
-      const uint32_t instruction =
-          dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, true, true, kTileM, chunks * kBlockK);
-      if (!warp_wait(&p.sum_empty[sums.stage], sums.parity ^ 1, p, a.limit_ns)) break;
-      dev::tmem_fence_after();
+      const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, true, true, 2 * kTileM,
+                                                        2 * g.chunks * kBlockK);
+      if (rank == 0) {
+        if (!warp_wait<true>(&p.sum_empty[sums.stage], sums.parity ^ 1, p, a.limit_ns)) break;
+        dev::tmem_fence_after();
+      }
       const uint32_t sum = p.tmem + sums.stage * kGradN;
       for (int k = 0; k < count; k += kBlockK) {
-        if (!warp_wait(&p.full[ring.stage], ring.parity, p, a.limit_ns)) {
-          ok = false;
-          break;
-        }
-        const int valid = min(kBlockK, count - k), depth = (valid + 15) / 16;
-        if (valid < depth * 16) {
-          const int pieces = (depth * 16 - valid) * 8 * (2 + chunks);  // 16 bytes each
-          for (int i = lane; i < pieces; i += 32) {
-            const int column = i / ((depth * 16 - valid) * 8), within = i % ((depth * 16 - valid) * 8);
-            *reinterpret_cast<uint4*>(base + ring.stage * kGradStage + column * (kBytesA / 2) + valid * 128 +
-                                      within * 16) = make_uint4(0, 0, 0, 0);
-          }
+        const bool end = has_end(count, k);
+        if (rank == 0) ok = warp_wait(&p.full[ring.stage], ring.parity, p, a.limit_ns);
+        else if (end) ok = warp_wait(&p.full[ring.stage], ends >> ring.stage & 1, p, a.limit_ns);
+        if (!ok) break;
+        const int valid = min(kBlockK, count - k), depth = (valid + 15) / 16, rest = depth * 16 - valid;
+        if (end) {
+          for (int i = lane; i < rest * 8 * (2 + g.chunks); i += 32)  // 16 bytes each
+            *reinterpret_cast<uint4*>(base + ring.stage * kGradStage + i / (rest * 8) * kChunkBytes +
+                                      valid * dev::kBoxRowBytes + i % (rest * 8) * 16) = make_uint4(0, 0, 0, 0);
           dev::fence_proxy_async_smem();
           __syncwarp();
+          if (rank != 0) {
+            if (lane == 0) dev::mbar_arrive_first(&p.end[ring.stage]);
+          } else {
+            ok = warp_wait<true>(&p.end[ring.stage], ends >> ring.stage & 1, p, a.limit_ns);
+            if (!ok) break;
+          }
+          ends ^= 1u << ring.stage;
         }
-        if (lane == 0) {
+        if (rank == 0 && lane == 0) {
           dev::tmem_fence_after();
           const uint32_t at = stages + ring.stage * kGradStage;
-          const uint64_t da = dev::operand_descriptor(at, kBytesA / 2, 1024);
-          const uint64_t db = dev::operand_descriptor(at + kBytesA, kBytesA / 2, 1024);
+          const uint64_t da = dev::operand_descriptor(at, kChunkBytes, 1024);
+          const uint64_t db = dev::operand_descriptor(at + kBytesA, kChunkBytes, 1024);
           for (int i = 0; i < depth; ++i)
-            dev::mma_issue(sum, da + i * 2048 / 16, db + i * 2048 / 16, instruction, k + i > 0);
-          dev::mma_commit(dev::smem_u32(&p.empty[ring.stage]));
+            dev::mma_issue<true>(sum, da + i * 2048 / 16, db + i * 2048 / 16, instruction, k + i > 0);
+          dev::mma_commit<true>(&p.empty[ring.stage]);
         }
         ring.next();
         __syncwarp();
       }
-      if (lane == 0) dev::mma_commit(dev::smem_u32(&p.sum_full[sums.stage]));
+      if (rank == 0 && lane == 0) dev::mma_commit<true>(&p.sum_full[sums.stage]);
       sums.next();
     }
   } else if (warp >= 4) {
@@ -508,13 +561,12 @@ __global__ void __launch_bounds__(kThreads, 1) grad_weights_kernel(const __grid_
     const int quarter = warp & 3;
     uint8_t* mine = staging + quarter * 32 * kGradPitch;
     const bool whole = a.fast_width % 8 == 0;
-    for (uint32_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-      const uint32_t local = t % per_expert;
-      const int expert = t / per_expert, m = local % a.slow_tiles * kTileM + quarter * 32,
-                n = local / a.slow_tiles * kGradN;
-      const int columns = min(kGradN, a.fast_width - n), rows = min(32, a.slow_width - m);
-      const bool empty = segment(a.segments, expert).y == 0;
-      T* out = static_cast<T*>(a.out) + ((int64_t)expert * a.slow_width + m) * a.fast_width + n;
+    for (uint32_t t = t0; t < tiles; t += t_step) {
+      const GradTile g = grad_tile(a, t);
+      const int m = g.slow + rank * kTileM + quarter * 32;
+      const int columns = min(2 * g.chunks * kBlockK, a.fast_width - g.fast), rows = min(32, a.slow_width - m);
+      const bool empty = g.segment.y == 0;
+      T* out = static_cast<T*>(a.out) + ((int64_t)g.expert * a.slow_width + m) * a.fast_width + g.fast;
       if (!empty) {
         if (!warp_wait(&p.sum_full[sums.stage], sums.parity, p, a.limit_ns)) break;
         dev::tmem_fence_after();
@@ -553,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_weights_kernel(const __grid_
       if (!empty) {
         dev::tmem_fence_before();
         __syncwarp();
-        if (lane == 0) dev::mbar_arrive(&p.sum_empty[sums.stage]);
+        if (lane == 0) release_sum(p, sums.stage);
         sums.next();
       }
     }
@@ -627,22 +679,26 @@ struct Operand {
 };
 
 template <typename Kernel, typename Args>
-cudaError_t run(Kernel kernel, const Args& a, int64_t tiles, size_t smem, cudaStream_t stream) {
+cudaError_t run(Kernel kernel, const Args& a, int64_t tiles, int ctas, size_t smem, cudaStream_t stream) {
   // the limit is the kernel's, not the call's: the same one from every host thread
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
   if (e) return e;
-  return launch_after_previous(kernel, std::max<int64_t>(1, std::min<int64_t>(kSms, tiles)), kThreads, smem, a, stream);
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(kSms / ctas, tiles)) * ctas;  // ctas to a tile
+  return launch_after_previous(kernel, grid, kThreads, smem, a, stream);
 }
 
-template <typename T, int BN, int STAGES>
-cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order, int64_t tiles, cudaStream_t stream) {
-  using Shape = ProductShape<BN, STAGES>;
+template <typename T, int BN, int STAGES, bool PAIR>
+cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order, int64_t row_tiles,
+                    cudaStream_t stream) {
+  using Shape = ProductShape<BN, STAGES, PAIR>;
+  a.width_tiles = (a.width + Shape::kTile - 1) / Shape::kTile;
   cudaError_t e = weights.map(&a.weights, false, in_order ? kTileM : kBlockK);
   if (!e) e = rows.map(&a.rows, true, Shape::kBoxRows);
   if (e) return e;
   const size_t smem = Shape::bytes(a.segments.experts);
-  return in_order ? run(product_kernel<T, BN, STAGES, true>, a, tiles, smem, stream)
-                  : run(product_kernel<T, BN, STAGES, false>, a, tiles, smem, stream);
+  const int64_t tiles = row_tiles * a.width_tiles;
+  return in_order ? run(product_kernel<T, BN, STAGES, PAIR, true>, a, tiles, Shape::kCtas, smem, stream)
+                  : run(product_kernel<T, BN, STAGES, PAIR, false>, a, tiles, Shape::kCtas, smem, stream);
 }
 
 bool half_type(int type) { return type == CUSORT_FLOAT_F16 || type == CUSORT_FLOAT_BF16; }
@@ -687,19 +743,18 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   a.out = d_out;
   a.in = (int)in;
   a.width = (int)out;
-  a.width_tiles = (int)((out + kTileM - 1) / kTileM);
   a.limit_ns = wait_limit_ns();
   // at most one part-filled tile to an expert, and no expert without a row
-  const int64_t tiles = (capacity / (few ? kFewRows : kManyRows) + std::min<int64_t>(num_experts, capacity)) * a.width_tiles;
-  if (tiles > INT32_MAX) return cudaErrorInvalidValue;
+  const int64_t tiles = capacity / (few ? kFewRows : kManyRows) + std::min<int64_t>(num_experts, capacity);
+  if (tiles * ((out + kTileM - 1) / kTileM) > INT32_MAX) return cudaErrorInvalidValue;
   uint8_t* temp = static_cast<uint8_t*>(d_temp_storage);
   cudaError_t e = rows.prepare(temp, nullptr, stream);
   if (!e) e = weights.prepare(temp, d_counts, stream);
   if (e) return e;
   const auto go = [&](auto t) {
     using T = decltype(t);
-    return few ? product<T, kFewRows, 8>(a, weights, rows, in_order, tiles, stream)
-               : product<T, kManyRows, 4>(a, weights, rows, in_order, tiles, stream);
+    return few ? product<T, kFewRows, 8, false>(a, weights, rows, in_order, tiles, stream)
+               : product<T, kManyRows, 6, true>(a, weights, rows, in_order, tiles, stream);
   };
   return type == CUSORT_FLOAT_F16 ? go(__half{}) : go(__nv_bfloat16{});
 }
@@ -730,7 +785,7 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
   a.out = d_grad_weights;
   a.slow_width = (int)slow.width;
   a.fast_width = (int)fast.width;
-  a.slow_tiles = (int)((slow.width + kTileM - 1) / kTileM);
+  a.slow_tiles = (int)((slow.width + 2 * kTileM - 1) / (2 * kTileM));
   a.fast_tiles = (int)((fast.width + kGradN - 1) / kGradN);
   a.limit_ns = wait_limit_ns();
   const int64_t tiles = (int64_t)a.slow_tiles * a.fast_tiles * num_experts;
@@ -741,8 +796,8 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
   if (!e) e = slow.map(&a.slow, true, kBlockK);
   if (!e) e = fast.map(&a.fast, true, kBlockK);
   if (e) return e;
-  return type == CUSORT_FLOAT_F16 ? run(grad_weights_kernel<__half>, a, tiles, grad_bytes(num_experts), stream)
-                                  : run(grad_weights_kernel<__nv_bfloat16>, a, tiles, grad_bytes(num_experts), stream);
+  return type == CUSORT_FLOAT_F16 ? run(grad_weights_kernel<__half>, a, tiles, 2, grad_bytes(), stream)
+                                  : run(grad_weights_kernel<__nv_bfloat16>, a, tiles, 2, grad_bytes(), stream);
 }
 
 extern "C" cudaError_t cusort_read_product_status(uint32_t* status, cudaStream_t stream) {
