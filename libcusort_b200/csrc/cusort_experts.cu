@@ -8,6 +8,8 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
+#include <utility>
 
 #include "../../include/cusort_b200.h"
 #include "cusort_dispatch.h"
@@ -50,7 +52,7 @@ namespace {
 using namespace cusort_b200;
 
 constexpr int kMaxExperts = 1024;
-constexpr int kThreads = 256;  // warp 0 brings tiles, 1 multiplies, 2 and 3 clear rows, 4 to 7 store
+constexpr int kThreads = 256;  // warps 0 and 2 bring operands, 1 multiplies, 3 clears rows, 4 to 7 store
 constexpr int kSms = 148;
 constexpr int kBlockK = 64;              // contracted elements to a stage: one swizzle row
 constexpr int kTileM = 128;              // lanes of a CTA's tensor memory
@@ -135,7 +137,8 @@ __device__ __forceinline__ int find(const int32_t* tiles, int experts, int t) {
 template <int STAGES, bool PAIR> struct Pipe {
   uint64_t full[STAGES];   // a stage's copies are there; those of both CTAs count on the first one's barrier
   uint64_t empty[STAGES];  // a stage was multiplied
-  uint64_t end[STAGES];    // in the first of two CTAs: the other's end of a segment is ready
+  uint64_t end[STAGES];    // a stage's copies of this CTA are there, which hold the end of a segment
+  uint64_t ended[STAGES];  // in the first of two CTAs: both have cleared what lies behind that
   uint64_t sum_full[2], sum_empty[2];
   uint32_t tmem, gave_up, sums[8];
 };
@@ -147,6 +150,7 @@ __device__ __forceinline__ void init_pipe(Pipe<STAGES, PAIR>& p, uint32_t column
       dev::mbar_init(&p.full[i], 1);
       dev::mbar_init(&p.empty[i], 1);
       dev::mbar_init(&p.end[i], 1);
+      dev::mbar_init(&p.ended[i], 2);
     }
     for (int i = 0; i < 2; ++i) dev::mbar_init(&p.sum_full[i], 1), dev::mbar_init(&p.sum_empty[i], PAIR ? 8 : 4);
     p.gave_up = 0;
@@ -179,6 +183,11 @@ template <int STAGES> struct Ring {
   uint32_t parity = 0;
   __device__ __forceinline__ void next() {
     if (++stage == STAGES) stage = 0, parity ^= 1;
+  }
+  __device__ __forceinline__ void skip(int n) {
+    stage += n;
+    parity ^= stage / STAGES & 1;
+    stage %= STAGES;
   }
 };
 
@@ -234,7 +243,7 @@ struct ProductArgs {
 template <int BN, int STAGES, bool PAIR> struct ProductShape {
   static constexpr int kCtas = PAIR ? 2 : 1, kTile = kTileM * kCtas;
   static constexpr int kRowStep = 16 * kCtas;       // the instruction's width comes in such steps
-  static constexpr int kBoxRows = BN / kCtas / 4;   // a tile of few rows brings few boxes
+  static constexpr int kBoxRows = PAIR ? 64 : 16;   // a tile of few rows brings few boxes
   static constexpr uint32_t kBytesB = BN / kCtas * kBlockK * 2, kStage = kBytesA + kBytesB;
   static constexpr uint32_t kBoxBytes = kBoxRows * dev::kBoxRowBytes;
   static constexpr uint32_t kColumns = 2 * BN;
@@ -290,8 +299,9 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
   const uint32_t t0 = blockIdx.x / Shape::kCtas, t_step = gridDim.x / Shape::kCtas;
   const uint32_t stages = dev::smem_u32(base);
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp == 0 || warp == 2) {
+    // one warp brings the weights, another the rows: together, one thread's issue would be what bounds the products
+    if (dev::elect_one()) {
       Ring<STAGES> ring;
       bool ok = true;
       for (uint32_t t = t0; ok && t < tiles; t += t_step) {
@@ -306,28 +316,33 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
           }
           const uint32_t at = stages + ring.stage * Shape::kStage;
           const uint32_t own = dev::smem_u32(&p.full[ring.stage]), bar = PAIR ? dev::in_first(own) : own;
-          // the first CTA's barrier counts the copies of both
-          if (rank == 0)
-            dev::mbar_arrive_expect_tx(&p.full[ring.stage], Shape::kCtas * (kBytesA + boxes * Shape::kBoxBytes));
-          if (IN_ORDER) {
-            dev::tma_load_3d<PAIR>(at, &a.weights, bar, k * kBlockK, column, tile.expert);
+          if (warp == 0) {
+            // the first CTA's barrier counts the copies of both
+            if (rank == 0)
+              dev::mbar_arrive_expect_tx(&p.full[ring.stage], Shape::kCtas * (kBytesA + boxes * Shape::kBoxBytes));
+            if (IN_ORDER) {
+              dev::tma_load_3d<PAIR>(at, &a.weights, bar, k * kBlockK, column, tile.expert);
+            } else {
+              dev::tma_load_3d<PAIR>(at, &a.weights, bar, column, k * kBlockK, tile.expert);
+              dev::tma_load_3d<PAIR>(at + kBytesA / 2, &a.weights, bar, column + kBlockK, k * kBlockK, tile.expert);
+            }
           } else {
-            dev::tma_load_3d<PAIR>(at, &a.weights, bar, column, k * kBlockK, tile.expert);
-            dev::tma_load_3d<PAIR>(at + kBytesA / 2, &a.weights, bar, column + kBlockK, k * kBlockK, tile.expert);
+            for (int b = 0; b < boxes; ++b)
+              dev::tma_load_2d<PAIR>(at + kBytesA + b * Shape::kBoxBytes, &a.rows, bar, k * kBlockK,
+                                     row + b * Shape::kBoxRows);
           }
-          for (int b = 0; b < boxes; ++b)
-            dev::tma_load_2d<PAIR>(at + kBytesA + b * Shape::kBoxBytes, &a.rows, bar, k * kBlockK,
-                                   row + b * Shape::kBoxRows);
           ring.next();
         }
       }
       if (!ok) settle();
     }
   } else if (warp == 1 && rank == 0) {
-    if (lane == 0) {
+    if (dev::elect_one()) {
       Ring<STAGES> ring;
       Ring<2> sums;
       bool ok = true;
+      const uint64_t first_a = dev::operand_descriptor(stages, IN_ORDER ? 16 : kBytesA / 2, 1024);
+      const uint64_t first_b = dev::operand_descriptor(stages + kBytesA, 16, 1024);
       for (uint32_t t = t0; ok && t < tiles; t += t_step) {
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, !IN_ORDER, false,
@@ -341,9 +356,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
             break;
           }
           dev::tmem_fence_after();
-          const uint32_t at = stages + ring.stage * Shape::kStage;
-          const uint64_t da = dev::operand_descriptor(at, IN_ORDER ? 16 : kBytesA / 2, 1024);
-          const uint64_t db = dev::operand_descriptor(at + kBytesA, 16, 1024);
+          const uint64_t da = first_a + ring.stage * (Shape::kStage / 16), db = first_b + ring.stage * (Shape::kStage / 16);
 #pragma unroll
           for (int i = 0; i < kBlockK / 16; ++i)
             dev::mma_issue<PAIR>(sum, da + i * (IN_ORDER ? 32 : 2048) / 16, db + i * 32 / 16, instruction, k + i > 0);
@@ -354,19 +367,18 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
         sums.next();
       }
     }
-  } else if (warp == 2 || warp == 3) {
+  } else if (warp == 3) {
     // rows that hold no pair: those between the segments by the expert before, those behind the last in equal parts
     uint16_t* out = static_cast<uint16_t*>(a.out);
-    const int thread = threadIdx.x - 64;
     for (int e = blockIdx.x; e < experts; e += gridDim.x) {
       const int end = s.first[e] + s.count[e];
-      if (e + 1 < experts) clear(out, (int64_t)end * a.width, (int64_t)s.first[e + 1] * a.width, thread, 64);
-      if (e == 0) clear(out, 0, (int64_t)s.first[0] * a.width, thread, 64);
+      if (e + 1 < experts) clear(out, (int64_t)end * a.width, (int64_t)s.first[e + 1] * a.width, lane, 32);
+      if (e == 0) clear(out, 0, (int64_t)s.first[0] * a.width, lane, 32);
     }
     const int end = s.first[experts - 1] + s.count[experts - 1], left = a.segments.capacity - end;
     const int per = (left + gridDim.x - 1) / gridDim.x;
     const int64_t r0 = end + (int64_t)min((int64_t)left, (int64_t)blockIdx.x * per);
-    clear(out, r0 * a.width, min(r0 + per, (int64_t)a.segments.capacity) * a.width, thread, 64);
+    clear(out, r0 * a.width, min(r0 + per, (int64_t)a.segments.capacity) * a.width, lane, 32);
   } else if (warp >= 4) {
     // the sums to 16 bits, through shared memory from a column of the result to a lane to a row's piece to a lane
     Ring<2> sums;
@@ -382,6 +394,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
       for (int c = 0; c < tile.rows; c += 32) {
         uint32_t v[32];
         dev::tmem_load32(p.tmem + sums.stage * BN + c + ((uint32_t)quarter << 21), v);
+        dev::tmem_load_wait();
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const uint32_t both = dev::from_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), T{});
@@ -420,22 +433,24 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
 // ---------------------------------------------------- the gradient of the weights
 
 struct GradArgs {
+  CUtensorMap out;         // where its rows lie on 16-byte boundaries
   CUtensorMap slow, fast;  // the rows whose width is the gradient's slower dimension, and those of the contiguous one
   SegmentArgs segments;
-  void* out;  // [experts][slow_width][fast_width]
+  void* result;  // [experts][slow_width][fast_width]
   int slow_width, fast_width, slow_tiles, fast_tiles;
   uint64_t limit_ns;
 };
 
 constexpr int kGradN = 256;
-constexpr int kGradStages = 6;
+constexpr int kGradStages = 5;
 constexpr uint32_t kGradStage = kBytesA + kGradN / 2 * kBlockK * 2;
-constexpr uint32_t kGradPitch = 80;  // bytes between the staged rows of 64: 8 lanes' 16-byte pieces fall on all banks
-constexpr uint32_t kGradStaging = 4 * 32 * kGradPitch;
+constexpr uint32_t kStoreBox = 32 * 128;             // 32 rows of 64 elements, stored as one box
+constexpr int kStoreBoxes = 3;                       // for each storing warp: one is filled, others are being stored
+constexpr uint32_t kGradStaging = 4 * kStoreBoxes * kStoreBox;
 constexpr int kChunkBytes = kBytesA / 2;  // 64 contracted rows of 64 elements
 
-size_t grad_bytes() {
-  return 1024 + kGradStages * kGradStage + kGradStaging + sizeof(Pipe<kGradStages, true>);
+size_t grad_bytes(int experts) {
+  return 1024 + kGradStages * kGradStage + kGradStaging + sizeof(Pipe<kGradStages, true>) + 8 * (size_t)experts;
 }
 
 struct GradTile {
@@ -443,14 +458,14 @@ struct GradTile {
   int2 segment;
 };
 
-__device__ __forceinline__ GradTile grad_tile(const GradArgs& a, uint32_t t) {
+__device__ __forceinline__ GradTile grad_tile(const GradArgs& a, const int2* segments, uint32_t t) {
   const uint32_t per_expert = (uint32_t)a.slow_tiles * a.fast_tiles, local = t % per_expert;
   GradTile g;
   g.expert = t / per_expert;
   g.slow = local % a.slow_tiles * (2 * kTileM);
   g.fast = local / a.slow_tiles * kGradN;
   g.chunks = min(kGradN / 2, (a.fast_width - g.fast + 1) / 2 + kBlockK - 1) / kBlockK;
-  g.segment = segment(a.segments, g.expert);
+  g.segment = segments[g.expert];
   return g;
 }
 
@@ -468,19 +483,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   uint8_t* staging = base + kGradStages * kGradStage;
   Pipe<kGradStages, true>& p = *reinterpret_cast<Pipe<kGradStages, true>*>(staging + kGradStaging);
 
+  int2* segments = reinterpret_cast<int2*>(&p + 1);
+
   init_pipe(p, 512);
   dev::wait_for_previous();
+  for (int e = threadIdx.x; e < a.segments.experts; e += kThreads) segments[e] = segment(a.segments, e);
+  __syncthreads();
   const uint32_t tiles = (uint32_t)a.slow_tiles * a.fast_tiles * a.segments.experts;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = dev::cluster_rank();
   const uint32_t t0 = blockIdx.x / 2, t_step = gridDim.x / 2;
   const uint32_t stages = dev::smem_u32(base);
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp == 0 || warp == 2) {  // an operand each
+    if (dev::elect_one()) {
       Ring<kGradStages> ring;
       bool ok = true;
       for (uint32_t t = t0; ok && t < tiles; t += t_step) {
-        const GradTile g = grad_tile(a, t);
+        const GradTile g = grad_tile(a, segments, t);
         const int slow = g.slow + rank * kTileM, fast = g.fast + rank * g.chunks * kBlockK;
         for (int k = 0; k < g.segment.y; k += kBlockK) {
           if (!dev::mbar_wait(&p.empty[ring.stage], ring.parity ^ 1, &p.gave_up, a.limit_ns)) {
@@ -488,119 +507,143 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             break;
           }
           const uint32_t at = stages + ring.stage * kGradStage, bytes = (2 + g.chunks) * kChunkBytes;
-          const uint32_t own = dev::smem_u32(&p.full[ring.stage]);
           const int row = g.segment.x + k;
-          // copies that the other CTA has to clear the end of count on its own barrier
+          // each CTA looks after the end of a segment in its own copies
           const bool end = has_end(g.segment.y, k);
-          if (rank == 0) dev::mbar_arrive_expect_tx(&p.full[ring.stage], end ? bytes : 2 * bytes);
-          else if (end) dev::mbar_arrive_expect_tx(&p.full[ring.stage], bytes);
-          const uint32_t bar = end ? own : dev::in_first(own);
-          dev::tma_load_2d<true>(at, &a.slow, bar, slow, row);
-          dev::tma_load_2d<true>(at + kChunkBytes, &a.slow, bar, slow + kBlockK, row);
-          for (int c = 0; c < g.chunks; ++c)
-            dev::tma_load_2d<true>(at + kBytesA + c * kChunkBytes, &a.fast, bar, fast + c * kBlockK, row);
+          const uint32_t bar =
+              end ? dev::smem_u32(&p.end[ring.stage]) : dev::in_first(dev::smem_u32(&p.full[ring.stage]));
+          if (warp == 0) {
+            if (end) dev::mbar_arrive_expect_tx(&p.end[ring.stage], bytes);
+            else if (rank == 0) dev::mbar_arrive_expect_tx(&p.full[ring.stage], 2 * bytes);
+            dev::tma_load_2d<true>(at, &a.slow, bar, slow, row);
+            dev::tma_load_2d<true>(at + kChunkBytes, &a.slow, bar, slow + kBlockK, row);
+          } else {
+            for (int c = 0; c < g.chunks; ++c)
+              dev::tma_load_2d<true>(at + kBytesA + c * kChunkBytes, &a.fast, bar, fast + c * kBlockK, row);
+          }
           ring.next();
         }
       }
       if (!ok) settle();
     }
-  } else if (warp == 1) {
-    // the first CTA multiplies; both look after the ends of segments in their own copies
-    Ring<kGradStages> ring;
-    Ring<2> sums;
-    uint32_t ends = 0;  // a bit for each stage: parity of its barrier of ends, or the other CTA's own barrier
-    bool ok = true;
-    for (uint32_t t = t0; ok && t < tiles; t += t_step) {
-      const GradTile g = grad_tile(a, t);
-      const int count = g.segment.y;
-      if (count == 0) continue;
-      const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, true, true, 2 * kTileM,
-                                                        2 * g.chunks * kBlockK);
-      if (rank == 0) {
-        if (!warp_wait<true>(&p.sum_empty[sums.stage], sums.parity ^ 1, p, a.limit_ns)) break;
+  } else if (warp == 1 && rank == 0) {
+    if (dev::elect_one()) {
+      Ring<kGradStages> ring;
+      Ring<2> sums;
+      const uint64_t first_a = dev::operand_descriptor(stages, kChunkBytes, 1024);
+      const uint64_t first_b = dev::operand_descriptor(stages + kBytesA, kChunkBytes, 1024);
+      uint32_t parity[2] = {0, 0};  // of each stage's barriers: of whole steps, of ends
+      bool ok = true;
+      for (uint32_t t = t0; ok && t < tiles; t += t_step) {
+        const GradTile g = grad_tile(a, segments, t);
+        const int count = g.segment.y;
+        if (count == 0) continue;
+        const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, true, true, 2 * kTileM,
+                                                          2 * g.chunks * kBlockK);
+        if (!dev::mbar_wait<true>(&p.sum_empty[sums.stage], sums.parity ^ 1, &p.gave_up, a.limit_ns)) break;
         dev::tmem_fence_after();
-      }
-      const uint32_t sum = p.tmem + sums.stage * kGradN;
-      for (int k = 0; k < count; k += kBlockK) {
-        const bool end = has_end(count, k);
-        if (rank == 0) ok = warp_wait(&p.full[ring.stage], ring.parity, p, a.limit_ns);
-        else if (end) ok = warp_wait(&p.full[ring.stage], ends >> ring.stage & 1, p, a.limit_ns);
-        if (!ok) break;
-        const int valid = min(kBlockK, count - k), depth = (valid + 15) / 16, rest = depth * 16 - valid;
-        if (end) {
-          for (int i = lane; i < rest * 8 * (2 + g.chunks); i += 32)  // 16 bytes each
-            *reinterpret_cast<uint4*>(base + ring.stage * kGradStage + i / (rest * 8) * kChunkBytes +
-                                      valid * dev::kBoxRowBytes + i % (rest * 8) * 16) = make_uint4(0, 0, 0, 0);
-          dev::fence_proxy_async_smem();
-          __syncwarp();
-          if (rank != 0) {
-            if (lane == 0) dev::mbar_arrive_first(&p.end[ring.stage]);
+        const uint32_t sum = p.tmem + sums.stage * kGradN;
+        for (int k = 0; k < count; k += kBlockK) {
+          if (has_end(count, k)) {
+            ok = dev::mbar_wait<true>(&p.ended[ring.stage], parity[1] >> ring.stage & 1, &p.gave_up, a.limit_ns);
+            parity[1] ^= 1u << ring.stage;
           } else {
-            ok = warp_wait<true>(&p.end[ring.stage], ends >> ring.stage & 1, p, a.limit_ns);
-            if (!ok) break;
+            ok = dev::mbar_wait(&p.full[ring.stage], parity[0] >> ring.stage & 1, &p.gave_up, a.limit_ns);
+            parity[0] ^= 1u << ring.stage;
           }
-          ends ^= 1u << ring.stage;
-        }
-        if (rank == 0 && lane == 0) {
+          if (!ok) break;
           dev::tmem_fence_after();
-          const uint32_t at = stages + ring.stage * kGradStage;
-          const uint64_t da = dev::operand_descriptor(at, kChunkBytes, 1024);
-          const uint64_t db = dev::operand_descriptor(at + kBytesA, kChunkBytes, 1024);
-          for (int i = 0; i < depth; ++i)
-            dev::mma_issue<true>(sum, da + i * 2048 / 16, db + i * 2048 / 16, instruction, k + i > 0);
+          const uint64_t da = first_a + ring.stage * (kGradStage / 16), db = first_b + ring.stage * (kGradStage / 16);
+          const int depth = min(kBlockK, count - k + 15) / 16;
+#pragma unroll
+          for (int i = 0; i < kBlockK / 16; ++i)
+            if (i < depth) dev::mma_issue<true>(sum, da + i * 2048 / 16, db + i * 2048 / 16, instruction, k + i > 0);
           dev::mma_commit<true>(&p.empty[ring.stage]);
+          ring.next();
         }
-        ring.next();
-        __syncwarp();
+        dev::mma_commit<true>(&p.sum_full[sums.stage]);
+        sums.next();
       }
-      if (rank == 0 && lane == 0) dev::mma_commit<true>(&p.sum_full[sums.stage]);
-      sums.next();
+    }
+  } else if (warp == 3) {
+    // the ends of segments, cleared as soon as they have come (by the multiplying warp, when it got there, the
+    // gradient of 32 experts of about 1024 rows took 685 us)
+    Ring<kGradStages> ring;
+    uint32_t ends = 0;  // parity of each stage's barrier
+    for (uint32_t t = t0; t < tiles; t += t_step) {
+      const GradTile g = grad_tile(a, segments, t);
+      const int count = g.segment.y, plain = (count + kBlockK - 1) / kBlockK - (count % 16 != 0);
+      ring.skip(plain);
+      if (count % 16 == 0) continue;
+      if (!warp_wait(&p.end[ring.stage], ends >> ring.stage & 1, p, a.limit_ns)) break;
+      const int valid = count - plain * kBlockK, depth = (valid + 15) / 16 * 16;
+      uint8_t* chunk = base + ring.stage * kGradStage + lane * 16;  // 8 lanes to a row
+      for (int c = 0; c < 2 + g.chunks; ++c, chunk += kChunkBytes)
+        for (int row = valid; row < depth; row += 4)
+          if (row + lane / 8 < depth) *reinterpret_cast<uint4*>(chunk + row * dev::kBoxRowBytes) = make_uint4(0, 0, 0, 0);
+      dev::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) dev::mbar_arrive_first(&p.ended[ring.stage]);
+      ends ^= 1u << ring.stage;
+      ring.next();
     }
   } else if (warp >= 4) {
     Ring<2> sums;
     const int quarter = warp & 3;
-    uint8_t* mine = staging + quarter * 32 * kGradPitch;
+    uint8_t* mine = staging + quarter * kStoreBoxes * kStoreBox;
     const bool whole = a.fast_width % 8 == 0;
+    int filled = 0;
     for (uint32_t t = t0; t < tiles; t += t_step) {
-      const GradTile g = grad_tile(a, t);
+      const GradTile g = grad_tile(a, segments, t);
       const int m = g.slow + rank * kTileM + quarter * 32;
       const int columns = min(2 * g.chunks * kBlockK, a.fast_width - g.fast), rows = min(32, a.slow_width - m);
       const bool empty = g.segment.y == 0;
-      T* out = static_cast<T*>(a.out) + ((int64_t)g.expert * a.slow_width + m) * a.fast_width + g.fast;
       if (!empty) {
         if (!warp_wait(&p.sum_full[sums.stage], sums.parity, p, a.limit_ns)) break;
         dev::tmem_fence_after();
       }
-      for (int c = 0; c < columns; c += 32) {
-        if (!empty) {
-          uint32_t v[32];
-          dev::tmem_load32(p.tmem + sums.stage * kGradN + c + ((uint32_t)quarter << 21), v);
+      for (int c = 0; c < columns; c += kBlockK, filled = (filled + 1) % kStoreBoxes) {
+        uint32_t v[2][32];
+        if (empty) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint4 w;
-            w.x = dev::from_float2(__uint_as_float(v[8 * j]), __uint_as_float(v[8 * j + 1]), T{});
-            w.y = dev::from_float2(__uint_as_float(v[8 * j + 2]), __uint_as_float(v[8 * j + 3]), T{});
-            w.z = dev::from_float2(__uint_as_float(v[8 * j + 4]), __uint_as_float(v[8 * j + 5]), T{});
-            w.w = dev::from_float2(__uint_as_float(v[8 * j + 6]), __uint_as_float(v[8 * j + 7]), T{});
-            *reinterpret_cast<uint4*>(mine + lane * kGradPitch + j * 16) = w;
+          for (int i = 0; i < 32; ++i) v[0][i] = v[1][i] = 0;
+        } else {
+          const uint32_t at = p.tmem + sums.stage * kGradN + c + ((uint32_t)quarter << 21);
+          dev::tmem_load32(at, v[0]);
+          dev::tmem_load32(at + 32, v[1]);
+          dev::tmem_load_wait();
+        }
+        if (rows <= 0) continue;
+        // 16-byte pieces in the order of the tiled copies: the piece's number within 128 bytes xor the row's within 8
+        uint8_t* box = mine + filled * kStoreBox;
+        dev::store_wait<kStoreBoxes - 1>();
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t* x = v[j / 4] + j % 4 * 8;
+          uint4 w;
+          w.x = dev::from_float2(__uint_as_float(x[0]), __uint_as_float(x[1]), T{});
+          w.y = dev::from_float2(__uint_as_float(x[2]), __uint_as_float(x[3]), T{});
+          w.z = dev::from_float2(__uint_as_float(x[4]), __uint_as_float(x[5]), T{});
+          w.w = dev::from_float2(__uint_as_float(x[6]), __uint_as_float(x[7]), T{});
+          *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) * 16)) = w;
+        }
+        if (whole) {
+          dev::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) dev::tma_store_3d(&a.out, dev::smem_u32(box), g.fast + c, m, g.expert);
+        } else {
+          __syncwarp();
+          T* out = static_cast<T*>(a.result) + ((int64_t)g.expert * a.slow_width + m) * a.fast_width + g.fast + c;
+          for (int half = 0; half < 2; ++half) {
+            const int i = half * 32 + lane;
+            if (c + i < columns)
+              for (int row = 0; row < rows; ++row)
+                out[(int64_t)row * a.fast_width + i] =
+                    *reinterpret_cast<const T*>(box + row * 128 + ((i / 8 ^ (row & 7)) * 16) + i % 8 * 2);
           }
           __syncwarp();
         }
-        if (whole) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = i * 8 + lane / 4, at = c + lane % 4 * 8;
-            if (row < rows && at < columns)
-              *reinterpret_cast<uint4*>(out + (int64_t)row * a.fast_width + at) =
-                  empty ? make_uint4(0, 0, 0, 0)
-                        : *reinterpret_cast<const uint4*>(mine + row * kGradPitch + lane % 4 * 16);
-          }
-        } else if (c + lane < columns) {
-          for (int row = 0; row < rows; ++row)
-            out[(int64_t)row * a.fast_width + c + lane] =
-                empty ? dev::from_float<T>(0.f) : *reinterpret_cast<const T*>(mine + row * kGradPitch + lane * 2);
-        }
-        __syncwarp();
       }
       if (!empty) {
         dev::tmem_fence_before();
@@ -609,6 +652,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         sums.next();
       }
     }
+    dev::store_wait<0>();
   }
   __syncwarp();
   close_pipe(p, 512);
@@ -782,7 +826,7 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
     return cudaErrorInvalidValue;
   GradArgs a;
   a.segments = {d_counts, d_offsets, num_experts, (int)capacity};
-  a.out = d_grad_weights;
+  a.result = d_grad_weights;
   a.slow_width = (int)slow.width;
   a.fast_width = (int)fast.width;
   a.slow_tiles = (int)((slow.width + 2 * kTileM - 1) / (2 * kTileM));
@@ -795,9 +839,13 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
   if (!e) e = fast.prepare(temp, nullptr, stream);
   if (!e) e = slow.map(&a.slow, true, kBlockK);
   if (!e) e = fast.map(&a.fast, true, kBlockK);
+  if (!e && fast.width % 8 == 0) {
+    const Operand out{d_grad_weights, num_experts, slow.width, fast.width, slow.width * fast.width, fast.width};
+    e = out.map(&a.out, false, 32);
+  }
   if (e) return e;
-  return type == CUSORT_FLOAT_F16 ? run(grad_weights_kernel<__half>, a, tiles, 2, grad_bytes(), stream)
-                                  : run(grad_weights_kernel<__nv_bfloat16>, a, tiles, 2, grad_bytes(), stream);
+  return type == CUSORT_FLOAT_F16 ? run(grad_weights_kernel<__half>, a, tiles, 2, grad_bytes(num_experts), stream)
+                                  : run(grad_weights_kernel<__nv_bfloat16>, a, tiles, 2, grad_bytes(num_experts), stream);
 }
 
 extern "C" cudaError_t cusort_read_product_status(uint32_t* status, cudaStream_t stream) {

@@ -53,6 +53,20 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// A box from shared memory, what lies outside the tensor left out; a group of
+// one.  The thread's groups but the last N have been read when store_wait
+// returns.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
+               "r"(src), "r"(x), "r"(y), "r"(z)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void store_wait() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+
 // Shared-memory matrix descriptor of a 128-byte-swizzled operand.  `leading`
 // and `stride` in bytes:
 //   contracted dimension contiguous: `stride` from one group of 8 rows to the
@@ -128,7 +142,8 @@ __device__ __forceinline__ void tmem_free(uint32_t address, uint32_t columns) {
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 32 columns of this warp's 32 lanes of tensor memory: v[i] = column i of this thread's lane.
+// 32 columns of this warp's 32 lanes of tensor memory: v[i] = column i of this thread's lane, after
+// tmem_load_wait.
 __device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -138,7 +153,16 @@ __device__ __forceinline__ void tmem_load32(uint32_t address, uint32_t (&v)[32])
         "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
         "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
       : "r"(address));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// v is there when this returns.
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// One thread of a whole warp, the same one each time.  Where copies and
+// products are issued under it, the compiler knows that a single thread does.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
 }
 
 // Number of this CTA in its cluster.
