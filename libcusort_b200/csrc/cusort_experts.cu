@@ -7,6 +7,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstddef>
 #include <cstdint>
 #include <type_traits>
 #include <utility>
@@ -143,6 +144,24 @@ template <int STAGES, bool PAIR> struct Pipe {
   uint32_t tmem, gave_up, sums[8];
 };
 
+// The barriers' addresses.
+template <int STAGES, bool PAIR> struct PipeAt {
+  using P = Pipe<STAGES, PAIR>;
+  uint32_t base;
+  __device__ __forceinline__ explicit PipeAt(const P& p) : base(dev::smem_u32(&p)) {}
+  __device__ __forceinline__ uint32_t full(int i) const { return base + offsetof(P, full) + 8 * i; }
+  __device__ __forceinline__ uint32_t empty(int i) const { return base + offsetof(P, empty) + 8 * i; }
+  __device__ __forceinline__ uint32_t end(int i) const { return base + offsetof(P, end) + 8 * i; }
+  __device__ __forceinline__ uint32_t ended(int i) const { return base + offsetof(P, ended) + 8 * i; }
+  __device__ __forceinline__ uint32_t sum_full(int i) const { return base + offsetof(P, sum_full) + 8 * i; }
+  __device__ __forceinline__ uint32_t sum_empty(int i) const { return base + offsetof(P, sum_empty) + 8 * i; }
+  // The storing warps have read a sum: one lane says so.
+  __device__ __forceinline__ void release_sum(int i) const {
+    if (PAIR) dev::arrive_first(sum_empty(i));
+    else dev::arrive(sum_empty(i));
+  }
+};
+
 template <int STAGES, bool PAIR>
 __device__ __forceinline__ void init_pipe(Pipe<STAGES, PAIR>& p, uint32_t columns) {
   if (threadIdx.x == 0) {
@@ -193,25 +212,17 @@ template <int STAGES> struct Ring {
 
 // After a wait ran out: copies in flight, which take microseconds, are given a
 // millisecond before the CTA ends.
-__device__ __forceinline__ void settle() {
+__device__ __forceinline__ void settle(const dev::WaitLimit& limit) {
+  if (!*limit.gave_up) return;
   const uint64_t t0 = dev::globaltimer_ns();
   while (dev::globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
 }
 
-// A wait of a whole warp.  One lane asks: 32 of them keep shared memory busy, which the copies and products need (a
-// third of the products' rate was lost to the storing warps' waits).
-template <bool CLUSTER = false, int STAGES, bool PAIR>
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, Pipe<STAGES, PAIR>& p, uint64_t limit_ns) {
+// A wait of a whole warp, by one lane: 32 of them keep shared memory busy.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const dev::WaitLimit& limit) {
   bool ok = true;
-  if ((threadIdx.x & 31) == 0) ok = dev::mbar_wait<CLUSTER>(bar, parity, &p.gave_up, limit_ns);
+  if ((threadIdx.x & 31) == 0) ok = dev::wait_for(bar, parity, limit);
   return __shfl_sync(kAll, ok, 0);
-}
-
-// The storing warps have read a sum: one lane says so.
-template <int STAGES, bool PAIR>
-__device__ __forceinline__ void release_sum(Pipe<STAGES, PAIR>& p, int sum) {
-  if (PAIR) dev::mbar_arrive_first(&p.sum_empty[sum]);
-  else dev::mbar_arrive(&p.sum_empty[sum]);
 }
 
 __device__ __forceinline__ uint32_t align_up(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
@@ -290,6 +301,9 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
   s.count = s.first + experts;
   s.tiles = s.count + experts;
 
+  const PipeAt<STAGES, PAIR> at(p);
+  const dev::WaitLimit limit{&p.gave_up, a.limit_ns};
+
   init_pipe(p, Shape::kColumns);
   dev::wait_for_previous();
   load_segments(a.segments, s, p.sums, [](int count) { return (count + BN - 1) / BN; });
@@ -303,68 +317,58 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
     // one warp brings the weights, another the rows: together, one thread's issue would be what bounds the products
     if (dev::elect_one()) {
       Ring<STAGES> ring;
-      bool ok = true;
-      for (uint32_t t = t0; ok && t < tiles; t += t_step) {
+      for (uint32_t t = t0; t < tiles; t += t_step) {
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const int column = tile.column + rank * kTileM;
         const int mine = align_up(tile.rows, Shape::kRowStep) / Shape::kCtas, row = tile.row + rank * mine;
         const int boxes = (mine + Shape::kBoxRows - 1) / Shape::kBoxRows;
-        for (int k = 0; k < steps; ++k) {
-          if (!dev::mbar_wait(&p.empty[ring.stage], ring.parity ^ 1, &p.gave_up, a.limit_ns)) {
-            ok = false;
-            break;
-          }
-          const uint32_t at = stages + ring.stage * Shape::kStage;
-          const uint32_t own = dev::smem_u32(&p.full[ring.stage]), bar = PAIR ? dev::in_first(own) : own;
+        const uint32_t bytes = Shape::kCtas * (kBytesA + boxes * Shape::kBoxBytes);
+        for (int k = 0; k < steps; ++k, ring.next()) {
+          if (!dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
+          const uint32_t to = stages + ring.stage * Shape::kStage, own = at.full(ring.stage);
+          const uint32_t bar = PAIR ? dev::in_first(own) : own;
           if (warp == 0) {
             // the first CTA's barrier counts the copies of both
-            if (rank == 0)
-              dev::mbar_arrive_expect_tx(&p.full[ring.stage], Shape::kCtas * (kBytesA + boxes * Shape::kBoxBytes));
+            if (rank == 0) dev::arrive_expect(own, bytes);
             if (IN_ORDER) {
-              dev::tma_load_3d<PAIR>(at, &a.weights, bar, k * kBlockK, column, tile.expert);
+              dev::tma_load_3d<PAIR>(to, &a.weights, bar, k * kBlockK, column, tile.expert);
             } else {
-              dev::tma_load_3d<PAIR>(at, &a.weights, bar, column, k * kBlockK, tile.expert);
-              dev::tma_load_3d<PAIR>(at + kBytesA / 2, &a.weights, bar, column + kBlockK, k * kBlockK, tile.expert);
+              dev::tma_load_3d<PAIR>(to, &a.weights, bar, column, k * kBlockK, tile.expert);
+              dev::tma_load_3d<PAIR>(to + kBytesA / 2, &a.weights, bar, column + kBlockK, k * kBlockK, tile.expert);
             }
           } else {
             for (int b = 0; b < boxes; ++b)
-              dev::tma_load_2d<PAIR>(at + kBytesA + b * Shape::kBoxBytes, &a.rows, bar, k * kBlockK,
+              dev::tma_load_2d<PAIR>(to + kBytesA + b * Shape::kBoxBytes, &a.rows, bar, k * kBlockK,
                                      row + b * Shape::kBoxRows);
           }
-          ring.next();
         }
       }
-      if (!ok) settle();
+      settle(limit);
     }
   } else if (warp == 1 && rank == 0) {
     if (dev::elect_one()) {
       Ring<STAGES> ring;
       Ring<2> sums;
-      bool ok = true;
       const uint64_t first_a = dev::operand_descriptor(stages, IN_ORDER ? 16 : kBytesA / 2, 1024);
       const uint64_t first_b = dev::operand_descriptor(stages + kBytesA, 16, 1024);
-      for (uint32_t t = t0; ok && t < tiles; t += t_step) {
+      for (uint32_t t = t0; t < tiles; t += t_step, sums.next()) {
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, !IN_ORDER, false,
                                                           Shape::kTile, align_up(tile.rows, Shape::kRowStep));
-        if (!dev::mbar_wait<PAIR>(&p.sum_empty[sums.stage], sums.parity ^ 1, &p.gave_up, a.limit_ns)) break;
-        dev::tmem_fence_after();
         const uint32_t sum = p.tmem + sums.stage * BN;
-        for (int k = 0; k < steps; ++k) {
-          if (!dev::mbar_wait(&p.full[ring.stage], ring.parity, &p.gave_up, a.limit_ns)) {
-            ok = false;
-            break;
-          }
+        dev::wait_for<PAIR>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
+        dev::tmem_fence_after();
+        for (int k = 0; k < steps; ++k, ring.next()) {
+          if (!dev::wait_for(at.full(ring.stage), ring.parity, limit)) continue;
           dev::tmem_fence_after();
-          const uint64_t da = first_a + ring.stage * (Shape::kStage / 16), db = first_b + ring.stage * (Shape::kStage / 16);
+          const uint32_t stage = ring.stage * (Shape::kStage / 16);
 #pragma unroll
           for (int i = 0; i < kBlockK / 16; ++i)
-            dev::mma_issue<PAIR>(sum, da + i * (IN_ORDER ? 32 : 2048) / 16, db + i * 32 / 16, instruction, k + i > 0);
-          dev::mma_commit<PAIR>(&p.empty[ring.stage]);
-          ring.next();
+            dev::mma_issue<PAIR>(sum, first_a + stage + i * (IN_ORDER ? 32 : 2048) / 16, first_b + stage + i * 32 / 16,
+                                 instruction, k + i > 0);
+          dev::mma_commit<PAIR>(at.empty(ring.stage));
         }
-        dev::mma_commit<PAIR>(&p.sum_full[sums.stage]);
-        sums.next();
+        dev::mma_commit<PAIR>(at.sum_full(sums.stage));
       }
     }
   } else if (warp == 3) {
@@ -386,9 +390,9 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
     uint8_t* mine = staging + quarter * 2048;
     T* out = static_cast<T*>(a.out);
     const bool whole = a.width % 8 == 0;  // the result's first byte lies on a 16-byte boundary
-    for (uint32_t t = t0; t < tiles; t += t_step) {
+    for (uint32_t t = t0; t < tiles; t += t_step, sums.next()) {
       const ProductTile tile = product_tile<Shape>(a, s, t);
-      if (!warp_wait(&p.sum_full[sums.stage], sums.parity, p, a.limit_ns)) break;
+      if (!warp_wait(at.sum_full(sums.stage), sums.parity, limit)) continue;
       dev::tmem_fence_after();
       const int column = tile.column + rank * kTileM + quarter * 32;
       for (int c = 0; c < tile.rows; c += 32) {
@@ -409,9 +413,9 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
         if (whole) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int row = i * 8 + lane / 4, at = column + lane % 4 * 8;
-            if (row < rows && at < a.width)
-              *reinterpret_cast<uint4*>(out + (first + row) * a.width + at) =
+            const int row = i * 8 + lane / 4, x = column + lane % 4 * 8;
+            if (row < rows && x < a.width)
+              *reinterpret_cast<uint4*>(out + (first + row) * a.width + x) =
                   *reinterpret_cast<const uint4*>(mine + row * 64 + lane % 4 * 16);
           }
         } else if (column + lane < a.width) {
@@ -422,8 +426,7 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
       }
       dev::tmem_fence_before();
       __syncwarp();
-      if (lane == 0) release_sum(p, sums.stage);
-      sums.next();
+      if (lane == 0) at.release_sum(sums.stage);
     }
   }
   __syncwarp();
@@ -485,6 +488,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   int2* segments = reinterpret_cast<int2*>(&p + 1);
 
+  const PipeAt<kGradStages, true> at(p);
+  const dev::WaitLimit limit{&p.gave_up, a.limit_ns};
+
   init_pipe(p, 512);
   dev::wait_for_previous();
   for (int e = threadIdx.x; e < a.segments.experts; e += kThreads) segments[e] = segment(a.segments, e);
@@ -497,34 +503,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == 0 || warp == 2) {  // an operand each
     if (dev::elect_one()) {
       Ring<kGradStages> ring;
-      bool ok = true;
-      for (uint32_t t = t0; ok && t < tiles; t += t_step) {
+      for (uint32_t t = t0; t < tiles; t += t_step) {
         const GradTile g = grad_tile(a, segments, t);
         const int slow = g.slow + rank * kTileM, fast = g.fast + rank * g.chunks * kBlockK;
-        for (int k = 0; k < g.segment.y; k += kBlockK) {
-          if (!dev::mbar_wait(&p.empty[ring.stage], ring.parity ^ 1, &p.gave_up, a.limit_ns)) {
-            ok = false;
-            break;
-          }
-          const uint32_t at = stages + ring.stage * kGradStage, bytes = (2 + g.chunks) * kChunkBytes;
+        const uint32_t bytes = (2 + g.chunks) * kChunkBytes;
+        for (int k = 0; k < g.segment.y; k += kBlockK, ring.next()) {
+          if (!dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
+          const uint32_t to = stages + ring.stage * kGradStage;
           const int row = g.segment.x + k;
           // each CTA looks after the end of a segment in its own copies
           const bool end = has_end(g.segment.y, k);
-          const uint32_t bar =
-              end ? dev::smem_u32(&p.end[ring.stage]) : dev::in_first(dev::smem_u32(&p.full[ring.stage]));
+          const uint32_t bar = end ? at.end(ring.stage) : dev::in_first(at.full(ring.stage));
           if (warp == 0) {
-            if (end) dev::mbar_arrive_expect_tx(&p.end[ring.stage], bytes);
-            else if (rank == 0) dev::mbar_arrive_expect_tx(&p.full[ring.stage], 2 * bytes);
-            dev::tma_load_2d<true>(at, &a.slow, bar, slow, row);
-            dev::tma_load_2d<true>(at + kChunkBytes, &a.slow, bar, slow + kBlockK, row);
+            if (end) dev::arrive_expect(at.end(ring.stage), bytes);
+            else if (rank == 0) dev::arrive_expect(at.full(ring.stage), 2 * bytes);
+            dev::tma_load_2d<true>(to, &a.slow, bar, slow, row);
+            dev::tma_load_2d<true>(to + kChunkBytes, &a.slow, bar, slow + kBlockK, row);
           } else {
             for (int c = 0; c < g.chunks; ++c)
-              dev::tma_load_2d<true>(at + kBytesA + c * kChunkBytes, &a.fast, bar, fast + c * kBlockK, row);
+              dev::tma_load_2d<true>(to + kBytesA + c * kChunkBytes, &a.fast, bar, fast + c * kBlockK, row);
           }
-          ring.next();
         }
       }
-      if (!ok) settle();
+      settle(limit);
     }
   } else if (warp == 1 && rank == 0) {
     if (dev::elect_one()) {
@@ -533,35 +534,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint64_t first_a = dev::operand_descriptor(stages, kChunkBytes, 1024);
       const uint64_t first_b = dev::operand_descriptor(stages + kBytesA, kChunkBytes, 1024);
       uint32_t parity[2] = {0, 0};  // of each stage's barriers: of whole steps, of ends
-      bool ok = true;
-      for (uint32_t t = t0; ok && t < tiles; t += t_step) {
+      for (uint32_t t = t0; t < tiles; t += t_step) {
         const GradTile g = grad_tile(a, segments, t);
         const int count = g.segment.y;
         if (count == 0) continue;
         const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, true, true, 2 * kTileM,
                                                           2 * g.chunks * kBlockK);
-        if (!dev::mbar_wait<true>(&p.sum_empty[sums.stage], sums.parity ^ 1, &p.gave_up, a.limit_ns)) break;
-        dev::tmem_fence_after();
         const uint32_t sum = p.tmem + sums.stage * kGradN;
-        for (int k = 0; k < count; k += kBlockK) {
+        dev::wait_for<true>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
+        dev::tmem_fence_after();
+        for (int k = 0; k < count; k += kBlockK, ring.next()) {
+          bool there;
           if (has_end(count, k)) {
-            ok = dev::mbar_wait<true>(&p.ended[ring.stage], parity[1] >> ring.stage & 1, &p.gave_up, a.limit_ns);
+            there = dev::wait_for<true>(at.ended(ring.stage), parity[1] >> ring.stage & 1, limit);
             parity[1] ^= 1u << ring.stage;
           } else {
-            ok = dev::mbar_wait(&p.full[ring.stage], parity[0] >> ring.stage & 1, &p.gave_up, a.limit_ns);
+            there = dev::wait_for(at.full(ring.stage), parity[0] >> ring.stage & 1, limit);
             parity[0] ^= 1u << ring.stage;
           }
-          if (!ok) break;
+          if (!there) continue;
           dev::tmem_fence_after();
-          const uint64_t da = first_a + ring.stage * (kGradStage / 16), db = first_b + ring.stage * (kGradStage / 16);
+          const uint32_t stage = ring.stage * (kGradStage / 16);
           const int depth = min(kBlockK, count - k + 15) / 16;
 #pragma unroll
           for (int i = 0; i < kBlockK / 16; ++i)
-            if (i < depth) dev::mma_issue<true>(sum, da + i * 2048 / 16, db + i * 2048 / 16, instruction, k + i > 0);
-          dev::mma_commit<true>(&p.empty[ring.stage]);
-          ring.next();
+            if (i < depth)
+              dev::mma_issue<true>(sum, first_a + stage + i * 2048 / 16, first_b + stage + i * 2048 / 16, instruction,
+                                   k + i > 0);
+          dev::mma_commit<true>(at.empty(ring.stage));
         }
-        dev::mma_commit<true>(&p.sum_full[sums.stage]);
+        dev::mma_commit<true>(at.sum_full(sums.stage));
         sums.next();
       }
     }
@@ -569,22 +571,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // the ends of segments, cleared as soon as they have come (by the multiplying warp, when it got there, the
     // gradient of 32 experts of about 1024 rows took 685 us)
     Ring<kGradStages> ring;
-    uint32_t ends = 0;  // parity of each stage's barrier
+    uint32_t parity = 0;  // of each stage's barrier of ends
     for (uint32_t t = t0; t < tiles; t += t_step) {
       const GradTile g = grad_tile(a, segments, t);
       const int count = g.segment.y, plain = (count + kBlockK - 1) / kBlockK - (count % 16 != 0);
       ring.skip(plain);
       if (count % 16 == 0) continue;
-      if (!warp_wait(&p.end[ring.stage], ends >> ring.stage & 1, p, a.limit_ns)) break;
-      const int valid = count - plain * kBlockK, depth = (valid + 15) / 16 * 16;
-      uint8_t* chunk = base + ring.stage * kGradStage + lane * 16;  // 8 lanes to a row
-      for (int c = 0; c < 2 + g.chunks; ++c, chunk += kChunkBytes)
-        for (int row = valid; row < depth; row += 4)
-          if (row + lane / 8 < depth) *reinterpret_cast<uint4*>(chunk + row * dev::kBoxRowBytes) = make_uint4(0, 0, 0, 0);
-      dev::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) dev::mbar_arrive_first(&p.ended[ring.stage]);
-      ends ^= 1u << ring.stage;
+      if (warp_wait(at.end(ring.stage), parity >> ring.stage & 1, limit)) {
+        const int valid = count - plain * kBlockK, depth = (valid + 15) / 16 * 16;
+        uint8_t* chunk = base + ring.stage * kGradStage + lane * 16;  // 8 lanes to a row
+        for (int c = 0; c < 2 + g.chunks; ++c, chunk += kChunkBytes)
+          for (int row = valid; row < depth; row += 4)
+            if (row + lane / 8 < depth)
+              *reinterpret_cast<uint4*>(chunk + row * dev::kBoxRowBytes) = make_uint4(0, 0, 0, 0);
+        dev::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) dev::arrive_first(at.ended(ring.stage));
+      }
+      parity ^= 1u << ring.stage;
       ring.next();
     }
   } else if (warp >= 4) {
@@ -599,7 +603,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int columns = min(2 * g.chunks * kBlockK, a.fast_width - g.fast), rows = min(32, a.slow_width - m);
       const bool empty = g.segment.y == 0;
       if (!empty) {
-        if (!warp_wait(&p.sum_full[sums.stage], sums.parity, p, a.limit_ns)) break;
+        if (!warp_wait(at.sum_full(sums.stage), sums.parity, limit)) {
+          sums.next();
+          continue;
+        }
         dev::tmem_fence_after();
       }
       for (int c = 0; c < columns; c += kBlockK, filled = (filled + 1) % kStoreBoxes) {
@@ -608,9 +615,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[0][i] = v[1][i] = 0;
         } else {
-          const uint32_t at = p.tmem + sums.stage * kGradN + c + ((uint32_t)quarter << 21);
-          dev::tmem_load32(at, v[0]);
-          dev::tmem_load32(at + 32, v[1]);
+          const uint32_t sum = p.tmem + sums.stage * kGradN + c + ((uint32_t)quarter << 21);
+          dev::tmem_load32(sum, v[0]);
+          dev::tmem_load32(sum + 32, v[1]);
           dev::tmem_load_wait();
         }
         if (rows <= 0) continue;
@@ -648,7 +655,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!empty) {
         dev::tmem_fence_before();
         __syncwarp();
-        if (lane == 0) release_sum(p, sums.stage);
+        if (lane == 0) at.release_sum(sums.stage);
         sums.next();
       }
     }

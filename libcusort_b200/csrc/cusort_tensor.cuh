@@ -107,16 +107,14 @@ __device__ __forceinline__ void mma_issue(uint32_t accumulator, uint64_t a, uint
 }
 // The barrier (PAIR: the one at this address in both CTAs) gets one arrival when the products issued so far are done.
 template <bool PAIR>
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
   if constexpr (PAIR)
     asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-            smem_u32(bar)),
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
         "h"((uint16_t)3)
         : "memory");
   else
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 template <bool PAIR>
 __device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t columns) {
@@ -182,43 +180,69 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+// Barriers by their shared-memory addresses.
+__device__ __forceinline__ void arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // At the barrier at this address of the cluster's first CTA.
-__device__ __forceinline__ void mbar_arrive_first(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_first(smem_u32(bar)))
-               : "memory");
+__device__ __forceinline__ void arrive_first(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_first(bar)) : "memory");
 }
-// A barrier at which other CTAs of the cluster arrive.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t* bar, uint32_t parity) {
+// Whether a phase is over.  CLUSTER: of a barrier at which other CTAs of the cluster arrive.
+template <bool CLUSTER>
+__device__ __forceinline__ bool is_over(uint32_t bar, uint32_t parity) {
   uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
+  if constexpr (CLUSTER)
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
   return ok != 0;
 }
 
-// Waits for a phase of a barrier, `limit_ns` at most and no longer than until
-// another thread of the CTA has given up (*gave_up, in shared memory).
-template <bool CLUSTER = false>
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t* gave_up, uint64_t limit_ns) {
-  const auto done = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
-  SpinGuard guard;
+// What ends a CTA's waits: a time, and a word in shared memory that says that
+// one of them ran out.  From then on they all return false at once.
+struct WaitLimit {
+  volatile uint32_t* gave_up;
+  uint64_t ns;
+};
+
+// The rest of wait_for, for a phase that was not over yet.  Not inlined: with
+// this loop in the loops that bring and multiply tiles a wait cost 380 cycles
+// even where the phase was over.
+template <bool CLUSTER>
+__device__ __noinline__ bool wait_long(uint32_t bar, uint32_t parity, WaitLimit limit) {
+  uint64_t t0 = 0;
   for (;;) {
-    // the clock is looked at now and then: reading it takes longer than most waits (a wait that read it after every
-    // try made the products twice as slow)
+    // the clock is looked at now and then: reading it takes longer than most waits
 #pragma unroll 1
     for (int i = 0; i < 64; ++i)
-      if (done()) return true;
-    if (guard.expired(gave_up, limit_ns)) {
-      if (gave_up != nullptr) *(volatile uint32_t*)gave_up = 1;
+      if (is_over<CLUSTER>(bar, parity)) return true;
+    if (*limit.gave_up) return false;
+    const uint64_t now = globaltimer_ns();
+    if (t0 == 0) t0 = now;
+    if (now - t0 > limit.ns) {
+      *limit.gave_up = 1;
       return false;
     }
   }
+}
+
+// Waits for a phase of a barrier; false: in vain.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, WaitLimit limit) {
+  return is_over<CLUSTER>(bar, parity) || wait_long<CLUSTER>(bar, parity, limit);
 }
 
 }  // namespace dev
