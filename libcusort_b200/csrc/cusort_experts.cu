@@ -53,7 +53,7 @@ namespace {
 using namespace cusort_b200;
 
 constexpr int kMaxExperts = 1024;
-constexpr int kThreads = 256;  // warps 0 and 2 bring operands, 1 multiplies, 3 clears rows, 4 to 7 store
+constexpr int kThreads = 320;  // warps 0, 2, 8 and 9 bring operands, 1 multiplies, 3 clears rows, 4 to 7 store
 constexpr int kSms = 148;
 constexpr int kBlockK = 64;              // contracted elements to a stage: one swizzle row
 constexpr int kTileM = 128;              // lanes of a CTA's tensor memory
@@ -85,7 +85,7 @@ __device__ __forceinline__ int2 segment(const SegmentArgs& a, int e) {
 template <typename F>
 __device__ __forceinline__ void load_segments(const SegmentArgs& a, const Segments& s, uint32_t* sums, F&& tiles) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int kEach = kMaxExperts / kThreads;
+  constexpr int kEach = (kMaxExperts + kThreads - 1) / kThreads;
   const int per = (a.experts + kThreads - 1) / kThreads;  // consecutive experts to a thread
   int mine[kEach], sum = 0;
 #pragma unroll
@@ -141,7 +141,8 @@ template <int STAGES, bool PAIR> struct Pipe {
   uint64_t end[STAGES];    // a stage's copies of this CTA are there, which hold the end of a segment
   uint64_t ended[STAGES];  // in the first of two CTAs: both have cleared what lies behind that
   uint64_t sum_full[2], sum_empty[2];
-  uint32_t tmem, gave_up, sums[8];
+  uint64_t parts;          // in the first CTA of a split tile: the others' sums are there
+  uint32_t tmem, gave_up, sums[kThreads / 32];
 };
 
 // The barriers' addresses.
@@ -155,6 +156,7 @@ template <int STAGES, bool PAIR> struct PipeAt {
   __device__ __forceinline__ uint32_t ended(int i) const { return base + offsetof(P, ended) + 8 * i; }
   __device__ __forceinline__ uint32_t sum_full(int i) const { return base + offsetof(P, sum_full) + 8 * i; }
   __device__ __forceinline__ uint32_t sum_empty(int i) const { return base + offsetof(P, sum_empty) + 8 * i; }
+  __device__ __forceinline__ uint32_t parts() const { return base + offsetof(P, parts); }
   // The storing warps have read a sum: one lane says so.
   __device__ __forceinline__ void release_sum(int i) const {
     if (PAIR) dev::arrive_first(sum_empty(i));
@@ -162,7 +164,7 @@ template <int STAGES, bool PAIR> struct PipeAt {
   }
 };
 
-template <int STAGES, bool PAIR>
+template <bool CLUSTER, int STAGES, bool PAIR>
 __device__ __forceinline__ void init_pipe(Pipe<STAGES, PAIR>& p, uint32_t columns) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
@@ -172,22 +174,23 @@ __device__ __forceinline__ void init_pipe(Pipe<STAGES, PAIR>& p, uint32_t column
       dev::mbar_init(&p.ended[i], 2);
     }
     for (int i = 0; i < 2; ++i) dev::mbar_init(&p.sum_full[i], 1), dev::mbar_init(&p.sum_empty[i], PAIR ? 8 : 4);
+    if (CLUSTER && !PAIR) dev::mbar_init(&p.parts, 4 * (dev::cluster_size() - 1));
     p.gave_up = 0;
     dev::fence_mbar_init();
   }
   __syncwarp();
   if (threadIdx.x / 32 == 1) dev::tmem_alloc<PAIR>(&p.tmem, columns);
   dev::tmem_fence_before();
-  if (PAIR) dev::cluster_sync();
+  if (CLUSTER) dev::cluster_sync();
   else __syncthreads();
   dev::tmem_fence_after();
 }
 
 // The end of every warp's work: tensor memory is given back.
-template <int STAGES, bool PAIR>
+template <bool CLUSTER, int STAGES, bool PAIR>
 __device__ __forceinline__ void close_pipe(Pipe<STAGES, PAIR>& p, uint32_t columns) {
   dev::tmem_fence_before();
-  if (PAIR) dev::cluster_sync();
+  if (CLUSTER) dev::cluster_sync();
   else __syncthreads();
   if (threadIdx.x == 0 && p.gave_up) atomicOr(&g_product_status, 1u);
   if (threadIdx.x / 32 == 1) {
@@ -219,11 +222,19 @@ __device__ __forceinline__ void settle(const dev::WaitLimit& limit) {
 }
 
 // A wait of a whole warp, by one lane: 32 of them keep shared memory busy.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const dev::WaitLimit& limit) {
   bool ok = true;
-  if ((threadIdx.x & 31) == 0) ok = dev::wait_for(bar, parity, limit);
+  if ((threadIdx.x & 31) == 0) ok = dev::wait_for<CLUSTER>(bar, parity, limit);
+  __syncwarp();
   return __shfl_sync(kAll, ok, 0);
 }
+
+// The warps that bring operands: 0 and 2 one of them, 8 and 9 the other, each
+// every second step.  A thread takes some 200 cycles to issue a tiled copy,
+// whatever its size: with one warp for all of them the products ran at half
+// the rate, with one for each operand a step took 350 cycles.
+__device__ __forceinline__ bool brings(int warp) { return warp == 0 || warp == 2 || warp >= 8; }
 
 __device__ __forceinline__ uint32_t align_up(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
 
@@ -251,7 +262,10 @@ struct ProductArgs {
 };
 
 // PAIR: tiles of 256 columns of the result, 128 in each of two CTAs, and half of the rows in each.
-template <int BN, int STAGES, bool PAIR> struct ProductShape {
+// SPLIT: the contracted dimension in equal parts over the CTAs of a cluster, kMostParts of them at most.
+constexpr int kMostParts = 3;
+template <int BN_, int STAGES, bool PAIR, bool SPLIT> struct ProductShape {
+  static constexpr int BN = BN_;
   static constexpr int kCtas = PAIR ? 2 : 1, kTile = kTileM * kCtas;
   static constexpr int kRowStep = 16 * kCtas;       // the instruction's width comes in such steps
   static constexpr int kBoxRows = PAIR ? 64 : 16;   // a tile of few rows brings few boxes
@@ -259,8 +273,10 @@ template <int BN, int STAGES, bool PAIR> struct ProductShape {
   static constexpr uint32_t kBoxBytes = kBoxRows * dev::kBoxRowBytes;
   static constexpr uint32_t kColumns = 2 * BN;
   static constexpr uint32_t kStaging = 4 * 2048;  // 32 x 32 16-bit elements for each storing warp
+  static constexpr uint32_t kPart = SPLIT ? BN * kTileM * 4 : 0;  // the sums of one of the other CTAs
   static size_t bytes(int experts) {
-    return 1024 + STAGES * kStage + kStaging + sizeof(Pipe<STAGES, PAIR>) + 4 * (3 * (size_t)experts + 1);
+    return 1024 + STAGES * kStage + (kMostParts - 1) * kPart + kStaging + sizeof(Pipe<STAGES, PAIR>) +
+           4 * (3 * (size_t)experts + 1);
   }
 };
 
@@ -287,13 +303,13 @@ __device__ __forceinline__ ProductTile product_tile(const ProductArgs& a, const 
 // the instruction's width is the number of rows, in steps of 16: an expert
 // with three rows costs a width of 16, and its weights stream through the
 // lanes.
-template <typename T, int BN, int STAGES, bool PAIR, bool IN_ORDER>
-__global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads, 1)
-    product_kernel(const __grid_constant__ ProductArgs a) {
-  using Shape = ProductShape<BN, STAGES, PAIR>;
+template <typename T, int BN, int STAGES, bool PAIR, bool SPLIT, bool IN_ORDER>
+__global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
+  using Shape = ProductShape<BN, STAGES, PAIR, SPLIT>;
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (align_up(dev::smem_u32(raw), 1024) - dev::smem_u32(raw));
-  uint8_t* staging = base + STAGES * Shape::kStage;
+  uint8_t* parts = base + STAGES * Shape::kStage;
+  uint8_t* staging = parts + (kMostParts - 1) * Shape::kPart;
   Pipe<STAGES, PAIR>& p = *reinterpret_cast<Pipe<STAGES, PAIR>*>(staging + Shape::kStaging);
   const int experts = a.segments.experts;
   Segments s;
@@ -304,19 +320,22 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
   const PipeAt<STAGES, PAIR> at(p);
   const dev::WaitLimit limit{&p.gave_up, a.limit_ns};
 
-  init_pipe(p, Shape::kColumns);
+  init_pipe<PAIR || SPLIT>(p, Shape::kColumns);
   dev::wait_for_previous();
   load_segments(a.segments, s, p.sums, [](int count) { return (count + BN - 1) / BN; });
   const uint32_t tiles = (uint32_t)s.tiles[experts] * a.width_tiles;
-  const int steps = (a.in + kBlockK - 1) / kBlockK;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = PAIR ? dev::cluster_rank() : 0;
-  const uint32_t t0 = blockIdx.x / Shape::kCtas, t_step = gridDim.x / Shape::kCtas;
+  const int part = SPLIT ? dev::cluster_rank() : 0, all_parts = SPLIT ? dev::cluster_size() : 1;
+  const int all_steps = (a.in + kBlockK - 1) / kBlockK;
+  const int first_step = all_steps * part / all_parts, steps = all_steps * (part + 1) / all_parts - first_step;
+  const int ctas = SPLIT ? all_parts : Shape::kCtas;  // to a tile
+  const uint32_t t0 = blockIdx.x / ctas, t_step = gridDim.x / ctas;
   const uint32_t stages = dev::smem_u32(base);
 
-  if (warp == 0 || warp == 2) {
-    // one warp brings the weights, another the rows: together, one thread's issue would be what bounds the products
+  if (brings(warp)) {
     if (dev::elect_one()) {
       Ring<STAGES> ring;
+      uint32_t turn = (warp == 2 || warp == 9);  // whether it takes the odd steps
       for (uint32_t t = t0; t < tiles; t += t_step) {
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const int column = tile.column + rank * kTileM;
@@ -324,22 +343,22 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
         const int boxes = (mine + Shape::kBoxRows - 1) / Shape::kBoxRows;
         const uint32_t bytes = Shape::kCtas * (kBytesA + boxes * Shape::kBoxBytes);
         for (int k = 0; k < steps; ++k, ring.next()) {
-          if (!dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
+          if ((turn ^= 1) == 0 || !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
           const uint32_t to = stages + ring.stage * Shape::kStage, own = at.full(ring.stage);
           const uint32_t bar = PAIR ? dev::in_first(own) : own;
-          if (warp == 0) {
+          const int x = (first_step + k) * kBlockK;
+          if (warp < 8) {
             // the first CTA's barrier counts the copies of both
             if (rank == 0) dev::arrive_expect(own, bytes);
             if (IN_ORDER) {
-              dev::tma_load_3d<PAIR>(to, &a.weights, bar, k * kBlockK, column, tile.expert);
+              dev::tma_load_3d<PAIR>(to, &a.weights, bar, x, column, tile.expert);
             } else {
-              dev::tma_load_3d<PAIR>(to, &a.weights, bar, column, k * kBlockK, tile.expert);
-              dev::tma_load_3d<PAIR>(to + kBytesA / 2, &a.weights, bar, column + kBlockK, k * kBlockK, tile.expert);
+              dev::tma_load_3d<PAIR>(to, &a.weights, bar, column, x, tile.expert);
+              dev::tma_load_3d<PAIR>(to + kBytesA / 2, &a.weights, bar, column + kBlockK, x, tile.expert);
             }
           } else {
             for (int b = 0; b < boxes; ++b)
-              dev::tma_load_2d<PAIR>(to + kBytesA + b * Shape::kBoxBytes, &a.rows, bar, k * kBlockK,
-                                     row + b * Shape::kBoxRows);
+              dev::tma_load_2d<PAIR>(to + kBytesA + b * Shape::kBoxBytes, &a.rows, bar, x, row + b * Shape::kBoxRows);
           }
         }
       }
@@ -371,19 +390,20 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
         dev::mma_commit<PAIR>(at.sum_full(sums.stage));
       }
     }
-  } else if (warp == 3) {
+  } else if (warp == 3 && part == 0) {
     // rows that hold no pair: those between the segments by the expert before, those behind the last in equal parts
     uint16_t* out = static_cast<uint16_t*>(a.out);
-    for (int e = blockIdx.x; e < experts; e += gridDim.x) {
+    const int clearing = PAIR ? gridDim.x : t_step, me = PAIR ? blockIdx.x : t0;
+    for (int e = me; e < experts; e += clearing) {
       const int end = s.first[e] + s.count[e];
       if (e + 1 < experts) clear(out, (int64_t)end * a.width, (int64_t)s.first[e + 1] * a.width, lane, 32);
       if (e == 0) clear(out, 0, (int64_t)s.first[0] * a.width, lane, 32);
     }
     const int end = s.first[experts - 1] + s.count[experts - 1], left = a.segments.capacity - end;
-    const int per = (left + gridDim.x - 1) / gridDim.x;
-    const int64_t r0 = end + (int64_t)min((int64_t)left, (int64_t)blockIdx.x * per);
+    const int per = (left + clearing - 1) / clearing;
+    const int64_t r0 = end + min((int64_t)left, (int64_t)me * per);
     clear(out, r0 * a.width, min(r0 + per, (int64_t)a.segments.capacity) * a.width, lane, 32);
-  } else if (warp >= 4) {
+  } else if (warp >= 4 && warp < 8) {
     // the sums to 16 bits, through shared memory from a column of the result to a lane to a row's piece to a lane
     Ring<2> sums;
     const int quarter = warp & 3;
@@ -395,10 +415,28 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
       if (!warp_wait(at.sum_full(sums.stage), sums.parity, limit)) continue;
       dev::tmem_fence_after();
       const int column = tile.column + rank * kTileM + quarter * 32;
+      if (SPLIT && part == 0) {
+        if (!warp_wait<true>(at.parts(), 0, limit)) continue;  // one tile to a cluster
+      }
       for (int c = 0; c < tile.rows; c += 32) {
         uint32_t v[32];
         dev::tmem_load32(p.tmem + sums.stage * BN + c + ((uint32_t)quarter << 21), v);
         dev::tmem_load_wait();
+        if constexpr (SPLIT) {
+          const int row = min(32, tile.rows - c);
+          float* sum = reinterpret_cast<float*>(parts) + c * kTileM + quarter * 32 + lane;  // [part][row][column]
+          if (part != 0) {
+            const uint32_t to = dev::in_first(dev::smem_u32(sum) + (part - 1) * Shape::kPart);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < row) dev::store_first(to + i * kTileM * 4, __uint_as_float(v[i]));
+            continue;
+          }
+          for (int q = 0; q + 1 < all_parts; ++q)  // in the order of the parts
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i < row) v[i] = __float_as_uint(__uint_as_float(v[i]) + sum[q * (Shape::kPart / 4) + i * kTileM]);
+        }
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const uint32_t both = dev::from_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), T{});
@@ -426,11 +464,14 @@ __global__ void __cluster_dims__(PAIR ? 2 : 1, 1, 1) __launch_bounds__(kThreads,
       }
       dev::tmem_fence_before();
       __syncwarp();
-      if (lane == 0) at.release_sum(sums.stage);
+      if (lane == 0) {
+        at.release_sum(sums.stage);
+        if (SPLIT && part != 0) dev::arrive_first(at.parts());
+      }
     }
   }
   __syncwarp();
-  close_pipe(p, Shape::kColumns);
+  close_pipe<PAIR || SPLIT>(p, Shape::kColumns);
 }
 
 // ---------------------------------------------------- the gradient of the weights
@@ -479,7 +520,7 @@ __device__ __forceinline__ bool has_end(int count, int k) { return count - k < k
 // dimension across.  Rows behind the segment's end that the last step brings along are cleared in shared memory: they
 // are another expert's, or anything at all.
 template <typename T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, 1)
     grad_weights_kernel(const __grid_constant__ GradArgs a) {
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (align_up(dev::smem_u32(raw), 1024) - dev::smem_u32(raw));
@@ -491,7 +532,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const PipeAt<kGradStages, true> at(p);
   const dev::WaitLimit limit{&p.gave_up, a.limit_ns};
 
-  init_pipe(p, 512);
+  init_pipe<true>(p, 512);
   dev::wait_for_previous();
   for (int e = threadIdx.x; e < a.segments.experts; e += kThreads) segments[e] = segment(a.segments, e);
   __syncthreads();
@@ -500,21 +541,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t t0 = blockIdx.x / 2, t_step = gridDim.x / 2;
   const uint32_t stages = dev::smem_u32(base);
 
-  if (warp == 0 || warp == 2) {  // an operand each
+  if (brings(warp)) {
     if (dev::elect_one()) {
       Ring<kGradStages> ring;
+      uint32_t turn = (warp == 2 || warp == 9);  // whether it takes the odd steps
       for (uint32_t t = t0; t < tiles; t += t_step) {
         const GradTile g = grad_tile(a, segments, t);
         const int slow = g.slow + rank * kTileM, fast = g.fast + rank * g.chunks * kBlockK;
         const uint32_t bytes = (2 + g.chunks) * kChunkBytes;
         for (int k = 0; k < g.segment.y; k += kBlockK, ring.next()) {
-          if (!dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
+          if ((turn ^= 1) == 0 || !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
           const uint32_t to = stages + ring.stage * kGradStage;
           const int row = g.segment.x + k;
           // each CTA looks after the end of a segment in its own copies
           const bool end = has_end(g.segment.y, k);
           const uint32_t bar = end ? at.end(ring.stage) : dev::in_first(at.full(ring.stage));
-          if (warp == 0) {
+          if (warp < 8) {
             if (end) dev::arrive_expect(at.end(ring.stage), bytes);
             else if (rank == 0) dev::arrive_expect(at.full(ring.stage), 2 * bytes);
             dev::tma_load_2d<true>(to, &a.slow, bar, slow, row);
@@ -591,7 +633,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       parity ^= 1u << ring.stage;
       ring.next();
     }
-  } else if (warp >= 4) {
+  } else if (warp >= 4 && warp < 8) {
     Ring<2> sums;
     const int quarter = warp & 3;
     uint8_t* mine = staging + quarter * kStoreBoxes * kStoreBox;
@@ -662,7 +704,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     dev::store_wait<0>();
   }
   __syncwarp();
-  close_pipe(p, 512);
+  close_pipe<true>(p, 512);
 }
 
 // --------------------------------------------------------- operands laid out anew
@@ -729,27 +771,28 @@ struct Operand {
   }
 };
 
+// Over `ctas` CTAs to a tile, a cluster.
 template <typename Kernel, typename Args>
 cudaError_t run(Kernel kernel, const Args& a, int64_t tiles, int ctas, size_t smem, cudaStream_t stream) {
   // the limit is the kernel's, not the call's: the same one from every host thread
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
   if (e) return e;
-  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(kSms / ctas, tiles)) * ctas;  // ctas to a tile
-  return launch_after_previous(kernel, grid, kThreads, smem, a, stream);
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(kSms / ctas, tiles)) * ctas;
+  return launch_after_previous(kernel, grid, kThreads, smem, a, stream, ctas);
 }
 
-template <typename T, int BN, int STAGES, bool PAIR>
-cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order, int64_t row_tiles,
+template <typename T, int BN, int STAGES, bool PAIR, bool SPLIT>
+cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order, int64_t row_tiles, int ctas,
                     cudaStream_t stream) {
-  using Shape = ProductShape<BN, STAGES, PAIR>;
+  using Shape = ProductShape<BN, STAGES, PAIR, SPLIT>;
   a.width_tiles = (a.width + Shape::kTile - 1) / Shape::kTile;
   cudaError_t e = weights.map(&a.weights, false, in_order ? kTileM : kBlockK);
   if (!e) e = rows.map(&a.rows, true, Shape::kBoxRows);
   if (e) return e;
   const size_t smem = Shape::bytes(a.segments.experts);
   const int64_t tiles = row_tiles * a.width_tiles;
-  return in_order ? run(product_kernel<T, BN, STAGES, PAIR, true>, a, tiles, Shape::kCtas, smem, stream)
-                  : run(product_kernel<T, BN, STAGES, PAIR, false>, a, tiles, Shape::kCtas, smem, stream);
+  return in_order ? run(product_kernel<T, BN, STAGES, PAIR, SPLIT, true>, a, tiles, ctas, smem, stream)
+                  : run(product_kernel<T, BN, STAGES, PAIR, SPLIT, false>, a, tiles, ctas, smem, stream);
 }
 
 bool half_type(int type) { return type == CUSORT_FLOAT_F16 || type == CUSORT_FLOAT_BF16; }
@@ -798,14 +841,18 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   // at most one part-filled tile to an expert, and no expert without a row
   const int64_t tiles = capacity / (few ? kFewRows : kManyRows) + std::min<int64_t>(num_experts, capacity);
   if (tiles * ((out + kTileM - 1) / kTileM) > INT32_MAX) return cudaErrorInvalidValue;
+  // Fewer tiles than SMs: several CTAs to a tile, which split what is contracted.
+  const int64_t all = tiles * ((out + kTileM - 1) / kTileM), steps = (in + kBlockK - 1) / kBlockK;
+  const int parts = (int)std::min<int64_t>({kMostParts, kSms / all, steps / 4});
   uint8_t* temp = static_cast<uint8_t*>(d_temp_storage);
   cudaError_t e = rows.prepare(temp, nullptr, stream);
   if (!e) e = weights.prepare(temp, d_counts, stream);
   if (e) return e;
   const auto go = [&](auto t) {
     using T = decltype(t);
-    return few ? product<T, kFewRows, 8, false>(a, weights, rows, in_order, tiles, stream)
-               : product<T, kManyRows, 6, true>(a, weights, rows, in_order, tiles, stream);
+    if (!few) return product<T, kManyRows, 6, true, false>(a, weights, rows, in_order, tiles, 2, stream);
+    return parts > 1 ? product<T, kFewRows, 5, false, true>(a, weights, rows, in_order, tiles, parts, stream)
+                     : product<T, kFewRows, 8, false, false>(a, weights, rows, in_order, tiles, 1, stream);
   };
   return type == CUSORT_FLOAT_F16 ? go(__half{}) : go(__nv_bfloat16{});
 }

@@ -24,21 +24,25 @@ __device__ __forceinline__ void wait_for_previous() { pdl_wait(); }
 
 }  // namespace dev
 
-// Launches a kernel that begins with wait_for_previous().
+// Launches a kernel that begins with wait_for_previous(), over clusters of
+// `cluster` CTAs.
 template <typename Args>
 cudaError_t launch_after_previous(void (*kernel)(Args), int64_t grid, int threads, size_t smem, const Args& args,
-                                  cudaStream_t stream) {
+                                  cudaStream_t stream, int cluster = 1) {
   if (grid < 1 || grid > INT32_MAX) return cudaErrorInvalidValue;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute at[2] = {};
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)cluster;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, args);
 }
 

@@ -87,6 +87,13 @@ def test_few_rows_an_expert(fin, fout, dtype, order):
 
 
 @pytest.mark.parametrize("order", ["in_out", "out_in"])
+@pytest.mark.parametrize("counts", [[1], [0, 2, 0, 64], [1, 33, 0, 5, 0, 0, 1, 70]], ids=str)
+@pytest.mark.parametrize("fin,fout", [(520, 136), (1032, 264), (2049, 200), (4096, 128)])
+def test_few_tiles_with_a_long_contracted_dimension(fin, fout, counts, order):
+    check(counts, fin, fout, "bf16", order)
+
+
+@pytest.mark.parametrize("order", ["in_out", "out_in"])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("fin,fout", [(64, 128), (264, 136), (136, 520)])
 def test_many_rows_an_expert(fin, fout, dtype, order):
