@@ -41,7 +41,7 @@ cudaError_t encode_map(CUtensorMap* map, const void* base, int rank, const uint6
   for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i];
   // both types have 16 bits, and nothing but zeros outside depends on which it is
   const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d, s, b, one,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
@@ -486,9 +486,9 @@ struct GradArgs {
 };
 
 constexpr int kGradN = 256;
-constexpr int kGradStages = 5;
+constexpr int kGradStages = 6;
 constexpr uint32_t kGradStage = kBytesA + kGradN / 2 * kBlockK * 2;
-constexpr uint32_t kStoreBox = 32 * 128;             // 32 rows of 64 elements, stored as one box
+constexpr uint32_t kStoreBox = 32 * 64;              // 32 rows of 32 elements, stored as one box
 constexpr int kStoreBoxes = 3;                       // for each storing warp: one is filled, others are being stored
 constexpr uint32_t kGradStaging = 4 * kStoreBoxes * kStoreBox;
 constexpr int kChunkBytes = kBytesA / 2;  // 64 contracted rows of 64 elements
@@ -651,31 +651,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         dev::tmem_fence_after();
       }
-      for (int c = 0; c < columns; c += kBlockK, filled = (filled + 1) % kStoreBoxes) {
-        uint32_t v[2][32];
+      for (int c = 0; c < columns; c += 32) {
+        uint32_t v[32];
         if (empty) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[0][i] = v[1][i] = 0;
+          for (int i = 0; i < 32; ++i) v[i] = 0;
         } else {
-          const uint32_t sum = p.tmem + sums.stage * kGradN + c + ((uint32_t)quarter << 21);
-          dev::tmem_load32(sum, v[0]);
-          dev::tmem_load32(sum + 32, v[1]);
+          dev::tmem_load32(p.tmem + sums.stage * kGradN + c + ((uint32_t)quarter << 21), v);
           dev::tmem_load_wait();
         }
         if (rows <= 0) continue;
-        // 16-byte pieces in the order of the tiled copies: the piece's number within 128 bytes xor the row's within 8
+        // 16-byte pieces in the order of the tiled copies of 64-byte rows: the piece's number xor that of the row pair
         uint8_t* box = mine + filled * kStoreBox;
         dev::store_wait<kStoreBoxes - 1>();
         __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t* x = v[j / 4] + j % 4 * 8;
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t* x = v + j * 8;
           uint4 w;
           w.x = dev::from_float2(__uint_as_float(x[0]), __uint_as_float(x[1]), T{});
           w.y = dev::from_float2(__uint_as_float(x[2]), __uint_as_float(x[3]), T{});
           w.z = dev::from_float2(__uint_as_float(x[4]), __uint_as_float(x[5]), T{});
           w.w = dev::from_float2(__uint_as_float(x[6]), __uint_as_float(x[7]), T{});
-          *reinterpret_cast<uint4*>(box + lane * 128 + ((j ^ (lane & 7)) * 16)) = w;
+          *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ (lane >> 1 & 3)) * 16)) = w;
         }
         if (whole) {
           dev::fence_proxy_async_smem();
@@ -684,15 +682,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           __syncwarp();
           T* out = static_cast<T*>(a.result) + ((int64_t)g.expert * a.slow_width + m) * a.fast_width + g.fast + c;
-          for (int half = 0; half < 2; ++half) {
-            const int i = half * 32 + lane;
-            if (c + i < columns)
-              for (int row = 0; row < rows; ++row)
-                out[(int64_t)row * a.fast_width + i] =
-                    *reinterpret_cast<const T*>(box + row * 128 + ((i / 8 ^ (row & 7)) * 16) + i % 8 * 2);
-          }
+          if (c + lane < columns)
+            for (int row = 0; row < rows; ++row)
+              out[(int64_t)row * a.fast_width + lane] =
+                  *reinterpret_cast<const T*>(box + row * 64 + ((lane / 8 ^ (row >> 1 & 3)) * 16) + lane % 8 * 2);
           __syncwarp();
         }
+        filled = (filled + 1) % kStoreBoxes;
       }
       if (!empty) {
         dev::tmem_fence_before();
@@ -761,12 +757,12 @@ struct Operand {
     return launch_after_previous(repack_kernel, std::min<int64_t>(kSms * 8, (a.rows + 7) / 8), 256, 0, a, stream);
   }
 
-  cudaError_t map(CUtensorMap* m, bool matrix, uint32_t box_rows) const {
+  cudaError_t map(CUtensorMap* m, bool matrix, uint32_t box_rows, uint32_t box_width = kBlockK) const {
     // strides of dimensions of one element are never used, but have to be in order
     const uint64_t row = (uint64_t)(rows > 1 ? row_stride : pitch()) * 2;
     const uint64_t dims[3] = {(uint64_t)width, (uint64_t)rows, (uint64_t)outer};
     const uint64_t strides[2] = {row, outer > 1 ? (uint64_t)outer_stride * 2 : row * rows};
-    const uint32_t box[3] = {kBlockK, box_rows, 1};
+    const uint32_t box[3] = {box_width, box_rows, 1};
     return encode_map(m, data, matrix ? 2 : 3, dims, strides, box);
   }
 };
@@ -843,7 +839,7 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   if (tiles * ((out + kTileM - 1) / kTileM) > INT32_MAX) return cudaErrorInvalidValue;
   // Fewer tiles than SMs: several CTAs to a tile, which split what is contracted.
   const int64_t all = tiles * ((out + kTileM - 1) / kTileM), steps = (in + kBlockK - 1) / kBlockK;
-  const int parts = (int)std::min<int64_t>({kMostParts, kSms / all, steps / 4});
+  const int parts = (int)std::min<int64_t>({kMostParts, all > 74 ? 1 : all > 45 ? 2 : 3, steps / 4});
   uint8_t* temp = static_cast<uint8_t*>(d_temp_storage);
   cudaError_t e = rows.prepare(temp, nullptr, stream);
   if (!e) e = weights.prepare(temp, d_counts, stream);
@@ -895,7 +891,7 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
   if (!e) e = fast.map(&a.fast, true, kBlockK);
   if (!e && fast.width % 8 == 0) {
     const Operand out{d_grad_weights, num_experts, slow.width, fast.width, slow.width * fast.width, fast.width};
-    e = out.map(&a.out, false, 32);
+    e = out.map(&a.out, false, 32, 32);
   }
   if (e) return e;
   return type == CUSORT_FLOAT_F16 ? run(grad_weights_kernel<__half>, a, tiles, 2, grad_bytes(num_experts), stream)

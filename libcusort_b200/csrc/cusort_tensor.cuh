@@ -54,8 +54,8 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 }
 
 // A box from shared memory, what lies outside the tensor left out; a group of
-// one.  The thread's groups but the last N have been read when store_wait
-// returns.
+// one.  All of the thread's groups but the last N have been read when
+// store_wait returns.
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map),
                "r"(src), "r"(x), "r"(y), "r"(z)
@@ -256,9 +256,9 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, WaitLimi
 
 }  // namespace dev
 
-// Tensor map of 16-bit elements with 128-byte swizzle, zeros outside.  dims
-// and box from the contiguous dimension on; strides in bytes, of the
-// dimensions after it.
+// Tensor map of 16-bit elements, zeros outside.  dims and box from the
+// contiguous dimension on; strides in bytes, of the dimensions after it.  The
+// box's rows are 128 or 64 bytes, whose swizzle it has.
 cudaError_t encode_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
                        const uint32_t* box);
 
