@@ -141,7 +141,6 @@ template <int STAGES, bool PAIR> struct Pipe {
   uint64_t end[STAGES];    // a stage's copies of this CTA are there, which hold the end of a segment
   uint64_t ended[STAGES];  // in the first of two CTAs: both have cleared what lies behind that
   uint64_t sum_full[2], sum_empty[2];
-  uint64_t parts;          // in the first CTA of a split tile: the others' sums are there
   uint32_t tmem, gave_up, sums[kThreads / 32];
 };
 
@@ -156,7 +155,6 @@ template <int STAGES, bool PAIR> struct PipeAt {
   __device__ __forceinline__ uint32_t ended(int i) const { return base + offsetof(P, ended) + 8 * i; }
   __device__ __forceinline__ uint32_t sum_full(int i) const { return base + offsetof(P, sum_full) + 8 * i; }
   __device__ __forceinline__ uint32_t sum_empty(int i) const { return base + offsetof(P, sum_empty) + 8 * i; }
-  __device__ __forceinline__ uint32_t parts() const { return base + offsetof(P, parts); }
   // The storing warps have read a sum: one lane says so.
   __device__ __forceinline__ void release_sum(int i) const {
     if (PAIR) dev::arrive_first(sum_empty(i));
@@ -164,7 +162,7 @@ template <int STAGES, bool PAIR> struct PipeAt {
   }
 };
 
-template <bool CLUSTER, int STAGES, bool PAIR>
+template <int STAGES, bool PAIR>
 __device__ __forceinline__ void init_pipe(Pipe<STAGES, PAIR>& p, uint32_t columns) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
@@ -174,23 +172,22 @@ __device__ __forceinline__ void init_pipe(Pipe<STAGES, PAIR>& p, uint32_t column
       dev::mbar_init(&p.ended[i], 2);
     }
     for (int i = 0; i < 2; ++i) dev::mbar_init(&p.sum_full[i], 1), dev::mbar_init(&p.sum_empty[i], PAIR ? 8 : 4);
-    if (CLUSTER && !PAIR) dev::mbar_init(&p.parts, 4 * (dev::cluster_size() - 1));
     p.gave_up = 0;
     dev::fence_mbar_init();
   }
   __syncwarp();
   if (threadIdx.x / 32 == 1) dev::tmem_alloc<PAIR>(&p.tmem, columns);
   dev::tmem_fence_before();
-  if (CLUSTER) dev::cluster_sync();
+  if (PAIR) dev::cluster_sync();
   else __syncthreads();
   dev::tmem_fence_after();
 }
 
 // The end of every warp's work: tensor memory is given back.
-template <bool CLUSTER, int STAGES, bool PAIR>
+template <int STAGES, bool PAIR>
 __device__ __forceinline__ void close_pipe(Pipe<STAGES, PAIR>& p, uint32_t columns) {
   dev::tmem_fence_before();
-  if (CLUSTER) dev::cluster_sync();
+  if (PAIR) dev::cluster_sync();
   else __syncthreads();
   if (threadIdx.x == 0 && p.gave_up) atomicOr(&g_product_status, 1u);
   if (threadIdx.x / 32 == 1) {
@@ -222,10 +219,9 @@ __device__ __forceinline__ void settle(const dev::WaitLimit& limit) {
 }
 
 // A wait of a whole warp, by one lane: 32 of them keep shared memory busy.
-template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const dev::WaitLimit& limit) {
   bool ok = true;
-  if ((threadIdx.x & 31) == 0) ok = dev::wait_for<CLUSTER>(bar, parity, limit);
+  if ((threadIdx.x & 31) == 0) ok = dev::wait_for(bar, parity, limit);
   __syncwarp();
   return __shfl_sync(kAll, ok, 0);
 }
@@ -262,21 +258,17 @@ struct ProductArgs {
 };
 
 // PAIR: tiles of 256 columns of the result, 128 in each of two CTAs, and half of the rows in each.
-// SPLIT: the contracted dimension in equal parts over the CTAs of a cluster, kMostParts of them at most.
-constexpr int kMostParts = 3;
-template <int BN_, int STAGES, bool PAIR, bool SPLIT> struct ProductShape {
-  static constexpr int BN = BN_;
+template <int BN, int STAGES, int SUB, bool PAIR> struct ProductShape {
   static constexpr int kCtas = PAIR ? 2 : 1, kTile = kTileM * kCtas;
   static constexpr int kRowStep = 16 * kCtas;       // the instruction's width comes in such steps
   static constexpr int kBoxRows = PAIR ? 64 : 16;   // a tile of few rows brings few boxes
-  static constexpr uint32_t kBytesB = BN / kCtas * kBlockK * 2, kStage = kBytesA + kBytesB;
+  // A stage holds SUB steps of kBlockK, each the weights' part and then the rows'.
+  static constexpr uint32_t kBytesB = BN / kCtas * kBlockK * 2, kStep = kBytesA + kBytesB, kStage = SUB * kStep;
   static constexpr uint32_t kBoxBytes = kBoxRows * dev::kBoxRowBytes;
   static constexpr uint32_t kColumns = 2 * BN;
   static constexpr uint32_t kStaging = 4 * 2048;  // 32 x 32 16-bit elements for each storing warp
-  static constexpr uint32_t kPart = SPLIT ? BN * kTileM * 4 : 0;  // the sums of one of the other CTAs
   static size_t bytes(int experts) {
-    return 1024 + STAGES * kStage + (kMostParts - 1) * kPart + kStaging + sizeof(Pipe<STAGES, PAIR>) +
-           4 * (3 * (size_t)experts + 1);
+    return 1024 + STAGES * kStage + kStaging + sizeof(Pipe<STAGES, PAIR>) + 4 * (3 * (size_t)experts + 1);
   }
 };
 
@@ -303,13 +295,12 @@ __device__ __forceinline__ ProductTile product_tile(const ProductArgs& a, const 
 // the instruction's width is the number of rows, in steps of 16: an expert
 // with three rows costs a width of 16, and its weights stream through the
 // lanes.
-template <typename T, int BN, int STAGES, bool PAIR, bool SPLIT, bool IN_ORDER>
+template <typename T, int BN, int STAGES, int SUB, bool PAIR, bool IN_ORDER>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
-  using Shape = ProductShape<BN, STAGES, PAIR, SPLIT>;
+  using Shape = ProductShape<BN, STAGES, SUB, PAIR>;
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (align_up(dev::smem_u32(raw), 1024) - dev::smem_u32(raw));
-  uint8_t* parts = base + STAGES * Shape::kStage;
-  uint8_t* staging = parts + (kMostParts - 1) * Shape::kPart;
+  uint8_t* staging = base + STAGES * Shape::kStage;
   Pipe<STAGES, PAIR>& p = *reinterpret_cast<Pipe<STAGES, PAIR>*>(staging + Shape::kStaging);
   const int experts = a.segments.experts;
   Segments s;
@@ -320,16 +311,13 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
   const PipeAt<STAGES, PAIR> at(p);
   const dev::WaitLimit limit{&p.gave_up, a.limit_ns};
 
-  init_pipe<PAIR || SPLIT>(p, Shape::kColumns);
+  init_pipe(p, Shape::kColumns);
   dev::wait_for_previous();
   load_segments(a.segments, s, p.sums, [](int count) { return (count + BN - 1) / BN; });
   const uint32_t tiles = (uint32_t)s.tiles[experts] * a.width_tiles;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = PAIR ? dev::cluster_rank() : 0;
-  const int part = SPLIT ? dev::cluster_rank() : 0, all_parts = SPLIT ? dev::cluster_size() : 1;
-  const int all_steps = (a.in + kBlockK - 1) / kBlockK;
-  const int first_step = all_steps * part / all_parts, steps = all_steps * (part + 1) / all_parts - first_step;
-  const int ctas = SPLIT ? all_parts : Shape::kCtas;  // to a tile
-  const uint32_t t0 = blockIdx.x / ctas, t_step = gridDim.x / ctas;
+  const int steps = (a.in + SUB * kBlockK - 1) / (SUB * kBlockK);
+  const uint32_t t0 = blockIdx.x / Shape::kCtas, t_step = gridDim.x / Shape::kCtas;
   const uint32_t stages = dev::smem_u32(base);
 
   if (brings(warp)) {
@@ -341,24 +329,27 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         const int column = tile.column + rank * kTileM;
         const int mine = align_up(tile.rows, Shape::kRowStep) / Shape::kCtas, row = tile.row + rank * mine;
         const int boxes = (mine + Shape::kBoxRows - 1) / Shape::kBoxRows;
-        const uint32_t bytes = Shape::kCtas * (kBytesA + boxes * Shape::kBoxBytes);
+        const uint32_t bytes = SUB * Shape::kCtas * (kBytesA + boxes * Shape::kBoxBytes);
         for (int k = 0; k < steps; ++k, ring.next()) {
           if ((turn ^= 1) == 0 || !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
           const uint32_t to = stages + ring.stage * Shape::kStage, own = at.full(ring.stage);
           const uint32_t bar = PAIR ? dev::in_first(own) : own;
-          const int x = (first_step + k) * kBlockK;
-          if (warp < 8) {
-            // the first CTA's barrier counts the copies of both
-            if (rank == 0) dev::arrive_expect(own, bytes);
-            if (IN_ORDER) {
-              dev::tma_load_3d<PAIR>(to, &a.weights, bar, x, column, tile.expert);
+          // the first CTA's barrier counts the copies of both
+          if (warp < 8 && rank == 0) dev::arrive_expect(own, bytes);
+#pragma unroll
+          for (int u = 0; u < SUB; ++u) {
+            const int x = (k * SUB + u) * kBlockK;
+            const uint32_t step = to + u * Shape::kStep;
+            if (warp >= 8) {
+              for (int b = 0; b < boxes; ++b)
+                dev::tma_load_2d<PAIR>(step + kBytesA + b * Shape::kBoxBytes, &a.rows, bar, x,
+                                       row + b * Shape::kBoxRows);
+            } else if (IN_ORDER) {
+              dev::tma_load_3d<PAIR>(step, &a.weights, bar, x, column, tile.expert);
             } else {
-              dev::tma_load_3d<PAIR>(to, &a.weights, bar, column, x, tile.expert);
-              dev::tma_load_3d<PAIR>(to + kBytesA / 2, &a.weights, bar, column + kBlockK, x, tile.expert);
+              dev::tma_load_3d<PAIR>(step, &a.weights, bar, column, x, tile.expert);
+              dev::tma_load_3d<PAIR>(step + kBytesA / 2, &a.weights, bar, column + kBlockK, x, tile.expert);
             }
-          } else {
-            for (int b = 0; b < boxes; ++b)
-              dev::tma_load_2d<PAIR>(to + kBytesA + b * Shape::kBoxBytes, &a.rows, bar, x, row + b * Shape::kBoxRows);
           }
         }
       }
@@ -382,18 +373,20 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           dev::tmem_fence_after();
           const uint32_t stage = ring.stage * (Shape::kStage / 16);
 #pragma unroll
-          for (int i = 0; i < kBlockK / 16; ++i)
-            dev::mma_issue<PAIR>(sum, first_a + stage + i * (IN_ORDER ? 32 : 2048) / 16, first_b + stage + i * 32 / 16,
-                                 instruction, k + i > 0);
+          for (int u = 0; u < SUB; ++u)
+#pragma unroll
+            for (int i = 0; i < kBlockK / 16; ++i)
+              dev::mma_issue<PAIR>(sum, first_a + stage + (u * Shape::kStep + i * (IN_ORDER ? 32 : 2048)) / 16,
+                                   first_b + stage + (u * Shape::kStep + i * 32) / 16, instruction, k + u + i > 0);
           dev::mma_commit<PAIR>(at.empty(ring.stage));
         }
         dev::mma_commit<PAIR>(at.sum_full(sums.stage));
       }
     }
-  } else if (warp == 3 && part == 0) {
+  } else if (warp == 3) {
     // rows that hold no pair: those between the segments by the expert before, those behind the last in equal parts
     uint16_t* out = static_cast<uint16_t*>(a.out);
-    const int clearing = PAIR ? gridDim.x : t_step, me = PAIR ? blockIdx.x : t0;
+    const int clearing = gridDim.x, me = blockIdx.x;
     for (int e = me; e < experts; e += clearing) {
       const int end = s.first[e] + s.count[e];
       if (e + 1 < experts) clear(out, (int64_t)end * a.width, (int64_t)s.first[e + 1] * a.width, lane, 32);
@@ -415,28 +408,10 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       if (!warp_wait(at.sum_full(sums.stage), sums.parity, limit)) continue;
       dev::tmem_fence_after();
       const int column = tile.column + rank * kTileM + quarter * 32;
-      if (SPLIT && part == 0) {
-        if (!warp_wait<true>(at.parts(), 0, limit)) continue;  // one tile to a cluster
-      }
       for (int c = 0; c < tile.rows; c += 32) {
         uint32_t v[32];
         dev::tmem_load32(p.tmem + sums.stage * BN + c + ((uint32_t)quarter << 21), v);
         dev::tmem_load_wait();
-        if constexpr (SPLIT) {
-          const int row = min(32, tile.rows - c);
-          float* sum = reinterpret_cast<float*>(parts) + c * kTileM + quarter * 32 + lane;  // [part][row][column]
-          if (part != 0) {
-            const uint32_t to = dev::in_first(dev::smem_u32(sum) + (part - 1) * Shape::kPart);
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < row) dev::store_first(to + i * kTileM * 4, __uint_as_float(v[i]));
-            continue;
-          }
-          for (int q = 0; q + 1 < all_parts; ++q)  // in the order of the parts
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (i < row) v[i] = __float_as_uint(__uint_as_float(v[i]) + sum[q * (Shape::kPart / 4) + i * kTileM]);
-        }
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const uint32_t both = dev::from_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), T{});
@@ -464,14 +439,11 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       }
       dev::tmem_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        at.release_sum(sums.stage);
-        if (SPLIT && part != 0) dev::arrive_first(at.parts());
-      }
+      if (lane == 0) at.release_sum(sums.stage);
     }
   }
   __syncwarp();
-  close_pipe<PAIR || SPLIT>(p, Shape::kColumns);
+  close_pipe(p, Shape::kColumns);
 }
 
 // ---------------------------------------------------- the gradient of the weights
@@ -532,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const PipeAt<kGradStages, true> at(p);
   const dev::WaitLimit limit{&p.gave_up, a.limit_ns};
 
-  init_pipe<true>(p, 512);
+  init_pipe(p, 512);
   dev::wait_for_previous();
   for (int e = threadIdx.x; e < a.segments.experts; e += kThreads) segments[e] = segment(a.segments, e);
   __syncthreads();
@@ -700,7 +672,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     dev::store_wait<0>();
   }
   __syncwarp();
-  close_pipe<true>(p, 512);
+  close_pipe(p, 512);
 }
 
 // --------------------------------------------------------- operands laid out anew
@@ -777,18 +749,18 @@ cudaError_t run(Kernel kernel, const Args& a, int64_t tiles, int ctas, size_t sm
   return launch_after_previous(kernel, grid, kThreads, smem, a, stream, ctas);
 }
 
-template <typename T, int BN, int STAGES, bool PAIR, bool SPLIT>
-cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order, int64_t row_tiles, int ctas,
+template <typename T, int BN, int STAGES, int SUB, bool PAIR>
+cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order, int64_t row_tiles,
                     cudaStream_t stream) {
-  using Shape = ProductShape<BN, STAGES, PAIR, SPLIT>;
+  using Shape = ProductShape<BN, STAGES, SUB, PAIR>;
   a.width_tiles = (a.width + Shape::kTile - 1) / Shape::kTile;
   cudaError_t e = weights.map(&a.weights, false, in_order ? kTileM : kBlockK);
   if (!e) e = rows.map(&a.rows, true, Shape::kBoxRows);
   if (e) return e;
   const size_t smem = Shape::bytes(a.segments.experts);
   const int64_t tiles = row_tiles * a.width_tiles;
-  return in_order ? run(product_kernel<T, BN, STAGES, PAIR, SPLIT, true>, a, tiles, ctas, smem, stream)
-                  : run(product_kernel<T, BN, STAGES, PAIR, SPLIT, false>, a, tiles, ctas, smem, stream);
+  return in_order ? run(product_kernel<T, BN, STAGES, SUB, PAIR, true>, a, tiles, Shape::kCtas, smem, stream)
+                  : run(product_kernel<T, BN, STAGES, SUB, PAIR, false>, a, tiles, Shape::kCtas, smem, stream);
 }
 
 bool half_type(int type) { return type == CUSORT_FLOAT_F16 || type == CUSORT_FLOAT_BF16; }
@@ -837,18 +809,14 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   // at most one part-filled tile to an expert, and no expert without a row
   const int64_t tiles = capacity / (few ? kFewRows : kManyRows) + std::min<int64_t>(num_experts, capacity);
   if (tiles * ((out + kTileM - 1) / kTileM) > INT32_MAX) return cudaErrorInvalidValue;
-  // Fewer tiles than SMs: several CTAs to a tile, which split what is contracted.
-  const int64_t all = tiles * ((out + kTileM - 1) / kTileM), steps = (in + kBlockK - 1) / kBlockK;
-  const int parts = (int)std::min<int64_t>({kMostParts, all > 74 ? 1 : all > 45 ? 2 : 3, steps / 4});
   uint8_t* temp = static_cast<uint8_t*>(d_temp_storage);
   cudaError_t e = rows.prepare(temp, nullptr, stream);
   if (!e) e = weights.prepare(temp, d_counts, stream);
   if (e) return e;
   const auto go = [&](auto t) {
     using T = decltype(t);
-    if (!few) return product<T, kManyRows, 6, true, false>(a, weights, rows, in_order, tiles, 2, stream);
-    return parts > 1 ? product<T, kFewRows, 5, false, true>(a, weights, rows, in_order, tiles, parts, stream)
-                     : product<T, kFewRows, 8, false, false>(a, weights, rows, in_order, tiles, 1, stream);
+    return few ? product<T, kFewRows, 4, 2, false>(a, weights, rows, in_order, tiles, stream)
+               : product<T, kManyRows, 6, 1, true>(a, weights, rows, in_order, tiles, stream);
   };
   return type == CUSORT_FLOAT_F16 ? go(__half{}) : go(__nv_bfloat16{});
 }
