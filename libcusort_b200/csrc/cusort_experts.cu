@@ -431,9 +431,15 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
               *reinterpret_cast<uint4*>(out + (first + row) * a.width + x) =
                   *reinterpret_cast<const uint4*>(mine + row * 64 + lane % 4 * 16);
           }
-        } else if (column + lane < a.width) {
-          for (int row = 0; row < rows; ++row)
-            out[(first + row) * a.width + column + lane] = *reinterpret_cast<const T*>(mine + row * 64 + lane * 2);
+        } else {
+          T x[32];
+#pragma unroll
+          for (int row = 0; row < 32; ++row) x[row] = *reinterpret_cast<const T*>(mine + row * 64 + lane * 2);
+          T* to = out + first * a.width + column + lane;
+          const int there = column + lane < a.width ? rows : 0;
+#pragma unroll
+          for (int row = 0; row < 32; ++row, to += a.width)
+            if (row < there) *to = x[row];
         }
         __syncwarp();
       }
@@ -654,10 +660,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           __syncwarp();
           T* out = static_cast<T*>(a.result) + ((int64_t)g.expert * a.slow_width + m) * a.fast_width + g.fast + c;
-          if (c + lane < columns)
-            for (int row = 0; row < rows; ++row)
-              out[(int64_t)row * a.fast_width + lane] =
-                  *reinterpret_cast<const T*>(box + row * 64 + ((lane / 8 ^ (row >> 1 & 3)) * 16) + lane % 8 * 2);
+          T x[32];
+#pragma unroll
+          for (int row = 0; row < 32; ++row)
+            x[row] = *reinterpret_cast<const T*>(box + row * 64 + ((lane / 8 ^ (row >> 1 & 3)) * 16) + lane % 8 * 2);
+          out += lane;
+          const int there = c + lane < columns ? rows : 0;
+#pragma unroll
+          for (int row = 0; row < 32; ++row, out += a.fast_width)
+            if (row < there) *out = x[row];
           __syncwarp();
         }
         filled = (filled + 1) % kStoreBoxes;
@@ -678,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // --------------------------------------------------------- operands laid out anew
 
 struct RepackArgs {
-  const uint16_t* x;
+  const uint16_t *x, *x_end;  // x_end: behind the last element of all
   uint16_t* y;
   int64_t outer_stride, row_stride, pitch;  // elements
   int64_t rows;                             // of all outer parts together
@@ -686,18 +697,68 @@ struct RepackArgs {
   const int32_t* counts;  // where it is given: outer parts with none are left out
 };
 
+// The 16-byte word at `word`, of which the elements in [x, end) are read.
+__device__ __forceinline__ uint4 load_word(const uint4* word, const uint16_t* x, const uint16_t* end) {
+  const uint16_t* e = reinterpret_cast<const uint16_t*>(word);
+  if (e >= x && e + 8 <= end) return *word;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t low = e + 2 * i >= x && e + 2 * i < end ? e[2 * i] : 0;
+    const uint32_t high = e + 2 * i + 1 >= x && e + 2 * i + 1 < end ? e[2 * i + 1] : 0;
+    w[i] = low | high << 16;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 16 bytes from byte `shift` (even, below 16) of two words on.
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, int shift) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  uint32_t v[5];
+  switch (shift >> 2) {  // the same in the whole warp
+#define TAKE(q) \
+  case q: \
+    _Pragma("unroll") for (int i = 0; i < 5; ++i) v[i] = w[q + i < 8 ? q + i : 7]; \
+    break;
+    TAKE(0) TAKE(1) TAKE(2) TAKE(3)
+#undef TAKE
+  }
+  const uint32_t order = shift & 2 ? 0x5432 : 0x3210;
+  return make_uint4(__byte_perm(v[0], v[1], order), __byte_perm(v[1], v[2], order), __byte_perm(v[2], v[3], order),
+                    __byte_perm(v[3], v[4], order));
+}
+
 // Rows of a width or at an address that the tiled copies do not take (they want 16-byte steps), copied to where they
-// do: y[r] = x's row r, `pitch` elements apart.  One warp to a row; bound by the narrow loads.
+// do: y[r] = x's row r, `pitch` elements apart, whole 16-byte words of it (what lies behind the row's end is anything).
+// One warp to a row, two aligned words shifted together for each one stored; bound by memory.
 __global__ void __launch_bounds__(256) repack_kernel(const __grid_constant__ RepackArgs a) {
   dev::wait_for_previous();
-  const int lane = threadIdx.x & 31;
+  constexpr int U = 4;
+  const int lane = threadIdx.x & 31, words = (a.width + 7) / 8;
   for (int64_t r = blockIdx.x * 8ll + (threadIdx.x >> 5); r < a.rows; r += gridDim.x * 8ll) {
     const int64_t outer = r / a.per_outer;
     if (a.counts != nullptr && a.counts[outer] <= 0) continue;
     const uint16_t* x = a.x + outer * a.outer_stride + (r - outer * a.per_outer) * a.row_stride;
-    uint16_t* y = a.y + r * a.pitch;
-#pragma unroll 8
-    for (int i = lane; i < a.width; i += 32) y[i] = x[i];
+    const int shift = reinterpret_cast<uintptr_t>(x) & 15;
+    const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(x) - shift);
+    const uint16_t* row_end = x + a.width;
+    uint4* to = reinterpret_cast<uint4*>(a.y + r * a.pitch);
+    for (int i0 = lane; i0 < words; i0 += 32 * U) {
+      uint4 w[U][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + 32 * u;
+        w[u][0] = w[u][1] = make_uint4(0, 0, 0, 0);
+        if (i < words) {
+          w[u][0] = load_word(from + i, a.x, a.x_end);
+          if (shift && reinterpret_cast<const uint16_t*>(from + i + 1) < row_end)
+            w[u][1] = load_word(from + i + 1, a.x, a.x_end);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (i0 + 32 * u < words) to[i0 + 32 * u] = shifted(w[u][0], w[u][1], shift);
+    }
   }
 }
 
@@ -720,8 +781,9 @@ struct Operand {
   cudaError_t prepare(uint8_t*& temp, const int32_t* counts, cudaStream_t stream) {
     if (ready()) return cudaSuccess;
     const size_t size = bytes();
-    RepackArgs a{static_cast<const uint16_t*>(data), reinterpret_cast<uint16_t*>(temp), outer_stride, row_stride,
-                 pitch(), outer * rows, (int)rows, (int)width, counts};
+    const uint16_t* x = static_cast<const uint16_t*>(data);
+    RepackArgs a{x, x + (outer - 1) * outer_stride + (rows - 1) * row_stride + width, reinterpret_cast<uint16_t*>(temp),
+                 outer_stride, row_stride, pitch(), outer * rows, (int)rows, (int)width, counts};
     data = temp;
     row_stride = pitch();
     outer_stride = rows * pitch();
