@@ -420,6 +420,69 @@ cudaError_t cusort_page_plan(const int32_t* d_cached_lens, const int32_t* d_new_
                              int64_t num_tokens, int64_t* d_slots, int32_t* d_positions, int32_t* d_starts,
                              uint8_t* d_served, int32_t* d_num_free_out, cudaStream_t stream);
 
+/* Blocks of a paged cache after cusort_page_plan gave them out.  A request
+ * holds the first ceil(len / block_size) blocks of its table.  d_shares[b] (of
+ * num_blocks blocks) is the number of tables that hold block b beyond the
+ * first: 0 for free blocks, and for those that one table holds.  A free list
+ * has room for num_blocks; *d_num_free of it are valid.  Nothing is written in
+ * place: the *_out arrays are other memory than the inputs, so a call can be
+ * made again; its caller goes on with the results.  Entries of tables outside
+ * [0, num_blocks) are kept and counted nowhere.  num_requests, num_children <=
+ * 16384, block_size <= 2^20, num_blocks <= 2^30.  Two-phase temp protocol.
+ *
+ * Requests that go on from others' (parallel samples, beams): child r takes
+ * over from request d_parents[r]; outside [0, num_requests) it is empty.  All
+ * num_requests tables are given up, those of the children hold in their place.
+ *   - Whole blocks are shared.  A part-filled last block goes to the request's
+ *     first child if no other table holds it (d_shares 0); any other child
+ *     gets a block from the end of the free list in its place, in the
+ *     children's order, and (d_sources[r], d_destinations[r]) says which to
+ *     copy (cusort_page_copy), both -1 where nothing is.  One for which there
+ *     is no free block is not served (d_served[r] 0) and empty.
+ *   - d_block_tables_out (num_children x table_width, contiguous): -1 behind
+ *     what is held.
+ *   - Blocks that no table holds any more come behind what is left of the free
+ *     list, ascending; -1 behind them.  A block to be copied from may be among
+ *     them: copy before the next step's blocks are written. */
+cudaError_t cusort_page_fork(void* d_temp_storage, size_t* temp_storage_bytes, const int32_t* d_block_tables,
+                             int64_t table_stride, int table_width, const int32_t* d_lens, int num_requests,
+                             const int32_t* d_parents, int num_children, int block_size, const int32_t* d_free_blocks,
+                             const int32_t* d_num_free, const int32_t* d_shares, int num_blocks,
+                             int32_t* d_block_tables_out, int32_t* d_lens_out, int32_t* d_sources,
+                             int32_t* d_destinations, uint8_t* d_served, int32_t* d_shares_out,
+                             int32_t* d_free_blocks_out, int32_t* d_num_free_out, cudaStream_t stream);
+
+/* Blocks given back: request r keeps the first d_keep_lens[r] of its tokens
+ * (0: it is done) and gives up the blocks behind; the free list as above.  The
+ * tables stay as they are. */
+cudaError_t cusort_page_free(void* d_temp_storage, size_t* temp_storage_bytes, const int32_t* d_block_tables,
+                             int64_t table_stride, int table_width, const int32_t* d_lens,
+                             const int32_t* d_keep_lens, int num_requests, int block_size,
+                             const int32_t* d_free_blocks, const int32_t* d_num_free, const int32_t* d_shares,
+                             int num_blocks, int32_t* d_shares_out, int32_t* d_free_blocks_out,
+                             int32_t* d_num_free_out, cudaStream_t stream);
+
+/* Used blocks moved together: with U blocks that the tables hold, those
+ * numbered U and more, ascending, go to the unused ones below U, ascending:
+ * block d_sources[i] to d_destinations[i] (num_blocks / 2 of each, -1 behind
+ * the last move).  Tables (contiguous, -1 behind what is held), shares (counted
+ * from the tables) and the free list (num_blocks - 1 down to U, so that the
+ * lowest are taken first; -1 behind) follow the new numbers. */
+cudaError_t cusort_page_compact(void* d_temp_storage, size_t* temp_storage_bytes, const int32_t* d_block_tables,
+                                int64_t table_stride, int table_width, const int32_t* d_lens, int num_requests,
+                                int block_size, int num_blocks, int32_t* d_block_tables_out, int32_t* d_sources,
+                                int32_t* d_destinations, int32_t* d_shares_out, int32_t* d_free_blocks_out,
+                                int32_t* d_num_free_out, cudaStream_t stream);
+
+/* Block d_sources[i] copied to block d_destinations[i] in every one of
+ * num_caches caches of num_blocks blocks (host arrays: address, bytes from one
+ * block to the next, bytes of a block).  Pairs with a number outside [0,
+ * num_blocks) or of one block are left out.  No block may be in two pairs
+ * unless it is a source in both. */
+cudaError_t cusort_page_copy(void* const* d_caches, const int64_t* block_strides, const size_t* block_bytes,
+                             int num_caches, int num_blocks, const int32_t* d_sources, const int32_t* d_destinations,
+                             int64_t num_pairs, cudaStream_t stream);
+
 /* ---- library state, status and diagnostics (no reference counterpart;
  *      the reference has compile-time macros only, libcusort.cuh:119-148) -- */
 

@@ -75,6 +75,11 @@ SIGNATURES = {
                                                  _i64, _i, _vp]),
     "cusort_read_product_status": (_i, [C.POINTER(_u32), _vp]),
     "cusort_page_plan": (_i, [_vp, _vp, _i, _i, _vp, _i64, _i, _vp, _i, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "cusort_page_fork": (_i, [_vp, _P_SZ, _vp, _i64, _i, _vp, _i, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp,
+                              _vp, _vp, _vp, _vp, _vp]),
+    "cusort_page_free": (_i, [_vp, _P_SZ, _vp, _i64, _i, _vp, _vp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp]),
+    "cusort_page_compact": (_i, [_vp, _P_SZ, _vp, _i64, _i, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "cusort_page_copy": (_i, [C.POINTER(_vp), C.POINTER(_i64), _P_SZ, _i, _i, _vp, _vp, _i64, _vp]),
     "cusort_version": (C.c_char_p, []),
     "cusort_set_launch_mode": (_i, [_i]),
     "cusort_read_device_status": (_i, [_vp, C.POINTER(_u32), _vp]),

@@ -1,0 +1,623 @@
+// cusort_pages.cu -- blocks of a paged cache after they were given out:
+// requests that go on from others' (forking), blocks given back, blocks
+// copied, and a pool whose used blocks are moved together.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "../../include/cusort_b200.h"
+#include "cusort_overlap.cuh"
+#include "cusort_tensor.cuh"
+
+namespace {
+
+using namespace cusort_b200;
+
+constexpr int kMaxRequests = 16384;
+constexpr int kThreads = 1024;
+constexpr int kWarps = kThreads / 32;
+constexpr int kSms = 148;
+constexpr int kCluster = 8;  // CTAs of the form with all phases in one launch
+constexpr int kTiles = kSms;  // of the pool, a CTA each
+constexpr int64_t kOneClusterEntries = 1 << 17;
+constexpr uint32_t kAll = 0xffffffffu;
+
+enum Op { kFork, kFree, kCompact };
+
+struct PagesArgs {
+  const int32_t* tables;
+  int64_t table_stride;
+  int width, requests, block_size, num_blocks;
+  const int32_t* lens;
+  const int32_t* parents;  // fork: of each child
+  int children;
+  const int32_t* keep;                             // free: tokens that a request keeps
+  const int32_t *free_blocks, *num_free, *shares;  // fork and free
+  // results
+  int32_t *tables_out, *lens_out, *sources, *destinations, *shares_out, *free_out, *num_free_out;
+  uint8_t* served;
+  // workspace
+  int32_t* tile_counts;    // [kTiles] blocks that a tile of the pool adds to the list; and the blocks taken
+  int32_t *holders, *map;  // compact: [num_blocks] tables that hold a block, less one; the move that a block takes part in
+  int phase;               // of the form with a launch for each
+};
+
+__device__ __forceinline__ int held_of(const PagesArgs& a, int len) {
+  return (int)min((int64_t)a.width, ((int64_t)max(len, 0) + a.block_size - 1) / a.block_size);
+}
+__device__ __forceinline__ bool in_pool(const PagesArgs& a, int block) { return block >= 0 && block < a.num_blocks; }
+
+// Sum of the CTA's values before this thread's; total: of all.
+__device__ __forceinline__ int scan(int v, int* sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int in = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int u = __shfl_up_sync(kAll, in, d);
+    if (lane >= d) in += u;
+  }
+  if (lane == 31) sums[warp] = in;
+  __syncthreads();
+  const int w = sums[lane];
+  total = __reduce_add_sync(kAll, w);
+  const int before = __reduce_add_sync(kAll, lane < warp ? w : 0);
+  __syncthreads();
+  return before + in - v;
+}
+
+// Blocks at the CTA's tile of the pool: a whole number of fours to a tile.
+struct Tile {
+  int begin, end;
+};
+__device__ __forceinline__ int tile_size(const PagesArgs& a) {
+  return (int)((((int64_t)a.num_blocks + gridDim.x - 1) / gridDim.x + 3) / 4 * 4);
+}
+__device__ __forceinline__ Tile tile_of(const PagesArgs& a, int i) {
+  const int64_t size = tile_size(a);
+  return {(int)min((int64_t)a.num_blocks, i * size), (int)min((int64_t)a.num_blocks, (i + 1) * size)};
+}
+
+// Whether a block goes on the list: one that nothing holds any more (fork,
+// free), one that is held (compact).  Written by atomics of other SMs before.
+template <Op OP>
+__device__ __forceinline__ bool listed(const PagesArgs& a, int block) {
+  return OP == kCompact ? __ldcg(a.holders + block) >= 0 : __ldcg(a.shares_out + block) < 0;
+}
+
+// The tiles' counts before tile i, and of all.
+__device__ __forceinline__ int2 counts_before(const PagesArgs& a, int i, int* sums) {
+  int total = 0, unused;
+  const int mine = threadIdx.x < gridDim.x ? __ldcg(a.tile_counts + threadIdx.x) : 0;
+  scan(mine, sums, total);
+  scan(threadIdx.x < i ? mine : 0, sums, unused);
+  return make_int2(unused, total);
+}
+
+// Of the num_free first free blocks, within the list.
+__device__ __forceinline__ int free_of(const PagesArgs& a) { return min(max(*a.num_free, 0), a.num_blocks); }
+
+// ------------------------------------------------------------------ forking
+
+// Every CTA works the children out for itself (they are few): for a request
+// its first child and the number of children that are served, for a child the
+// number of blocks taken before its own.
+struct Children {
+  int *first, *count;  // [requests]
+  int* rank;           // [children] blocks taken before; -1: takes none, -2: no parent or not served
+};
+
+// The block that a request's last token lies in, where that is part-filled; -1 otherwise.
+__device__ __forceinline__ int last_part(const PagesArgs& a, int request, int len) {
+  const int64_t held = ((int64_t)len + a.block_size - 1) / a.block_size;
+  return len <= 0 || len % a.block_size == 0 || held > a.width ? -1
+                                                                 : a.tables[request * a.table_stride + held - 1];
+}
+// Whether its first child keeps that block: no other table holds it.
+__device__ __forceinline__ bool stays(const PagesArgs& a, int block) {
+  return in_pool(a, block) && a.shares[block] == 0;
+}
+
+__device__ __forceinline__ int plan_children(const PagesArgs& a, const Children& c, int* sums) {
+  for (int p = threadIdx.x; p < a.requests; p += kThreads) c.first[p] = a.children, c.count[p] = 0;
+  __syncthreads();
+  for (int r = threadIdx.x; r < a.children; r += kThreads) {
+    const int p = a.parents[r];
+    if (p >= 0 && p < a.requests) atomicMin(c.first + p, r);
+  }
+  __syncthreads();
+  const int left = free_of(a);
+  int taken = 0;
+  for (int r0 = 0; r0 < a.children; r0 += kThreads) {
+    const int r = r0 + threadIdx.x, p = r < a.children ? a.parents[r] : -1;
+    const bool valid = p >= 0 && p < a.requests;
+    bool need = false;
+    if (valid) {
+      const int len = a.lens[p];
+      const int64_t held = ((int64_t)max(len, 0) + a.block_size - 1) / a.block_size;
+      const bool part = len > 0 && len % a.block_size != 0 && held <= a.width;
+      need = part && !(c.first[p] == r && stays(a, a.tables[p * a.table_stride + held - 1]));
+    }
+    int total;
+    const int rank = taken + scan(need, sums, total);
+    taken += total;
+    if (r < a.children) {
+      const bool ok = valid && (!need || rank < left);
+      c.rank[r] = !ok ? -2 : need ? rank : -1;
+      if (ok) atomicAdd(c.count + p, 1);
+    }
+  }
+  __syncthreads();
+  return min(taken, left);
+}
+
+// The children's results, their tables, and the holders that their parents' blocks win and lose.
+__device__ __forceinline__ void fork_tables(const PagesArgs& a, const Children& c) {
+  const int left = free_of(a), me = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads;
+  for (int r = me; r < a.children; r += all) {
+    const int rank = c.rank[r], p = a.parents[r];
+    const bool valid = p >= 0 && p < a.requests;
+    a.lens_out[r] = rank == -2 ? 0 : max(a.lens[p], 0);
+    a.sources[r] = rank >= 0 ? last_part(a, p, a.lens[p]) : -1;
+    a.destinations[r] = rank >= 0 ? a.free_blocks[left - 1 - rank] : -1;
+    a.served[r] = !valid || rank != -2;
+  }
+  const int lane = threadIdx.x & 31, warp = me >> 5, warps = all >> 5;
+  for (int r = warp; r < a.children; r += warps) {
+    const int rank = c.rank[r], p = rank == -2 ? 0 : a.parents[r], held = rank == -2 ? 0 : held_of(a, a.lens[p]);
+    const int32_t* from = a.tables + p * a.table_stride;
+    int32_t* to = a.tables_out + (int64_t)r * a.width;
+#pragma unroll 4
+    for (int i = lane; i < a.width; i += 32) {
+      int block = -1;
+      if (i < held) block = rank >= 0 && i == held - 1 ? a.free_blocks[left - 1 - rank] : from[i];
+      to[i] = block;
+    }
+  }
+  for (int p = warp; p < a.requests; p += warps) {
+    const int len = a.lens[p], held = held_of(a, len), more = c.count[p] - 1;
+    const bool part = len > 0 && len % a.block_size != 0 && held == ((int64_t)len + a.block_size - 1) / a.block_size;
+    const int32_t* from = a.tables + p * a.table_stride;
+#pragma unroll 4
+    for (int i = lane; i < held; i += 32) {
+      const int block = from[i];
+      int delta = more;
+      if (part && i == held - 1) delta = c.first[p] < a.children && stays(a, block) ? 0 : -1;
+      if (delta != 0 && in_pool(a, block)) atomicAdd(a.shares_out + block, delta);
+    }
+  }
+}
+
+// ------------------------------------------------------------ the phases
+
+// 0: what later phases add to is set up.
+template <Op OP>
+__device__ __forceinline__ void set_up(const PagesArgs& a) {
+  const int me = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads;
+  if (OP == kCompact) {
+    for (int b = me; b < a.num_blocks; b += all) {
+      a.holders[b] = -1;
+      if (b < a.num_blocks / 2) a.sources[b] = a.destinations[b] = -1;
+    }
+  } else {
+    for (int b = me; b < a.num_blocks; b += all) a.shares_out[b] = a.shares[b];
+  }
+}
+
+// 1: holders are counted.
+template <Op OP>
+__device__ __forceinline__ void count_holders(const PagesArgs& a, const Children& c) {
+  const int me = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads;
+  if (OP == kFork) {
+    fork_tables(a, c);
+    return;
+  }
+  const int lane = threadIdx.x & 31;
+  for (int r = me >> 5; r < a.requests; r += all >> 5) {
+    const int len = a.lens[r], held = held_of(a, len);
+    const int first = OP == kFree ? held_of(a, min(a.keep[r], len)) : 0;
+    const int32_t* from = a.tables + r * a.table_stride;
+#pragma unroll 4
+    for (int i = first + lane; i < held; i += 32) {
+      const int block = from[i];
+      if (in_pool(a, block)) atomicAdd(OP == kFree ? a.shares_out + block : a.holders + block, OP == kFree ? -1 : 1);
+    }
+  }
+}
+
+// 2: listed blocks of the CTA's tile are counted.
+template <Op OP>
+__device__ __forceinline__ void count_listed(const PagesArgs& a, int* sums) {
+  const Tile t = tile_of(a, blockIdx.x);
+  int n = 0, total;
+#pragma unroll 4
+  for (int b = t.begin + threadIdx.x; b < t.end; b += kThreads) n += listed<OP>(a, b);
+  scan(n, sums, total);
+  if (threadIdx.x == 0) a.tile_counts[blockIdx.x] = total;
+}
+
+// 3, fork and free: the free list, and behind what is left of it the blocks that nothing holds any more.
+__device__ __forceinline__ void write_free(const PagesArgs& a, int left, int* sums) {
+  const Tile t = tile_of(a, blockIdx.x);
+  const int2 before = counts_before(a, blockIdx.x, sums);
+  int at = left + before.x;
+  for (int b0 = t.begin; b0 < t.end; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    const bool gone = b < t.end && listed<kFree>(a, b);
+    int total;
+    const int place = at + scan(gone, sums, total);
+    at += total;
+    if (gone) {
+      if (place < a.num_blocks) a.free_out[place] = b;
+      a.shares_out[b] = 0;
+    }
+  }
+  const int end = (int)min((int64_t)a.num_blocks, (int64_t)left + before.y);
+  for (int i = blockIdx.x * kThreads + threadIdx.x; i < a.num_blocks; i += gridDim.x * kThreads)
+    if (i < left || i >= end) a.free_out[i] = i < left ? a.free_blocks[i] : -1;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.num_free_out = end;
+}
+
+// 3, compact: with U used blocks, those from U on are numbered in order, and so are the holes below it.
+__device__ __forceinline__ void write_moves(const PagesArgs& a, int* sums) {
+  const Tile t = tile_of(a, blockIdx.x);
+  const int2 before = counts_before(a, blockIdx.x, sums);
+  const int used = before.y;
+  // used blocks below U: those of the tiles before U's, and those of its own before it
+  const int of = min((int)(used / max(tile_size(a), 1)), (int)gridDim.x - 1);
+  int inside = counts_before(a, of, sums).x, n = 0, total;
+#pragma unroll 4
+  for (int b = tile_of(a, of).begin + threadIdx.x; b < used; b += kThreads) n += listed<kCompact>(a, b);
+  scan(n, sums, total);
+  inside += total;
+  int at = before.x;
+  for (int b0 = t.begin; b0 < t.end; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    const bool in = b < t.end && listed<kCompact>(a, b);
+    const int below = at + scan(in, sums, total);  // used blocks below b
+    at += total;
+    if (b < t.end && in && b >= used) {
+      a.sources[below - inside] = b;
+      a.map[b] = below - inside;
+    } else if (b < t.end && !in && b < used) {
+      a.destinations[b - below] = b;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.num_free_out = a.num_blocks - used;
+}
+
+// 4, compact: tables, shares and free list by the new numbers.
+__device__ __forceinline__ void renumber(const PagesArgs& a) {
+  const int me = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads, lane = threadIdx.x & 31;
+  const int used = a.num_blocks - __ldcg(a.num_free_out);
+  for (int r = me >> 5; r < a.requests; r += all >> 5) {
+    const int held = held_of(a, a.lens[r]);
+    const int32_t* from = a.tables + r * a.table_stride;
+    int32_t* to = a.tables_out + (int64_t)r * a.width;
+#pragma unroll 4
+    for (int i = lane; i < a.width; i += 32) {
+      int block = i < held ? from[i] : -1;
+      if (block >= used && block < a.num_blocks) block = __ldcg(a.destinations + __ldcg(a.map + block));
+      to[i] = block;
+    }
+  }
+  for (int b = me; b < a.num_blocks; b += all) {
+    const int holders = __ldcg(a.holders + b);
+    if (b >= used) {
+      a.shares_out[b] = 0;
+      if (holders >= 0) a.shares_out[__ldcg(a.destinations + __ldcg(a.map + b))] = holders;
+    } else if (holders >= 0) {
+      a.shares_out[b] = holders;
+    }
+    a.free_out[b] = b < a.num_blocks - used ? a.num_blocks - 1 - b : -1;
+  }
+}
+
+// ONE: all phases, over one cluster of CTAs with its barrier between them;
+// otherwise the phase a.phase, over any number of them.  Small steps are bound
+// by the latency of launches, barriers and dependent loads.
+template <Op OP, bool ONE>
+__global__ void __launch_bounds__(kThreads, 1) pages_kernel(const __grid_constant__ PagesArgs a) {
+  extern __shared__ int s_children[];
+  __shared__ int sums[kWarps];
+  static_assert(kWarps == 32, "scan() takes a sum to a lane");
+  const Children c{s_children, s_children + a.requests, s_children + 2 * a.requests};
+  dev::wait_for_previous();
+  if (ONE || a.phase == 0) set_up<OP>(a);
+  int taken = 0;
+  if (OP == kFork && (ONE || a.phase == 1)) {
+    taken = plan_children(a, c, sums);
+    if (!ONE && blockIdx.x == 0 && threadIdx.x == 0) a.tile_counts[kTiles] = taken;
+  }
+  if (OP == kFork && !ONE && a.phase == 3) taken = a.tile_counts[kTiles];
+  if (ONE) dev::cluster_sync();
+  if (ONE || a.phase == 1) count_holders<OP>(a, c);
+  if (ONE) dev::cluster_sync();
+  if (ONE || a.phase == 2) count_listed<OP>(a, sums);
+  if (ONE) dev::cluster_sync();
+  if (ONE || a.phase == 3) {
+    if (OP == kCompact) write_moves(a, sums);
+    else write_free(a, free_of(a) - taken, sums);
+  }
+  if (OP == kCompact) {
+    if (ONE) dev::cluster_sync();
+    if (ONE || a.phase == 4) renumber(a);
+  }
+}
+
+template <Op OP>
+cudaError_t run(PagesArgs a, cudaStream_t stream) {
+  const size_t smem = OP == kFork ? sizeof(int) * (2 * (size_t)a.requests + a.children) : 0;
+  const size_t most = OP == kFork ? sizeof(int) * 3 * kMaxRequests : 0;
+  const auto limit = [&](auto kernel) {
+    // the limit is the kernel's, not the call's: the same one from every host thread
+    return smem > 40 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most)
+                            : cudaSuccess;
+  };
+  const int64_t entries = (int64_t)(a.requests + a.children) * a.width + a.num_blocks;
+  if (entries <= kOneClusterEntries) {
+    const cudaError_t e = limit(pages_kernel<OP, true>);
+    return e ? e : launch_after_previous(pages_kernel<OP, true>, kCluster, kThreads, smem, a, stream, kCluster);
+  }
+  cudaError_t e = limit(pages_kernel<OP, false>);
+  const int grid = (int)std::min<int64_t>(kSms, (entries + kThreads - 1) / kThreads);
+  for (a.phase = 0; !e && a.phase < (OP == kCompact ? 5 : 4); ++a.phase)
+    e = launch_after_previous(pages_kernel<OP, false>, grid, kThreads, OP == kFork && a.phase == 1 ? smem : 0, a,
+                              stream);
+  return e;
+}
+
+// ------------------------------------------------------------------ copying
+
+constexpr int kCopyThreads = 128;
+constexpr int kCopyPiece = 16384;  // bytes that a CTA copies at a time
+constexpr int kCopyCaches = 64;    // to a launch
+
+struct CopyArgs {
+  struct Cache {
+    char* data;
+    int64_t stride, bytes;  // between blocks; of a block
+    int pieces_before;      // in the caches before it
+  } caches[kCopyCaches];
+  const int32_t *sources, *destinations;
+  int64_t pairs;
+  int num_blocks, num_caches, pieces;  // pieces of a pair over all caches
+  int groups, parts;                   // pairs p with p % groups == g in turn, the pieces of each over `parts` CTAs
+};
+
+// Pairs that are none cost a look each: a CTA looks at 128 of its pairs at a
+// time and copies the blocks of those that are.  Bound by memory.
+template <typename V>
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ CopyArgs a) {
+  __shared__ int2 pairs[kCopyThreads];
+  __shared__ int found;
+  dev::wait_for_previous();
+  const int g = blockIdx.x % a.groups, part = blockIdx.x / a.groups;
+  for (int64_t p0 = 0; p0 * a.groups < a.pairs; p0 += kCopyThreads) {
+    const int64_t p = (p0 + threadIdx.x) * a.groups + g;
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    if (p < a.pairs) {
+      const int from = a.sources[p], to = a.destinations[p];
+      if (from >= 0 && from < a.num_blocks && to >= 0 && to < a.num_blocks && from != to)
+        pairs[atomicAdd(&found, 1)] = make_int2(from, to);
+    }
+    __syncthreads();
+    for (int i = 0; i < found; ++i) {
+      const int2 pair = pairs[i];
+      int cache = 0;
+      for (int piece = part; piece < a.pieces; piece += a.parts) {
+        while (cache + 1 < a.num_caches && piece >= a.caches[cache + 1].pieces_before) ++cache;
+        const CopyArgs::Cache& c = a.caches[cache];
+        const int64_t begin = (int64_t)(piece - c.pieces_before) * kCopyPiece;
+        const int n = (int)(min((int64_t)kCopyPiece, c.bytes - begin) / (int64_t)sizeof(V));
+        const V* from = reinterpret_cast<const V*>(c.data + pair.x * c.stride + begin);
+        V* to = reinterpret_cast<V*>(c.data + pair.y * c.stride + begin);
+        constexpr int U = 8;
+        for (int j0 = threadIdx.x; j0 < n; j0 += kCopyThreads * U) {
+          V v[U];
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (j0 + u * kCopyThreads < n) v[u] = from[j0 + u * kCopyThreads];
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (j0 + u * kCopyThreads < n) to[j0 + u * kCopyThreads] = v[u];
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+bool pool_ok(int num_requests, int block_size, int64_t table_stride, int table_width, int num_blocks) {
+  return num_requests >= 0 && num_requests <= kMaxRequests && block_size >= 1 && block_size <= (1 << 20) &&
+         table_width >= 0 && table_stride >= table_width && num_blocks >= 0 && num_blocks <= (1 << 30);
+}
+
+// The two-phase protocol's answer: true where the call ends with *e.
+bool temp_done(void* temp, size_t* bytes, size_t need, cudaError_t* e) {
+  if (bytes == nullptr) {
+    *e = cudaErrorInvalidValue;
+    return true;
+  }
+  if (temp == nullptr) {
+    *bytes = need;
+    *e = cudaSuccess;
+    return true;
+  }
+  *e = *bytes < need || (reinterpret_cast<uintptr_t>(temp) & 15) != 0 ? cudaErrorInvalidValue : cudaSuccess;
+  return *e != cudaSuccess;
+}
+
+constexpr size_t kCountBytes = ((kTiles + 1) * sizeof(int32_t) + 15) / 16 * 16;
+
+}  // namespace
+
+extern "C" cudaError_t cusort_page_fork(void* d_temp_storage, size_t* temp_storage_bytes,
+                                        const int32_t* d_block_tables, int64_t table_stride, int table_width,
+                                        const int32_t* d_lens, int num_requests, const int32_t* d_parents,
+                                        int num_children, int block_size, const int32_t* d_free_blocks,
+                                        const int32_t* d_num_free, const int32_t* d_shares, int num_blocks,
+                                        int32_t* d_block_tables_out, int32_t* d_lens_out, int32_t* d_sources,
+                                        int32_t* d_destinations, uint8_t* d_served, int32_t* d_shares_out,
+                                        int32_t* d_free_blocks_out, int32_t* d_num_free_out, cudaStream_t stream) {
+  cudaError_t e;
+  if (!pool_ok(num_requests, block_size, table_stride, table_width, num_blocks) || num_children < 0 ||
+      num_children > kMaxRequests)
+    return cudaErrorInvalidValue;
+  if (temp_done(d_temp_storage, temp_storage_bytes, kCountBytes, &e)) return e;
+  const bool tables = num_requests > 0 && table_width > 0;
+  if ((tables && d_block_tables == nullptr) || (num_requests > 0 && d_lens == nullptr) ||
+      (num_children > 0 && (d_parents == nullptr || d_lens_out == nullptr || d_sources == nullptr ||
+                            d_destinations == nullptr || d_served == nullptr ||
+                            (table_width > 0 && d_block_tables_out == nullptr))) ||
+      (num_blocks > 0 && (d_free_blocks == nullptr || d_shares == nullptr || d_shares_out == nullptr ||
+                          d_free_blocks_out == nullptr)) ||
+      d_num_free == nullptr || d_num_free_out == nullptr)
+    return cudaErrorInvalidValue;
+  // what is read by every CTA, whenever it comes to run, must not be written meanwhile
+  if (d_num_free == d_num_free_out || (num_blocks > 0 && (d_free_blocks == d_free_blocks_out || d_shares == d_shares_out)) ||
+      (tables && d_block_tables == d_block_tables_out) || (num_children > 0 && num_requests > 0 && d_lens == d_lens_out))
+    return cudaErrorInvalidValue;
+  PagesArgs a{};
+  a.tables = d_block_tables;
+  a.table_stride = table_stride;
+  a.width = table_width;
+  a.requests = num_requests;
+  a.block_size = block_size;
+  a.num_blocks = num_blocks;
+  a.lens = d_lens;
+  a.parents = d_parents;
+  a.children = num_children;
+  a.free_blocks = d_free_blocks;
+  a.num_free = d_num_free;
+  a.shares = d_shares;
+  a.tables_out = d_block_tables_out;
+  a.lens_out = d_lens_out;
+  a.sources = d_sources;
+  a.destinations = d_destinations;
+  a.served = d_served;
+  a.shares_out = d_shares_out;
+  a.free_out = d_free_blocks_out;
+  a.num_free_out = d_num_free_out;
+  a.tile_counts = static_cast<int32_t*>(d_temp_storage);
+  return run<kFork>(a, stream);
+}
+
+extern "C" cudaError_t cusort_page_free(void* d_temp_storage, size_t* temp_storage_bytes,
+                                        const int32_t* d_block_tables, int64_t table_stride, int table_width,
+                                        const int32_t* d_lens, const int32_t* d_keep_lens, int num_requests,
+                                        int block_size, const int32_t* d_free_blocks, const int32_t* d_num_free,
+                                        const int32_t* d_shares, int num_blocks, int32_t* d_shares_out,
+                                        int32_t* d_free_blocks_out, int32_t* d_num_free_out, cudaStream_t stream) {
+  cudaError_t e;
+  if (!pool_ok(num_requests, block_size, table_stride, table_width, num_blocks)) return cudaErrorInvalidValue;
+  if (temp_done(d_temp_storage, temp_storage_bytes, kCountBytes, &e)) return e;
+  if ((num_requests > 0 && ((table_width > 0 && d_block_tables == nullptr) || d_lens == nullptr ||
+                            d_keep_lens == nullptr)) ||
+      (num_blocks > 0 && (d_free_blocks == nullptr || d_shares == nullptr || d_shares_out == nullptr ||
+                          d_free_blocks_out == nullptr)) ||
+      d_num_free == nullptr || d_num_free_out == nullptr || d_num_free == d_num_free_out ||
+      (num_blocks > 0 && (d_free_blocks == d_free_blocks_out || d_shares == d_shares_out)))
+    return cudaErrorInvalidValue;
+  PagesArgs a{};
+  a.tables = d_block_tables;
+  a.table_stride = table_stride;
+  a.width = table_width;
+  a.requests = num_requests;
+  a.block_size = block_size;
+  a.num_blocks = num_blocks;
+  a.lens = d_lens;
+  a.keep = d_keep_lens;
+  a.free_blocks = d_free_blocks;
+  a.num_free = d_num_free;
+  a.shares = d_shares;
+  a.shares_out = d_shares_out;
+  a.free_out = d_free_blocks_out;
+  a.num_free_out = d_num_free_out;
+  a.tile_counts = static_cast<int32_t*>(d_temp_storage);
+  return run<kFree>(a, stream);
+}
+
+extern "C" cudaError_t cusort_page_compact(void* d_temp_storage, size_t* temp_storage_bytes,
+                                           const int32_t* d_block_tables, int64_t table_stride, int table_width,
+                                           const int32_t* d_lens, int num_requests, int block_size, int num_blocks,
+                                           int32_t* d_block_tables_out, int32_t* d_sources, int32_t* d_destinations,
+                                           int32_t* d_shares_out, int32_t* d_free_blocks_out,
+                                           int32_t* d_num_free_out, cudaStream_t stream) {
+  cudaError_t e;
+  if (!pool_ok(num_requests, block_size, table_stride, table_width, num_blocks)) return cudaErrorInvalidValue;
+  if (temp_done(d_temp_storage, temp_storage_bytes, kCountBytes + 8 * (size_t)num_blocks, &e)) return e;
+  if ((num_requests > 0 && (d_lens == nullptr || (table_width > 0 && (d_block_tables == nullptr ||
+                                                                     d_block_tables_out == nullptr ||
+                                                                     d_block_tables == d_block_tables_out)))) ||
+      (num_blocks > 1 && (d_sources == nullptr || d_destinations == nullptr)) ||
+      (num_blocks > 0 && (d_shares_out == nullptr || d_free_blocks_out == nullptr)) || d_num_free_out == nullptr)
+    return cudaErrorInvalidValue;
+  PagesArgs a{};
+  a.tables = d_block_tables;
+  a.table_stride = table_stride;
+  a.width = table_width;
+  a.requests = num_requests;
+  a.block_size = block_size;
+  a.num_blocks = num_blocks;
+  a.lens = d_lens;
+  a.tables_out = d_block_tables_out;
+  a.sources = d_sources;
+  a.destinations = d_destinations;
+  a.shares_out = d_shares_out;
+  a.free_out = d_free_blocks_out;
+  a.num_free_out = d_num_free_out;
+  a.tile_counts = static_cast<int32_t*>(d_temp_storage);
+  a.holders = reinterpret_cast<int32_t*>(static_cast<char*>(d_temp_storage) + kCountBytes);
+  a.map = a.holders + num_blocks;
+  return run<kCompact>(a, stream);
+}
+
+extern "C" cudaError_t cusort_page_copy(void* const* d_caches, const int64_t* block_strides, const size_t* block_bytes,
+                                        int num_caches, int num_blocks, const int32_t* d_sources,
+                                        const int32_t* d_destinations, int64_t num_pairs, cudaStream_t stream) {
+  if (num_caches < 0 || num_blocks < 0 || num_pairs < 0 || num_pairs > INT32_MAX ||
+      (num_caches > 0 && (d_caches == nullptr || block_strides == nullptr || block_bytes == nullptr)) ||
+      (num_pairs > 0 && (d_sources == nullptr || d_destinations == nullptr)))
+    return cudaErrorInvalidValue;
+  for (int c = 0; c < num_caches; ++c)
+    if ((block_bytes[c] > 0 && num_blocks > 0 && d_caches[c] == nullptr) || block_bytes[c] > (size_t)1 << 40 ||
+        (num_blocks > 1 && block_strides[c] < (int64_t)block_bytes[c]))
+      return cudaErrorInvalidValue;
+  if (num_pairs == 0 || num_blocks < 2) return cudaSuccess;
+  for (int c = 0; c < num_caches;) {
+    CopyArgs a{};
+    a.sources = d_sources;
+    a.destinations = d_destinations;
+    a.pairs = num_pairs;
+    a.num_blocks = num_blocks;
+    uintptr_t bits = 0;
+    int64_t pieces = 0;
+    for (; c < num_caches && a.num_caches < kCopyCaches; ++c) {
+      if (block_bytes[c] == 0) continue;
+      const int64_t of = ((int64_t)block_bytes[c] + kCopyPiece - 1) / kCopyPiece;
+      if (pieces + of > INT32_MAX) {
+        if (pieces == 0) return cudaErrorInvalidValue;
+        break;
+      }
+      a.caches[a.num_caches++] = {static_cast<char*>(d_caches[c]), block_strides[c], (int64_t)block_bytes[c], (int)pieces};
+      pieces += of;
+      bits |= reinterpret_cast<uintptr_t>(d_caches[c]) | (uintptr_t)block_strides[c] | (uintptr_t)block_bytes[c];
+    }
+    if (pieces == 0) continue;
+    a.pieces = (int)pieces;
+    // every pair has its CTAs where there are few, every CTA several pairs where there are many
+    constexpr int64_t kCtas = kSms * 12;
+    a.groups = (int)std::min<int64_t>(num_pairs, kCtas);
+    a.parts = (int)std::min<int64_t>(pieces, std::max<int64_t>(1, kCtas / a.groups));
+    const int64_t grid = (int64_t)a.groups * a.parts;
+    const cudaError_t e = (bits & 15) == 0  ? launch_after_previous(copy_kernel<uint4>, grid, kCopyThreads, 0, a, stream)
+                          : (bits & 7) == 0 ? launch_after_previous(copy_kernel<uint2>, grid, kCopyThreads, 0, a, stream)
+                          : (bits & 3) == 0 ? launch_after_previous(copy_kernel<uint32_t>, grid, kCopyThreads, 0, a, stream)
+                          : (bits & 1) == 0 ? launch_after_previous(copy_kernel<uint16_t>, grid, kCopyThreads, 0, a, stream)
+                                            : launch_after_previous(copy_kernel<uint8_t>, grid, kCopyThreads, 0, a, stream);
+    if (e) return e;
+  }
+  return cudaSuccess;
+}

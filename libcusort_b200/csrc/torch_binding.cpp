@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <string>
+#include <vector>
 
 #include "../../include/cusort_b200.h"
 
@@ -192,7 +193,7 @@ class Outputs {
   bool separate_;
   int count_ = 0;
   int64_t bytes_ = 0;
-  Output outputs_[5];
+  Output outputs_[8];
 };
 
 template <typename T>
@@ -562,6 +563,159 @@ PyObject* page_plan(PyObject* const* p) {
   return out.tuple(left < 0);
 }
 
+// Block tables [requests, width] of int32 whose rows do not overlap, and the requests' lengths.
+void check_tables(const at::Tensor& tables, const at::Tensor& lens) {
+  if (lens.dim() != 1 || lens.numel() > kMaxRequests)
+    refuse(PyExc_ValueError, "lens must be 1-D with at most ", kMaxRequests, " requests (got shape ", shape_of(lens),
+           ")");
+  check(lens, "lens", at::kInt, lens.device(), {lens.numel()});
+  check_rows(tables, "block_tables");
+  if (tables.scalar_type() != at::kInt || tables.device() != lens.device() || tables.size(0) != lens.numel())
+    refuse(PyExc_ValueError, "block_tables must be int32 with ", lens.numel(), " rows on ", lens.device(), " (got ",
+           name_of(tables.scalar_type()), ", ", shape_of(tables), ", ", tables.device(), ")");
+  if (tables.size(0) > 1 && tables.numel() > 0 && tables.stride(0) < tables.size(1))
+    refuse(PyExc_ValueError, "block_tables' rows must not overlap (strides ", tables.strides(), ")");
+  if (tables.size(1) > INT32_MAX) refuse(PyExc_ValueError, "block_tables must be at most 2^31 - 1 blocks wide");
+}
+
+void check_block_size(int64_t block) {
+  if (block < 1 || block > 1 << 20)
+    refuse(PyExc_ValueError, "block_size must be between 1 and 2^20 (got ", block, ")");
+}
+
+// A pool's free list, its length and its blocks' shares; the number of blocks.
+int64_t check_pool(const at::Tensor& free, const at::Tensor& num_free, const at::Tensor& shares, at::Device device) {
+  if (shares.dim() != 1 || shares.numel() > 1 << 30)
+    refuse(PyExc_ValueError, "shares must be 1-D with at most 2^30 blocks (got shape ", shape_of(shares), ")");
+  check(shares, "shares", at::kInt, device, {shares.numel()});
+  check(free, "free_blocks", at::kInt, device, {shares.numel()});
+  check(num_free, "num_free", at::kInt, device, {1});
+  return shares.numel();
+}
+
+int64_t stride_of(const at::Tensor& tables) { return std::max(tables.stride(0), tables.size(1)); }
+
+// block_tables, lens, parents, block_size, free_blocks, num_free, shares, separate
+PyObject* page_fork(PyObject* const* p) {
+  const at::Tensor &tables = tensor(p[0], "block_tables"), &lens = tensor(p[1], "lens"),
+                   &parents = tensor(p[2], "parents"), &free = tensor(p[4], "free_blocks"),
+                   &num_free = tensor(p[5], "num_free"), &shares = tensor(p[6], "shares");
+  const int64_t block = whole(p[3]);
+  check_tables(tables, lens);
+  check_block_size(block);
+  const at::Device device = lens.device();
+  if (parents.dim() != 1 || parents.numel() > kMaxRequests)
+    refuse(PyExc_ValueError, "parents must be 1-D with at most ", kMaxRequests, " requests (got shape ",
+           shape_of(parents), ")");
+  const int64_t children = parents.numel(), width = tables.size(1);
+  check(parents, "parents", at::kInt, device, {children});
+  const int64_t blocks = check_pool(free, num_free, shares, device);
+  check_cuda(lens, "lens");
+  Outputs out(device, truth(p[7]));
+  const int new_tables = out.add({children, width}, at::kInt), new_lens = out.add({children}, at::kInt);
+  const int sources = out.add({children}, at::kInt), destinations = out.add({children}, at::kInt);
+  const int served = out.add({children}, at::kBool), new_shares = out.add({blocks}, at::kInt);
+  const int new_free = out.add({blocks}, at::kInt), left = out.add({1}, at::kInt);
+  out.allocate();
+  launch_with_temp("cusort_page_fork", device, [&](void* temp, size_t* bytes, cudaStream_t s) {
+    return cusort_page_fork(temp, bytes, ptr<int32_t>(tables), stride_of(tables), (int)width, ptr<int32_t>(lens),
+                            (int)lens.numel(), ptr<int32_t>(parents), (int)children, (int)block, ptr<int32_t>(free),
+                            ptr<int32_t>(num_free), ptr<int32_t>(shares), (int)blocks, out.ptr<int32_t>(new_tables),
+                            out.ptr<int32_t>(new_lens), out.ptr<int32_t>(sources), out.ptr<int32_t>(destinations),
+                            out.ptr<uint8_t>(served), out.ptr<int32_t>(new_shares), out.ptr<int32_t>(new_free),
+                            out.ptr<int32_t>(left), s);
+  });
+  return out.tuple();
+}
+
+// block_tables, lens, keep_lens, block_size, free_blocks, num_free, shares, separate
+PyObject* page_free(PyObject* const* p) {
+  const at::Tensor &tables = tensor(p[0], "block_tables"), &lens = tensor(p[1], "lens"),
+                   &keep = tensor(p[2], "keep_lens"), &free = tensor(p[4], "free_blocks"),
+                   &num_free = tensor(p[5], "num_free"), &shares = tensor(p[6], "shares");
+  const int64_t block = whole(p[3]);
+  check_tables(tables, lens);
+  check_block_size(block);
+  const at::Device device = lens.device();
+  check(keep, "keep_lens", at::kInt, device, {lens.numel()});
+  const int64_t blocks = check_pool(free, num_free, shares, device);
+  check_cuda(lens, "lens");
+  Outputs out(device, truth(p[7]));
+  const int new_shares = out.add({blocks}, at::kInt), new_free = out.add({blocks}, at::kInt);
+  const int left = out.add({1}, at::kInt);
+  out.allocate();
+  launch_with_temp("cusort_page_free", device, [&](void* temp, size_t* bytes, cudaStream_t s) {
+    return cusort_page_free(temp, bytes, ptr<int32_t>(tables), stride_of(tables), (int)tables.size(1),
+                            ptr<int32_t>(lens), ptr<int32_t>(keep), (int)lens.numel(), (int)block, ptr<int32_t>(free),
+                            ptr<int32_t>(num_free), ptr<int32_t>(shares), (int)blocks, out.ptr<int32_t>(new_shares),
+                            out.ptr<int32_t>(new_free), out.ptr<int32_t>(left), s);
+  });
+  return out.tuple();
+}
+
+// block_tables, lens, block_size, num_blocks, separate
+PyObject* page_compact(PyObject* const* p) {
+  const at::Tensor &tables = tensor(p[0], "block_tables"), &lens = tensor(p[1], "lens");
+  const int64_t block = whole(p[2]), blocks = whole(p[3]);
+  check_tables(tables, lens);
+  check_block_size(block);
+  if (blocks < 0 || blocks > 1 << 30)
+    refuse(PyExc_ValueError, "num_blocks must be between 0 and 2^30 (got ", blocks, ")");
+  check_cuda(lens, "lens");
+  const at::Device device = lens.device();
+  Outputs out(device, truth(p[4]));
+  const int new_tables = out.add(tables.sizes(), at::kInt), sources = out.add({blocks / 2}, at::kInt);
+  const int destinations = out.add({blocks / 2}, at::kInt), shares = out.add({blocks}, at::kInt);
+  const int free = out.add({blocks}, at::kInt), left = out.add({1}, at::kInt);
+  out.allocate();
+  launch_with_temp("cusort_page_compact", device, [&](void* temp, size_t* bytes, cudaStream_t s) {
+    return cusort_page_compact(temp, bytes, ptr<int32_t>(tables), stride_of(tables), (int)tables.size(1),
+                               ptr<int32_t>(lens), (int)lens.numel(), (int)block, (int)blocks,
+                               out.ptr<int32_t>(new_tables), out.ptr<int32_t>(sources), out.ptr<int32_t>(destinations),
+                               out.ptr<int32_t>(shares), out.ptr<int32_t>(free), out.ptr<int32_t>(left), s);
+  });
+  return out.tuple();
+}
+
+// caches (a list or tuple), sources, destinations
+PyObject* page_copy(PyObject* const* p) {
+  if (!PyList_Check(p[0]) && !PyTuple_Check(p[0])) refuse(PyExc_TypeError, "caches must be a list or tuple of tensors");
+  const Py_ssize_t count = PySequence_Fast_GET_SIZE(p[0]);
+  const at::Tensor &sources = tensor(p[1], "sources"), &destinations = tensor(p[2], "destinations");
+  const at::Device device = sources.device();
+  check(sources, "sources", at::kInt, device, {sources.numel()});
+  check(destinations, "destinations", at::kInt, device, {sources.numel()});
+  if (sources.numel() > INT32_MAX) refuse(PyExc_ValueError, "at most 2^31 - 1 pairs are supported");
+  std::vector<void*> data;
+  std::vector<int64_t> strides;
+  std::vector<size_t> bytes;
+  int64_t blocks = 0;
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    const at::Tensor& t = tensor(PySequence_Fast_GET_ITEM(p[0], i), "every cache");
+    if (t.dim() < 1) refuse(PyExc_ValueError, "every cache must be [blocks, ...] (got shape ", shape_of(t), ")");
+    if (i == 0) blocks = t.size(0);
+    int64_t of = 1;
+    bool dense = t.device() == device && t.size(0) == blocks && blocks <= 1 << 30;
+    for (int64_t d = t.dim() - 1; d > 0; --d) {
+      dense = dense && (t.size(d) == 1 || t.stride(d) == of || t.numel() == 0);
+      of *= t.size(d);
+    }
+    if (!dense || (blocks > 1 && t.stride(0) < of && t.numel() > 0))
+      refuse(PyExc_ValueError, "every cache must be on ", device, " with ", blocks,
+             " blocks (2^30 at most), each contiguous in itself, that do not overlap (got shape ", shape_of(t),
+             ", strides ", t.strides(), ", ", t.device(), ")");
+    data.push_back(t.data_ptr());
+    strides.push_back(t.stride(0) * (int64_t)t.element_size());
+    bytes.push_back((size_t)(t.numel() == 0 ? 0 : of) * t.element_size());
+  }
+  check_cuda(sources, "sources");
+  launch("cusort_page_copy", device, [&](cudaStream_t s) {
+    return cusort_page_copy(data.data(), strides.data(), bytes.data(), (int)count, (int)blocks, ptr<int32_t>(sources),
+                            ptr<int32_t>(destinations), sources.numel(), s);
+  });
+  Py_RETURN_NONE;
+}
+
 // The boundary: no C++ exception leaves through it.
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
@@ -585,7 +739,9 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
 PyMethodDef kMethods[] = {ENTRY(route, 9),   ENTRY(route_backward, 7), ENTRY(plan_dispatch, 4),
                           ENTRY(dispatch, 3), ENTRY(combine, 5),       ENTRY(combine_backward, 5),
                           ENTRY(expert_products, 6), ENTRY(expert_products_grad_weights, 5),
-                          ENTRY(weights_in_contiguous, 1), ENTRY(page_plan, 8), {nullptr, nullptr, 0, nullptr}};
+                          ENTRY(weights_in_contiguous, 1), ENTRY(page_plan, 8),
+                          ENTRY(page_fork, 8), ENTRY(page_free, 8),
+                          ENTRY(page_compact, 5), ENTRY(page_copy, 3), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_cusort_torch", nullptr, -1, kMethods};
 
