@@ -40,9 +40,21 @@ cudaError_t encode_map(CUtensorMap* map, const void* base, int rank, const uint6
   for (int i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i];
   for (int i = 0; i + 1 < rank; ++i) s[i] = strides[i];
   // both types have 16 bits, and nothing but zeros outside depends on which it is
-  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d, s, b, one,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const auto call = [&] {
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), d, s, b, one,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  box[0] == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = call();
+  if (r != CUDA_SUCCESS) {
+    // a host thread that has made no call of the runtime yet (as one that runs a backward pass) has no context
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (!e) e = cudaSetDevice(device);
+    if (e) return e;
+    r = call();
+  }
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 

@@ -8,7 +8,6 @@
 
 #include "../../include/cusort_b200.h"
 #include "cusort_overlap.cuh"
-#include "cusort_tensor.cuh"
 
 namespace {
 
@@ -18,9 +17,13 @@ constexpr int kMaxRequests = 16384;
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSms = 148;
-constexpr int kCluster = 8;  // CTAs of the form with all phases in one launch
-constexpr int kTiles = kSms;  // of the pool, a CTA each
-constexpr int64_t kOneClusterEntries = 1 << 17;
+constexpr int kTiles = kSms;                  // of the pool, a CTA each
+// One CTA does it all in shared memory while tables and pool have up to so
+// many entries.  In one CTA and in a launch for each phase: freeing 200 entries
+// 3.8 and 6.8 us, 5000 6.0 and 7.2, 14000 9.0 and 6.9; forking 140 entries 6.7
+// and 10.0, 9200 9.5 and 9.8, 12600 12.9 and 11.7; compacting 7500 9.8 and
+// 12.1, 26900 24 and 12.
+constexpr int64_t kFewEntries = 1 << 13;
 constexpr uint32_t kAll = 0xffffffffu;
 
 enum Op { kFork, kFree, kCompact };
@@ -41,6 +44,7 @@ struct PagesArgs {
   int32_t* tile_counts;    // [kTiles] blocks that a tile of the pool adds to the list; and the blocks taken
   int32_t *holders, *map;  // compact: [num_blocks] tables that hold a block, less one; the move that a block takes part in
   int phase;               // of the form with a launch for each
+  int row_lanes, row_parts;  // see for_rows
 };
 
 __device__ __forceinline__ int held_of(const PagesArgs& a, int len) {
@@ -78,20 +82,62 @@ __device__ __forceinline__ Tile tile_of(const PagesArgs& a, int i) {
   return {(int)min((int64_t)a.num_blocks, i * size), (int)min((int64_t)a.num_blocks, (i + 1) * size)};
 }
 
-// Whether a block goes on the list: one that nothing holds any more (fork,
-// free), one that is held (compact).  Written by atomics of other SMs before.
-template <Op OP>
-__device__ __forceinline__ bool listed(const PagesArgs& a, int block) {
-  return OP == kCompact ? __ldcg(a.holders + block) >= 0 : __ldcg(a.shares_out + block) < 0;
-}
+// What is counted for each block: the tables that hold it, less one.  ONE: in
+// shared memory, else in global memory, by all SMs.
+template <Op OP, bool ONE> struct Holders {
+  int* of;
+  int* tiles;  // in shared memory: what this CTA adds to the tiles' counts
+  __device__ __forceinline__ int operator[](int block) const { return ONE ? of[block] : __ldcg(of + block); }
+  // Whether a block goes on the list: one that nothing holds any more (fork, free), one that is held (compact).
+  __device__ __forceinline__ bool listed(int block) const { return ((*this)[block] < 0) != (OP == kCompact); }
+  // Adds, and keeps count of the listed blocks of each tile: however often a block gets on the list and off it again
+  // meanwhile, in whatever order, its ups and downs come to what it is at the end.  All additions are under way before
+  // the first one's result is looked at.
+  template <int N>
+  __device__ __forceinline__ void add(const PagesArgs& a, const int (&block)[N], const int (&n)[N]) const {
+    int old[N] = {};
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (n[i] != 0 && in_pool(a, block[i])) old[i] = atomicAdd(of + block[i], n[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (!ONE && n[i] != 0 && in_pool(a, block[i]) && (old[i] < 0) != (old[i] + n[i] < 0))
+        atomicAdd(tiles + block[i] / tile_size(a), (old[i] + n[i] < 0) != (OP == kCompact) ? 1 : -1);
+  }
+};
 
-// The tiles' counts before tile i, and of all.
-__device__ __forceinline__ int2 counts_before(const PagesArgs& a, int i, int* sums) {
+// Listed blocks of the tiles before tile i, and of all.
+template <Op OP, bool ONE>
+__device__ __forceinline__ int2 counts_before(const PagesArgs& a, const Holders<OP, ONE>& h, int i, int* sums) {
   int total = 0, unused;
+  if (ONE) {
+    int n = 0;
+    for (int b = threadIdx.x; b < a.num_blocks; b += kThreads) n += h.listed(b);
+    scan(n, sums, total);
+    return make_int2(0, total);
+  }
   const int mine = threadIdx.x < gridDim.x ? __ldcg(a.tile_counts + threadIdx.x) : 0;
   scan(mine, sums, total);
   scan(threadIdx.x < i ? mine : 0, sums, unused);
   return make_int2(unused, total);
+}
+
+// f(row, entries) for every thread's shares of the rows: kEach entries each, of which those below the width are any.
+// A long row is shared by several warps, several short ones by a warp.
+constexpr int kEach = 4;
+template <typename F>
+__device__ __forceinline__ void for_rows(const PagesArgs& a, int rows, F&& f) {
+  const int shift = __ffs(a.row_lanes) - 1, lane = threadIdx.x & (a.row_lanes - 1);
+  const int64_t all = gridDim.x * kThreads >> shift, units = (int64_t)rows * a.row_parts;
+  for (int64_t u = (blockIdx.x * kThreads + threadIdx.x) >> shift; u < units; u += all) {
+    // a long division where it has to be
+    const int r = units <= INT32_MAX ? (int)((uint32_t)u / (uint32_t)a.row_parts) : (int)(u / a.row_parts);
+    const int first = (int)(u - (int64_t)r * a.row_parts) * a.row_lanes * kEach + lane;
+    int at[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) at[i] = first + i * a.row_lanes;
+    f(r, at);
+  }
 }
 
 // Of the num_free first free blocks, within the list.
@@ -152,7 +198,8 @@ __device__ __forceinline__ int plan_children(const PagesArgs& a, const Children&
 }
 
 // The children's results, their tables, and the holders that their parents' blocks win and lose.
-__device__ __forceinline__ void fork_tables(const PagesArgs& a, const Children& c) {
+template <bool ONE>
+__device__ __forceinline__ void fork_tables(const PagesArgs& a, const Children& c, const Holders<kFork, ONE>& h) {
   const int left = free_of(a), me = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads;
   for (int r = me; r < a.children; r += all) {
     const int rank = c.rank[r], p = a.parents[r];
@@ -162,95 +209,84 @@ __device__ __forceinline__ void fork_tables(const PagesArgs& a, const Children& 
     a.destinations[r] = rank >= 0 ? a.free_blocks[left - 1 - rank] : -1;
     a.served[r] = !valid || rank != -2;
   }
-  const int lane = threadIdx.x & 31, warp = me >> 5, warps = all >> 5;
-  for (int r = warp; r < a.children; r += warps) {
+  for_rows(a, a.children, [&](int r, const int (&at)[kEach]) {
     const int rank = c.rank[r], p = rank == -2 ? 0 : a.parents[r], held = rank == -2 ? 0 : held_of(a, a.lens[p]);
     const int32_t* from = a.tables + p * a.table_stride;
     int32_t* to = a.tables_out + (int64_t)r * a.width;
-#pragma unroll 4
-    for (int i = lane; i < a.width; i += 32) {
-      int block = -1;
-      if (i < held) block = rank >= 0 && i == held - 1 ? a.free_blocks[left - 1 - rank] : from[i];
-      to[i] = block;
-    }
-  }
-  for (int p = warp; p < a.requests; p += warps) {
+    int block[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      block[i] = at[i] >= held ? -1 : rank >= 0 && at[i] == held - 1 ? a.free_blocks[left - 1 - rank] : from[at[i]];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (at[i] < a.width) to[at[i]] = block[i];
+  });
+  for_rows(a, a.requests, [&](int p, const int (&at)[kEach]) {
     const int len = a.lens[p], held = held_of(a, len), more = c.count[p] - 1;
     const bool part = len > 0 && len % a.block_size != 0 && held == ((int64_t)len + a.block_size - 1) / a.block_size;
     const int32_t* from = a.tables + p * a.table_stride;
-#pragma unroll 4
-    for (int i = lane; i < held; i += 32) {
-      const int block = from[i];
-      int delta = more;
-      if (part && i == held - 1) delta = c.first[p] < a.children && stays(a, block) ? 0 : -1;
-      if (delta != 0 && in_pool(a, block)) atomicAdd(a.shares_out + block, delta);
+    if (more == 0 && !part) return;
+    int block[kEach], delta[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      block[i] = at[i] < held ? from[at[i]] : -1;
+      delta[i] = more;
     }
-  }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (part && at[i] == held - 1) delta[i] = c.first[p] < a.children && stays(a, block[i]) ? 0 : -1;
+    h.add(a, block, delta);
+  });
 }
 
 // ------------------------------------------------------------ the phases
 
 // 0: what later phases add to is set up.
-template <Op OP>
-__device__ __forceinline__ void set_up(const PagesArgs& a) {
+template <Op OP, bool ONE>
+__device__ __forceinline__ void set_up(const PagesArgs& a, const Holders<OP, ONE>& h) {
   const int me = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads;
-  if (OP == kCompact) {
-    for (int b = me; b < a.num_blocks; b += all) {
-      a.holders[b] = -1;
-      if (b < a.num_blocks / 2) a.sources[b] = a.destinations[b] = -1;
-    }
-  } else {
-    for (int b = me; b < a.num_blocks; b += all) a.shares_out[b] = a.shares[b];
-  }
+#pragma unroll 4
+  for (int b = me; b < a.num_blocks; b += all) h.of[b] = OP == kCompact ? -1 : a.shares[b];
+  if (OP == kCompact)
+    for (int i = me; i < a.num_blocks / 2; i += all) a.sources[i] = a.destinations[i] = -1;
+  if (!ONE && me < kTiles) a.tile_counts[me] = 0;
 }
 
 // 1: holders are counted.
-template <Op OP>
-__device__ __forceinline__ void count_holders(const PagesArgs& a, const Children& c) {
-  const int me = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads;
-  if (OP == kFork) {
-    fork_tables(a, c);
-    return;
-  }
-  const int lane = threadIdx.x & 31;
-  for (int r = me >> 5; r < a.requests; r += all >> 5) {
-    const int len = a.lens[r], held = held_of(a, len);
-    const int first = OP == kFree ? held_of(a, min(a.keep[r], len)) : 0;
-    const int32_t* from = a.tables + r * a.table_stride;
-#pragma unroll 4
-    for (int i = first + lane; i < held; i += 32) {
-      const int block = from[i];
-      if (in_pool(a, block)) atomicAdd(OP == kFree ? a.shares_out + block : a.holders + block, OP == kFree ? -1 : 1);
-    }
+template <Op OP, bool ONE>
+__device__ __forceinline__ void count_holders(const PagesArgs& a, const Children& c, const Holders<OP, ONE>& h) {
+  if constexpr (OP == kFork) {
+    fork_tables(a, c, h);
+  } else {
+    for_rows(a, a.requests, [&](int r, const int (&at)[kEach]) {
+      const int len = a.lens[r], held = held_of(a, len);
+      const int kept = OP == kFree ? held_of(a, min(a.keep[r], len)) : 0;
+      const int32_t* from = a.tables + r * a.table_stride;
+      int block[kEach], n[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        n[i] = OP == kFree ? -1 : 1;
+        block[i] = at[i] >= kept && at[i] < held ? from[at[i]] : -1;
+      }
+      h.add(a, block, n);
+    });
   }
 }
 
-// 2: listed blocks of the CTA's tile are counted.
-template <Op OP>
-__device__ __forceinline__ void count_listed(const PagesArgs& a, int* sums) {
+// 2, fork and free: the free list, and behind what is left of it the blocks that nothing holds any more.
+template <Op OP, bool ONE>
+__device__ __forceinline__ void write_free(const PagesArgs& a, const Holders<OP, ONE>& h, int left, int* sums) {
   const Tile t = tile_of(a, blockIdx.x);
-  int n = 0, total;
-#pragma unroll 4
-  for (int b = t.begin + threadIdx.x; b < t.end; b += kThreads) n += listed<OP>(a, b);
-  scan(n, sums, total);
-  if (threadIdx.x == 0) a.tile_counts[blockIdx.x] = total;
-}
-
-// 3, fork and free: the free list, and behind what is left of it the blocks that nothing holds any more.
-__device__ __forceinline__ void write_free(const PagesArgs& a, int left, int* sums) {
-  const Tile t = tile_of(a, blockIdx.x);
-  const int2 before = counts_before(a, blockIdx.x, sums);
+  const int2 before = counts_before(a, h, blockIdx.x, sums);
   int at = left + before.x;
   for (int b0 = t.begin; b0 < t.end; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
-    const bool gone = b < t.end && listed<kFree>(a, b);
+    const bool gone = b < t.end && h.listed(b);
     int total;
     const int place = at + scan(gone, sums, total);
     at += total;
-    if (gone) {
-      if (place < a.num_blocks) a.free_out[place] = b;
-      a.shares_out[b] = 0;
-    }
+    if (gone && place < a.num_blocks) a.free_out[place] = b;
+    if (gone || (ONE && b < t.end)) a.shares_out[b] = gone ? 0 : h[b];
   }
   const int end = (int)min((int64_t)a.num_blocks, (int64_t)left + before.y);
   for (int i = blockIdx.x * kThreads + threadIdx.x; i < a.num_blocks; i += gridDim.x * kThreads)
@@ -258,27 +294,28 @@ __device__ __forceinline__ void write_free(const PagesArgs& a, int left, int* su
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.num_free_out = end;
 }
 
-// 3, compact: with U used blocks, those from U on are numbered in order, and so are the holes below it.
-__device__ __forceinline__ void write_moves(const PagesArgs& a, int* sums) {
+// 2, compact: with U used blocks, those from U on are numbered in order, and so are the holes below it.
+template <bool ONE>
+__device__ __forceinline__ void write_moves(const PagesArgs& a, const Holders<kCompact, ONE>& h, int* map, int* sums) {
   const Tile t = tile_of(a, blockIdx.x);
-  const int2 before = counts_before(a, blockIdx.x, sums);
+  const int2 before = counts_before(a, h, blockIdx.x, sums);
   const int used = before.y;
   // used blocks below U: those of the tiles before U's, and those of its own before it
   const int of = min((int)(used / max(tile_size(a), 1)), (int)gridDim.x - 1);
-  int inside = counts_before(a, of, sums).x, n = 0, total;
+  int inside = counts_before(a, h, of, sums).x, n = 0, total;
 #pragma unroll 4
-  for (int b = tile_of(a, of).begin + threadIdx.x; b < used; b += kThreads) n += listed<kCompact>(a, b);
+  for (int b = tile_of(a, of).begin + threadIdx.x; b < used; b += kThreads) n += h.listed(b);
   scan(n, sums, total);
   inside += total;
   int at = before.x;
   for (int b0 = t.begin; b0 < t.end; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
-    const bool in = b < t.end && listed<kCompact>(a, b);
+    const bool in = b < t.end && h.listed(b);
     const int below = at + scan(in, sums, total);  // used blocks below b
     at += total;
     if (b < t.end && in && b >= used) {
       a.sources[below - inside] = b;
-      a.map[b] = below - inside;
+      map[b] = below - inside;
     } else if (b < t.end && !in && b < used) {
       a.destinations[b - below] = b;
     }
@@ -286,26 +323,31 @@ __device__ __forceinline__ void write_moves(const PagesArgs& a, int* sums) {
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.num_free_out = a.num_blocks - used;
 }
 
-// 4, compact: tables, shares and free list by the new numbers.
-__device__ __forceinline__ void renumber(const PagesArgs& a) {
-  const int me = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads, lane = threadIdx.x & 31;
+// 3, compact: tables, shares and free list by the new numbers.
+template <bool ONE>
+__device__ __forceinline__ void renumber(const PagesArgs& a, const Holders<kCompact, ONE>& h, const int* map) {
+  const int me = blockIdx.x * kThreads + threadIdx.x, all = gridDim.x * kThreads;
   const int used = a.num_blocks - __ldcg(a.num_free_out);
-  for (int r = me >> 5; r < a.requests; r += all >> 5) {
+  const auto moved = [&](int block) { return __ldcg(a.destinations + (ONE ? map[block] : __ldcg(map + block))); };
+  for_rows(a, a.requests, [&](int r, const int (&at)[kEach]) {
     const int held = held_of(a, a.lens[r]);
     const int32_t* from = a.tables + r * a.table_stride;
     int32_t* to = a.tables_out + (int64_t)r * a.width;
-#pragma unroll 4
-    for (int i = lane; i < a.width; i += 32) {
-      int block = i < held ? from[i] : -1;
-      if (block >= used && block < a.num_blocks) block = __ldcg(a.destinations + __ldcg(a.map + block));
-      to[i] = block;
-    }
-  }
+    int block[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) block[i] = at[i] < held ? from[at[i]] : -1;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (block[i] >= used && block[i] < a.num_blocks) block[i] = moved(block[i]);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (at[i] < a.width) to[at[i]] = block[i];
+  });
   for (int b = me; b < a.num_blocks; b += all) {
-    const int holders = __ldcg(a.holders + b);
+    const int holders = h[b];
     if (b >= used) {
       a.shares_out[b] = 0;
-      if (holders >= 0) a.shares_out[__ldcg(a.destinations + __ldcg(a.map + b))] = holders;
+      if (holders >= 0) a.shares_out[moved(b)] = holders;
     } else if (holders >= 0) {
       a.shares_out[b] = holders;
     }
@@ -313,57 +355,72 @@ __device__ __forceinline__ void renumber(const PagesArgs& a) {
   }
 }
 
-// ONE: all phases, over one cluster of CTAs with its barrier between them;
-// otherwise the phase a.phase, over any number of them.  Small steps are bound
-// by the latency of launches, barriers and dependent loads.
+// ONE: all phases, in one CTA; otherwise the phase a.phase, over any number of
+// them, a launch for each.  Bound by the latency of launches (2.3 us each) and
+// of dependent loads: a child's parent, its length, its last block, that
+// block's shares.  256 requests of up to 545 blocks freed in 7.9 us (before the
+// entries of long rows were shared among warps, four at a time to a thread:
+// 18), 2048 forked in 14.6, 1024 tables of up to 273 blocks compacted in 13.5.
+// One cluster of eight CTAs for all phases took 6.3 to 12.6 us where one CTA
+// takes 3.8 to 9.5.
 template <Op OP, bool ONE>
 __global__ void __launch_bounds__(kThreads, 1) pages_kernel(const __grid_constant__ PagesArgs a) {
-  extern __shared__ int s_children[];
-  __shared__ int sums[kWarps];
+  extern __shared__ int s_all[];  // ONE: holders, and for compact the map; the children
+  __shared__ int sums[kWarps], tiles[kTiles];
   static_assert(kWarps == 32, "scan() takes a sum to a lane");
+  int* const values = ONE ? s_all : OP == kCompact ? a.holders : a.shares_out;
+  int* const map = ONE ? s_all + a.num_blocks : a.map;
+  int* const s_children = s_all + (ONE ? a.num_blocks : 0);
   const Children c{s_children, s_children + a.requests, s_children + 2 * a.requests};
+  const Holders<OP, ONE> h{values, tiles};
   dev::wait_for_previous();
-  if (ONE || a.phase == 0) set_up<OP>(a);
+  if (ONE || a.phase == 0) set_up<OP, ONE>(a, h);
   int taken = 0;
   if (OP == kFork && (ONE || a.phase == 1)) {
     taken = plan_children(a, c, sums);
     if (!ONE && blockIdx.x == 0 && threadIdx.x == 0) a.tile_counts[kTiles] = taken;
   }
-  if (OP == kFork && !ONE && a.phase == 3) taken = a.tile_counts[kTiles];
-  if (ONE) dev::cluster_sync();
-  if (ONE || a.phase == 1) count_holders<OP>(a, c);
-  if (ONE) dev::cluster_sync();
-  if (ONE || a.phase == 2) count_listed<OP>(a, sums);
-  if (ONE) dev::cluster_sync();
-  if (ONE || a.phase == 3) {
-    if (OP == kCompact) write_moves(a, sums);
-    else write_free(a, free_of(a) - taken, sums);
+  if (OP == kFork && !ONE && a.phase == 2) taken = a.tile_counts[kTiles];
+  if (ONE) __syncthreads();
+  if (!ONE && a.phase == 1) {
+    if (threadIdx.x < kTiles) tiles[threadIdx.x] = 0;
+    __syncthreads();
   }
-  if (OP == kCompact) {
-    if (ONE) dev::cluster_sync();
-    if (ONE || a.phase == 4) renumber(a);
+  if (ONE || a.phase == 1) count_holders<OP, ONE>(a, c, h);
+  if (ONE || a.phase == 1) __syncthreads();
+  if (!ONE && a.phase == 1 && threadIdx.x < kTiles && tiles[threadIdx.x] != 0)
+    atomicAdd(a.tile_counts + threadIdx.x, tiles[threadIdx.x]);
+  if constexpr (OP == kCompact) {
+    if (ONE || a.phase == 2) write_moves<ONE>(a, h, map, sums);
+    if (ONE) __syncthreads();
+    if (ONE || a.phase == 3) renumber<ONE>(a, h, map);
+  } else {
+    if (ONE || a.phase == 2) write_free<OP, ONE>(a, h, free_of(a) - taken, sums);
   }
 }
 
 template <Op OP>
 cudaError_t run(PagesArgs a, cudaStream_t stream) {
-  const size_t smem = OP == kFork ? sizeof(int) * (2 * (size_t)a.requests + a.children) : 0;
-  const size_t most = OP == kFork ? sizeof(int) * 3 * kMaxRequests : 0;
-  const auto limit = [&](auto kernel) {
-    // the limit is the kernel's, not the call's: the same one from every host thread
-    return smem > 40 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most)
-                            : cudaSuccess;
+  const size_t children = OP == kFork ? sizeof(int) * (2 * (size_t)a.requests + a.children) : 0;
+  const size_t all = children + sizeof(int) * (size_t)a.num_blocks * (OP == kCompact ? 2 : 1);
+  // the limit is the kernel's, not the call's: the same one from every host thread
+  constexpr size_t kMost = 226 * 1024, kPlain = 40 * 1024;
+  const auto limit = [&](auto kernel, size_t smem) {
+    return smem > kPlain ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost)
+                         : cudaSuccess;
   };
   const int64_t entries = (int64_t)(a.requests + a.children) * a.width + a.num_blocks;
-  if (entries <= kOneClusterEntries) {
-    const cudaError_t e = limit(pages_kernel<OP, true>);
-    return e ? e : launch_after_previous(pages_kernel<OP, true>, kCluster, kThreads, smem, a, stream, kCluster);
+  a.row_lanes = 1;
+  while (a.row_lanes < 32 && a.row_lanes * kEach < a.width) a.row_lanes *= 2;
+  a.row_parts = std::max(1, (a.width + a.row_lanes * kEach - 1) / (a.row_lanes * kEach));
+  if (entries <= kFewEntries && all <= kMost) {
+    const cudaError_t e = limit(pages_kernel<OP, true>, all);
+    return e ? e : launch_after_previous(pages_kernel<OP, true>, 1, kThreads, all, a, stream);
   }
-  cudaError_t e = limit(pages_kernel<OP, false>);
-  const int grid = (int)std::min<int64_t>(kSms, (entries + kThreads - 1) / kThreads);
-  for (a.phase = 0; !e && a.phase < (OP == kCompact ? 5 : 4); ++a.phase)
-    e = launch_after_previous(pages_kernel<OP, false>, grid, kThreads, OP == kFork && a.phase == 1 ? smem : 0, a,
-                              stream);
+  cudaError_t e = limit(pages_kernel<OP, false>, children);
+  const int grid = (int)std::min<int64_t>(kTiles, (entries + kThreads - 1) / kThreads);
+  for (a.phase = 0; !e && a.phase < (OP == kCompact ? 4 : 3); ++a.phase)
+    e = launch_after_previous(pages_kernel<OP, false>, grid, kThreads, a.phase == 1 ? children : 0, a, stream);
   return e;
 }
 
@@ -386,7 +443,9 @@ struct CopyArgs {
 };
 
 // Pairs that are none cost a look each: a CTA looks at 128 of its pairs at a
-// time and copies the blocks of those that are.  Bound by memory.
+// time and copies the blocks of those that are.  Bound by memory: 5923 blocks
+// of 32 KB in four caches 263 us, 5.9 TB/s (90 % of the copy rate), 596 of 16
+// KB 14 us, 5.6 TB/s.
 template <typename V>
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ CopyArgs a) {
   __shared__ int2 pairs[kCopyThreads];

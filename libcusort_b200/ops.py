@@ -18,9 +18,18 @@ Importing this module registers, in the ``cusort`` namespace:
   Tensor sources, Tensor positions)``
 * ``dispatch(Tensor x, Tensor sources, Tensor positions) -> Tensor``
 * ``combine(Tensor rows, Tensor weights, Tensor sources, Tensor positions, Tensor? residual=None) -> Tensor``
+* ``expert_products(Tensor rows, Tensor weights, Tensor counts, Tensor offsets) -> Tensor``
 * ``page_plan(Tensor cached_lens, Tensor new_lens, Tensor(a!) block_tables, int block_size, int num_tokens,
   Tensor free_blocks, Tensor num_free) -> (Tensor slots, Tensor positions, Tensor starts, Tensor served,
   Tensor num_free)``
+* ``page_fork(Tensor block_tables, Tensor lens, Tensor parents, int block_size, Tensor free_blocks, Tensor num_free,
+  Tensor shares) -> (Tensor block_tables, Tensor lens, Tensor sources, Tensor destinations, Tensor served,
+  Tensor shares, Tensor free_blocks, Tensor num_free)``
+* ``page_free(Tensor block_tables, Tensor lens, Tensor keep_lens, int block_size, Tensor free_blocks, Tensor num_free,
+  Tensor shares) -> (Tensor shares, Tensor free_blocks, Tensor num_free)``
+* ``page_compact(Tensor block_tables, Tensor lens, int block_size, int num_blocks) -> (Tensor block_tables,
+  Tensor sources, Tensor destinations, Tensor shares, Tensor free_blocks, Tensor num_free)``
+* ``page_copy(Tensor(a!)[] caches, Tensor sources, Tensor destinations) -> ()``
 
 ``sort_pairs`` takes payload rows of any width (rows of 1, 2, 4, 8 or 16 bytes move with the keys,
 others are gathered by the sorted permutation).  The segmented operators sort every segment
@@ -29,9 +38,11 @@ outside every segment keep their input.
 
 The routing operators are those of ``libcusort_b200.routing`` (its docstrings have the details), with
 gradients through autograd: ``route`` to the logits, ``dispatch`` to the rows (float32, float16 or bfloat16
-ones), ``combine`` to the rows, the weights and the residual.  ``page_plan`` is that of ``libcusort_b200.paging`` with a free list.
+ones), ``combine`` to the rows, the weights and the residual.  ``expert_products`` is that of ``libcusort_b200.experts``,
+with gradients to the rows and the weights.  ``page_plan`` (with a free list) and the other page operators are those of
+``libcusort_b200.paging``.
 
-All of them are stable, allocate fresh outputs (the inputs are never written, except ``page_plan``'s block tables), run on torch's current
+All of them are stable, allocate fresh outputs (the inputs are never written, except ``page_plan``'s block tables and ``page_copy``'s caches), run on torch's current
 CUDA stream through the C ABI (``cusort_sort_keys``, ``cusort_sort_pairs``, ``cusort_route`` and so on) and have
 fake (meta) implementations, so they trace under ``torch.compile`` / ``torch.export`` as opaque
 calls.  ``end_bit = -1`` means all key bits.  There is no CPU implementation: a CPU tensor raises.
@@ -42,7 +53,7 @@ from __future__ import annotations
 
 import torch
 
-from . import paging, routing
+from . import experts as _experts, paging, routing
 from .torch_sort import radix_sort, segmented_sort
 
 
@@ -240,6 +251,59 @@ def _combine_grad(ctx, grad_out):
 combine.register_autograd(_combine_grad, setup_context=_combine_setup)
 
 
+@torch.library.custom_op("cusort::expert_products", mutates_args=())
+def expert_products(rows: torch.Tensor, weights: torch.Tensor, counts: torch.Tensor,
+                    offsets: torch.Tensor) -> torch.Tensor:
+    return _experts.expert_products(rows, weights, counts, offsets)
+
+
+@expert_products.register_fake
+def _(rows, weights, counts, offsets):
+    return rows.new_empty((rows.shape[0], weights.shape[2]))
+
+
+@torch.library.custom_op("cusort::expert_products_grad_rows", mutates_args=())
+def expert_products_grad_rows(grad_out: torch.Tensor, weights: torch.Tensor, counts: torch.Tensor,
+                              offsets: torch.Tensor) -> torch.Tensor:
+    return _experts.expert_products_grad_rows(_rowwise(grad_out), weights, counts, offsets)
+
+
+@expert_products_grad_rows.register_fake
+def _(grad_out, weights, counts, offsets):
+    return grad_out.new_empty((grad_out.shape[0], weights.shape[1]))
+
+
+@torch.library.custom_op("cusort::expert_products_grad_weights", mutates_args=())
+def expert_products_grad_weights(grad_out: torch.Tensor, rows: torch.Tensor, counts: torch.Tensor,
+                                 offsets: torch.Tensor, in_contiguous: bool = False) -> torch.Tensor:
+    return _experts.expert_products_grad_weights(_rowwise(grad_out), rows, counts, offsets, in_contiguous=in_contiguous)
+
+
+@expert_products_grad_weights.register_fake
+def _(grad_out, rows, counts, offsets, in_contiguous=False):
+    shape = counts.shape[0], rows.shape[1], grad_out.shape[1]
+    return rows.new_empty((shape[0], shape[2], shape[1])).transpose(1, 2) if in_contiguous else rows.new_empty(shape)
+
+
+def _products_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
+
+
+def _products_grad(ctx, grad_out):
+    rows, weights, counts, offsets = ctx.saved_tensors
+    grad_rows = grad_weights = None
+    if ctx.needs_input_grad[0]:
+        grad_rows = torch.ops.cusort.expert_products_grad_rows(grad_out, weights, counts, offsets)
+    if ctx.needs_input_grad[1]:
+        # in the weights' order: their contiguous dimension is that of the gradient
+        in_contiguous = weights.stride(2) != 1 and weights.shape[2] != 1
+        grad_weights = torch.ops.cusort.expert_products_grad_weights(grad_out, rows, counts, offsets, in_contiguous)
+    return grad_rows, grad_weights, None, None
+
+
+expert_products.register_autograd(_products_grad, setup_context=_products_setup)
+
+
 @torch.library.custom_op("cusort::page_plan", mutates_args=("block_tables",))
 def page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: torch.Tensor, block_size: int,
               num_tokens: int, free_blocks: torch.Tensor, num_free: torch.Tensor
@@ -254,3 +318,55 @@ def _(cached_lens, new_lens, block_tables, block_size, num_tokens, free_blocks, 
     new = cached_lens.new_empty
     return (new(num_tokens, dtype=torch.int64), new(num_tokens), new(requests + 1), new(requests, dtype=torch.bool),
             new(1))
+
+
+@torch.library.custom_op("cusort::page_fork", mutates_args=())
+def page_fork(block_tables: torch.Tensor, lens: torch.Tensor, parents: torch.Tensor, block_size: int,
+              free_blocks: torch.Tensor, num_free: torch.Tensor, shares: torch.Tensor
+              ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor,
+                         torch.Tensor, torch.Tensor]:
+    return tuple(paging.page_fork(block_tables, lens, parents, block_size, free_blocks=free_blocks, num_free=num_free,
+                                  shares=shares, separate=True))
+
+
+@page_fork.register_fake
+def _(block_tables, lens, parents, block_size, free_blocks, num_free, shares):
+    new, children, blocks = lens.new_empty, parents.shape[0], shares.shape[0]
+    return (new((children, block_tables.shape[1])), new(children), new(children), new(children),
+            new(children, dtype=torch.bool), new(blocks), new(blocks), new(1))
+
+
+@torch.library.custom_op("cusort::page_free", mutates_args=())
+def page_free(block_tables: torch.Tensor, lens: torch.Tensor, keep_lens: torch.Tensor, block_size: int,
+              free_blocks: torch.Tensor, num_free: torch.Tensor, shares: torch.Tensor
+              ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return tuple(paging.page_free(block_tables, lens, keep_lens, block_size, free_blocks=free_blocks,
+                                  num_free=num_free, shares=shares, separate=True))
+
+
+@page_free.register_fake
+def _(block_tables, lens, keep_lens, block_size, free_blocks, num_free, shares):
+    blocks = shares.shape[0]
+    return lens.new_empty(blocks), lens.new_empty(blocks), lens.new_empty(1)
+
+
+@torch.library.custom_op("cusort::page_compact", mutates_args=())
+def page_compact(block_tables: torch.Tensor, lens: torch.Tensor, block_size: int, num_blocks: int
+                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return tuple(paging.page_compact(block_tables, lens, block_size, num_blocks, separate=True))
+
+
+@page_compact.register_fake
+def _(block_tables, lens, block_size, num_blocks):
+    new, half = lens.new_empty, num_blocks // 2
+    return new(block_tables.shape), new(half), new(half), new(num_blocks), new(num_blocks), new(1)
+
+
+@torch.library.custom_op("cusort::page_copy", mutates_args=("caches",))
+def page_copy(caches: list[torch.Tensor], sources: torch.Tensor, destinations: torch.Tensor) -> None:
+    paging.page_copy(list(caches), sources, destinations)
+
+
+@page_copy.register_fake
+def _(caches, sources, destinations):
+    return None

@@ -1,6 +1,8 @@
 """The experts' products and their gradients against a plain implementation in 64 bits."""
 from __future__ import annotations
 
+import threading
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -176,6 +178,19 @@ def test_same_result_again_and_on_another_stream():
         again = (X.expert_products(x, w, c, o), *X.expert_products_backward(g, x, w, c, o))
     stream.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(first, again))
+
+
+def test_from_another_host_thread():
+    """A thread that has made no CUDA call before."""
+    c, o, capacity, _ = plan([100, 30])
+    x, w = matrix(capacity, 64, torch.bfloat16), weights_of(2, 64, 72, torch.bfloat16, "in_out")
+    here, there = X.expert_products(x, w, c, o), []
+    torch.cuda.synchronize()
+    thread = threading.Thread(target=lambda: there.append(X.expert_products(x, w, c, o)))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert torch.equal(here, there[0])
 
 
 def test_segments_that_are_no_plan_stay_inside():
