@@ -272,7 +272,7 @@ struct ProductArgs {
 // PAIR: tiles of 256 columns of the result, 128 in each of two CTAs, and half of the rows in each.
 template <int BN, int STAGES, int SUB, bool PAIR> struct ProductShape {
   static constexpr int kCtas = PAIR ? 2 : 1, kTile = kTileM * kCtas;
-  static constexpr int kRowStep = 16 * kCtas;       // the instruction's width comes in such steps
+  static constexpr int kRowStep = 16;               // the instruction's width comes in such steps
   static constexpr int kBoxRows = PAIR ? 64 : 16;   // a tile of few rows brings few boxes
   // A stage holds SUB steps of kBlockK, each the weights' part and then the rows'.
   static constexpr uint32_t kBytesB = BN / kCtas * kBlockK * 2, kStep = kBytesA + kBytesB, kStage = SUB * kStep;
