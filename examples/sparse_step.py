@@ -26,7 +26,7 @@ cusort = torch.ops.cusort
 class SparseLayer(torch.nn.Module):
     """x + the weighted sum of each token's k experts' two-layer networks."""
 
-    ALIGN = 16  # rows to a product tile: no tile holds two experts' rows
+    ALIGN = 16  # every expert's rows begin at a multiple of it
 
     def __init__(self, hidden: int, inner: int, experts: int, k: int, **how):
         super().__init__()
@@ -39,18 +39,9 @@ class SparseLayer(torch.nn.Module):
         weights, experts = cusort.route(x @ self.router, self.k, renormalize=True)
         counts, offsets, sources, positions = cusort.plan_dispatch(experts, self.router.shape[1], self.ALIGN)
         rows = cusort.dispatch(x, sources, positions)
-        if x.dtype != torch.float32:
-            inner = torch.relu(cusort.expert_products(rows, self.up, counts, offsets))
-            return cusort.combine(cusort.expert_products(inner, self.down, counts, offsets), weights, sources,
-                                  positions, x)
-        # 32-bit weights, which the products do not take: the rows in tiles, each with its expert's matrices; rows that hold no pair are zeros, and so are their products
-        tiles = -(-rows.shape[0] // self.ALIGN)
-        rows = torch.nn.functional.pad(rows, (0, 0, 0, tiles * self.ALIGN - rows.shape[0]))
-        first = torch.arange(tiles, device=x.device, dtype=torch.int32) * self.ALIGN
-        expert = torch.searchsorted(offsets[1:], first, right=True).clamp(max=self.router.shape[1] - 1)
-        inner = torch.relu(rows.view(tiles, self.ALIGN, -1) @ self.up[expert])
-        y = (inner @ self.down[expert]).view(tiles * self.ALIGN, -1)[:sources.shape[0]]
-        return cusort.combine(y.contiguous(), weights, sources, positions, x)
+        inner = torch.relu(cusort.expert_products(rows, self.up, counts, offsets))
+        y = cusort.expert_products(inner, self.down, counts, offsets)
+        return cusort.combine(y, weights, sources, positions, x)
 
     def dense(self, x: torch.Tensor) -> torch.Tensor:
         """The same by every expert on every token."""

@@ -363,17 +363,17 @@ cudaError_t cusort_combine_rows_backward(cusort_float_type type, const void* d_g
  * (d_offsets[e] <= r < d_offsets[e] + d_counts[e], as cusort_plan_dispatch
  * gives them)
  *   d_out[r] = d_rows[r] x weights[e],
- * zeros for rows of no segment.  float16 or bfloat16 alone; sums in 32 bits,
- * rounded once.  d_rows: `capacity` rows of `in` contiguous elements,
+ * zeros for rows of no segment.  Sums in 32 bits, rounded once; 32-bit
+ * operands are multiplied as they are (and not on the tensor cores).  d_rows: `capacity` rows of `in` contiguous elements,
  * row_stride elements apart; weights[e][i][o] at d_weights + e * expert_stride
  * + i * in_stride + o * out_stride, one of the last two strides 1; d_out:
  * capacity x out, contiguous, on a 16-byte boundary.  With weights and widths
  * the other way round it is the gradient of the rows.
  * Segments beyond the capacity are cut there; they must not overlap.
  * 1 <= in, out <= 2^20, capacity < 2^31, num_experts <= 1024.
- * Two-phase temp protocol, with the same arguments in both calls: operands
- * whose addresses and strides are all multiples of 16 bytes need none, others
- * are laid out anew there (at a 16-byte boundary). */
+ * Two-phase temp protocol, with the same arguments in both calls: 16-bit
+ * operands whose addresses or strides are no multiples of 16 bytes are laid
+ * out anew there (at a 16-byte boundary), others need none. */
 cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp_storage_bytes, cusort_float_type type,
                                    const void* d_rows, int64_t row_stride, const void* d_weights,
                                    int64_t expert_stride, int64_t in_stride, int64_t out_stride,

@@ -1,6 +1,7 @@
 // cusort_experts.cu -- the experts' matrix products: every row of a segment
 // times its expert's weights, and the gradient of the weights.  (The gradient
-// of the rows is the product with the weights' other order.)
+// of the rows is the product with the weights' other order.)  16-bit operands
+// here, on the tensor cores; 32-bit ones in cusort_experts_f32.cu.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -14,6 +15,7 @@
 
 #include "../../include/cusort_b200.h"
 #include "cusort_dispatch.h"
+#include "cusort_experts.cuh"
 #include "cusort_float.cuh"
 #include "cusort_overlap.cuh"
 #include "cusort_tensor.cuh"
@@ -64,7 +66,6 @@ namespace {
 
 using namespace cusort_b200;
 
-constexpr int kMaxExperts = 1024;
 constexpr int kThreads = 320;  // warps 0, 2, 8 and 9 bring operands, 1 multiplies, 3 clears rows, 4 to 7 store
 constexpr int kSms = 148;
 constexpr int kBlockK = 64;              // contracted elements to a stage: one swizzle row
@@ -74,76 +75,6 @@ constexpr uint32_t kAll = 0xffffffffu;
 
 // Products that gave up waiting (a bounded wait ran out): 1.
 __device__ uint32_t g_product_status;
-
-// Expert segments as the CTA keeps them in shared memory.
-struct Segments {
-  int32_t* first;  // [experts] rows: clamped into [0, capacity]
-  int32_t* count;
-  int32_t* tiles;  // [experts + 1] sums of the tiles before each expert
-};
-
-struct SegmentArgs {
-  const int32_t *counts, *offsets;
-  int experts, capacity;
-};
-
-// First row and number of rows of an expert's segment, within the rows there are.
-__device__ __forceinline__ int2 segment(const SegmentArgs& a, int e) {
-  const int first = min(max(a.offsets[e], 0), a.capacity);
-  return make_int2(first, min(max(a.counts[e], 0), a.capacity - first));
-}
-
-// All threads: fills s; tiles(count) is the number of tiles of an expert with that many rows.
-template <typename F>
-__device__ __forceinline__ void load_segments(const SegmentArgs& a, const Segments& s, uint32_t* sums, F&& tiles) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int kEach = (kMaxExperts + kThreads - 1) / kThreads;
-  const int per = (a.experts + kThreads - 1) / kThreads;  // consecutive experts to a thread
-  int mine[kEach], sum = 0;
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int e = threadIdx.x * per + i;
-    mine[i] = 0;
-    if (i < per && e < a.experts) {
-      const int2 seg = segment(a, e);
-      s.first[e] = seg.x;
-      s.count[e] = seg.y;
-      mine[i] = tiles(seg.y);
-    }
-    sum += mine[i];
-  }
-  int scan = sum;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int v = __shfl_up_sync(kAll, scan, d);
-    if (lane >= d) scan += v;
-  }
-  if (lane == 31) sums[warp] = scan;
-  __syncthreads();
-  int before = scan - sum;
-  for (int w = 0; w < warp; ++w) before += sums[w];
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int e = threadIdx.x * per + i;
-    if (i < per && e < a.experts) {
-      s.tiles[e] = before;
-      before += mine[i];
-      if (e == a.experts - 1) s.tiles[a.experts] = before;
-    }
-  }
-  __syncthreads();
-}
-
-// The expert whose tiles hold tile t.
-__device__ __forceinline__ int find(const int32_t* tiles, int experts, int t) {
-  int low = 0, high = experts;  // tiles[low] <= t < tiles[high]
-  while (high - low > 1) {
-    const int mid = (low + high) >> 1;
-    if (tiles[mid] <= t) low = mid;
-    else high = mid;
-  }
-  return low;
-}
 
 // Barriers and flags of one CTA.  PAIR: two CTAs work on one tile, each with
 // half of either operand; the first one multiplies.
@@ -244,20 +175,6 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const d
 // the rate, with one for each operand a step took 350 cycles.
 __device__ __forceinline__ bool brings(int warp) { return warp == 0 || warp == 2 || warp >= 8; }
 
-__device__ __forceinline__ uint32_t align_up(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
-
-// Zeros in 16-bit elements [begin, end) of x, by `threads` threads.
-__device__ __forceinline__ void clear(uint16_t* x, int64_t begin, int64_t end, int thread, int threads) {
-  if (begin >= end) return;
-  const int64_t head = min(end, begin + (int64_t)((16 - (reinterpret_cast<uintptr_t>(x + begin) & 15)) % 16) / 2);
-  const int64_t words = (end - head) / 8;
-  uint4* body = reinterpret_cast<uint4*>(x + head);
-  if (begin + thread < head) x[begin + thread] = 0;
-#pragma unroll 4
-  for (int64_t i = thread; i < words; i += threads) body[i] = make_uint4(0, 0, 0, 0);
-  if (head + words * 8 + thread < end) x[head + words * 8 + thread] = 0;
-}
-
 // ---------------------------------------------------------------- the products
 
 struct ProductArgs {
@@ -325,7 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 
   init_pipe(p, Shape::kColumns);
   dev::wait_for_previous();
-  load_segments(a.segments, s, p.sums, [](int count) { return (count + BN - 1) / BN; });
+  load_segments<kThreads>(a.segments, s, p.sums, [](int count) { return (count + BN - 1) / BN; });
   const uint32_t tiles = (uint32_t)s.tiles[experts] * a.width_tiles;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = PAIR ? dev::cluster_rank() : 0;
   const int steps = (a.in + SUB * kBlockK - 1) / (SUB * kBlockK);
@@ -396,18 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       }
     }
   } else if (warp == 3) {
-    // rows that hold no pair: those between the segments by the expert before, those behind the last in equal parts
-    uint16_t* out = static_cast<uint16_t*>(a.out);
-    const int clearing = gridDim.x, me = blockIdx.x;
-    for (int e = me; e < experts; e += clearing) {
-      const int end = s.first[e] + s.count[e];
-      if (e + 1 < experts) clear(out, (int64_t)end * a.width, (int64_t)s.first[e + 1] * a.width, lane, 32);
-      if (e == 0) clear(out, 0, (int64_t)s.first[0] * a.width, lane, 32);
-    }
-    const int end = s.first[experts - 1] + s.count[experts - 1], left = a.segments.capacity - end;
-    const int per = (left + clearing - 1) / clearing;
-    const int64_t r0 = end + min((int64_t)left, (int64_t)me * per);
-    clear(out, r0 * a.width, min(r0 + per, (int64_t)a.segments.capacity) * a.width, lane, 32);
+    clear_other_rows(static_cast<uint16_t*>(a.out), a.width, a.segments, s, blockIdx.x, gridDim.x);
   } else if (warp >= 4 && warp < 8) {
     // the sums to 16 bits, through shared memory from a column of the result to a lane to a row's piece to a lane
     Ring<2> sums;
@@ -837,8 +743,6 @@ cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order
                   : run(product_kernel<T, BN, STAGES, SUB, PAIR, false>, a, tiles, Shape::kCtas, smem, stream);
 }
 
-bool half_type(int type) { return type == CUSORT_FLOAT_F16 || type == CUSORT_FLOAT_BF16; }
-
 // Rows of a tile where experts have few rows on average, and where they have many.
 constexpr int kFewRows = 64, kManyRows = 256;
 
@@ -855,15 +759,16 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
                                               const int32_t* d_counts, const int32_t* d_offsets, void* d_out,
                                               int64_t capacity, int64_t in, int64_t out, int num_experts,
                                               cudaStream_t stream) {
-  if (temp_storage_bytes == nullptr || !half_type(type) || !sizes_fit(capacity, in, out, num_experts) ||
+  if (temp_storage_bytes == nullptr || float_type_bytes(type) == 0 || !sizes_fit(capacity, in, out, num_experts) ||
       row_stride < 0 || expert_stride < 0 || in_stride < 0 || out_stride < 0)
     return cudaErrorInvalidValue;
   const bool in_order = !(out_stride == 1 || out == 1);
   if (in_order && in_stride != 1 && in != 1) return cudaErrorInvalidValue;
+  const bool whole = type == CUSORT_FLOAT_F32;  // its loads take any address and stride
   Operand rows{d_rows, 1, capacity, in, 0, row_stride};
   Operand weights{d_weights, num_experts, in_order ? out : in, in_order ? in : out, expert_stride,
                   in_order ? out_stride : in_stride};
-  const size_t need = std::max<size_t>(1, capacity == 0 ? 0 : rows.bytes() + weights.bytes());
+  const size_t need = std::max<size_t>(1, capacity == 0 || whole ? 0 : rows.bytes() + weights.bytes());
   if (d_temp_storage == nullptr) {
     *temp_storage_bytes = need;
     return cudaSuccess;
@@ -873,9 +778,14 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   if (d_rows == nullptr || d_weights == nullptr || d_counts == nullptr || d_offsets == nullptr || d_out == nullptr ||
       (reinterpret_cast<uintptr_t>(d_out) & 15) != 0 || (need > 1 && (reinterpret_cast<uintptr_t>(d_temp_storage) & 15) != 0))
     return cudaErrorInvalidValue;
+  const SegmentArgs segments{d_counts, d_offsets, num_experts, (int)capacity};
+  if (whole)
+    return float_products(static_cast<const float*>(d_rows), row_stride, static_cast<const float*>(d_weights),
+                          expert_stride, in_stride, out_stride, segments, static_cast<float*>(d_out), (int)in, (int)out,
+                          stream);
   const bool few = capacity <= (int64_t)kFewRows * num_experts;
   ProductArgs a;
-  a.segments = {d_counts, d_offsets, num_experts, (int)capacity};
+  a.segments = segments;
   a.out = d_out;
   a.in = (int)in;
   a.width = (int)out;
@@ -900,24 +810,30 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
     const void* d_grad_out, int64_t grad_stride, const int32_t* d_counts, const int32_t* d_offsets,
     void* d_grad_weights, int in_contiguous, int64_t capacity, int64_t in, int64_t out, int num_experts,
     cudaStream_t stream) {
-  if (temp_storage_bytes == nullptr || !half_type(type) || !sizes_fit(capacity, in, out, num_experts) ||
+  if (temp_storage_bytes == nullptr || float_type_bytes(type) == 0 || !sizes_fit(capacity, in, out, num_experts) ||
       row_stride < 0 || grad_stride < 0)
     return cudaErrorInvalidValue;
   Operand slow{d_rows, 1, capacity, in, 0, row_stride}, fast{d_grad_out, 1, capacity, out, 0, grad_stride};
   if (in_contiguous) std::swap(slow, fast);
-  const size_t need = std::max<size_t>(1, capacity == 0 ? 0 : slow.bytes() + fast.bytes());
+  const bool whole = type == CUSORT_FLOAT_F32;
+  const size_t need = std::max<size_t>(1, capacity == 0 || whole ? 0 : slow.bytes() + fast.bytes());
   if (d_temp_storage == nullptr) {
     *temp_storage_bytes = need;
     return cudaSuccess;
   }
   if (*temp_storage_bytes < need) return cudaErrorInvalidValue;
   if (d_grad_weights == nullptr || (reinterpret_cast<uintptr_t>(d_grad_weights) & 15) != 0) return cudaErrorInvalidValue;
-  if (capacity == 0) return cudaMemsetAsync(d_grad_weights, 0, (size_t)num_experts * in * out * 2, stream);
+  if (capacity == 0) return cudaMemsetAsync(d_grad_weights, 0, (size_t)num_experts * in * out * float_type_bytes(type), stream);
   if (d_rows == nullptr || d_grad_out == nullptr || d_counts == nullptr || d_offsets == nullptr ||
       (need > 1 && (reinterpret_cast<uintptr_t>(d_temp_storage) & 15) != 0))
     return cudaErrorInvalidValue;
+  const SegmentArgs segments{d_counts, d_offsets, num_experts, (int)capacity};
+  if (whole)
+    return float_products_grad(static_cast<const float*>(slow.data), slow.row_stride,
+                               static_cast<const float*>(fast.data), fast.row_stride, segments,
+                               static_cast<float*>(d_grad_weights), (int)slow.width, (int)fast.width, stream);
   GradArgs a;
-  a.segments = {d_counts, d_offsets, num_experts, (int)capacity};
+  a.segments = segments;
   a.result = d_grad_weights;
   a.slow_width = (int)slow.width;
   a.fast_width = (int)fast.width;

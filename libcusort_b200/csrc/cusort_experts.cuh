@@ -1,0 +1,124 @@
+// cusort_experts.cuh -- what the experts' products of 16-bit and of 32-bit
+// operands share: the segments of a plan, and rows of none.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace cusort_b200 {
+
+constexpr int kMaxExperts = 1024;
+
+// Expert segments as the CTA keeps them in shared memory.
+struct Segments {
+  int32_t* first;  // [experts] rows: clamped into [0, capacity]
+  int32_t* count;
+  int32_t* tiles;  // [experts + 1] sums of the tiles before each expert
+};
+
+struct SegmentArgs {
+  const int32_t *counts, *offsets;
+  int experts, capacity;
+};
+
+// First row and number of rows of an expert's segment, within the rows there are.
+__device__ __forceinline__ int2 segment(const SegmentArgs& a, int e) {
+  const int first = min(max(a.offsets[e], 0), a.capacity);
+  return make_int2(first, min(max(a.counts[e], 0), a.capacity - first));
+}
+
+// All threads: fills s; tiles(count) is the number of tiles of an expert with that many rows.
+template <int THREADS, typename F>
+__device__ __forceinline__ void load_segments(const SegmentArgs& a, const Segments& s, uint32_t* sums, F&& tiles) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr uint32_t kAll = 0xffffffffu;
+  constexpr int kEach = (kMaxExperts + THREADS - 1) / THREADS;
+  const int per = (a.experts + THREADS - 1) / THREADS;  // consecutive experts to a thread
+  int mine[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = threadIdx.x * per + i;
+    mine[i] = 0;
+    if (i < per && e < a.experts) {
+      const int2 seg = segment(a, e);
+      s.first[e] = seg.x;
+      s.count[e] = seg.y;
+      mine[i] = tiles(seg.y);
+    }
+    sum += mine[i];
+  }
+  int scan = sum;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(kAll, scan, d);
+    if (lane >= d) scan += v;
+  }
+  if (lane == 31) sums[warp] = scan;
+  __syncthreads();
+  int before = scan - sum;
+  for (int w = 0; w < warp; ++w) before += sums[w];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int e = threadIdx.x * per + i;
+    if (i < per && e < a.experts) {
+      s.tiles[e] = before;
+      before += mine[i];
+      if (e == a.experts - 1) s.tiles[a.experts] = before;
+    }
+  }
+  __syncthreads();
+}
+
+// The expert whose tiles hold tile t.
+__device__ __forceinline__ int find(const int32_t* tiles, int experts, int t) {
+  int low = 0, high = experts;  // tiles[low] <= t < tiles[high]
+  while (high - low > 1) {
+    const int mid = (low + high) >> 1;
+    if (tiles[mid] <= t) low = mid;
+    else high = mid;
+  }
+  return low;
+}
+
+__device__ __forceinline__ uint32_t align_up(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
+
+// Zeros in 16-bit elements [begin, end) of x, by `threads` threads.
+__device__ __forceinline__ void clear(uint16_t* x, int64_t begin, int64_t end, int thread, int threads) {
+  if (begin >= end) return;
+  const int64_t head = min(end, begin + (int64_t)((16 - (reinterpret_cast<uintptr_t>(x + begin) & 15)) % 16) / 2);
+  const int64_t words = (end - head) / 8;
+  uint4* body = reinterpret_cast<uint4*>(x + head);
+  if (begin + thread < head) x[begin + thread] = 0;
+#pragma unroll 4
+  for (int64_t i = thread; i < words; i += threads) body[i] = make_uint4(0, 0, 0, 0);
+  if (head + words * 8 + thread < end) x[head + words * 8 + thread] = 0;
+}
+
+// One warp's part in clearing the rows that belong to no segment (16-bit
+// elements, `width` to a row; warp `me` of `all`): those between the segments
+// by the expert before, those behind the last in equal parts.
+__device__ __forceinline__ void clear_other_rows(uint16_t* out, int64_t width, const SegmentArgs& a, const Segments& s,
+                                                 int me, int all) {
+  const int lane = threadIdx.x & 31;
+  for (int e = me; e < a.experts; e += all) {
+    const int end = s.first[e] + s.count[e];
+    if (e + 1 < a.experts) clear(out, end * width, s.first[e + 1] * width, lane, 32);
+    if (e == 0) clear(out, 0, s.first[0] * width, lane, 32);
+  }
+  const int end = s.first[a.experts - 1] + s.count[a.experts - 1], left = a.capacity - end;
+  const int per = (left + all - 1) / all;
+  const int64_t r0 = end + min((int64_t)left, (int64_t)me * per);
+  clear(out, r0 * width, min(r0 + per, (int64_t)a.capacity) * width, lane, 32);
+}
+
+// The products of 32-bit operands (cusort_experts_f32.cu).
+// out[r] = rows[r] x weights[e], element (i, o) of them i * in_stride + o * out_stride behind their start.
+cudaError_t float_products(const float* rows, int64_t row_stride, const float* weights, int64_t expert_stride,
+                           int64_t in_stride, int64_t out_stride, const SegmentArgs& segments, float* out, int in,
+                           int width, cudaStream_t stream);
+// grad[e] = slow_e^T x fast_e, [experts][slow_width][fast_width].
+cudaError_t float_products_grad(const float* slow, int64_t slow_stride, const float* fast, int64_t fast_stride,
+                                const SegmentArgs& segments, float* grad, int slow_width, int fast_width,
+                                cudaStream_t stream);
+
+}  // namespace cusort_b200

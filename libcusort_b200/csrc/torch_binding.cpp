@@ -411,12 +411,6 @@ PyObject* combine_backward(PyObject* const* p) {
   return tuple(wrap(std::move(grad_rows)), wrap(std::move(grad_weights)));
 }
 
-cusort_float_type half_type(const at::Tensor& t, const char* name) {
-  if (t.scalar_type() != at::kHalf && t.scalar_type() != at::kBFloat16)
-    refuse(PyExc_TypeError, name, " must be float16 or bfloat16 (got ", name_of(t.scalar_type()), ")");
-  return float_type(t, name);
-}
-
 // A plan's segments over the rows of t.
 void check_segments(const at::Tensor& counts, const at::Tensor& offsets, const at::Tensor& t) {
   if (counts.dim() != 1 || counts.numel() < 1 || counts.numel() > kMaxExperts)
@@ -457,7 +451,7 @@ PyObject* expert_products(PyObject* const* p) {
   const at::Tensor &rows = tensor(p[0], name), &weights = tensor(p[1], "weights"), &counts = tensor(p[2], "counts"),
                    &offsets = tensor(p[3], "offsets");
   const bool back = truth(p[4]);
-  const cusort_float_type type = half_type(rows, name);
+  const cusort_float_type type = float_type(rows, name);
   check_rows(rows, name);
   check_segments(counts, offsets, rows);
   const int64_t experts = counts.numel(), capacity = rows.size(0);
@@ -486,7 +480,7 @@ PyObject* expert_products_grad_weights(PyObject* const* p) {
   const at::Tensor &grad = tensor(p[0], "grad_out"), &rows = tensor(p[1], "rows"), &counts = tensor(p[2], "counts"),
                    &offsets = tensor(p[3], "offsets");
   const bool in_last = truth(p[4]);
-  const cusort_float_type type = half_type(rows, "rows");
+  const cusort_float_type type = float_type(rows, "rows");
   check_rows(rows, "rows");
   check_segments(counts, offsets, rows);
   const int64_t experts = counts.numel(), capacity = rows.size(0), in = rows.size(1);

@@ -34,9 +34,10 @@ def expert_products(rows: torch.Tensor, weights: torch.Tensor, counts: torch.Ten
 
     ``rows`` [capacity, in] (rows any distance apart) and ``weights`` [experts, in, out] (contiguous
     along either of the last two dimensions, so that linear layers' [experts, out, in] go in as
-    ``w.transpose(1, 2)``) are float16 or bfloat16; sums are held in 32 bits and rounded once.  What
-    lies in ``rows`` outside the segments has no influence, whatever it is.  Rows or weights
-    whose addresses and strides are no multiples of 16 bytes are copied to a workspace first."""
+    ``w.transpose(1, 2)``) are bfloat16, float16 or float32; sums are held in 32 bits and rounded once.
+    What lies in ``rows`` outside the segments has no influence, whatever it is.  16-bit rows or
+    weights whose addresses and strides are no multiples of 16 bytes are copied to a workspace first;
+    32-bit ones are multiplied as they are, without the tensor cores, which would round them."""
     return _capi.native().expert_products(rows, weights, counts, offsets, False, "rows")
 
 

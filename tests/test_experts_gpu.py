@@ -11,7 +11,7 @@ from libcusort_b200 import experts as X  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
-TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 
 
 @pytest.fixture(autouse=True)
@@ -55,7 +55,7 @@ def close(got, want, size, depth):
     """One rounding of the result (half a step: eps / 2 of it, and half the smallest subnormal), and `depth` 32-bit
     additions, each off by a step (2^-23) of at most the sum of all products' sizes."""
     info = torch.finfo(got.dtype)
-    tiny = 2.0 ** -25 if got.dtype == torch.float16 else 2.0 ** -134
+    tiny = info.smallest_normal * info.eps / 2
     bound = info.eps / 2 * want.abs() + (1 + info.eps) * depth * 2.0 ** -23 * size + tiny
     bad = ~((got.double() - want).abs() <= bound)
     assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist(), got[bad][:4], want[bad][:4])
@@ -82,7 +82,7 @@ def check(counts, fin, fout, dtype="bf16", order="in_out", align=1, tail=0, pitc
 
 
 @pytest.mark.parametrize("order", ["in_out", "out_in"])
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("fin,fout", [(64, 128), (128, 64), (72, 200), (8, 8), (512, 264), (200, 1032)])
 def test_few_rows_an_expert(fin, fout, dtype, order):
     check([0, 1, 3, 0, 16, 17, 33, 64, 0, 40], fin, fout, dtype, order)
@@ -96,39 +96,44 @@ def test_few_tiles_with_a_long_contracted_dimension(fin, fout, counts, order):
 
 
 @pytest.mark.parametrize("order", ["in_out", "out_in"])
-@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("fin,fout", [(64, 128), (264, 136), (136, 520)])
 def test_many_rows_an_expert(fin, fout, dtype, order):
     check([0, 255, 1, 256, 257, 0, 300, 1000, 63, 65], fin, fout, dtype, order)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("align,tail", [(16, 0), (128, 70), (7, 1000), (1, 333)])
 @pytest.mark.parametrize("fin,fout", [(64, 136), (40, 33)])
-def test_rows_of_no_segment_are_zeros_and_not_read(fin, fout, align, tail):
-    check([5, 0, 128, 130, 0, 1, 0], fin, fout, "bf16", align=align, tail=tail)
+def test_rows_of_no_segment_are_zeros_and_not_read(fin, fout, align, tail, dtype):
+    check([5, 0, 128, 130, 0, 1, 0], fin, fout, dtype, align=align, tail=tail)
 
 
 @pytest.mark.parametrize("order", ["in_out", "out_in"])
 @pytest.mark.parametrize("fin,fout", [(1, 1), (7, 5), (1, 64), (64, 1), (33, 130), (771, 257), (66, 72), (72, 66)])
 def test_widths_of_no_16_bytes(fin, fout, order):
     check([3, 0, 70, 1, 20], fin, fout, "f16", order)
+    check([3, 0, 70, 1, 20], fin, fout, "f32", order)
 
 
 @pytest.mark.parametrize("pitch,shift,grad_pitch", [(80, 0, 72), (72, 4, 64), (65, 0, 67), (64, 8, 64), (64, 1, 71)])
 def test_rows_apart_and_off_16_bytes(pitch, shift, grad_pitch):
     check([9, 130, 0, 31], 64, 64, "bf16", pitch=pitch, shift=shift, grad_pitch=grad_pitch)
+    check([9, 130, 0, 31], 64, 64, "f32", pitch=pitch, shift=shift, grad_pitch=grad_pitch)
 
 
 def test_one_expert_and_the_most():
     check([700], 136, 72)
     check([1], 64, 64)
     check([i % 3 for i in range(1024)], 64, 72)
+    check([i % 3 for i in range(1024)], 24, 40, "f32")
 
 
 def test_nothing_to_do():
     check([0, 0, 0], 64, 72)
     check([0, 0, 0], 64, 72, tail=50)
     check([0], 33, 5, "f16")
+    check([0, 0, 0], 64, 72, "f32", tail=50)
 
 
 def test_expanded_rows_and_weights():

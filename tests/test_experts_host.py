@@ -34,8 +34,8 @@ def _pool(blocks=9, **other):
 
 @pytest.mark.parametrize("call,match", [
     (lambda: _products(), "CUDA"),
-    (lambda: _products(rows=_t(20, 16, dtype=torch.float32)), "float16 or bfloat16"),
-    (lambda: _products(rows=_t(20, 16, dtype=torch.float64)), "float16 or bfloat16"),
+    (lambda: _products(rows=_t(20, 16, dtype=torch.float32)), "weights"),
+    (lambda: _products(rows=_t(20, 16, dtype=torch.float64)), "float32, float16 or bfloat16"),
     (lambda: _products(rows=_t(20, 16, dtype=torch.float16)), "weights"),
     (lambda: _products(rows=_t(16, 20).t()), "rows are contiguous"),
     (lambda: _products(rows=_t(20)), "2-D"),
@@ -132,7 +132,7 @@ def _call(temp=P, room=1 << 40, kind=2, rows=P, row_stride=64, weights=P, expert
 
 
 def test_products_arguments():
-    for bad in (dict(kind=0), dict(kind=3), dict(capacity=-1), dict(capacity=1 << 31), dict(width=0),
+    for bad in (dict(kind=-1), dict(kind=3), dict(capacity=-1), dict(capacity=1 << 31), dict(width=0),
                 dict(width=(1 << 20) + 1), dict(result=0), dict(result=(1 << 20) + 1), dict(num=0), dict(num=1025),
                 dict(row_stride=-1), dict(expert=-8), dict(fin=-1), dict(fin=3, fout=2), dict(rows=None),
                 dict(weights=None), dict(counts=None), dict(offsets=None), dict(out=None),
@@ -154,6 +154,7 @@ def test_products_size_query():
     assert weights >= 3 * 64 * 72 * 2
     assert _call(temp=None, row_stride=65, fin=73, expert=64 * 73)[1] == rows + weights
     assert _call(temp=None, fin=1, fout=64)[1] == 1  # the other order
+    assert _call(temp=None, kind=0, row_stride=65, rows=C.c_void_p(0x10004))[1] == 1  # 32 bits: wherever they are
 
 
 def test_products_gradient_arguments():
@@ -163,7 +164,7 @@ def test_products_gradient_arguments():
         return _capi.load().cusort_expert_products_grad_weights(temp, C.byref(nb), kind, rows, row_stride, grad,
                                                                 grad_stride, counts, offsets, out, order, capacity,
                                                                 fin, fout, num, None), nb.value
-    for bad in (dict(kind=0), dict(capacity=-1), dict(fin=0), dict(fout=0), dict(num=0), dict(num=1025),
+    for bad in (dict(kind=3), dict(capacity=-1), dict(fin=0), dict(fout=0), dict(num=0), dict(num=1025),
                 dict(row_stride=-1), dict(grad_stride=-1), dict(rows=None), dict(grad=None), dict(counts=None),
                 dict(offsets=None), dict(out=None), dict(out=C.c_void_p(0x10008)), dict(grad_stride=73, room=1)):
         assert call(**bad)[0] == INVALID, bad
