@@ -182,14 +182,15 @@ struct ProductArgs {
   SegmentArgs segments;
   void* out;
   int in, width;      // of a row, and of a row of the result
-  int width_tiles;    // tiles of kTileM of the result's width
+  int width_tiles;    // tiles of the result's width
+  uint32_t most;      // tiles of rows
   uint64_t limit_ns;  // bound on every wait
 };
 
 // PAIR: tiles of 256 columns of the result, 128 in each of two CTAs, and half of the rows in each.
 template <int BN, int STAGES, int SUB, bool PAIR> struct ProductShape {
   static constexpr int kCtas = PAIR ? 2 : 1, kTile = kTileM * kCtas;
-  static constexpr int kRowStep = 16;               // the instruction's width comes in such steps
+  static constexpr int kRowStep = 16 * kCtas;       // the instruction's width comes in such steps
   static constexpr int kBoxRows = PAIR ? 64 : 16;   // a tile of few rows brings few boxes
   // A stage holds SUB steps of kBlockK, each the weights' part and then the rows'.
   static constexpr uint32_t kBytesB = BN / kCtas * kBlockK * 2, kStep = kBytesA + kBytesB, kStage = SUB * kStep;
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 
   init_pipe(p, Shape::kColumns);
   dev::wait_for_previous();
-  load_segments<kThreads>(a.segments, s, p.sums, [](int count) { return (count + BN - 1) / BN; });
+  load_segments<kThreads>(a.segments, s, p.sums, a.most, [](int count) { return (count + BN - 1) / BN; });
   const uint32_t tiles = (uint32_t)s.tiles[experts] * a.width_tiles;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = PAIR ? dev::cluster_rank() : 0;
   const int steps = (a.in + SUB * kBlockK - 1) / (SUB * kBlockK);
@@ -734,6 +735,7 @@ cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order
                     cudaStream_t stream) {
   using Shape = ProductShape<BN, STAGES, SUB, PAIR>;
   a.width_tiles = (a.width + Shape::kTile - 1) / Shape::kTile;
+  a.most = (uint32_t)row_tiles;
   cudaError_t e = weights.map(&a.weights, false, in_order ? kTileM : kBlockK);
   if (!e) e = rows.map(&a.rows, true, Shape::kBoxRows);
   if (e) return e;
@@ -746,8 +748,11 @@ cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order
 // Rows of a tile where experts have few rows on average, and where they have many.
 constexpr int kFewRows = 64, kManyRows = 256;
 
+// Tiles begin before this many rows and end within 32 bits.
+constexpr int64_t kMaxRows = INT32_MAX - 1024;
+
 bool sizes_fit(int64_t capacity, int64_t in, int64_t out, int experts) {
-  return capacity >= 0 && capacity <= INT32_MAX && in >= 1 && in <= (1 << 20) && out >= 1 && out <= (1 << 20) &&
+  return capacity >= 0 && capacity <= kMaxRows && in >= 1 && in <= (1 << 20) && out >= 1 && out <= (1 << 20) &&
          experts >= 1 && experts <= kMaxExperts;
 }
 
@@ -792,7 +797,7 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   a.limit_ns = wait_limit_ns();
   // at most one part-filled tile to an expert, and no expert without a row
   const int64_t tiles = capacity / (few ? kFewRows : kManyRows) + std::min<int64_t>(num_experts, capacity);
-  if (tiles * ((out + kTileM - 1) / kTileM) > INT32_MAX) return cudaErrorInvalidValue;
+  if (tiles * ((out + kTileM - 1) / kTileM) > 1 << 30) return cudaErrorInvalidValue;
   uint8_t* temp = static_cast<uint8_t*>(d_temp_storage);
   cudaError_t e = rows.prepare(temp, nullptr, stream);
   if (!e) e = weights.prepare(temp, d_counts, stream);

@@ -27,14 +27,20 @@ __device__ __forceinline__ int2 segment(const SegmentArgs& a, int e) {
   return make_int2(first, min(max(a.counts[e], 0), a.capacity - first));
 }
 
-// All threads: fills s; tiles(count) is the number of tiles of an expert with that many rows.
+// Sums of tiles stop at 2^30, more than there are of any plan's.
+__device__ __forceinline__ uint32_t add_tiles(uint32_t a, uint32_t b) { return min(a + b, 1u << 30); }
+
+// All threads: fills s; tiles(count) is the number of tiles of an expert with
+// that many rows.  Segments that do not overlap have `most` tiles at most; of
+// others those that go beyond it are left out, and all after them.
 template <int THREADS, typename F>
-__device__ __forceinline__ void load_segments(const SegmentArgs& a, const Segments& s, uint32_t* sums, F&& tiles) {
+__device__ __forceinline__ void load_segments(const SegmentArgs& a, const Segments& s, uint32_t* sums, uint32_t most,
+                                              F&& tiles) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   constexpr uint32_t kAll = 0xffffffffu;
   constexpr int kEach = (kMaxExperts + THREADS - 1) / THREADS;
   const int per = (a.experts + THREADS - 1) / THREADS;  // consecutive experts to a thread
-  int mine[kEach], sum = 0;
+  uint32_t mine[kEach], sum = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int e = threadIdx.x * per + i;
@@ -45,25 +51,38 @@ __device__ __forceinline__ void load_segments(const SegmentArgs& a, const Segmen
       s.count[e] = seg.y;
       mine[i] = tiles(seg.y);
     }
-    sum += mine[i];
+    sum = add_tiles(sum, mine[i]);
   }
-  int scan = sum;
+  uint32_t scan = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int v = __shfl_up_sync(kAll, scan, d);
-    if (lane >= d) scan += v;
+    const uint32_t v = __shfl_up_sync(kAll, scan, d);
+    if (lane >= d) scan = add_tiles(scan, v);
   }
   if (lane == 31) sums[warp] = scan;
+  if (threadIdx.x == 0) s.tiles[a.experts] = 0;
+  uint32_t before = __shfl_up_sync(kAll, scan, 1);
+  if (lane == 0) before = 0;
   __syncthreads();
-  int before = scan - sum;
-  for (int w = 0; w < warp; ++w) before += sums[w];
+  for (int w = 0; w < warp; ++w) before = add_tiles(before, sums[w]);
+  const uint32_t begin = before;
+  uint32_t last = 0;  // the end of the last one that stays
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    before = add_tiles(before, mine[i]);
+    if (before <= most) last = before;
+  }
+  atomicMax(s.tiles + a.experts, (int)last);
+  __syncthreads();
+  const uint32_t end = s.tiles[a.experts];
+  before = begin;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int e = threadIdx.x * per + i;
     if (i < per && e < a.experts) {
-      s.tiles[e] = before;
-      before += mine[i];
-      if (e == a.experts - 1) s.tiles[a.experts] = before;
+      s.tiles[e] = (int)min(before, end);
+      before = add_tiles(before, mine[i]);
+      if (before > end) s.count[e] = 0;
     }
   }
   __syncthreads();

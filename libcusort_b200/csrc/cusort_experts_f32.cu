@@ -41,6 +41,7 @@ struct FloatArgs {
   int64_t am, ak, bk, bn, b_expert, cm, c_expert;
   SegmentArgs segments;
   int m, n, k;
+  uint32_t most;  // tiles along m of all experts
 };
 
 // RAGGED_K: the rows of a segment are what is contracted (the gradient of the
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(kThreads, Shape<U, K>::kCtas)
   const Segments s{s_segments, s_segments + experts, s_segments + 2 * experts};
   dev::wait_for_previous();
   const int m_tiles = (a.m + kM - 1) / kM, n_tiles = (a.n + kN - 1) / kN;
-  load_segments<kThreads>(a.segments, s, sums, [&](int count) { return RAGGED_K ? m_tiles : (count + kM - 1) / kM; });
+  load_segments<kThreads>(a.segments, s, sums, a.most, [&](int count) { return RAGGED_K ? m_tiles : (count + kM - 1) / kM; });
   const uint32_t tiles = (uint32_t)s.tiles[experts] * n_tiles;
   if (!RAGGED_K)
     clear_other_rows(reinterpret_cast<uint16_t*>(a.c), 2 * (int64_t)a.n, a.segments, s,
@@ -145,12 +146,13 @@ __global__ void __launch_bounds__(kThreads, Shape<U, K>::kCtas)
 }
 
 template <int U, int K, bool RAGGED_K, bool B_ALONG>
-cudaError_t run(const FloatArgs& a, cudaStream_t stream) {
+cudaError_t run(FloatArgs a, cudaStream_t stream) {
   constexpr int kM = 16 * U;
   const int64_t row_tiles = RAGGED_K ? (int64_t)a.segments.experts * ((a.m + kM - 1) / kM)
                                      : a.segments.capacity / kM + std::min(a.segments.experts, a.segments.capacity);
   const int64_t tiles = row_tiles * ((a.n + kN - 1) / kN);
-  if (tiles > INT32_MAX) return cudaErrorInvalidValue;
+  if (tiles > 1 << 30) return cudaErrorInvalidValue;
+  a.most = (uint32_t)row_tiles;
   const auto kernel = float_products_kernel<U, K, RAGGED_K, B_ALONG>;
   // the limit is the kernel's, not the call's: the same one from every host thread
   constexpr size_t kMost = sizeof(Shape<U, K>) + 4 * (3 * kMaxExperts + 1);
@@ -170,7 +172,7 @@ cudaError_t float_products(const float* rows, int64_t row_stride, const float* w
                            int64_t in_stride, int64_t out_stride, const SegmentArgs& segments, float* out, int in,
                            int width, cudaStream_t stream) {
   const FloatArgs a{rows, weights, out, row_stride, 1, in_stride, out_stride, expert_stride, width, 0, segments, 0,
-                    width, in};
+                    width, in, 0};
   const bool fewest = segments.capacity <= (int64_t)kFewestRows * segments.experts;
   const bool few = segments.capacity <= (int64_t)kFewRows * segments.experts, along = out_stride != 1;
   if (fewest) return along ? run<1, 32, false, true>(a, stream) : run<1, 32, false, false>(a, stream);
@@ -182,7 +184,7 @@ cudaError_t float_products_grad(const float* slow, int64_t slow_stride, const fl
                                 const SegmentArgs& segments, float* grad, int slow_width, int fast_width,
                                 cudaStream_t stream) {
   const FloatArgs a{slow, fast, grad, 1, slow_stride, fast_stride, 1, 0, fast_width, (int64_t)slow_width * fast_width,
-                    segments, slow_width, fast_width, 0};
+                    segments, slow_width, fast_width, 0, 0};
   return run<8, 16, true, false>(a, stream);
 }
 

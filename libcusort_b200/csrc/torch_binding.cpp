@@ -418,7 +418,8 @@ void check_segments(const at::Tensor& counts, const at::Tensor& offsets, const a
            ")");
   check(counts, "counts", at::kInt, t.device(), {counts.numel()});
   check(offsets, "offsets", at::kInt, t.device(), {counts.numel() + 1});
-  if (t.size(0) > INT32_MAX) refuse(PyExc_ValueError, "2^31 rows and more are not supported (got ", t.size(0), ")");
+  if (t.size(0) > INT32_MAX - 1024)
+    refuse(PyExc_ValueError, "fewer than 2^31 - 1024 rows are supported (got ", t.size(0), ")");
 }
 
 void check_width(const char* name, int64_t width) {
@@ -439,7 +440,9 @@ bool in_contiguous(const at::Tensor& weights) {
 template <typename F>
 void launch_with_temp(const char* what, at::Device device, F&& f) {
   size_t bytes = 0;
-  launch(what, device, [&](cudaStream_t s) { return f(nullptr, &bytes, s); });
+  if (f(nullptr, &bytes, nullptr) != cudaSuccess) {
+    launch(what, device, [&](cudaStream_t s) { return f(nullptr, &bytes, s); });  // says so
+  }
   // one byte is asked for where nothing is needed: any address does
   const at::Tensor temp = bytes > 1 ? empty({(int64_t)bytes}, at::kByte, device) : at::Tensor();
   launch(what, device, [&](cudaStream_t s) { return f(bytes > 1 ? temp.data_ptr() : (void*)&bytes, &bytes, s); });

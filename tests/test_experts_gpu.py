@@ -198,6 +198,22 @@ def test_from_another_host_thread():
     assert torch.equal(here, there[0])
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", [300, 40_000])
+def test_segments_on_top_of_each_other_end(rows, dtype):
+    """Every expert claims all rows: what does not fit the number of tiles of a plan is left out, the first stays."""
+    x, w = matrix(rows, 64, TYPES[dtype]), weights_of(700, 64, 72, TYPES[dtype], "in_out")
+    c = torch.full((700,), 1 << 30, dtype=torch.int32, device="cuda")
+    o = torch.zeros(701, dtype=torch.int32, device="cuda")
+    out = X.expert_products(x, w, c, o)
+    assert out.shape == (rows, 72)
+    c[1:] = 0
+    c[0] = rows
+    o[1:] = rows
+    out = X.expert_products(x, w, c, o)
+    close(out, x.double() @ w[0].double(), x.double().abs() @ w[0].double().abs(), 64)
+
+
 def test_segments_that_are_no_plan_stay_inside():
     """Counts and offsets beyond the rows are cut there; nothing outside the tensors is touched."""
     x = matrix(40, 64, torch.bfloat16)

@@ -132,12 +132,12 @@ def _call(temp=P, room=1 << 40, kind=2, rows=P, row_stride=64, weights=P, expert
 
 
 def test_products_arguments():
-    for bad in (dict(kind=-1), dict(kind=3), dict(capacity=-1), dict(capacity=1 << 31), dict(width=0),
+    for bad in (dict(kind=-1), dict(kind=3), dict(capacity=-1), dict(capacity=1 << 31), dict(capacity=(1 << 31) - 1024), dict(width=0),
                 dict(width=(1 << 20) + 1), dict(result=0), dict(result=(1 << 20) + 1), dict(num=0), dict(num=1025),
                 dict(row_stride=-1), dict(expert=-8), dict(fin=-1), dict(fin=3, fout=2), dict(rows=None),
                 dict(weights=None), dict(counts=None), dict(offsets=None), dict(out=None),
                 dict(out=C.c_void_p(0x10002)), dict(row_stride=65, room=16), dict(row_stride=65, temp=C.c_void_p(8)),
-                dict(capacity=(1 << 31) - 1, result=1 << 20, num=1024)):
+                dict(capacity=(1 << 31) - 2000, result=1 << 20, num=1024)):
         assert _call(**bad)[0] == INVALID, bad
     assert _call(capacity=0, rows=None, weights=None, counts=None, offsets=None, out=None)[0] == 0
     assert _capi.load().cusort_expert_products(P, None, 2, P, 64, P, 64, 72, 1, P, P, P, 10, 64, 72, 3, None) == INVALID
