@@ -178,7 +178,7 @@ __device__ __forceinline__ bool brings(int warp) { return warp == 0 || warp == 2
 // ---------------------------------------------------------------- the products
 
 struct ProductArgs {
-  CUtensorMap weights, rows;
+  CUtensorMap weights, rows[3];  // the rows by boxes of 64, 32 and 16
   SegmentArgs segments;
   void* out;
   int in, width;      // of a row, and of a row of the result
@@ -191,10 +191,8 @@ struct ProductArgs {
 template <int BN, int STAGES, int SUB, bool PAIR> struct ProductShape {
   static constexpr int kCtas = PAIR ? 2 : 1, kTile = kTileM * kCtas;
   static constexpr int kRowStep = 16 * kCtas;       // the instruction's width comes in such steps
-  static constexpr int kBoxRows = PAIR ? 64 : 16;   // a tile of few rows brings few boxes
   // A stage holds SUB steps of kBlockK, each the weights' part and then the rows'.
   static constexpr uint32_t kBytesB = BN / kCtas * kBlockK * 2, kStep = kBytesA + kBytesB, kStage = SUB * kStep;
-  static constexpr uint32_t kBoxBytes = kBoxRows * dev::kBoxRowBytes;
   static constexpr uint32_t kColumns = 2 * BN;
   static constexpr uint32_t kStaging = 4 * 2048;  // 32 x 32 16-bit elements for each storing warp
   static size_t bytes(int experts) {
@@ -258,8 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const int column = tile.column + rank * kTileM;
         const int mine = align_up(tile.rows, Shape::kRowStep) / Shape::kCtas, row = tile.row + rank * mine;
-        const int boxes = (mine + Shape::kBoxRows - 1) / Shape::kBoxRows;
-        const uint32_t bytes = SUB * Shape::kCtas * (kBytesA + boxes * Shape::kBoxBytes);
+        const uint32_t bytes = SUB * Shape::kCtas * (kBytesA + mine * dev::kBoxRowBytes);
         for (int k = 0; k < steps; ++k, ring.next()) {
           if ((turn ^= 1) == 0 || !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
           const uint32_t to = stages + ring.stage * Shape::kStage, own = at.full(ring.stage);
@@ -271,9 +268,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
             const int x = (k * SUB + u) * kBlockK;
             const uint32_t step = to + u * Shape::kStep;
             if (warp >= 8) {
-              for (int b = 0; b < boxes; ++b)
-                dev::tma_load_2d<PAIR>(step + kBytesA + b * Shape::kBoxBytes, &a.rows, bar, x,
-                                       row + b * Shape::kBoxRows);
+              // no more rows than are multiplied: what an SM takes in is what bounds the products
+              int r = 0;
+              for (; mine - r >= 64; r += 64)
+                dev::tma_load_2d<PAIR>(step + kBytesA + r * dev::kBoxRowBytes, &a.rows[0], bar, x, row + r);
+              if (mine & 32) {
+                dev::tma_load_2d<PAIR>(step + kBytesA + r * dev::kBoxRowBytes, &a.rows[1], bar, x, row + r);
+                r += 32;
+              }
+              if (mine & 16)
+                dev::tma_load_2d<PAIR>(step + kBytesA + r * dev::kBoxRowBytes, &a.rows[2], bar, x, row + r);
             } else if (IN_ORDER) {
               dev::tma_load_3d<PAIR>(step, &a.weights, bar, x, column, tile.expert);
             } else {
@@ -737,7 +741,7 @@ cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order
   a.width_tiles = (a.width + Shape::kTile - 1) / Shape::kTile;
   a.most = (uint32_t)row_tiles;
   cudaError_t e = weights.map(&a.weights, false, in_order ? kTileM : kBlockK);
-  if (!e) e = rows.map(&a.rows, true, Shape::kBoxRows);
+  for (int i = 0; !e && i < 3; ++i) e = rows.map(&a.rows[i], true, 64 >> i);
   if (e) return e;
   const size_t smem = Shape::bytes(a.segments.experts);
   const int64_t tiles = row_tiles * a.width_tiles;
