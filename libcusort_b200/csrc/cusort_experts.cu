@@ -220,9 +220,23 @@ __device__ __forceinline__ ProductTile product_tile(const ProductArgs& a, const 
 
 // out^T = weights^T x rows^T by tiles of 128 (PAIR: 256) of the result's
 // columns (the lanes of tensor memory) and up to BN rows of one segment.  So
-// the instruction's width is the number of rows, in steps of 16: an expert
-// with three rows costs a width of 16, and its weights stream through the
-// lanes.
+// the instruction's width is the number of rows, in steps of 16 (PAIR: 32): an
+// expert with three rows costs a width of 16, and its weights stream through
+// the lanes.  Two sums in tensor memory: one is stored while the next grows.
+//
+// Many rows an expert, a pair of CTAs to a tile, so that each takes in half of
+// either operand: bound by what an SM takes in from L2 (32 KB to a step of 512
+// cycles of the tensor cores: 51 to 57 bytes a cycle) and by the power cap.
+// One expert of 8192 rows, 4096 -> 4096: 188 us, 1.46 PFLOP/s (the library's
+// batched product: 184); 64 experts of 700, 2048 -> 1408: 216 us (215); of
+// about 400, whose tiles are no wider than 224 rows, 129 (115).  With a CTA to
+// each 128 x 256 tile: 354 us for the first.
+// Few rows, a CTA to a tile, two steps of 64 to a stage: bound by memory (128
+// experts with 4 rows each, 2048 -> 1536: 118 us, 6.8 TB/s), below that by the
+// time of a step (six rows of six experts, 2048 -> 1024: 8.3 us, 4.2 of it
+// without the contraction).  Splitting the contraction over clusters of two or
+// three CTAs took as long or longer (11.4 us): their barriers and the joining
+// cost what the shorter loops gained.
 template <typename T, int BN, int STAGES, int SUB, bool PAIR, bool IN_ORDER>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
   using Shape = ProductShape<BN, STAGES, SUB, PAIR>;
@@ -420,6 +434,12 @@ __device__ __forceinline__ bool has_end(int count, int k) { return count - k < k
 // gradient[e] = slow_e^T x fast_e, contracted over the rows of e's segment: both operands lie with the contracted
 // dimension across.  Rows behind the segment's end that the last step brings along are cleared in shared memory: they
 // are another expert's, or anything at all.
+//
+// Always by pairs of CTAs.  Many rows: bound as the products are (8192 rows, 4096 x 4096: 196 us, 1.40 PFLOP/s; 32
+// experts of 1024, 2048 x 4096: 403 us; of 1023, with an end to clear: 453, about a microsecond a tile that its stages
+// do not hide).  Few: by writing the gradient, for which 3.9 TB/s is all that a plain fill comes to (128 experts of 128
+// rows, 2048 x 1024: 181 us, 3.0 TB/s; without the stores 120).  Stored by tiled copies of 64-byte rows: whole
+// sectors straight from registers took 194 us there, and 271 instead of 233 where rows are 2800 bytes.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     grad_weights_kernel(const __grid_constant__ GradArgs a) {
