@@ -3,7 +3,8 @@ cusort::DeviceRadixSort of IlyaGrebnov/libcusort behind the C ABI in
 include/cusort_b200.h (C++ callers: include/cusort_b200.cuh).
 
 Beside it: token routing for sparse models and block tables of a paged cache
-(routing.py, paging.py), which are the same work, keys to positions.
+(routing.py, paging.py), which are the same work, keys to positions, and the
+experts' products between them (experts.py).
 
 Python modules here are thin bindings for tests, the benchmark and PyTorch
 callers; the sort itself is the CUDA library libcusort_b200/_lib/libcusort_b200.so.

@@ -232,11 +232,14 @@ __device__ __forceinline__ ProductTile product_tile(const ProductArgs& a, const 
 // about 400, whose tiles are no wider than 224 rows, 129 (115).  With a CTA to
 // each 128 x 256 tile: 354 us for the first.
 // Few rows, a CTA to a tile, two steps of 64 to a stage: bound by memory (128
-// experts with 4 rows each, 2048 -> 1536: 118 us, 6.8 TB/s), below that by the
-// time of a step (six rows of six experts, 2048 -> 1024: 8.3 us, 4.2 of it
-// without the contraction).  Splitting the contraction over clusters of two or
-// three CTAs took as long or longer (11.4 us): their barriers and the joining
-// cost what the shorter loops gained.
+// experts with 4 rows each, 2048 -> 1536: 118 us, 6.8 TB/s), below that by how
+// much of the weights each of the few CTAs has under way.  So where no expert
+// can have more than 16 rows their part of a stage is small and there are five
+// stages, not four (six rows of six experts, 2048 -> 1024, from memory 9.4 us,
+// with four 10.5; 4096 -> 1024 14.7, 17.3; 4.2 us are there without any
+// contraction).  Splitting the contraction over clusters of two or three CTAs
+// took as long or longer (11.4 us for the first): their barriers and the
+// joining cost what the shorter loops gained.
 template <typename T, int BN, int STAGES, int SUB, bool PAIR, bool IN_ORDER>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
   using Shape = ProductShape<BN, STAGES, SUB, PAIR>;
@@ -769,8 +772,9 @@ cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order
                   : run(product_kernel<T, BN, STAGES, SUB, PAIR, false>, a, tiles, Shape::kCtas, smem, stream);
 }
 
-// Rows of a tile where experts have few rows on average, and where they have many.
-constexpr int kFewRows = 64, kManyRows = 256;
+// Rows of a tile where no expert can have more, where experts have few on
+// average, and where they have many.
+constexpr int kFewestRows = 16, kFewRows = 64, kManyRows = 256;
 
 // Tiles begin before this many rows and end within 32 bits.
 constexpr int64_t kMaxRows = INT32_MAX - 1024;
@@ -820,7 +824,8 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   a.width = (int)out;
   a.limit_ns = wait_limit_ns();
   // at most one part-filled tile to an expert, and no expert without a row
-  const int64_t tiles = capacity / (few ? kFewRows : kManyRows) + std::min<int64_t>(num_experts, capacity);
+  const int64_t tiles = capacity / (capacity <= kFewestRows ? kFewestRows : few ? kFewRows : kManyRows) +
+                        std::min<int64_t>(num_experts, capacity);
   if (tiles * ((out + kTileM - 1) / kTileM) > 1 << 30) return cudaErrorInvalidValue;
   uint8_t* temp = static_cast<uint8_t*>(d_temp_storage);
   cudaError_t e = rows.prepare(temp, nullptr, stream);
@@ -828,6 +833,7 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   if (e) return e;
   const auto go = [&](auto t) {
     using T = decltype(t);
+    if (capacity <= kFewestRows) return product<T, kFewestRows, 5, 2, false>(a, weights, rows, in_order, tiles, stream);
     return few ? product<T, kFewRows, 4, 2, false>(a, weights, rows, in_order, tiles, stream)
                : product<T, kManyRows, 6, 1, true>(a, weights, rows, in_order, tiles, stream);
   };

@@ -18,9 +18,6 @@ namespace dev {
 constexpr int kBoxElements = 64;
 constexpr int kBoxRowBytes = 128;
 
-__device__ __forceinline__ void tma_prefetch(const CUtensorMap* map) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
-}
 // A box into this CTA's shared memory, counted on the barrier `bar` (PAIR: of either CTA of a cluster of two).
 template <bool PAIR = false>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
