@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       for (int c = 0; c < tile.rows; c += 32) {
         uint32_t v[32];
         dev::tmem_load32(p.tmem + sums.stage * BN + c + ((uint32_t)quarter << 21), v);
-        dev::tmem_load_wait();
+        dev::tmem_load_wait(v);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const uint32_t both = dev::from_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), T{});
@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 32; ++i) v[i] = 0;
         } else {
           dev::tmem_load32(p.tmem + sums.stage * kGradN + c + ((uint32_t)quarter << 21), v);
-          dev::tmem_load_wait();
+          dev::tmem_load_wait(v);
         }
         if (rows <= 0) continue;
         // 16-byte pieces in the order of the tiled copies of 64-byte rows: the piece's number xor that of the row pair
