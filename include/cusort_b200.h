@@ -508,7 +508,8 @@ cudaError_t cusort_read_device_status(const void* d_temp_storage, uint32_t* stat
 uint64_t cusort_set_wait_limit_ns(uint64_t ns);
 
 /* Fault injection for tests: tile `tile` of every pass never publishes its
- * lookback descriptors (-1 = off, the default).  Per host thread. */
+ * lookback descriptors, and the copies of step `tile` of every CTA of the
+ * experts' products never come (-1 = off, the default).  Per host thread. */
 int64_t cusort_debug_set_skip_tile(int64_t tile);
 
 /* Per-kernel timing for the benchmark: when enabled, every sort records CUDA

@@ -719,6 +719,7 @@ void twiddle_constants_of(int kt, bool desc, uint64_t* c, uint64_t* f) {
 }
 
 uint64_t wait_limit_ns() { return g_ts.wait_limit_ns; }
+int64_t debug_skip_tile() { return g_ts.skip_tile; }
 
 cudaError_t occupancy_of(const KernelInfo& k, int* sms, int* ctas_per_sm) {
   int dev = 0;

@@ -89,6 +89,8 @@ cudaError_t digit_counts_u64(int key_type, bool descending, const void* keys, in
 // bound on device-side waits (cusort_set_wait_limit_ns).
 void twiddle_constants_of(int key_type, bool descending, uint64_t* c, uint64_t* f);
 uint64_t wait_limit_ns();
+// Its tile or step that never comes (cusort_debug_set_skip_tile).
+int64_t debug_skip_tile();
 // Resident CTAs per SM of a kernel on the current device (cached).
 cudaError_t occupancy_of(const KernelInfo& k, int* sms, int* ctas_per_sm);
 

@@ -185,6 +185,7 @@ struct ProductArgs {
   int width_tiles;    // tiles of the result's width
   uint32_t most;      // tiles of rows
   uint64_t limit_ns;  // bound on every wait
+  int64_t skip;       // for tests: every CTA's step that is never brought; -1: none
 };
 
 // PAIR: tiles of 256 columns of the result, 128 in each of two CTAs, and half of the rows in each.
@@ -269,13 +270,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     if (dev::elect_one()) {
       Ring<STAGES> ring;
       uint32_t turn = (warp == 2 || warp == 9);  // whether it takes the odd steps
+      int64_t step_of_cta = -1;
       for (uint32_t t = t0; t < tiles; t += t_step) {
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const int column = tile.column + rank * kTileM;
         const int mine = align_up(tile.rows, Shape::kRowStep) / Shape::kCtas, row = tile.row + rank * mine;
         const uint32_t bytes = SUB * Shape::kCtas * (kBytesA + mine * dev::kBoxRowBytes);
         for (int k = 0; k < steps; ++k, ring.next()) {
+          ++step_of_cta;
           if ((turn ^= 1) == 0 || !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
+          if (step_of_cta == a.skip) continue;
           const uint32_t to = stages + ring.stage * Shape::kStage, own = at.full(ring.stage);
           const uint32_t bar = PAIR ? dev::in_first(own) : own;
           // the first CTA's barrier counts the copies of both
@@ -401,6 +405,7 @@ struct GradArgs {
   void* result;  // [experts][slow_width][fast_width]
   int slow_width, fast_width, slow_tiles, fast_tiles;
   uint64_t limit_ns;
+  int64_t skip;
 };
 
 constexpr int kGradN = 256;
@@ -469,12 +474,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (dev::elect_one()) {
       Ring<kGradStages> ring;
       uint32_t turn = (warp == 2 || warp == 9);  // whether it takes the odd steps
+      int64_t step_of_cta = -1;
       for (uint32_t t = t0; t < tiles; t += t_step) {
         const GradTile g = grad_tile(a, segments, t);
         const int slow = g.slow + rank * kTileM, fast = g.fast + rank * g.chunks * kBlockK;
         const uint32_t bytes = (2 + g.chunks) * kChunkBytes;
         for (int k = 0; k < g.segment.y; k += kBlockK, ring.next()) {
+          ++step_of_cta;
           if ((turn ^= 1) == 0 || !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
+          if (step_of_cta == a.skip) continue;
           const uint32_t to = stages + ring.stage * kGradStage;
           const int row = g.segment.x + k;
           // each CTA looks after the end of a segment in its own copies
@@ -823,6 +831,7 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   a.in = (int)in;
   a.width = (int)out;
   a.limit_ns = wait_limit_ns();
+  a.skip = debug_skip_tile();
   // at most one part-filled tile to an expert, and no expert without a row
   const int64_t tiles = capacity / (capacity <= kFewestRows ? kFewestRows : few ? kFewRows : kManyRows) +
                         std::min<int64_t>(num_experts, capacity);
@@ -875,6 +884,7 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
   a.slow_tiles = (int)((slow.width + 2 * kTileM - 1) / (2 * kTileM));
   a.fast_tiles = (int)((fast.width + kGradN - 1) / kGradN);
   a.limit_ns = wait_limit_ns();
+  a.skip = debug_skip_tile();
   const int64_t tiles = (int64_t)a.slow_tiles * a.fast_tiles * num_experts;
   if (tiles > INT32_MAX) return cudaErrorInvalidValue;
   uint8_t* temp = static_cast<uint8_t*>(d_temp_storage);

@@ -7,7 +7,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from libcusort_b200 import experts as X  # noqa: E402
+from libcusort_b200 import _capi, experts as X  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +18,63 @@ TYPES = {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}
 def no_wait_ran_out():
     yield
     assert X.product_status() == 0
+
+
+def _few(x, w, g):
+    return X.expert_products(x[:40], w, torch.tensor([20, 20], dtype=torch.int32, device="cuda"),
+                             torch.tensor([0, 20, 40], dtype=torch.int32, device="cuda"))
+
+
+def _many(x, w, g):
+    return X.expert_products(x, w, *plan([300, 500])[:2])
+
+
+def _gradient(x, w, g):
+    return X.expert_products_grad_weights(g, x, *plan([300, 500])[:2])
+
+
+@pytest.mark.parametrize("skip", [0, 3, 13])
+@pytest.mark.parametrize("call", [_few, _many, _gradient])
+def test_a_wait_that_runs_out_is_told(call, skip):
+    """Copies that never come: the kernel ends after a millisecond with a status, and the next call is right again."""
+    x, w, g = (matrix(800, 1024, torch.bfloat16), weights_of(2, 1024, 2048, torch.bfloat16, "in_out"),
+               matrix(800, 2048, torch.bfloat16, seed=4))
+    right, lib = call(x, w, g), _capi.load()
+    before = lib.cusort_set_wait_limit_ns(1_000_000)
+    lib.cusort_debug_set_skip_tile(skip)
+    try:
+        call(x, w, g)
+    finally:
+        lib.cusort_debug_set_skip_tile(-1)
+        lib.cusort_set_wait_limit_ns(before)
+    told = X.product_status(), X.product_status()
+    # every CTA has one tile at most here: of 1024 / 128 or 1024 / 64 steps, or of the segments' 300 and 500 rows by 64
+    steps = {_few: 8, _many: 16, _gradient: 8}[call]
+    assert told == ((1, 0) if skip < steps else (0, 0))
+    assert torch.equal(call(x, w, g), right)
+
+
+def test_results_and_weights_beyond_32_bits():
+    c, o, capacity, _ = plan([400_000, 200_000])
+    x, w = matrix(capacity, 64, torch.bfloat16), weights_of(2, 64, 4096, torch.bfloat16, "in_out")
+    out = X.expert_products(x, w, c, o)  # 4.9 GB
+    for at, e in ((slice(0, 50), 0), (slice(399_950, 400_000), 0), (slice(400_000, 400_050), 1),
+                  (slice(capacity - 50, capacity), 1)):
+        xe, we = x[at].double(), w[e].double()
+        close(out[at], xe @ we, xe.abs() @ we.abs(), 64)
+    del out, x, w
+    counts = [0] * 540
+    counts[0], counts[539] = 40, 70
+    c, o, capacity, _ = plan(counts)
+    x, g = matrix(capacity, 2048, torch.bfloat16), matrix(capacity, 2048, torch.bfloat16, seed=2)
+    w = torch.zeros(540, 2048, 2048, dtype=torch.bfloat16, device="cuda")  # 4.5 GB
+    w[0], w[539] = weights_of(2, 2048, 2048, torch.bfloat16, "in_out")
+    out, grad = X.expert_products(x, w, c, o), X.expert_products_grad_weights(g, x, c, o)
+    for at, e in ((slice(0, 40), 0), (slice(40, 110), 539)):
+        xe, ge, we = x[at].double(), g[at].double(), w[e].double()
+        close(out[at], xe @ we, xe.abs() @ we.abs(), 2048)
+        close(grad[e], xe.T @ ge, xe.T.abs() @ ge.abs(), 70)
+    assert not grad[1:539].any()
 
 
 def plan(counts, align=1, tail=0):
