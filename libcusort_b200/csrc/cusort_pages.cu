@@ -47,9 +47,11 @@ struct PagesArgs {
   int row_lanes, row_parts;  // see for_rows
 };
 
-__device__ __forceinline__ int held_of(const PagesArgs& a, int len) {
-  return (int)min((int64_t)a.width, ((int64_t)max(len, 0) + a.block_size - 1) / a.block_size);
+// Blocks that a length needs, and those of them that the table has.
+__device__ __forceinline__ int blocks_of(const PagesArgs& a, int len) {
+  return (int)(((uint32_t)max(len, 0) + (uint32_t)a.block_size - 1) / (uint32_t)a.block_size);
 }
+__device__ __forceinline__ int held_of(const PagesArgs& a, int len) { return min(a.width, blocks_of(a, len)); }
 __device__ __forceinline__ bool in_pool(const PagesArgs& a, int block) { return block >= 0 && block < a.num_blocks; }
 
 // Sum of the CTA's values before this thread's; total: of all.
@@ -149,40 +151,41 @@ __device__ __forceinline__ int free_of(const PagesArgs& a) { return min(max(*a.n
 // its first child and the number of children that are served, for a child the
 // number of blocks taken before its own.
 struct Children {
-  int *first, *count;  // [requests]
+  int *first, *count;  // [requests]; the count above two bits: kPart, kStays
   int* rank;           // [children] blocks taken before; -1: takes none, -2: no parent or not served
 };
+constexpr int kPart = 2;   // the request's last block is part-filled
+constexpr int kStays = 1;  // and its first child keeps it: no other table holds it
 
-// The block that a request's last token lies in, where that is part-filled; -1 otherwise.
-__device__ __forceinline__ int last_part(const PagesArgs& a, int request, int len) {
-  const int64_t held = ((int64_t)len + a.block_size - 1) / a.block_size;
-  return len <= 0 || len % a.block_size == 0 || held > a.width ? -1
-                                                                 : a.tables[request * a.table_stride + held - 1];
-}
-// Whether its first child keeps that block: no other table holds it.
-__device__ __forceinline__ bool stays(const PagesArgs& a, int block) {
-  return in_pool(a, block) && a.shares[block] == 0;
-}
-
+// What is read first is on its way before anything else: a chain of a length,
+// a table's entry and its shares beside that of the parents.
 __device__ __forceinline__ int plan_children(const PagesArgs& a, const Children& c, int* sums) {
-  for (int p = threadIdx.x; p < a.requests; p += kThreads) c.first[p] = a.children, c.count[p] = 0;
+  const int t = threadIdx.x;
+  const int parent0 = t < a.children ? a.parents[t] : -1, len0 = t < a.requests ? a.lens[t] : 0, left = free_of(a);
+  for (int p = t; p < a.requests; p += kThreads) c.first[p] = a.children;
   __syncthreads();
-  for (int r = threadIdx.x; r < a.children; r += kThreads) {
-    const int p = a.parents[r];
+  for (int p = t; p < a.requests; p += kThreads) {
+    const int len = p == t ? len0 : a.lens[p], blocks = blocks_of(a, len);
+    int bits = 0;
+    if (len > 0 && len % a.block_size != 0 && blocks <= a.width) {
+      const int last = a.tables[p * a.table_stride + blocks - 1];
+      bits = in_pool(a, last) && a.shares[last] == 0 ? kPart | kStays : kPart;
+    }
+    c.count[p] = bits;
+  }
+  for (int r = t; r < a.children; r += kThreads) {
+    const int p = r == t ? parent0 : a.parents[r];
     if (p >= 0 && p < a.requests) atomicMin(c.first + p, r);
   }
   __syncthreads();
-  const int left = free_of(a);
   int taken = 0;
   for (int r0 = 0; r0 < a.children; r0 += kThreads) {
-    const int r = r0 + threadIdx.x, p = r < a.children ? a.parents[r] : -1;
+    const int r = r0 + t, p = r0 == 0 ? parent0 : r < a.children ? a.parents[r] : -1;
     const bool valid = p >= 0 && p < a.requests;
     bool need = false;
     if (valid) {
-      const int len = a.lens[p];
-      const int64_t held = ((int64_t)max(len, 0) + a.block_size - 1) / a.block_size;
-      const bool part = len > 0 && len % a.block_size != 0 && held <= a.width;
-      need = part && !(c.first[p] == r && stays(a, a.tables[p * a.table_stride + held - 1]));
+      const int bits = c.count[p] & (kPart | kStays);
+      need = bits == kPart || (bits != 0 && c.first[p] != r);
     }
     int total;
     const int rank = taken + scan(need, sums, total);
@@ -190,7 +193,7 @@ __device__ __forceinline__ int plan_children(const PagesArgs& a, const Children&
     if (r < a.children) {
       const bool ok = valid && (!need || rank < left);
       c.rank[r] = !ok ? -2 : need ? rank : -1;
-      if (ok) atomicAdd(c.count + p, 1);
+      if (ok) atomicAdd(c.count + p, 4);
     }
   }
   __syncthreads();
@@ -204,8 +207,9 @@ __device__ __forceinline__ void fork_tables(const PagesArgs& a, const Children& 
   for (int r = me; r < a.children; r += all) {
     const int rank = c.rank[r], p = a.parents[r];
     const bool valid = p >= 0 && p < a.requests;
-    a.lens_out[r] = rank == -2 ? 0 : max(a.lens[p], 0);
-    a.sources[r] = rank >= 0 ? last_part(a, p, a.lens[p]) : -1;
+    const int len = rank == -2 ? 0 : max(a.lens[p], 0);
+    a.lens_out[r] = len;
+    a.sources[r] = rank >= 0 ? a.tables[p * a.table_stride + blocks_of(a, len) - 1] : -1;
     a.destinations[r] = rank >= 0 ? a.free_blocks[left - 1 - rank] : -1;
     a.served[r] = !valid || rank != -2;
   }
@@ -222,19 +226,17 @@ __device__ __forceinline__ void fork_tables(const PagesArgs& a, const Children& 
       if (at[i] < a.width) to[at[i]] = block[i];
   });
   for_rows(a, a.requests, [&](int p, const int (&at)[kEach]) {
-    const int len = a.lens[p], held = held_of(a, len), more = c.count[p] - 1;
-    const bool part = len > 0 && len % a.block_size != 0 && held == ((int64_t)len + a.block_size - 1) / a.block_size;
+    const int held = held_of(a, a.lens[p]), count = c.count[p], more = (count >> 2) - 1;
     const int32_t* from = a.tables + p * a.table_stride;
-    if (more == 0 && !part) return;
+    if (more == 0 && !(count & kPart)) return;
+    // what becomes of a part-filled last block
+    const int last = (count & kStays) && c.first[p] < a.children ? 0 : -1;
     int block[kEach], delta[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       block[i] = at[i] < held ? from[at[i]] : -1;
-      delta[i] = more;
+      delta[i] = (count & kPart) && at[i] == held - 1 ? last : more;
     }
-#pragma unroll
-    for (int i = 0; i < kEach; ++i)
-      if (part && at[i] == held - 1) delta[i] = c.first[p] < a.children && stays(a, block[i]) ? 0 : -1;
     h.add(a, block, delta);
   });
 }
