@@ -76,13 +76,16 @@ constexpr uint32_t kAll = 0xffffffffu;
 // Products that gave up waiting (a bounded wait ran out): 1.
 __device__ uint32_t g_product_status;
 
+constexpr int kEnds = 4;  // buffers for the ends of segments, in the gradient of the weights
+
 // Barriers and flags of one CTA.  PAIR: two CTAs work on one tile, each with
 // half of either operand; the first one multiplies.
 template <int STAGES, bool PAIR> struct Pipe {
   uint64_t full[STAGES];   // a stage's copies are there; those of both CTAs count on the first one's barrier
   uint64_t empty[STAGES];  // a stage was multiplied
-  uint64_t end[STAGES];    // a stage's copies of this CTA are there, which hold the end of a segment
-  uint64_t ended[STAGES];  // in the first of two CTAs: both have cleared what lies behind that
+  // the same of the buffers for the ends of segments, of this CTA alone; in the first of two CTAs: both have cleared
+  // what lies behind the end; multiplied
+  uint64_t end_full[kEnds], end_cleared[kEnds], end_empty[kEnds];
   uint64_t sum_full[2], sum_empty[2];
   uint32_t tmem, gave_up, sums[kThreads / 32];
 };
@@ -94,8 +97,9 @@ template <int STAGES, bool PAIR> struct PipeAt {
   __device__ __forceinline__ explicit PipeAt(const P& p) : base(dev::smem_u32(&p)) {}
   __device__ __forceinline__ uint32_t full(int i) const { return base + offsetof(P, full) + 8 * i; }
   __device__ __forceinline__ uint32_t empty(int i) const { return base + offsetof(P, empty) + 8 * i; }
-  __device__ __forceinline__ uint32_t end(int i) const { return base + offsetof(P, end) + 8 * i; }
-  __device__ __forceinline__ uint32_t ended(int i) const { return base + offsetof(P, ended) + 8 * i; }
+  __device__ __forceinline__ uint32_t end_full(int i) const { return base + offsetof(P, end_full) + 8 * i; }
+  __device__ __forceinline__ uint32_t end_cleared(int i) const { return base + offsetof(P, end_cleared) + 8 * i; }
+  __device__ __forceinline__ uint32_t end_empty(int i) const { return base + offsetof(P, end_empty) + 8 * i; }
   __device__ __forceinline__ uint32_t sum_full(int i) const { return base + offsetof(P, sum_full) + 8 * i; }
   __device__ __forceinline__ uint32_t sum_empty(int i) const { return base + offsetof(P, sum_empty) + 8 * i; }
   // The storing warps have read a sum: one lane says so.
@@ -111,8 +115,11 @@ __device__ __forceinline__ void init_pipe(Pipe<STAGES, PAIR>& p, uint32_t column
     for (int i = 0; i < STAGES; ++i) {
       dev::mbar_init(&p.full[i], 1);
       dev::mbar_init(&p.empty[i], 1);
-      dev::mbar_init(&p.end[i], 1);
-      dev::mbar_init(&p.ended[i], 2);
+    }
+    for (int i = 0; i < kEnds; ++i) {
+      dev::mbar_init(&p.end_full[i], 1);
+      dev::mbar_init(&p.end_cleared[i], 2);
+      dev::mbar_init(&p.end_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) dev::mbar_init(&p.sum_full[i], 1), dev::mbar_init(&p.sum_empty[i], PAIR ? 8 : 4);
     p.gave_up = 0;
@@ -145,11 +152,6 @@ template <int STAGES> struct Ring {
   uint32_t parity = 0;
   __device__ __forceinline__ void next() {
     if (++stage == STAGES) stage = 0, parity ^= 1;
-  }
-  __device__ __forceinline__ void skip(int n) {
-    stage += n;
-    parity ^= stage / STAGES & 1;
-    stage %= STAGES;
   }
 };
 
@@ -400,7 +402,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
 
 struct GradArgs {
   CUtensorMap out;         // where its rows lie on 16-byte boundaries
-  CUtensorMap slow, fast;  // the rows whose width is the gradient's slower dimension, and those of the contiguous one
+  // the rows whose width is the gradient's slower dimension, and those of the contiguous one; by boxes of 16 for ends
+  CUtensorMap slow, fast, slow_end, fast_end;
   SegmentArgs segments;
   void* result;  // [experts][slow_width][fast_width]
   int slow_width, fast_width, slow_tiles, fast_tiles;
@@ -409,20 +412,26 @@ struct GradArgs {
 };
 
 constexpr int kGradN = 256;
-constexpr int kGradStages = 6;
+constexpr int kGradStages = 5;
 constexpr uint32_t kGradStage = kBytesA + kGradN / 2 * kBlockK * 2;
 constexpr uint32_t kStoreBox = 32 * 64;              // 32 rows of 32 elements, stored as one box
 constexpr int kStoreBoxes = 3;                       // for each storing warp: one is filled, others are being stored
 constexpr uint32_t kGradStaging = 4 * kStoreBoxes * kStoreBox;
 constexpr int kChunkBytes = kBytesA / 2;  // 64 contracted rows of 64 elements
+constexpr int kEndRows = 16;              // contracted by one instruction
+constexpr int kEndChunk = kEndRows * 128, kEndBytes = 4 * kEndChunk;
 
 size_t grad_bytes(int experts) {
-  return 1024 + kGradStages * kGradStage + kGradStaging + sizeof(Pipe<kGradStages, true>) + 8 * (size_t)experts;
+  return 1024 + kGradStages * kGradStage + kEnds * kEndBytes + kGradStaging + sizeof(Pipe<kGradStages, true>) + 8 * (size_t)experts;
 }
 
 struct GradTile {
   int expert, slow, fast, chunks;  // first elements; 64-element chunks of the contiguous dimension in each of the CTAs
   int2 segment;
+  // The segment's rows in whole instructions, by steps of kBlockK; its end, fewer than kEndRows, is one by itself.
+  __device__ __forceinline__ int whole() const { return segment.y / kEndRows * kEndRows; }
+  __device__ __forceinline__ int steps() const { return (whole() + kBlockK - 1) / kBlockK; }
+  __device__ __forceinline__ int end() const { return segment.y % kEndRows; }
 };
 
 __device__ __forceinline__ GradTile grad_tile(const GradArgs& a, const int2* segments, uint32_t t) {
@@ -436,24 +445,21 @@ __device__ __forceinline__ GradTile grad_tile(const GradArgs& a, const int2* seg
   return g;
 }
 
-// Whether the step from row k of a segment on ends inside one of the instruction's 16 contracted rows.
-__device__ __forceinline__ bool has_end(int count, int k) { return count - k < kBlockK && count % 16 != 0; }
-
 // gradient[e] = slow_e^T x fast_e, contracted over the rows of e's segment: both operands lie with the contracted
-// dimension across.  Rows behind the segment's end that the last step brings along are cleared in shared memory: they
-// are another expert's, or anything at all.
+// dimension across.  Rows behind a segment's end are another expert's, or anything at all: the last fewer than 16 rows
+// come by themselves, and what comes with them is cleared in shared memory.
 //
-// Always by pairs of CTAs.  Many rows: bound as the products are (8192 rows, 4096 x 4096: 196 us, 1.40 PFLOP/s; 32
-// experts of 1024, 2048 x 4096: 403 us; of 1023, with an end to clear: 453, about a microsecond a tile that its stages
-// do not hide).  Few: by writing the gradient, for which 3.9 TB/s is all that a plain fill comes to (128 experts of 128
-// rows, 2048 x 1024: 181 us, 3.0 TB/s; without the stores 120).  Stored by tiled copies of 64-byte rows: whole
+// Always by pairs of CTAs.  Many rows: bound as the products are (8192 rows, 4096 x 4096: 192 us, 1.43 PFLOP/s; 32
+// experts of 1024, 2048 x 4096: 395 us).  Few: by writing the gradient, for which 3.9 TB/s is all that a plain fill
+// comes to (128 experts of 128 rows, 2048 x 1024: 183 us, 2.9 TB/s; without the stores 120).  Stored by tiled copies of 64-byte rows: whole
 // sectors straight from registers took 194 us there, and 271 instead of 233 where rows are 2800 bytes.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     grad_weights_kernel(const __grid_constant__ GradArgs a) {
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (align_up(dev::smem_u32(raw), 1024) - dev::smem_u32(raw));
-  uint8_t* staging = base + kGradStages * kGradStage;
+  uint8_t* ends = base + kGradStages * kGradStage;
+  uint8_t* staging = ends + kEnds * kEndBytes;
   Pipe<kGradStages, true>& p = *reinterpret_cast<Pipe<kGradStages, true>*>(staging + kGradStaging);
 
   int2* segments = reinterpret_cast<int2*>(&p + 1);
@@ -473,24 +479,38 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (brings(warp)) {
     if (dev::elect_one()) {
       Ring<kGradStages> ring;
+      Ring<kEnds> end;
       uint32_t turn = (warp == 2 || warp == 9);  // whether it takes the odd steps
       int64_t step_of_cta = -1;
       for (uint32_t t = t0; t < tiles; t += t_step) {
         const GradTile g = grad_tile(a, segments, t);
         const int slow = g.slow + rank * kTileM, fast = g.fast + rank * g.chunks * kBlockK;
         const uint32_t bytes = (2 + g.chunks) * kChunkBytes;
-        for (int k = 0; k < g.segment.y; k += kBlockK, ring.next()) {
+        const int steps = g.steps();
+        if (g.end()) {
+          // ahead of the steps, into a buffer of its own, so that it is there and cleared when they are done
+          if ((warp == 2 || warp == 9) && dev::wait_for(at.end_empty(end.stage), end.parity ^ 1, limit)) {
+            const uint32_t to = dev::smem_u32(ends) + end.stage * kEndBytes, bar = at.end_full(end.stage);
+            const int row = g.segment.x + g.whole();
+            if (warp < 8) {
+              dev::arrive_expect(bar, (2 + g.chunks) * kEndChunk);
+              for (int c = 0; c < 2; ++c)
+                dev::tma_load_2d(to + c * kEndChunk, &a.slow_end, bar, slow + c * kBlockK, row);
+            } else {
+              for (int c = 0; c < g.chunks; ++c)
+                dev::tma_load_2d(to + (2 + c) * kEndChunk, &a.fast_end, bar, fast + c * kBlockK, row);
+            }
+          }
+          end.next();
+        }
+        for (int k = 0; k < steps; ++k, ring.next()) {
           ++step_of_cta;
           if ((turn ^= 1) == 0 || !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
           if (step_of_cta == a.skip) continue;
-          const uint32_t to = stages + ring.stage * kGradStage;
-          const int row = g.segment.x + k;
-          // each CTA looks after the end of a segment in its own copies
-          const bool end = has_end(g.segment.y, k);
-          const uint32_t bar = end ? at.end(ring.stage) : dev::in_first(at.full(ring.stage));
+          const uint32_t to = stages + ring.stage * kGradStage, bar = dev::in_first(at.full(ring.stage));
+          const int row = g.segment.x + k * kBlockK;
           if (warp < 8) {
-            if (end) dev::arrive_expect(at.end(ring.stage), bytes);
-            else if (rank == 0) dev::arrive_expect(at.full(ring.stage), 2 * bytes);
+            if (rank == 0) dev::arrive_expect(at.full(ring.stage), 2 * bytes);
             dev::tma_load_2d<true>(to, &a.slow, bar, slow, row);
             dev::tma_load_2d<true>(to + kChunkBytes, &a.slow, bar, slow + kBlockK, row);
           } else {
@@ -507,29 +527,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       Ring<2> sums;
       const uint64_t first_a = dev::operand_descriptor(stages, kChunkBytes, 1024);
       const uint64_t first_b = dev::operand_descriptor(stages + kBytesA, kChunkBytes, 1024);
-      uint32_t parity[2] = {0, 0};  // of each stage's barriers: of whole steps, of ends
+      Ring<kEnds> end;
+      const uint64_t end_a = dev::operand_descriptor(dev::smem_u32(ends), kEndChunk, 1024);
+      const uint64_t end_b = dev::operand_descriptor(dev::smem_u32(ends) + 2 * kEndChunk, kEndChunk, 1024);
       for (uint32_t t = t0; t < tiles; t += t_step) {
         const GradTile g = grad_tile(a, segments, t);
-        const int count = g.segment.y;
-        if (count == 0) continue;
+        if (g.segment.y == 0) continue;
         const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, true, true, 2 * kTileM,
                                                           2 * g.chunks * kBlockK);
         const uint32_t sum = p.tmem + sums.stage * kGradN;
+        const int whole = g.whole(), steps = g.steps();
         dev::wait_for<true>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
-        dev::tmem_fence_after();
-        for (int k = 0; k < count; k += kBlockK, ring.next()) {
-          bool there;
-          if (has_end(count, k)) {
-            there = dev::wait_for<true>(at.ended(ring.stage), parity[1] >> ring.stage & 1, limit);
-            parity[1] ^= 1u << ring.stage;
-          } else {
-            there = dev::wait_for(at.full(ring.stage), parity[0] >> ring.stage & 1, limit);
-            parity[0] ^= 1u << ring.stage;
-          }
-          if (!there) continue;
+        for (int k = 0; k < steps; ++k, ring.next()) {
+          if (!dev::wait_for(at.full(ring.stage), ring.parity, limit)) continue;
           dev::tmem_fence_after();
           const uint32_t stage = ring.stage * (kGradStage / 16);
-          const int depth = min(kBlockK, count - k + 15) / 16;
+          const int depth = min(kBlockK, whole - k * kBlockK) / 16;
 #pragma unroll
           for (int i = 0; i < kBlockK / 16; ++i)
             if (i < depth)
@@ -537,33 +550,38 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    k + i > 0);
           dev::mma_commit<true>(at.empty(ring.stage));
         }
+        if (g.end()) {
+          if (dev::wait_for<true>(at.end_cleared(end.stage), end.parity, limit)) {
+            dev::tmem_fence_after();
+            const uint32_t buffer = end.stage * (kEndBytes / 16);
+            dev::mma_issue<true>(sum, end_a + buffer, end_b + buffer, instruction, steps > 0);
+            dev::mma_commit<true>(at.end_empty(end.stage));
+          }
+          end.next();
+        }
         dev::mma_commit<true>(at.sum_full(sums.stage));
         sums.next();
       }
     }
   } else if (warp == 3) {
-    // the ends of segments, cleared as soon as they have come (by the multiplying warp, when it got there, the
-    // gradient of 32 experts of about 1024 rows took 685 us)
-    Ring<kGradStages> ring;
-    uint32_t parity = 0;  // of each stage's barrier of ends
+    // What came with the ends of segments is cleared.  With the ends in the stages, among the steps, this took about a
+    // microsecond that nothing hid (32 experts of 1023 rows, 2048 x 4096: 441 us, 399 now, 395 of 1024 rows); done
+    // by the multiplying warp, 685.
+    Ring<kEnds> end;
     for (uint32_t t = t0; t < tiles; t += t_step) {
       const GradTile g = grad_tile(a, segments, t);
-      const int count = g.segment.y, plain = (count + kBlockK - 1) / kBlockK - (count % 16 != 0);
-      ring.skip(plain);
-      if (count % 16 == 0) continue;
-      if (warp_wait(at.end(ring.stage), parity >> ring.stage & 1, limit)) {
-        const int valid = count - plain * kBlockK, depth = (valid + 15) / 16 * 16;
-        uint8_t* chunk = base + ring.stage * kGradStage + lane * 16;  // 8 lanes to a row
-        for (int c = 0; c < 2 + g.chunks; ++c, chunk += kChunkBytes)
-          for (int row = valid; row < depth; row += 4)
-            if (row + lane / 8 < depth)
+      if (!g.end()) continue;
+      if (warp_wait(at.end_full(end.stage), end.parity, limit)) {
+        uint8_t* chunk = ends + end.stage * kEndBytes + lane * 16;  // 8 lanes to a row
+        for (int c = 0; c < 2 + g.chunks; ++c, chunk += kEndChunk)
+          for (int row = g.end(); row < kEndRows; row += 4)
+            if (row + lane / 8 < kEndRows)
               *reinterpret_cast<uint4*>(chunk + row * dev::kBoxRowBytes) = make_uint4(0, 0, 0, 0);
         dev::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) dev::arrive_first(at.ended(ring.stage));
+        if (lane == 0) dev::arrive_first(at.end_cleared(end.stage));
       }
-      parity ^= 1u << ring.stage;
-      ring.next();
+      end.next();
     }
   } else if (warp >= 4 && warp < 8) {
     Ring<2> sums;
@@ -781,7 +799,9 @@ cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order
 }
 
 // Rows of a tile where no expert can have more, where experts have few on
-// average, and where they have many.
+// average, and where they have many (by pairs of CTAs).  64 experts, 2048 ->
+// 1536, by the second and the third: 8 rows each 65 and 69 us, 64 71 and 75, 80
+// 84 and 76, 128 89 and 80.
 constexpr int kFewestRows = 16, kFewRows = 64, kManyRows = 256;
 
 // Tiles begin before this many rows and end within 32 bits.
@@ -892,6 +912,8 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
   if (!e) e = fast.prepare(temp, nullptr, stream);
   if (!e) e = slow.map(&a.slow, true, kBlockK);
   if (!e) e = fast.map(&a.fast, true, kBlockK);
+  if (!e) e = slow.map(&a.slow_end, true, kEndRows);
+  if (!e) e = fast.map(&a.fast_end, true, kEndRows);
   if (!e && fast.width % 8 == 0) {
     const Operand out{d_grad_weights, num_experts, slow.width, fast.width, slow.width * fast.width, fast.width};
     e = out.map(&a.out, false, 32, 32);

@@ -162,6 +162,9 @@ cudaError_t run(FloatArgs a, cudaStream_t stream) {
                                sizeof(Shape<U, K>) + 4 * (3 * (size_t)a.segments.experts + 1), a, stream);
 }
 
+// Rows an expert on average up to which tiles have 16 and 64 rows.  64 experts,
+// 1024 -> 2048, in tiles of 16, 64 and 128 rows: 16 rows each 415, 608 and 846
+// us; 24 752, 611, 848; 64 1430, 632, 886; 96 2132, 1076, 925.
 constexpr int kFewestRows = 16, kFewRows = 64;
 
 }  // namespace
