@@ -12,10 +12,9 @@
 namespace cusort_b200 {
 namespace dev {
 
-// A tile of 64 16-bit elements (128 bytes) along the contiguous dimension: the
-// width of every box that the tiled copies bring, whose 16-byte pieces they
-// permute within each 8 rows (128-byte swizzle).
-constexpr int kBoxElements = 64;
+// 64 16-bit elements along the contiguous dimension: the width of every box
+// that the tiled copies bring, whose 16-byte pieces they permute within each 8
+// rows (128-byte swizzle).
 constexpr int kBoxRowBytes = 128;
 
 // A box into this CTA's shared memory, counted on the barrier `bar` (PAIR: of either CTA of a cluster of two).
