@@ -70,7 +70,7 @@ constexpr int kThreads = 320;  // warps 0, 2, 8 and 9 bring operands, 1 multipli
 constexpr int kSms = 148;
 constexpr int kBlockK = 64;              // contracted elements to a stage: one swizzle row
 constexpr int kTileM = 128;              // lanes of a CTA's tensor memory
-constexpr uint32_t kBytesA = kTileM * kBlockK * 2;
+constexpr uint32_t kBoxBytes = kBlockK * dev::kBoxRowBytes;  // 64 rows of 64 elements
 constexpr uint32_t kAll = 0xffffffffu;
 
 // Products that gave up waiting (a bounded wait ran out): 1.
@@ -190,9 +190,12 @@ struct ProductArgs {
   int64_t skip;       // for tests: every CTA's step that is never brought; -1: none
 };
 
-// PAIR: tiles of 256 columns of the result, 128 in each of two CTAs, and half of the rows in each.
-template <int BN, int STAGES, int SUB, bool PAIR> struct ProductShape {
-  static constexpr int kCtas = PAIR ? 2 : 1, kTile = kTileM * kCtas;
+// PAIR: tiles of 256 columns of the result, 128 in each of two CTAs, and half of the rows in each.  COLUMNS: 128, or 64
+// (not by pairs): the other 64 lanes of tensor memory get products of what lies behind in shared memory, and nobody
+// looks at them.
+template <int BN, int COLUMNS, int STAGES, int SUB, bool PAIR> struct ProductShape {
+  static constexpr int kCtas = PAIR ? 2 : 1, kTile = COLUMNS * kCtas;
+  static constexpr uint32_t kBytesA = COLUMNS * kBlockK * 2;
   static constexpr int kRowStep = 16 * kCtas;       // the instruction's width comes in such steps
   // A stage holds SUB steps of kBlockK, each the weights' part and then the rows'.
   static constexpr uint32_t kBytesB = BN / kCtas * kBlockK * 2, kStep = kBytesA + kBytesB, kStage = SUB * kStep;
@@ -238,14 +241,17 @@ __device__ __forceinline__ ProductTile product_tile(const ProductArgs& a, const 
 // experts with 4 rows each, 2048 -> 1536: 118 us, 6.8 TB/s), below that by how
 // much of the weights each of the few CTAs has under way.  So where no expert
 // can have more than 16 rows their part of a stage is small and there are five
-// stages, not four (six rows of six experts, 2048 -> 1024, from memory 9.4 us,
-// with four 10.5; 4096 -> 1024 14.7, 17.3; 4.2 us are there without any
-// contraction).  Splitting the contraction over clusters of two or three CTAs
+// stages, not four, and tiles of 64 columns where that still leaves no more
+// than one to an SM (six rows of six experts, 2048 -> 1024, from memory: 10.5
+// us with four stages, 9.4 with five, 8.9 with half the columns; 4096 -> 1024
+// 17.3, 14.7, 12.6; 4.2 us are there without any contraction).  Splitting the contraction over clusters of two or three CTAs
 // took as long or longer (11.4 us for the first): their barriers and the
 // joining cost what the shorter loops gained.
-template <typename T, int BN, int STAGES, int SUB, bool PAIR, bool IN_ORDER>
+template <typename T, int BN, int COLUMNS, int STAGES, int SUB, bool PAIR, bool IN_ORDER>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
-  using Shape = ProductShape<BN, STAGES, SUB, PAIR>;
+  using Shape = ProductShape<BN, COLUMNS, STAGES, SUB, PAIR>;
+  constexpr uint32_t kBytesA = Shape::kBytesA;
+  static_assert(COLUMNS == 128 || (COLUMNS == 64 && !PAIR), "");
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (align_up(dev::smem_u32(raw), 1024) - dev::smem_u32(raw));
   uint8_t* staging = base + STAGES * Shape::kStage;
@@ -305,7 +311,8 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
               dev::tma_load_3d<PAIR>(step, &a.weights, bar, x, column, tile.expert);
             } else {
               dev::tma_load_3d<PAIR>(step, &a.weights, bar, column, x, tile.expert);
-              dev::tma_load_3d<PAIR>(step + kBytesA / 2, &a.weights, bar, column + kBlockK, x, tile.expert);
+              if (COLUMNS == 128)
+                dev::tma_load_3d<PAIR>(step + kBytesA / 2, &a.weights, bar, column + kBlockK, x, tile.expert);
             }
           }
         }
@@ -316,12 +323,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     if (dev::elect_one()) {
       Ring<STAGES> ring;
       Ring<2> sums;
-      const uint64_t first_a = dev::operand_descriptor(stages, IN_ORDER ? 16 : kBytesA / 2, 1024);
+      const uint64_t first_a = dev::operand_descriptor(stages, IN_ORDER ? 16 : kBoxBytes, 1024);
       const uint64_t first_b = dev::operand_descriptor(stages + kBytesA, 16, 1024);
       for (uint32_t t = t0; t < tiles; t += t_step, sums.next()) {
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, !IN_ORDER, false,
-                                                          Shape::kTile, align_up(tile.rows, Shape::kRowStep));
+                                                          kTileM * Shape::kCtas, align_up(tile.rows, Shape::kRowStep));
         const uint32_t sum = p.tmem + sums.stage * BN;
         dev::wait_for<PAIR>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
         dev::tmem_fence_after();
@@ -354,7 +361,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       if (!warp_wait(at.sum_full(sums.stage), sums.parity, limit)) continue;
       dev::tmem_fence_after();
       const int column = tile.column + rank * kTileM + quarter * 32;
-      for (int c = 0; c < tile.rows; c += 32) {
+      for (int c = 0; c < tile.rows && quarter * 32 < COLUMNS; c += 32) {
         uint32_t v[32];
         dev::tmem_load32(p.tmem + sums.stage * BN + c + ((uint32_t)quarter << 21), v);
         dev::tmem_load_wait(v);
@@ -413,11 +420,11 @@ struct GradArgs {
 
 constexpr int kGradN = 256;
 constexpr int kGradStages = 5;
-constexpr uint32_t kGradStage = kBytesA + kGradN / 2 * kBlockK * 2;
+constexpr uint32_t kGradStage = 4 * kBoxBytes;
 constexpr uint32_t kStoreBox = 32 * 64;              // 32 rows of 32 elements, stored as one box
 constexpr int kStoreBoxes = 3;                       // for each storing warp: one is filled, others are being stored
 constexpr uint32_t kGradStaging = 4 * kStoreBoxes * kStoreBox;
-constexpr int kChunkBytes = kBytesA / 2;  // 64 contracted rows of 64 elements
+constexpr int kChunkBytes = kBoxBytes;    // 64 contracted rows of 64 elements
 constexpr int kEndRows = 16;              // contracted by one instruction
 constexpr int kEndChunk = kEndRows * 128, kEndBytes = 4 * kEndChunk;
 
@@ -515,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             dev::tma_load_2d<true>(to + kChunkBytes, &a.slow, bar, slow + kBlockK, row);
           } else {
             for (int c = 0; c < g.chunks; ++c)
-              dev::tma_load_2d<true>(to + kBytesA + c * kChunkBytes, &a.fast, bar, fast + c * kBlockK, row);
+              dev::tma_load_2d<true>(to + (2 + c) * kChunkBytes, &a.fast, bar, fast + c * kBlockK, row);
           }
         }
       }
@@ -526,7 +533,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Ring<kGradStages> ring;
       Ring<2> sums;
       const uint64_t first_a = dev::operand_descriptor(stages, kChunkBytes, 1024);
-      const uint64_t first_b = dev::operand_descriptor(stages + kBytesA, kChunkBytes, 1024);
+      const uint64_t first_b = dev::operand_descriptor(stages + 2 * kChunkBytes, kChunkBytes, 1024);
       Ring<kEnds> end;
       const uint64_t end_a = dev::operand_descriptor(dev::smem_u32(ends), kEndChunk, 1024);
       const uint64_t end_b = dev::operand_descriptor(dev::smem_u32(ends) + 2 * kEndChunk, kEndChunk, 1024);
@@ -783,19 +790,19 @@ cudaError_t run(Kernel kernel, const Args& a, int64_t tiles, int ctas, size_t sm
   return launch_after_previous(kernel, grid, kThreads, smem, a, stream, ctas);
 }
 
-template <typename T, int BN, int STAGES, int SUB, bool PAIR>
+template <typename T, int BN, int COLUMNS, int STAGES, int SUB, bool PAIR>
 cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order, int64_t row_tiles,
                     cudaStream_t stream) {
-  using Shape = ProductShape<BN, STAGES, SUB, PAIR>;
+  using Shape = ProductShape<BN, COLUMNS, STAGES, SUB, PAIR>;
   a.width_tiles = (a.width + Shape::kTile - 1) / Shape::kTile;
   a.most = (uint32_t)row_tiles;
-  cudaError_t e = weights.map(&a.weights, false, in_order ? kTileM : kBlockK);
+  cudaError_t e = weights.map(&a.weights, false, in_order ? COLUMNS : kBlockK);
   for (int i = 0; !e && i < 3; ++i) e = rows.map(&a.rows[i], true, 64 >> i);
   if (e) return e;
   const size_t smem = Shape::bytes(a.segments.experts);
   const int64_t tiles = row_tiles * a.width_tiles;
-  return in_order ? run(product_kernel<T, BN, STAGES, SUB, PAIR, true>, a, tiles, Shape::kCtas, smem, stream)
-                  : run(product_kernel<T, BN, STAGES, SUB, PAIR, false>, a, tiles, Shape::kCtas, smem, stream);
+  return in_order ? run(product_kernel<T, BN, COLUMNS, STAGES, SUB, PAIR, true>, a, tiles, Shape::kCtas, smem, stream)
+                  : run(product_kernel<T, BN, COLUMNS, STAGES, SUB, PAIR, false>, a, tiles, Shape::kCtas, smem, stream);
 }
 
 // Rows of a tile where no expert can have more, where experts have few on
@@ -862,9 +869,12 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   if (e) return e;
   const auto go = [&](auto t) {
     using T = decltype(t);
-    if (capacity <= kFewestRows) return product<T, kFewestRows, 5, 2, false>(a, weights, rows, in_order, tiles, stream);
-    return few ? product<T, kFewRows, 4, 2, false>(a, weights, rows, in_order, tiles, stream)
-               : product<T, kManyRows, 6, 1, true>(a, weights, rows, in_order, tiles, stream);
+    if (capacity <= kFewestRows)
+      return tiles * ((out + kTileM - 1) / kTileM) <= kSms / 2
+                 ? product<T, kFewestRows, 64, 9, 2, false>(a, weights, rows, in_order, tiles, stream)
+                 : product<T, kFewestRows, 128, 5, 2, false>(a, weights, rows, in_order, tiles, stream);
+    return few ? product<T, kFewRows, 128, 4, 2, false>(a, weights, rows, in_order, tiles, stream)
+               : product<T, kManyRows, 128, 6, 1, true>(a, weights, rows, in_order, tiles, stream);
   };
   return type == CUSORT_FLOAT_F16 ? go(__half{}) : go(__nv_bfloat16{});
 }

@@ -146,10 +146,17 @@ def test_few_rows_an_expert(fin, fout, dtype, order):
 
 
 @pytest.mark.parametrize("order", ["in_out", "out_in"])
-@pytest.mark.parametrize("counts", [[1], [0, 2, 0, 64], [1, 33, 0, 5, 0, 0, 1, 70]], ids=str)
+@pytest.mark.parametrize("counts", [[1], [3, 0, 5, 1, 0, 7], [0, 2, 0, 64], [1, 33, 0, 5, 0, 0, 1, 70]], ids=str)
 @pytest.mark.parametrize("fin,fout", [(520, 136), (1032, 264), (2049, 200), (4096, 128)])
 def test_few_tiles_with_a_long_contracted_dimension(fin, fout, counts, order):
     check(counts, fin, fout, "bf16", order)
+
+
+@pytest.mark.parametrize("order", ["in_out", "out_in"])
+@pytest.mark.parametrize("fin,fout", [(200, 4744), (1032, 9608), (64, 70)])
+def test_sixteen_rows_at_most_over_wide_results(fin, fout, order):
+    check([9, 0, 7], fin, fout, "bf16", order)
+    check([16], fin, fout, "f16", order)
 
 
 @pytest.mark.parametrize("order", ["in_out", "out_in"])
