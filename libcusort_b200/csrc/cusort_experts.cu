@@ -68,8 +68,6 @@ using namespace cusort_b200;
 
 constexpr int kThreads = 320;  // warps 0, 2, 8 and 9 bring operands, 1 multiplies, 3 clears rows, 4 to 7 store
 constexpr int kSms = 148;
-constexpr int kBlockK = 64;              // contracted elements to a stage: one swizzle row
-constexpr int kTileM = 128;              // lanes of a CTA's tensor memory
 constexpr uint32_t kBoxBytes = kBlockK * dev::kBoxRowBytes;  // 64 rows of 64 elements
 constexpr uint32_t kAll = 0xffffffffu;
 
@@ -190,21 +188,10 @@ struct ProductArgs {
   int64_t skip;       // for tests: every CTA's step that is never brought; -1: none
 };
 
-// PAIR: tiles of 256 columns of the result, 128 in each of two CTAs, and half of the rows in each.  COLUMNS: 128, or 64
-// (not by pairs): the other 64 lanes of tensor memory get products of what lies behind in shared memory, and nobody
-// looks at them.
-template <int BN, int COLUMNS, int STAGES, int SUB, bool PAIR> struct ProductShape {
-  static constexpr int kCtas = PAIR ? 2 : 1, kTile = COLUMNS * kCtas;
-  static constexpr uint32_t kBytesA = COLUMNS * kBlockK * 2;
-  static constexpr int kRowStep = 16 * kCtas;       // the instruction's width comes in such steps
-  // A stage holds SUB steps of kBlockK, each the weights' part and then the rows'.
-  static constexpr uint32_t kBytesB = BN / kCtas * kBlockK * 2, kStep = kBytesA + kBytesB, kStage = SUB * kStep;
-  static constexpr uint32_t kColumns = 2 * BN;
-  static constexpr uint32_t kStaging = 4 * 2048;  // 32 x 32 16-bit elements for each storing warp
-  static size_t bytes(int experts) {
-    return 1024 + STAGES * kStage + kStaging + sizeof(Pipe<STAGES, PAIR>) + 4 * (3 * (size_t)experts + 1);
-  }
-};
+template <typename Shape> size_t product_bytes(int experts) {
+  return 1024 + Shape::kStages * Shape::kStage + Shape::kStaging + sizeof(Pipe<Shape::kStages, Shape::kPair>) +
+         4 * (3 * (size_t)experts + 1);
+}
 
 struct ProductTile {
   int expert, row, rows, column;  // first row and number of rows; first column of the result
@@ -247,11 +234,11 @@ __device__ __forceinline__ ProductTile product_tile(const ProductArgs& a, const 
 // 17.3, 14.7, 12.6; 4.2 us are there without any contraction).  Splitting the contraction over clusters of two or three CTAs
 // took as long or longer (11.4 us for the first): their barriers and the
 // joining cost what the shorter loops gained.
-template <typename T, int BN, int COLUMNS, int STAGES, int SUB, bool PAIR, bool IN_ORDER>
+template <typename T, typename Shape, bool IN_ORDER>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
-  using Shape = ProductShape<BN, COLUMNS, STAGES, SUB, PAIR>;
+  constexpr int BN = Shape::kRows, COLUMNS = Shape::kWeightColumns, STAGES = Shape::kStages, SUB = Shape::kSub;
+  constexpr bool PAIR = Shape::kPair;
   constexpr uint32_t kBytesA = Shape::kBytesA;
-  static_assert(COLUMNS == 128 || (COLUMNS == 64 && !PAIR), "");
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (align_up(dev::smem_u32(raw), 1024) - dev::smem_u32(raw));
   uint8_t* staging = base + STAGES * Shape::kStage;
@@ -329,7 +316,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, !IN_ORDER, false,
                                                           kTileM * Shape::kCtas, align_up(tile.rows, Shape::kRowStep));
-        const uint32_t sum = p.tmem + sums.stage * BN;
+        const uint32_t sum = p.tmem + sums.stage * Shape::kSumColumns;
         dev::wait_for<PAIR>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
         dev::tmem_fence_after();
         for (int k = 0; k < steps; ++k, ring.next()) {
@@ -363,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       const int column = tile.column + rank * kTileM + quarter * 32;
       for (int c = 0; c < tile.rows && quarter * 32 < COLUMNS; c += 32) {
         uint32_t v[32];
-        dev::tmem_load32(p.tmem + sums.stage * BN + c + ((uint32_t)quarter << 21), v);
+        dev::tmem_load32(p.tmem + sums.stage * Shape::kSumColumns + c + ((uint32_t)quarter << 21), v);
         dev::tmem_load_wait(v);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
@@ -790,26 +777,19 @@ cudaError_t run(Kernel kernel, const Args& a, int64_t tiles, int ctas, size_t sm
   return launch_after_previous(kernel, grid, kThreads, smem, a, stream, ctas);
 }
 
-template <typename T, int BN, int COLUMNS, int STAGES, int SUB, bool PAIR>
+template <typename T, typename Shape>
 cudaError_t product(ProductArgs& a, Operand weights, Operand rows, bool in_order, int64_t row_tiles,
                     cudaStream_t stream) {
-  using Shape = ProductShape<BN, COLUMNS, STAGES, SUB, PAIR>;
   a.width_tiles = (a.width + Shape::kTile - 1) / Shape::kTile;
   a.most = (uint32_t)row_tiles;
-  cudaError_t e = weights.map(&a.weights, false, in_order ? COLUMNS : kBlockK);
+  cudaError_t e = weights.map(&a.weights, false, in_order ? Shape::kWeightColumns : kBlockK);
   for (int i = 0; !e && i < 3; ++i) e = rows.map(&a.rows[i], true, 64 >> i);
   if (e) return e;
-  const size_t smem = Shape::bytes(a.segments.experts);
+  const size_t smem = product_bytes<Shape>(a.segments.experts);
   const int64_t tiles = row_tiles * a.width_tiles;
-  return in_order ? run(product_kernel<T, BN, COLUMNS, STAGES, SUB, PAIR, true>, a, tiles, Shape::kCtas, smem, stream)
-                  : run(product_kernel<T, BN, COLUMNS, STAGES, SUB, PAIR, false>, a, tiles, Shape::kCtas, smem, stream);
+  return in_order ? run(product_kernel<T, Shape, true>, a, tiles, Shape::kCtas, smem, stream)
+                  : run(product_kernel<T, Shape, false>, a, tiles, Shape::kCtas, smem, stream);
 }
-
-// Rows of a tile where no expert can have more, where experts have few on
-// average, and where they have many (by pairs of CTAs).  64 experts, 2048 ->
-// 1536, by the second and the third: 8 rows each 65 and 69 us, 64 71 and 75, 80
-// 84 and 76, 128 89 and 80.
-constexpr int kFewestRows = 16, kFewRows = 64, kManyRows = 256;
 
 // Tiles begin before this many rows and end within 32 bits.
 constexpr int64_t kMaxRows = INT32_MAX - 1024;
@@ -871,10 +851,10 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
     using T = decltype(t);
     if (capacity <= kFewestRows)
       return tiles * ((out + kTileM - 1) / kTileM) <= kSms / 2
-                 ? product<T, kFewestRows, 64, 9, 2, false>(a, weights, rows, in_order, tiles, stream)
-                 : product<T, kFewestRows, 128, 5, 2, false>(a, weights, rows, in_order, tiles, stream);
-    return few ? product<T, kFewRows, 128, 4, 2, false>(a, weights, rows, in_order, tiles, stream)
-               : product<T, kManyRows, 128, 6, 1, true>(a, weights, rows, in_order, tiles, stream);
+                 ? product<T, ProductFewestNarrow>(a, weights, rows, in_order, tiles, stream)
+                 : product<T, ProductFewest>(a, weights, rows, in_order, tiles, stream);
+    return few ? product<T, ProductFew>(a, weights, rows, in_order, tiles, stream)
+               : product<T, ProductMany>(a, weights, rows, in_order, tiles, stream);
   };
   return type == CUSORT_FLOAT_F16 ? go(__half{}) : go(__nv_bfloat16{});
 }

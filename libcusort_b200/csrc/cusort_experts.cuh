@@ -9,6 +9,41 @@ namespace cusort_b200 {
 
 constexpr int kMaxExperts = 1024;
 
+// The products of 16-bit operands.
+constexpr int kBlockK = 64;   // contracted elements to a step: one swizzle row
+constexpr int kTileM = 128;   // lanes of a CTA's tensor memory
+constexpr int kSumLoad = 32;  // columns of a sum that a warp reads at a time
+
+// PAIR: tiles of 256 columns of the result, 128 in each of two CTAs, and half of the rows in each.  COLUMNS: 128, or 64
+// (not by pairs): the other 64 lanes of tensor memory get products of what lies behind in shared memory, and nobody
+// looks at them.
+template <int BN, int COLUMNS, int STAGES, int SUB, bool PAIR> struct ProductShape {
+  static_assert(COLUMNS == 128 || (COLUMNS == 64 && !PAIR), "");
+  static constexpr int kRows = BN, kWeightColumns = COLUMNS, kStages = STAGES, kSub = SUB;
+  static constexpr bool kPair = PAIR;
+  static constexpr int kCtas = PAIR ? 2 : 1, kTile = COLUMNS * kCtas;
+  static constexpr uint32_t kBytesA = COLUMNS * kBlockK * 2;
+  static constexpr int kRowStep = 16 * kCtas;       // the instruction's width comes in such steps
+  // A stage holds SUB steps of kBlockK, each the weights' part and then the rows'.
+  static constexpr uint32_t kBytesB = BN / kCtas * kBlockK * 2, kStep = kBytesA + kBytesB, kStage = SUB * kStep;
+  // Each of the two sums has the columns that are read of it, which in the form for the fewest rows are more than it has
+  // rows: one that is read has no columns of the other, which grows meanwhile, nor any that were not allocated.
+  static constexpr uint32_t kSumColumns = (BN + kSumLoad - 1) / kSumLoad * kSumLoad, kColumns = 2 * kSumColumns;
+  static constexpr uint32_t kStaging = 4 * 2048;  // 32 x 32 16-bit elements for each storing warp
+};
+
+// Rows of a tile where no expert can have more, where experts have few on
+// average, and where they have many (by pairs of CTAs).  64 experts, 2048 ->
+// 1536, by the second and the third: 8 rows each 65 and 69 us, 64 71 and 75, 80
+// 84 and 76, 128 89 and 80.  The rule goes by averages, since the counts stay
+// on the device, and these are of experts with equal counts: a batch whose rows
+// nearly all go to one expert takes tiles that are smaller than they could be.
+constexpr int kFewestRows = 16, kFewRows = 64, kManyRows = 256;
+using ProductFewestNarrow = ProductShape<kFewestRows, 64, 9, 2, false>;
+using ProductFewest = ProductShape<kFewestRows, 128, 5, 2, false>;
+using ProductFew = ProductShape<kFewRows, 128, 4, 2, false>;
+using ProductMany = ProductShape<kManyRows, 128, 6, 1, true>;
+
 // Expert segments as the CTA keeps them in shared memory.
 struct Segments {
   int32_t* first;  // [experts] rows: clamped into [0, capacity]
