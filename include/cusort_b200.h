@@ -428,7 +428,8 @@ cudaError_t cusort_page_plan(const int32_t* d_cached_lens, const int32_t* d_new_
  * place: the *_out arrays are other memory than the inputs, so a call can be
  * made again; its caller goes on with the results.  Entries of tables outside
  * [0, num_blocks) are kept and counted nowhere.  num_requests, num_children <=
- * 16384, block_size <= 2^20, num_blocks <= 2^30.  Two-phase temp protocol.
+ * 16384, block_size <= 2^20, table_width, num_blocks <= 2^30.  Two-phase temp
+ * protocol.
  *
  * Requests that go on from others' (parallel samples, beams): child r takes
  * over from request d_parents[r]; outside [0, num_requests) it is empty.  All

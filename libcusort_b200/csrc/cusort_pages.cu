@@ -14,6 +14,7 @@ namespace {
 using namespace cusort_b200;
 
 constexpr int kMaxRequests = 16384;
+constexpr int kMaxWidth = 1 << 30;  // entries of a table: for_rows numbers them, and some behind the last, in 32 bits
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kSms = 148;
@@ -492,7 +493,8 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
 
 bool pool_ok(int num_requests, int block_size, int64_t table_stride, int table_width, int num_blocks) {
   return num_requests >= 0 && num_requests <= kMaxRequests && block_size >= 1 && block_size <= (1 << 20) &&
-         table_width >= 0 && table_stride >= table_width && num_blocks >= 0 && num_blocks <= (1 << 30);
+         table_width >= 0 && table_width <= kMaxWidth && table_stride >= table_width && num_blocks >= 0 &&
+         num_blocks <= (1 << 30);
 }
 
 // The two-phase protocol's answer: true where the call ends with *e.

@@ -572,7 +572,7 @@ void check_tables(const at::Tensor& tables, const at::Tensor& lens) {
            name_of(tables.scalar_type()), ", ", shape_of(tables), ", ", tables.device(), ")");
   if (tables.size(0) > 1 && tables.numel() > 0 && tables.stride(0) < tables.size(1))
     refuse(PyExc_ValueError, "block_tables' rows must not overlap (strides ", tables.strides(), ")");
-  if (tables.size(1) > INT32_MAX) refuse(PyExc_ValueError, "block_tables must be at most 2^31 - 1 blocks wide");
+  if (tables.size(1) > 1 << 30) refuse(PyExc_ValueError, "block_tables must be at most 2^30 blocks wide");
 }
 
 void check_block_size(int64_t block) {
