@@ -371,6 +371,7 @@ cudaError_t cusort_combine_rows_backward(cusort_float_type type, const void* d_g
  * the other way round it is the gradient of the rows.
  * Segments beyond the capacity are cut there; they must not overlap.
  * 1 <= in, out <= 2^20, capacity < 2^31 - 1024, num_experts <= 1024.
+ * Operands lie at multiples of their elements' size.
  * Two-phase temp protocol, with the same arguments in both calls: 16-bit
  * operands whose addresses or strides are no multiples of 16 bytes are laid
  * out anew there (at a 16-byte boundary), others need none. */

@@ -799,6 +799,12 @@ bool sizes_fit(int64_t capacity, int64_t in, int64_t out, int experts) {
          experts >= 1 && experts <= kMaxExperts;
 }
 
+// Whether elements of the type can be loaded from these addresses.
+bool on_elements(cusort_float_type type, const void* x, const void* y) {
+  return ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & (uintptr_t)(float_type_bytes(type) - 1)) ==
+         0;
+}
+
 }  // namespace
 
 extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp_storage_bytes, cusort_float_type type,
@@ -808,7 +814,7 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
                                               int64_t capacity, int64_t in, int64_t out, int num_experts,
                                               cudaStream_t stream) {
   if (temp_storage_bytes == nullptr || float_type_bytes(type) == 0 || !sizes_fit(capacity, in, out, num_experts) ||
-      row_stride < 0 || expert_stride < 0 || in_stride < 0 || out_stride < 0)
+      row_stride < 0 || expert_stride < 0 || in_stride < 0 || out_stride < 0 || !on_elements(type, d_rows, d_weights))
     return cudaErrorInvalidValue;
   const bool in_order = !(out_stride == 1 || out == 1);
   if (in_order && in_stride != 1 && in != 1) return cudaErrorInvalidValue;
@@ -865,7 +871,7 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
     void* d_grad_weights, int in_contiguous, int64_t capacity, int64_t in, int64_t out, int num_experts,
     cudaStream_t stream) {
   if (temp_storage_bytes == nullptr || float_type_bytes(type) == 0 || !sizes_fit(capacity, in, out, num_experts) ||
-      row_stride < 0 || grad_stride < 0)
+      row_stride < 0 || grad_stride < 0 || !on_elements(type, d_rows, d_grad_out))
     return cudaErrorInvalidValue;
   Operand slow{d_rows, 1, capacity, in, 0, row_stride}, fast{d_grad_out, 1, capacity, out, 0, grad_stride};
   if (in_contiguous) std::swap(slow, fast);
