@@ -148,21 +148,56 @@ __device__ __forceinline__ void clear(uint16_t* x, int64_t begin, int64_t end, i
   if (head + words * 8 + thread < end) x[head + words * 8 + thread] = 0;
 }
 
-// One warp's part in clearing the rows that belong to no segment (16-bit
-// elements, `width` to a row; warp `me` of `all`): those between the segments
-// by the expert before, those behind the last in equal parts.
+// Where rows of no segment that begin at row r end, by experts e0, e0 + step and so on: at the segment that begins next,
+// the capacity where none does, r itself where a segment covers it.
+__host__ __device__ inline int no_segment_until(const Segments& s, int experts, int capacity, int r, int e0, int step) {
+  int until = capacity;
+  for (int e = e0; e < experts; e += step)
+    if (s.count[e] > 0 && s.first[e] + s.count[e] > r) {
+      const int begin = s.first[e] > r ? s.first[e] : r;
+      until = begin < until ? begin : until;
+    }
+  return until;
+}
+// Where the last segment ends, by the same experts.
+__host__ __device__ inline int segments_end(const Segments& s, int experts, int e0, int step) {
+  int end = 0;
+  for (int e = e0; e < experts; e += step)
+    if (s.count[e] > 0 && s.first[e] + s.count[e] > end) end = s.first[e] + s.count[e];
+  return end;
+}
+
+// f(begin, end) for part `me` of `all` of the rows that belong to no segment:
+// those behind a segment by its expert, whatever the segments' order, those
+// behind the last one in equal parts.  Each of the lanes of a warp looks at its
+// share of the experts for what comes next.
+#pragma nv_exec_check_disable
+template <typename Lanes, typename F>
+__host__ __device__ inline void other_rows(const Segments& s, int experts, int capacity, int me, int all,
+                                           const Lanes& lanes, F&& f) {
+  const int end = lanes.highest(segments_end(s, experts, lanes.lane, lanes.count));
+  for (int e = me; e <= experts; e += all) {  // the last: before the first segment
+    if (e < experts && s.count[e] == 0) continue;
+    const int r = e < experts ? s.first[e] + s.count[e] : 0;
+    if (r < end) f(r, lanes.lowest(no_segment_until(s, experts, capacity, r, lanes.lane, lanes.count)));
+  }
+  const int left = capacity - end, per = (left + all - 1) / all;
+  const int64_t part = (int64_t)me * per;
+  if (part < left) f((int)(end + part), (int)(part + per < left ? end + part + per : capacity));
+}
+
+struct WarpLanes {
+  int lane, count = 32;
+  __device__ __forceinline__ int highest(int v) const { return __reduce_max_sync(0xffffffffu, v); }
+  __device__ __forceinline__ int lowest(int v) const { return __reduce_min_sync(0xffffffffu, v); }
+};
+
+// One warp's part in clearing the rows that belong to no segment (16-bit elements, `width` to a row; warp `me` of `all`).
 __device__ __forceinline__ void clear_other_rows(uint16_t* out, int64_t width, const SegmentArgs& a, const Segments& s,
                                                  int me, int all) {
-  const int lane = threadIdx.x & 31;
-  for (int e = me; e < a.experts; e += all) {
-    const int end = s.first[e] + s.count[e];
-    if (e + 1 < a.experts) clear(out, end * width, s.first[e + 1] * width, lane, 32);
-    if (e == 0) clear(out, 0, s.first[0] * width, lane, 32);
-  }
-  const int end = s.first[a.experts - 1] + s.count[a.experts - 1], left = a.capacity - end;
-  const int per = (left + all - 1) / all;
-  const int64_t r0 = end + min((int64_t)left, (int64_t)me * per);
-  clear(out, r0 * width, min(r0 + per, (int64_t)a.capacity) * width, lane, 32);
+  const WarpLanes lanes{(int)(threadIdx.x & 31)};
+  other_rows(s, a.experts, a.capacity, me, all, lanes,
+             [&](int begin, int end) { clear(out, begin * width, end * width, lanes.lane, 32); });
 }
 
 // The products of 32-bit operands (cusort_experts_f32.cu).

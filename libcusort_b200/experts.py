@@ -30,7 +30,8 @@ MAX_WIDTH = 1 << 20
 def expert_products(rows: torch.Tensor, weights: torch.Tensor, counts: torch.Tensor,
                     offsets: torch.Tensor) -> torch.Tensor:
     """out[r] = rows[r] @ weights[e] for the rows r of expert e's segment, ``offsets[e] <= r <
-    offsets[e] + counts[e]`` (int32, as ``plan_dispatch`` gives them), zeros for all others.
+    offsets[e] + counts[e]`` (int32, as ``plan_dispatch`` gives them; the segments may come in any order, but
+    must not overlap), zeros for all others.
 
     ``rows`` [capacity, in] (rows any distance apart) and ``weights`` [experts, in, out] (contiguous
     along either of the last two dimensions, so that linear layers' [experts, out, in] go in as

@@ -1,0 +1,65 @@
+// Which rows of the experts' products are cleared: those of no segment, each
+// once or more, and none of a segment, whatever the segments' order.  Built and
+// run by tests/test_experts_shapes.py (no GPU needed).  Prints "ok".
+#include <algorithm>
+#include <cstdint>
+#include <cstdio>
+#include <random>
+#include <vector>
+
+#include "cusort_experts.cuh"
+
+using namespace cusort_b200;
+
+struct OneLane {
+  int lane = 0, count = 1;
+  int highest(int v) const { return v; }
+  int lowest(int v) const { return v; }
+};
+
+static int bad = 0;
+
+// A plan of segments that do not overlap: shuffled experts, gaps between them, rows behind; empty experts anywhere.
+static void check(int experts, int most, int gap, int all, bool shuffled, unsigned seed) {
+  std::mt19937 rng(seed);
+  std::vector<int> order(experts), first(experts), count(experts);
+  for (int e = 0; e < experts; ++e) order[e] = e;
+  if (shuffled) std::shuffle(order.begin(), order.end(), rng);
+  int at = gap ? rng() % (gap + 1) : 0;
+  for (int e : order) {
+    count[e] = rng() % 3 ? rng() % (most + 1) : 0;
+    first[e] = at;
+    at += count[e] + (gap ? rng() % (gap + 1) : 0);
+  }
+  for (int e : order)
+    if (count[e] == 0 && shuffled) first[e] = rng() % (at + 1);
+  const int capacity = at;
+  std::vector<int> cleared(capacity, 0);
+  const Segments s{first.data(), count.data(), nullptr};
+  for (int me = 0; me < all; ++me)
+    other_rows(s, experts, capacity, me, all, OneLane(), [&](int begin, int end) {
+      if (begin < 0 || begin > end || end > capacity) {
+        ++bad;
+        std::printf("rows %d to %d of %d\n", begin, end, capacity);
+        return;
+      }
+      for (int r = begin; r < end; ++r) ++cleared[r];
+    });
+  std::vector<int> there(capacity, 0);
+  for (int e = 0; e < experts; ++e)
+    for (int r = first[e]; r < first[e] + count[e]; ++r) ++there[r];
+  for (int r = 0; r < capacity; ++r)
+    if ((cleared[r] > 0) != (there[r] == 0)) {
+      if (++bad < 20)
+        std::printf("%d experts, seed %u: row %d is %s\n", experts, seed, r, there[r] ? "cleared" : "left");
+    }
+}
+
+int main() {
+  for (unsigned seed = 0; seed < 40; ++seed)
+    for (int experts : {1, 2, 7, 64, 300})
+      for (int gap : {0, 5})
+        for (int all : {1, 6, 148, 1184}) check(experts, 9, gap, all, seed % 4 != 0, seed);
+  if (bad == 0) std::printf("ok\n");
+  return bad != 0;
+}
