@@ -181,8 +181,7 @@ __host__ __device__ inline void other_rows(const Segments& s, int experts, int c
     const int r = e < experts ? s.first[e] + s.count[e] : 0;
     if (r < end) f(r, lanes.lowest(no_segment_until(s, experts, capacity, r, lanes.lane, lanes.count)));
   }
-  const int left = capacity - end, per = (left + all - 1) / all;
-  const int64_t part = (int64_t)me * per;
+  const int64_t left = capacity - end, per = (left + all - 1) / all, part = me * per;
   if (part < left) f((int)(end + part), (int)(part + per < left ? end + part + per : capacity));
 }
 

@@ -55,7 +55,28 @@ static void check(int experts, int most, int gap, int all, bool shuffled, unsign
     }
 }
 
+// As many rows as there may be, of which the first ones belong to an expert: the parts begin and end where they should.
+static void check_most(int capacity, int taken, int all) {
+  int first = 0, count = taken;
+  const Segments s{&first, &count, nullptr};
+  int64_t next = taken;
+  for (int me = 0; me < all; ++me)
+    other_rows(s, 1, capacity, me, all, OneLane(), [&](int begin, int end) {
+      if (begin == end) return;  // before a segment that begins at row 0
+      if (begin != next || end < begin || end > capacity) {
+        ++bad;
+        std::printf("part %d of %d: rows %d to %d of %d, %lld come next\n", me, all, begin, end, capacity,
+                    (long long)next);
+      }
+      next = end;
+    });
+  if (next != capacity) ++bad, std::printf("%lld of %d rows\n", (long long)next, capacity);
+}
+
 int main() {
+  for (int capacity : {INT32_MAX - 1024, INT32_MAX - 1500, INT32_MAX - 5000})
+    for (int taken : {0, 1, 700})
+      for (int all : {1, 148, 2368, 4736}) check_most(capacity, taken, all);
   for (unsigned seed = 0; seed < 40; ++seed)
     for (int experts : {1, 2, 7, 64, 300})
       for (int gap : {0, 5})
