@@ -369,8 +369,8 @@ cudaError_t cusort_combine_rows_backward(cusort_float_type type, const void* d_g
  * + i * in_stride + o * out_stride, one of the last two strides 1; d_out:
  * capacity x out, contiguous, on a 16-byte boundary.  With weights and widths
  * the other way round it is the gradient of the rows.
- * Segments beyond the capacity are cut there; they may come in any order, but
- * must not overlap.
+ * Segments are cut to the rows there are; they may come in any order, but must
+ * not overlap.
  * 1 <= in, out <= 2^20, capacity < 2^31 - 1024, num_experts <= 1024.
  * Operands lie at multiples of their elements' size.
  * Two-phase temp protocol, with the same arguments in both calls: 16-bit

@@ -57,9 +57,10 @@ struct SegmentArgs {
 };
 
 // First row and number of rows of an expert's segment, within the rows there are.
-__device__ __forceinline__ int2 segment(const SegmentArgs& a, int e) {
-  const int first = min(max(a.offsets[e], 0), a.capacity);
-  return make_int2(first, min(max(a.counts[e], 0), a.capacity - first));
+__host__ __device__ inline int2 segment(const SegmentArgs& a, int e) {
+  const int offset = a.offsets[e], first = min(max(offset, 0), a.capacity);
+  const int64_t end = min((int64_t)offset + a.counts[e], (int64_t)a.capacity);
+  return make_int2(first, (int)max(end - first, (int64_t)0));
 }
 
 // Sums of tiles stop at 2^30, more than there are of any plan's.

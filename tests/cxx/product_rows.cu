@@ -1,6 +1,6 @@
 // Which rows of the experts' products are cleared: those of no segment, each
-// once or more, and none of a segment, whatever the segments' order.  Built and
-// run by tests/test_experts_shapes.py (no GPU needed).  Prints "ok".
+// once or more, and none of a segment, whatever the segments' order; and which
+// rows a segment has.  Built and run by tests/test_experts_shapes.py (no GPU needed).  Prints "ok".
 #include <algorithm>
 #include <cstdint>
 #include <cstdio>
@@ -73,7 +73,23 @@ static void check_most(int capacity, int taken, int all) {
   if (next != capacity) ++bad, std::printf("%lld of %d rows\n", (long long)next, capacity);
 }
 
+// The rows r with offset <= r < offset + count, of those there are.
+static void check_segment(int offset, int count, int capacity) {
+  const SegmentArgs a{&count, &offset, 1, capacity};
+  const int2 got = segment(a, 0);
+  const int64_t begin = std::max<int64_t>(offset, 0), end = std::min<int64_t>((int64_t)offset + count, capacity);
+  const int64_t rows = std::max<int64_t>(end - begin, 0);
+  if (got.y != rows || (rows > 0 && got.x != begin) || got.x < 0 || got.x > capacity) {
+    ++bad;
+    std::printf("offset %d, count %d of %d rows: %d from %d on\n", offset, count, capacity, got.y, got.x);
+  }
+}
+
 int main() {
+  for (int capacity : {1, 40, INT32_MAX - 1025})
+    for (int offset : {0, 1, 39, 40, 41, -1, -5, -100, INT32_MAX, INT32_MIN, -INT32_MAX})
+      for (int count : {0, 1, 5, 6, 40, 41, 140, 1 << 30, INT32_MAX, -1, INT32_MIN})
+        check_segment(offset, count, capacity);
   for (int capacity : {INT32_MAX - 1024, INT32_MAX - 1500, INT32_MAX - 5000})
     for (int taken : {0, 1, 700})
       for (int all : {1, 148, 2368, 4736}) check_most(capacity, taken, all);

@@ -66,6 +66,13 @@ def test_segments_in_any_order(first, count, capacity, order, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_segments_that_begin_before_the_rows(dtype):
+    """Only the rows that there are: of ten from -4 on the first six."""
+    check([-4, 6, -30, 90], [10, 20, 25, 1 << 30], 100, 72, 136, dtype)
+    check([-2 ** 31, -1], [2 ** 31 - 1, 8], 300, 72, 40, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("most", [3, 40])
 def test_many_experts_in_any_order(most, dtype):
     gen = torch.Generator().manual_seed(most)
