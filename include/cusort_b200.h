@@ -394,8 +394,8 @@ cudaError_t cusort_expert_products_grad_weights(void* d_temp_storage, size_t* te
                                                 cudaStream_t stream);
 
 /* Whether a wait inside one of these products ran out on the current device
- * since the last call (cusort_set_wait_limit_ns): 0, or 1 and their results
- * are not to be used.  Synchronises `stream`. */
+ * since the last call (cusort_set_wait_limit_ns): 0, or 1 and what the wait
+ * has cost is NaN in their results.  Synchronises `stream`. */
 cudaError_t cusort_read_product_status(uint32_t* status, cudaStream_t stream);
 
 /* Placement of one serving step in a paged cache of blocks of block_size

@@ -161,6 +161,17 @@ __device__ __forceinline__ void settle(const dev::WaitLimit& limit) {
   while (dev::globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
 }
 
+// What stands in the results in the place of sums that a wait in vain has cost: NaN.  A role whose wait ran out stops
+// there, so that nobody takes a barrier's phase for another one: stages that are not multiplied any more, sums that are
+// not handed on.  Those who wait for them run out in turn, at once in this CTA, after their own limit in the other of a
+// pair; the storing warps go on to the end.
+constexpr uint32_t kLost = 0x7fffffffu;
+
+__device__ __forceinline__ void fill(uint32_t (&v)[32], uint32_t value) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = value;
+}
+
 // A wait of a whole warp, by one lane: 32 of them keep shared memory busy.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const dev::WaitLimit& limit) {
   bool ok = true;
@@ -266,14 +277,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       Ring<STAGES> ring;
       uint32_t turn = (warp == 2 || warp == 9);  // whether it takes the odd steps
       int64_t step_of_cta = -1;
-      for (uint32_t t = t0; t < tiles; t += t_step) {
+      bool lost = false;
+      for (uint32_t t = t0; t < tiles && !lost; t += t_step) {
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const int column = tile.column + rank * kTileM;
         const int mine = align_up(tile.rows, Shape::kRowStep) / Shape::kCtas, row = tile.row + rank * mine;
         const uint32_t bytes = SUB * Shape::kCtas * (kBytesA + mine * dev::kBoxRowBytes);
         for (int k = 0; k < steps; ++k, ring.next()) {
           ++step_of_cta;
-          if ((turn ^= 1) == 0 || !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
+          if ((turn ^= 1) == 0) continue;
+          if ((lost = !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit))) break;
           if (step_of_cta == a.skip) continue;
           const uint32_t to = stages + ring.stage * Shape::kStage, own = at.full(ring.stage);
           const uint32_t bar = PAIR ? dev::in_first(own) : own;
@@ -312,15 +325,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       Ring<2> sums;
       const uint64_t first_a = dev::operand_descriptor(stages, IN_ORDER ? 16 : kBoxBytes, 1024);
       const uint64_t first_b = dev::operand_descriptor(stages + kBytesA, 16, 1024);
-      for (uint32_t t = t0; t < tiles; t += t_step, sums.next()) {
+      bool lost = false;
+      for (uint32_t t = t0; t < tiles && !lost; t += t_step, sums.next()) {
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, !IN_ORDER, false,
                                                           kTileM * Shape::kCtas, align_up(tile.rows, Shape::kRowStep));
         const uint32_t sum = p.tmem + sums.stage * Shape::kSumColumns;
-        dev::wait_for<PAIR>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
+        lost = !dev::wait_for<PAIR>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
         dev::tmem_fence_after();
-        for (int k = 0; k < steps; ++k, ring.next()) {
-          if (!dev::wait_for(at.full(ring.stage), ring.parity, limit)) continue;
+        for (int k = 0; k < steps && !lost; ++k, ring.next()) {
+          if ((lost = !dev::wait_for(at.full(ring.stage), ring.parity, limit))) break;
           dev::tmem_fence_after();
           const uint32_t stage = ring.stage * (Shape::kStage / 16);
 #pragma unroll
@@ -331,8 +345,9 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
                                    first_b + stage + (u * Shape::kStep + i * 32) / 16, instruction, k + u + i > 0);
           dev::mma_commit<PAIR>(at.empty(ring.stage));
         }
-        dev::mma_commit<PAIR>(at.sum_full(sums.stage));
+        if (!lost) dev::mma_commit<PAIR>(at.sum_full(sums.stage));
       }
+      settle(limit);
     }
   } else if (warp == 3) {
     clear_other_rows(static_cast<uint16_t*>(a.out), a.width, a.segments, s, blockIdx.x, gridDim.x);
@@ -343,15 +358,20 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
     uint8_t* mine = staging + quarter * 2048;
     T* out = static_cast<T*>(a.out);
     const bool whole = a.width % 8 == 0;  // the result's first byte lies on a 16-byte boundary
+    bool lost = false;
     for (uint32_t t = t0; t < tiles; t += t_step, sums.next()) {
       const ProductTile tile = product_tile<Shape>(a, s, t);
-      if (!warp_wait(at.sum_full(sums.stage), sums.parity, limit)) continue;
+      lost = lost || !warp_wait(at.sum_full(sums.stage), sums.parity, limit);
       dev::tmem_fence_after();
       const int column = tile.column + rank * kTileM + quarter * 32;
       for (int c = 0; c < tile.rows && quarter * 32 < COLUMNS; c += 32) {
         uint32_t v[32];
-        dev::tmem_load32(p.tmem + sums.stage * Shape::kSumColumns + c + ((uint32_t)quarter << 21), v);
-        dev::tmem_load_wait(v);
+        if (lost) {
+          fill(v, kLost);
+        } else {
+          dev::tmem_load32(p.tmem + sums.stage * Shape::kSumColumns + c + ((uint32_t)quarter << 21), v);
+          dev::tmem_load_wait(v);
+        }
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const uint32_t both = dev::from_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), T{});
@@ -385,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       }
       dev::tmem_fence_before();
       __syncwarp();
-      if (lane == 0) at.release_sum(sums.stage);
+      if (lane == 0 && !lost) at.release_sum(sums.stage);
     }
   }
   __syncwarp();
@@ -476,14 +496,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       Ring<kEnds> end;
       uint32_t turn = (warp == 2 || warp == 9);  // whether it takes the odd steps
       int64_t step_of_cta = -1;
-      for (uint32_t t = t0; t < tiles; t += t_step) {
+      bool lost = false;
+      for (uint32_t t = t0; t < tiles && !lost; t += t_step) {
         const GradTile g = grad_tile(a, segments, t);
         const int slow = g.slow + rank * kTileM, fast = g.fast + rank * g.chunks * kBlockK;
         const uint32_t bytes = (2 + g.chunks) * kChunkBytes;
         const int steps = g.steps();
         if (g.end()) {
           // ahead of the steps, into a buffer of its own, so that it is there and cleared when they are done
-          if ((warp == 2 || warp == 9) && dev::wait_for(at.end_empty(end.stage), end.parity ^ 1, limit)) {
+          if (warp == 2 || warp == 9) {
+            if ((lost = !dev::wait_for(at.end_empty(end.stage), end.parity ^ 1, limit))) break;
             const uint32_t to = dev::smem_u32(ends) + end.stage * kEndBytes, bar = at.end_full(end.stage);
             const int row = g.segment.x + g.whole();
             if (warp < 8) {
@@ -499,7 +521,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int k = 0; k < steps; ++k, ring.next()) {
           ++step_of_cta;
-          if ((turn ^= 1) == 0 || !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit)) continue;
+          if ((turn ^= 1) == 0) continue;
+          if ((lost = !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit))) break;
           if (step_of_cta == a.skip) continue;
           const uint32_t to = stages + ring.stage * kGradStage, bar = dev::in_first(at.full(ring.stage));
           const int row = g.segment.x + k * kBlockK;
@@ -524,16 +547,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       Ring<kEnds> end;
       const uint64_t end_a = dev::operand_descriptor(dev::smem_u32(ends), kEndChunk, 1024);
       const uint64_t end_b = dev::operand_descriptor(dev::smem_u32(ends) + 2 * kEndChunk, kEndChunk, 1024);
-      for (uint32_t t = t0; t < tiles; t += t_step) {
+      bool lost = false;
+      for (uint32_t t = t0; t < tiles && !lost; t += t_step) {
         const GradTile g = grad_tile(a, segments, t);
         if (g.segment.y == 0) continue;
         const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, true, true, 2 * kTileM,
                                                           2 * g.chunks * kBlockK);
         const uint32_t sum = p.tmem + sums.stage * kGradN;
         const int whole = g.whole(), steps = g.steps();
-        dev::wait_for<true>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
-        for (int k = 0; k < steps; ++k, ring.next()) {
-          if (!dev::wait_for(at.full(ring.stage), ring.parity, limit)) continue;
+        lost = !dev::wait_for<true>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
+        for (int k = 0; k < steps && !lost; ++k, ring.next()) {
+          if ((lost = !dev::wait_for(at.full(ring.stage), ring.parity, limit))) break;
           dev::tmem_fence_after();
           const uint32_t stage = ring.stage * (kGradStage / 16);
           const int depth = min(kBlockK, whole - k * kBlockK) / 16;
@@ -544,8 +568,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    k + i > 0);
           dev::mma_commit<true>(at.empty(ring.stage));
         }
-        if (g.end()) {
-          if (dev::wait_for<true>(at.end_cleared(end.stage), end.parity, limit)) {
+        if (g.end() && !lost) {
+          lost = !dev::wait_for<true>(at.end_cleared(end.stage), end.parity, limit);
+          if (!lost) {
             dev::tmem_fence_after();
             const uint32_t buffer = end.stage * (kEndBytes / 16);
             dev::mma_issue<true>(sum, end_a + buffer, end_b + buffer, instruction, steps > 0);
@@ -553,9 +578,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           end.next();
         }
-        dev::mma_commit<true>(at.sum_full(sums.stage));
+        if (!lost) dev::mma_commit<true>(at.sum_full(sums.stage));
         sums.next();
       }
+      settle(limit);
     }
   } else if (warp == 3) {
     // What came with the ends of segments is cleared.  With the ends in the stages, among the steps, this took about a
@@ -565,16 +591,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t t = t0; t < tiles; t += t_step) {
       const GradTile g = grad_tile(a, segments, t);
       if (!g.end()) continue;
-      if (warp_wait(at.end_full(end.stage), end.parity, limit)) {
-        uint8_t* chunk = ends + end.stage * kEndBytes + lane * 16;  // 8 lanes to a row
-        for (int c = 0; c < 2 + g.chunks; ++c, chunk += kEndChunk)
-          for (int row = g.end(); row < kEndRows; row += 4)
-            if (row + lane / 8 < kEndRows)
-              *reinterpret_cast<uint4*>(chunk + row * dev::kBoxRowBytes) = make_uint4(0, 0, 0, 0);
-        dev::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) dev::arrive_first(at.end_cleared(end.stage));
-      }
+      if (!warp_wait(at.end_full(end.stage), end.parity, limit)) break;
+      uint8_t* chunk = ends + end.stage * kEndBytes + lane * 16;  // 8 lanes to a row
+      for (int c = 0; c < 2 + g.chunks; ++c, chunk += kEndChunk)
+        for (int row = g.end(); row < kEndRows; row += 4)
+          if (row + lane / 8 < kEndRows)
+            *reinterpret_cast<uint4*>(chunk + row * dev::kBoxRowBytes) = make_uint4(0, 0, 0, 0);
+      dev::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) dev::arrive_first(at.end_cleared(end.stage));
       end.next();
     }
   } else if (warp >= 4 && warp < 8) {
@@ -583,23 +608,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* mine = staging + quarter * kStoreBoxes * kStoreBox;
     const bool whole = a.fast_width % 8 == 0;
     int filled = 0;
+    bool lost = false;
     for (uint32_t t = t0; t < tiles; t += t_step) {
       const GradTile g = grad_tile(a, segments, t);
       const int m = g.slow + rank * kTileM + quarter * 32;
       const int columns = min(2 * g.chunks * kBlockK, a.fast_width - g.fast), rows = min(32, a.slow_width - m);
       const bool empty = g.segment.y == 0;
       if (!empty) {
-        if (!warp_wait(at.sum_full(sums.stage), sums.parity, limit)) {
-          sums.next();
-          continue;
-        }
+        lost = lost || !warp_wait(at.sum_full(sums.stage), sums.parity, limit);
         dev::tmem_fence_after();
       }
       for (int c = 0; c < columns; c += 32) {
         uint32_t v[32];
-        if (empty) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0;
+        if (empty || lost) {
+          fill(v, empty ? 0 : kLost);
         } else {
           dev::tmem_load32(p.tmem + sums.stage * kGradN + c + ((uint32_t)quarter << 21), v);
           dev::tmem_load_wait(v);
@@ -642,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!empty) {
         dev::tmem_fence_before();
         __syncwarp();
-        if (lane == 0) at.release_sum(sums.stage);
+        if (lane == 0 && !lost) at.release_sum(sums.stage);
         sums.next();
       }
     }

@@ -65,8 +65,10 @@ def expert_products_backward(grad_out: torch.Tensor, rows: torch.Tensor, weights
 
 
 def product_status(device: torch.device | int | None = None) -> int:
-    """1 if a bounded wait inside one of these products ran out on the device since the last call
-    (their results are not to be used), else 0.  Synchronises the current stream."""
+    """1 if a bounded wait inside one of these products ran out on the device since the last call, else 0.
+    What such a wait has cost is NaN in the results; nothing else says so before this call, which
+    synchronises the current stream.  The bound (``cusort_set_wait_limit_ns``, 2 s where nothing is set)
+    is the calling host thread's, and autograd computes gradients in threads of its own."""
     status = C.c_uint32()
     with torch.cuda.device(device):
         _capi.check(_capi.load().cusort_read_product_status(
