@@ -859,7 +859,7 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
     return float_products(static_cast<const float*>(d_rows), row_stride, static_cast<const float*>(d_weights),
                           expert_stride, in_stride, out_stride, segments, static_cast<float*>(d_out), (int)in, (int)out,
                           stream);
-  const bool few = capacity <= (int64_t)kFewRows * num_experts;
+  const bool few = capacity <= (int64_t)kProductFewRows * num_experts;
   ProductArgs a;
   a.segments = segments;
   a.out = d_out;
@@ -868,7 +868,7 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   a.limit_ns = wait_limit_ns();
   a.skip = debug_skip_tile();
   // at most one part-filled tile to an expert, and no expert without a row
-  const int64_t tiles = capacity / (capacity <= kFewestRows ? kFewestRows : few ? kFewRows : kManyRows) +
+  const int64_t tiles = capacity / (capacity <= kProductFewestRows ? kProductFewestRows : few ? kProductFewRows : kProductManyRows) +
                         std::min<int64_t>(num_experts, capacity);
   if (tiles * ((out + kTileM - 1) / kTileM) > 1 << 30) return cudaErrorInvalidValue;
   uint8_t* temp = static_cast<uint8_t*>(d_temp_storage);
@@ -877,7 +877,7 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   if (e) return e;
   const auto go = [&](auto t) {
     using T = decltype(t);
-    if (capacity <= kFewestRows)
+    if (capacity <= kProductFewestRows)
       return tiles * ((out + kTileM - 1) / kTileM) <= kSms / 2
                  ? product<T, ProductFewestNarrow>(a, weights, rows, in_order, tiles, stream)
                  : product<T, ProductFewest>(a, weights, rows, in_order, tiles, stream);

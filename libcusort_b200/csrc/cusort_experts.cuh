@@ -38,11 +38,11 @@ template <int BN, int COLUMNS, int STAGES, int SUB, bool PAIR> struct ProductSha
 // 84 and 76, 128 89 and 80.  The rule goes by averages, since the counts stay
 // on the device, and these are of experts with equal counts: a batch whose rows
 // nearly all go to one expert takes tiles that are smaller than they could be.
-constexpr int kFewestRows = 16, kFewRows = 64, kManyRows = 256;
-using ProductFewestNarrow = ProductShape<kFewestRows, 64, 9, 2, false>;
-using ProductFewest = ProductShape<kFewestRows, 128, 5, 2, false>;
-using ProductFew = ProductShape<kFewRows, 128, 4, 2, false>;
-using ProductMany = ProductShape<kManyRows, 128, 6, 1, true>;
+constexpr int kProductFewestRows = 16, kProductFewRows = 64, kProductManyRows = 256;
+using ProductFewestNarrow = ProductShape<kProductFewestRows, 64, 9, 2, false>;
+using ProductFewest = ProductShape<kProductFewestRows, 128, 5, 2, false>;
+using ProductFew = ProductShape<kProductFewRows, 128, 4, 2, false>;
+using ProductMany = ProductShape<kProductManyRows, 128, 6, 1, true>;
 
 // Expert segments as the CTA keeps them in shared memory.
 struct Segments {
