@@ -161,16 +161,12 @@ __device__ __forceinline__ void settle(const dev::WaitLimit& limit) {
   while (dev::globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
 }
 
-// What stands in the results in the place of sums that a wait in vain has cost: NaN.  A role whose wait ran out stops
-// there, so that nobody takes a barrier's phase for another one: stages that are not multiplied any more, sums that are
-// not handed on.  Those who wait for them run out in turn, at once in this CTA, after their own limit in the other of a
-// pair; the storing warps go on to the end.
-constexpr uint32_t kLost = 0x7fffffffu;
-
-__device__ __forceinline__ void fill(uint32_t (&v)[32], uint32_t value) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = value;
-}
+// What stands in the results in the place of two sums that a wait in vain has cost: NaN, in either type.  A role whose
+// wait ran out waits and hands on no more, so that nobody takes a barrier's phase for another one: no stages are filled or
+// multiplied any more.  Those who wait for them run out in turn, at once in this CTA, after their own limit in the other of
+// a pair; the storing warps go on to the end.  (The roles' loops run on with nothing to do: left early they made a call of
+// 8.0 us one of 8.4.)
+constexpr uint32_t kLost = 0x7fff7fffu;
 
 // A wait of a whole warp, by one lane: 32 of them keep shared memory busy.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const dev::WaitLimit& limit) {
@@ -278,16 +274,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       uint32_t turn = (warp == 2 || warp == 9);  // whether it takes the odd steps
       int64_t step_of_cta = -1;
       bool lost = false;
-      for (uint32_t t = t0; t < tiles && !lost; t += t_step) {
+      for (uint32_t t = t0; t < tiles; t += t_step) {
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const int column = tile.column + rank * kTileM;
         const int mine = align_up(tile.rows, Shape::kRowStep) / Shape::kCtas, row = tile.row + rank * mine;
         const uint32_t bytes = SUB * Shape::kCtas * (kBytesA + mine * dev::kBoxRowBytes);
         for (int k = 0; k < steps; ++k, ring.next()) {
           ++step_of_cta;
-          if ((turn ^= 1) == 0) continue;
-          if ((lost = !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit))) break;
-          if (step_of_cta == a.skip) continue;
+          if ((turn ^= 1) == 0 || lost) continue;
+          lost = !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit);
+          if (lost || step_of_cta == a.skip) continue;
           const uint32_t to = stages + ring.stage * Shape::kStage, own = at.full(ring.stage);
           const uint32_t bar = PAIR ? dev::in_first(own) : own;
           // the first CTA's barrier counts the copies of both
@@ -326,15 +322,16 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       const uint64_t first_a = dev::operand_descriptor(stages, IN_ORDER ? 16 : kBoxBytes, 1024);
       const uint64_t first_b = dev::operand_descriptor(stages + kBytesA, 16, 1024);
       bool lost = false;
-      for (uint32_t t = t0; t < tiles && !lost; t += t_step, sums.next()) {
+      for (uint32_t t = t0; t < tiles; t += t_step, sums.next()) {
         const ProductTile tile = product_tile<Shape>(a, s, t);
         const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, !IN_ORDER, false,
                                                           kTileM * Shape::kCtas, align_up(tile.rows, Shape::kRowStep));
         const uint32_t sum = p.tmem + sums.stage * Shape::kSumColumns;
-        lost = !dev::wait_for<PAIR>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
+        lost = lost || !dev::wait_for<PAIR>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
         dev::tmem_fence_after();
-        for (int k = 0; k < steps && !lost; ++k, ring.next()) {
-          if ((lost = !dev::wait_for(at.full(ring.stage), ring.parity, limit))) break;
+        for (int k = 0; k < steps; ++k, ring.next()) {
+          lost = lost || !dev::wait_for(at.full(ring.stage), ring.parity, limit);
+          if (lost) continue;
           dev::tmem_fence_after();
           const uint32_t stage = ring.stage * (Shape::kStage / 16);
 #pragma unroll
@@ -366,15 +363,12 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
       const int column = tile.column + rank * kTileM + quarter * 32;
       for (int c = 0; c < tile.rows && quarter * 32 < COLUMNS; c += 32) {
         uint32_t v[32];
-        if (lost) {
-          fill(v, kLost);
-        } else {
-          dev::tmem_load32(p.tmem + sums.stage * Shape::kSumColumns + c + ((uint32_t)quarter << 21), v);
-          dev::tmem_load_wait(v);
-        }
+        dev::tmem_load32(p.tmem + sums.stage * Shape::kSumColumns + c + ((uint32_t)quarter << 21), v);
+        dev::tmem_load_wait(v);
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const uint32_t both = dev::from_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), T{});
+          const uint32_t both =
+              dev::from_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]), T{}) | (lost ? kLost : 0);
           const uint32_t other = __shfl_xor_sync(kAll, both, 1);
           // even lanes: row 2j, odd ones: row 2j + 1, each of this column and its neighbour
           const uint32_t word = lane & 1 ? __byte_perm(other, both, 0x7632) : __byte_perm(both, other, 0x5410);
@@ -497,15 +491,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t turn = (warp == 2 || warp == 9);  // whether it takes the odd steps
       int64_t step_of_cta = -1;
       bool lost = false;
-      for (uint32_t t = t0; t < tiles && !lost; t += t_step) {
+      for (uint32_t t = t0; t < tiles; t += t_step) {
         const GradTile g = grad_tile(a, segments, t);
         const int slow = g.slow + rank * kTileM, fast = g.fast + rank * g.chunks * kBlockK;
         const uint32_t bytes = (2 + g.chunks) * kChunkBytes;
         const int steps = g.steps();
         if (g.end()) {
           // ahead of the steps, into a buffer of its own, so that it is there and cleared when they are done
-          if (warp == 2 || warp == 9) {
-            if ((lost = !dev::wait_for(at.end_empty(end.stage), end.parity ^ 1, limit))) break;
+          if (warp == 2 || warp == 9) lost = lost || !dev::wait_for(at.end_empty(end.stage), end.parity ^ 1, limit);
+          if ((warp == 2 || warp == 9) && !lost) {
             const uint32_t to = dev::smem_u32(ends) + end.stage * kEndBytes, bar = at.end_full(end.stage);
             const int row = g.segment.x + g.whole();
             if (warp < 8) {
@@ -521,9 +515,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int k = 0; k < steps; ++k, ring.next()) {
           ++step_of_cta;
-          if ((turn ^= 1) == 0) continue;
-          if ((lost = !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit))) break;
-          if (step_of_cta == a.skip) continue;
+          if ((turn ^= 1) == 0 || lost) continue;
+          lost = !dev::wait_for(at.empty(ring.stage), ring.parity ^ 1, limit);
+          if (lost || step_of_cta == a.skip) continue;
           const uint32_t to = stages + ring.stage * kGradStage, bar = dev::in_first(at.full(ring.stage));
           const int row = g.segment.x + k * kBlockK;
           if (warp < 8) {
@@ -548,16 +542,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t end_a = dev::operand_descriptor(dev::smem_u32(ends), kEndChunk, 1024);
       const uint64_t end_b = dev::operand_descriptor(dev::smem_u32(ends) + 2 * kEndChunk, kEndChunk, 1024);
       bool lost = false;
-      for (uint32_t t = t0; t < tiles && !lost; t += t_step) {
+      for (uint32_t t = t0; t < tiles; t += t_step) {
         const GradTile g = grad_tile(a, segments, t);
         if (g.segment.y == 0) continue;
         const uint32_t instruction = dev::mma_instruction(std::is_same_v<T, __nv_bfloat16>, true, true, 2 * kTileM,
                                                           2 * g.chunks * kBlockK);
         const uint32_t sum = p.tmem + sums.stage * kGradN;
         const int whole = g.whole(), steps = g.steps();
-        lost = !dev::wait_for<true>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
-        for (int k = 0; k < steps && !lost; ++k, ring.next()) {
-          if ((lost = !dev::wait_for(at.full(ring.stage), ring.parity, limit))) break;
+        lost = lost || !dev::wait_for<true>(at.sum_empty(sums.stage), sums.parity ^ 1, limit);
+        for (int k = 0; k < steps; ++k, ring.next()) {
+          lost = lost || !dev::wait_for(at.full(ring.stage), ring.parity, limit);
+          if (lost) continue;
           dev::tmem_fence_after();
           const uint32_t stage = ring.stage * (kGradStage / 16);
           const int depth = min(kBlockK, whole - k * kBlockK) / 16;
@@ -568,8 +563,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                    k + i > 0);
           dev::mma_commit<true>(at.empty(ring.stage));
         }
-        if (g.end() && !lost) {
-          lost = !dev::wait_for<true>(at.end_cleared(end.stage), end.parity, limit);
+        if (g.end()) {
+          lost = lost || !dev::wait_for<true>(at.end_cleared(end.stage), end.parity, limit);
           if (!lost) {
             dev::tmem_fence_after();
             const uint32_t buffer = end.stage * (kEndBytes / 16);
@@ -591,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t t = t0; t < tiles; t += t_step) {
       const GradTile g = grad_tile(a, segments, t);
       if (!g.end()) continue;
-      if (!warp_wait(at.end_full(end.stage), end.parity, limit)) break;
+      if (!warp_wait(at.end_full(end.stage), end.parity, limit)) break;  // every later one is lost too
       uint8_t* chunk = ends + end.stage * kEndBytes + lane * 16;  // 8 lanes to a row
       for (int c = 0; c < 2 + g.chunks; ++c, chunk += kEndChunk)
         for (int row = g.end(); row < kEndRows; row += 4)
@@ -618,10 +613,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         lost = lost || !warp_wait(at.sum_full(sums.stage), sums.parity, limit);
         dev::tmem_fence_after();
       }
+      const uint32_t gone = lost && !empty ? kLost : 0;
       for (int c = 0; c < columns; c += 32) {
         uint32_t v[32];
-        if (empty || lost) {
-          fill(v, empty ? 0 : kLost);
+        if (empty) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = 0;
         } else {
           dev::tmem_load32(p.tmem + sums.stage * kGradN + c + ((uint32_t)quarter << 21), v);
           dev::tmem_load_wait(v);
@@ -635,10 +632,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 4; ++j) {
           const uint32_t* x = v + j * 8;
           uint4 w;
-          w.x = dev::from_float2(__uint_as_float(x[0]), __uint_as_float(x[1]), T{});
-          w.y = dev::from_float2(__uint_as_float(x[2]), __uint_as_float(x[3]), T{});
-          w.z = dev::from_float2(__uint_as_float(x[4]), __uint_as_float(x[5]), T{});
-          w.w = dev::from_float2(__uint_as_float(x[6]), __uint_as_float(x[7]), T{});
+          w.x = dev::from_float2(__uint_as_float(x[0]), __uint_as_float(x[1]), T{}) | gone;
+          w.y = dev::from_float2(__uint_as_float(x[2]), __uint_as_float(x[3]), T{}) | gone;
+          w.z = dev::from_float2(__uint_as_float(x[4]), __uint_as_float(x[5]), T{}) | gone;
+          w.w = dev::from_float2(__uint_as_float(x[6]), __uint_as_float(x[7]), T{}) | gone;
           *reinterpret_cast<uint4*>(box + lane * 64 + ((j ^ (lane >> 1 & 3)) * 16)) = w;
         }
         if (whole) {
