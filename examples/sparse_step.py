@@ -109,7 +109,8 @@ def sample(samples: int = 4, steps: int = 24, hidden: int = 64, block: int = 16,
     left = torch.tensor([blocks], dtype=torch.int32, device="cuda")
     shares = torch.zeros(blocks, dtype=torch.int32, device="cuda")
     tables = torch.full((len(prompts), 8), -1, dtype=torch.int32, device="cuda")
-    cache = torch.zeros(blocks + 1, block, hidden, device="cuda", dtype=torch.bfloat16)  # the last takes what has no slot
+    # the last block takes what has no slot
+    cache = torch.zeros(blocks + 1, block, hidden, device="cuda", dtype=torch.bfloat16)
     caches = [cache[:blocks]]
     rows = torch.zeros(len(prompts), 8 * block, hidden, device="cuda", dtype=torch.bfloat16)  # what should be found
 
@@ -119,7 +120,8 @@ def sample(samples: int = 4, steps: int = 24, hidden: int = 64, block: int = 16,
         with torch.no_grad():
             x = layer(torch.randn(tokens, hidden, device="cuda").bfloat16())
         cache.view(-1, hidden)[torch.where(plan.slots >= 0, plan.slots, blocks * block)] = x
-        request = torch.searchsorted(plan.starts[1:], torch.arange(tokens, device="cuda", dtype=torch.int32), right=True)
+        token = torch.arange(tokens, device="cuda", dtype=torch.int32)
+        request = torch.searchsorted(plan.starts[1:], token, right=True)
         there = request < len(lens)
         rows[request[there], plan.positions[there].long()] = x[there]
         lens, left = lens + new, plan.num_free

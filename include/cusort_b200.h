@@ -364,11 +364,12 @@ cudaError_t cusort_combine_rows_backward(cusort_float_type type, const void* d_g
  * gives them)
  *   d_out[r] = d_rows[r] x weights[e],
  * zeros for rows of no segment.  Sums in 32 bits, rounded once; 32-bit
- * operands are multiplied as they are (and not on the tensor cores).  d_rows: `capacity` rows of `in` contiguous elements,
- * row_stride elements apart; weights[e][i][o] at d_weights + e * expert_stride
- * + i * in_stride + o * out_stride, one of the last two strides 1; d_out:
- * capacity x out, contiguous, on a 16-byte boundary.  With weights and widths
- * the other way round it is the gradient of the rows.
+ * operands are multiplied as they are (and not on the tensor cores).  d_rows:
+ * `capacity` rows of `in` contiguous elements, row_stride elements apart;
+ * weights[e][i][o] at d_weights + e * expert_stride + i * in_stride
+ * + o * out_stride, one of the last two strides 1; d_out: capacity x out,
+ * contiguous, on a 16-byte boundary.  With weights and widths the other way
+ * round it is the gradient of the rows.
  * Segments are cut to the rows there are; they may come in any order, but must
  * not overlap.
  * 1 <= in, out <= 2^20, capacity < 2^31 - 1024, num_experts <= 1024.

@@ -120,7 +120,8 @@ def load() -> C.CDLL:
 
 
 def native():
-    """The native half of the PyTorch functions in routing.py, experts.py and paging.py (raises if it has not been built)."""
+    """The native half of the PyTorch functions in routing.py, experts.py and paging.py (raises if it has not been
+    built)."""
     global _native
     if _native is None:
         if not NATIVE_PATH.exists():

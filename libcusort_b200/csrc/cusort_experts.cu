@@ -161,11 +161,13 @@ __device__ __forceinline__ void settle(const dev::WaitLimit& limit) {
   while (dev::globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
 }
 
-// What stands in the results in the place of two sums that a wait in vain has cost: NaN, in either type.  A role whose
-// wait ran out waits and hands on no more, so that nobody takes a barrier's phase for another one: no stages are filled or
-// multiplied any more.  Those who wait for them run out in turn, at once in this CTA, after their own limit in the other of
-// a pair; the storing warps go on to the end.  (The roles' loops run on with nothing to do: left early they made a call of
-// 8.0 us one of 8.4.)
+// What stands in the results in the place of two sums that a wait in vain has
+// cost: NaN, in either type.  A role whose wait ran out waits and hands on no
+// more, so that nobody takes a barrier's phase for another one or arrives twice
+// in one: no stages are filled or multiplied any more.  Those who wait for them
+// run out in turn, at once in this CTA, after their own limit in the other of a
+// pair; the storing warps go on to the end.  (The roles' loops run on with
+// nothing to do: left early they made a call of 8.2 us one of 8.4.)
 constexpr uint32_t kLost = 0x7fff7fffu;
 
 // A wait of a whole warp, by one lane: 32 of them keep shared memory busy.
@@ -238,9 +240,16 @@ __device__ __forceinline__ ProductTile product_tile(const ProductArgs& a, const 
 // stages, not four, and tiles of 64 columns where that still leaves no more
 // than one to an SM (six rows of six experts, 2048 -> 1024, from memory: 10.5
 // us with four stages, 9.4 with five, 8.9 with half the columns; 4096 -> 1024
-// 17.3, 14.7, 12.6; 4.2 us are there without any contraction).  Splitting the contraction over clusters of two or three CTAs
-// took as long or longer (11.4 us for the first): their barriers and the
-// joining cost what the shorter loops gained.
+// 17.3, 14.7, 12.6; 4.2 us are there without any contraction).  Splitting the
+// contraction over clusters of two or three CTAs took as long or longer (11.4 us
+// for the first): their barriers and the joining cost what the shorter loops
+// gained.
+//
+// The tensor cores cut what an addition leaves beyond 32 bits instead of
+// rounding it: of 2048 to 4096 products' sums 0.1 to 0.2 % come to the
+// neighbour of the 16-bit number nearest to the exact sum, 0.01 to 0.04 % where
+// every addition is rounded; the distance from the exact sums, which that one
+// rounding makes, is the same in five digits (1.65e-3 of them in bfloat16).
 template <typename T, typename Shape, bool IN_ORDER>
 __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_constant__ ProductArgs a) {
   constexpr int BN = Shape::kRows, COLUMNS = Shape::kWeightColumns, STAGES = Shape::kStages, SUB = Shape::kSub;
@@ -430,7 +439,8 @@ constexpr int kEndRows = 16;              // contracted by one instruction
 constexpr int kEndChunk = kEndRows * 128, kEndBytes = 4 * kEndChunk;
 
 size_t grad_bytes(int experts) {
-  return 1024 + kGradStages * kGradStage + kEnds * kEndBytes + kGradStaging + sizeof(Pipe<kGradStages, true>) + 8 * (size_t)experts;
+  return 1024 + kGradStages * kGradStage + kEnds * kEndBytes + kGradStaging + sizeof(Pipe<kGradStages, true>) +
+         8 * (size_t)experts;
 }
 
 struct GradTile {
@@ -458,9 +468,11 @@ __device__ __forceinline__ GradTile grad_tile(const GradArgs& a, const int2* seg
 // come by themselves, and what comes with them is cleared in shared memory.
 //
 // Always by pairs of CTAs.  Many rows: bound as the products are (8192 rows, 4096 x 4096: 192 us, 1.43 PFLOP/s; 32
-// experts of 1024, 2048 x 4096: 395 us).  Few: by writing the gradient, for which 3.9 TB/s is all that a plain fill
-// comes to (128 experts of 128 rows, 2048 x 1024: 183 us, 2.9 TB/s; without the stores 120).  Stored by tiled copies of 64-byte rows: whole
-// sectors straight from registers took 194 us there, and 271 instead of 233 where rows are 2800 bytes.
+// experts of 1024, 2048 x 4096: 395 to 400 us).  Few (128 experts of 128 rows, 2048 x 1024): 183 to 199 us, 2.7 to 2.9
+// TB/s written, of which 120 are left without the stores, while a plain fill of as many bytes takes 78 to 96.  So neither
+// memory nor the tensor cores (16 % busy) bound it: a sum of 256 columns a CTA is there after two steps, and then four
+// warps have to read, round and stage it.  Stored by tiled copies of 64-byte rows: whole sectors straight from
+// registers took 194 us where these took 181, and 271 instead of 233 where rows are 2800 bytes.
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     grad_weights_kernel(const __grid_constant__ GradArgs a) {
@@ -580,8 +592,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 3) {
     // What came with the ends of segments is cleared.  With the ends in the stages, among the steps, this took about a
-    // microsecond that nothing hid (32 experts of 1023 rows, 2048 x 4096: 441 us, 399 now, 395 of 1024 rows); done
-    // by the multiplying warp, 685.
+    // microsecond that nothing hid (32 experts of 1023 rows, 2048 x 4096: 457 us where this way took 414; 399 to 408 in
+    // later runs, 396 to 400 of 1024 rows); done by the multiplying warp, 685.
     Ring<kEnds> end;
     for (uint32_t t = t0; t < tiles; t += t_step) {
       const GradTile g = grad_tile(a, segments, t);
@@ -820,8 +832,8 @@ bool sizes_fit(int64_t capacity, int64_t in, int64_t out, int experts) {
 
 // Whether elements of the type can be loaded from these addresses.
 bool on_elements(cusort_float_type type, const void* x, const void* y) {
-  return ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & (uintptr_t)(float_type_bytes(type) - 1)) ==
-         0;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y);
+  return (bits & (uintptr_t)(float_type_bytes(type) - 1)) == 0;
 }
 
 }  // namespace
@@ -849,7 +861,8 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   if (*temp_storage_bytes < need) return cudaErrorInvalidValue;
   if (capacity == 0) return cudaSuccess;
   if (d_rows == nullptr || d_weights == nullptr || d_counts == nullptr || d_offsets == nullptr || d_out == nullptr ||
-      (reinterpret_cast<uintptr_t>(d_out) & 15) != 0 || (need > 1 && (reinterpret_cast<uintptr_t>(d_temp_storage) & 15) != 0))
+      (reinterpret_cast<uintptr_t>(d_out) & 15) != 0 ||
+      (need > 1 && (reinterpret_cast<uintptr_t>(d_temp_storage) & 15) != 0))
     return cudaErrorInvalidValue;
   const SegmentArgs segments{d_counts, d_offsets, num_experts, (int)capacity};
   if (whole)
@@ -865,8 +878,9 @@ extern "C" cudaError_t cusort_expert_products(void* d_temp_storage, size_t* temp
   a.limit_ns = wait_limit_ns();
   a.skip = debug_skip_tile();
   // at most one part-filled tile to an expert, and no expert without a row
-  const int64_t tiles = capacity / (capacity <= kProductFewestRows ? kProductFewestRows : few ? kProductFewRows : kProductManyRows) +
-                        std::min<int64_t>(num_experts, capacity);
+  const int rows_of_tile =
+      capacity <= kProductFewestRows ? kProductFewestRows : few ? kProductFewRows : kProductManyRows;
+  const int64_t tiles = capacity / rows_of_tile + std::min<int64_t>(num_experts, capacity);
   if (tiles * ((out + kTileM - 1) / kTileM) > 1 << 30) return cudaErrorInvalidValue;
   uint8_t* temp = static_cast<uint8_t*>(d_temp_storage);
   cudaError_t e = rows.prepare(temp, nullptr, stream);
@@ -901,8 +915,10 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
     return cudaSuccess;
   }
   if (*temp_storage_bytes < need) return cudaErrorInvalidValue;
-  if (d_grad_weights == nullptr || (reinterpret_cast<uintptr_t>(d_grad_weights) & 15) != 0) return cudaErrorInvalidValue;
-  if (capacity == 0) return cudaMemsetAsync(d_grad_weights, 0, (size_t)num_experts * in * out * float_type_bytes(type), stream);
+  if (d_grad_weights == nullptr || (reinterpret_cast<uintptr_t>(d_grad_weights) & 15) != 0)
+    return cudaErrorInvalidValue;
+  if (capacity == 0)
+    return cudaMemsetAsync(d_grad_weights, 0, (size_t)num_experts * in * out * float_type_bytes(type), stream);
   if (d_rows == nullptr || d_grad_out == nullptr || d_counts == nullptr || d_offsets == nullptr ||
       (need > 1 && (reinterpret_cast<uintptr_t>(d_temp_storage) & 15) != 0))
     return cudaErrorInvalidValue;
@@ -934,8 +950,9 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
     e = out.map(&a.out, false, 32, 32);
   }
   if (e) return e;
-  return type == CUSORT_FLOAT_F16 ? run(grad_weights_kernel<__half>, a, tiles, 2, grad_bytes(num_experts), stream)
-                                  : run(grad_weights_kernel<__nv_bfloat16>, a, tiles, 2, grad_bytes(num_experts), stream);
+  const size_t smem = grad_bytes(num_experts);
+  return type == CUSORT_FLOAT_F16 ? run(grad_weights_kernel<__half>, a, tiles, 2, smem, stream)
+                                  : run(grad_weights_kernel<__nv_bfloat16>, a, tiles, 2, smem, stream);
 }
 
 extern "C" cudaError_t cusort_read_product_status(uint32_t* status, cudaStream_t stream) {

@@ -26,8 +26,8 @@ template <int BN, int COLUMNS, int STAGES, int SUB, bool PAIR> struct ProductSha
   static constexpr int kRowStep = 16 * kCtas;       // the instruction's width comes in such steps
   // A stage holds SUB steps of kBlockK, each the weights' part and then the rows'.
   static constexpr uint32_t kBytesB = BN / kCtas * kBlockK * 2, kStep = kBytesA + kBytesB, kStage = SUB * kStep;
-  // Each of the two sums has the columns that are read of it, which in the form for the fewest rows are more than it has
-  // rows: one that is read has no columns of the other, which grows meanwhile, nor any that were not allocated.
+  // Each of the two sums has the columns that are read of it, which in the form for the fewest rows are more than it
+  // has rows: one that is read has no columns of the other, which grows meanwhile, nor any that were not allocated.
   static constexpr uint32_t kSumColumns = (BN + kSumLoad - 1) / kSumLoad * kSumLoad, kColumns = 2 * kSumColumns;
   static constexpr uint32_t kStaging = 4 * 2048;  // 32 x 32 16-bit elements for each storing warp
 };
@@ -149,8 +149,9 @@ __device__ __forceinline__ void clear(uint16_t* x, int64_t begin, int64_t end, i
   if (head + words * 8 + thread < end) x[head + words * 8 + thread] = 0;
 }
 
-// Where rows of no segment that begin at row r end, by experts e0, e0 + step and so on: at the segment that begins next,
-// the capacity where none does, r itself where a segment covers it.
+// Where rows of no segment that begin at row r end, by experts e0, e0 + step and
+// so on: at the segment that begins next, the capacity where none does, r itself
+// where a segment covers it.
 __host__ __device__ inline int no_segment_until(const Segments& s, int experts, int capacity, int r, int e0, int step) {
   int until = capacity;
   for (int e = e0; e < experts; e += step)
@@ -192,7 +193,8 @@ struct WarpLanes {
   __device__ __forceinline__ int lowest(int v) const { return __reduce_min_sync(0xffffffffu, v); }
 };
 
-// One warp's part in clearing the rows that belong to no segment (16-bit elements, `width` to a row; warp `me` of `all`).
+// One warp's part in clearing the rows that belong to no segment (16-bit
+// elements, `width` to a row; warp `me` of `all`).
 __device__ __forceinline__ void clear_other_rows(uint16_t* out, int64_t width, const SegmentArgs& a, const Segments& s,
                                                  int me, int all) {
   const WarpLanes lanes{(int)(threadIdx.x & 31)};

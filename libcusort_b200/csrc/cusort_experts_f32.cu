@@ -51,10 +51,15 @@ struct FloatArgs {
 // Each step is loaded into registers while the one before is multiplied.
 // Where experts have many rows, 8 x 8 sums to a thread: 32 experts of 1024
 // rows, 1024 -> 2048, 3.3 ms, 41 TFLOP/s; 4 x 8, two multiply-adds at a time
-// or not, 4.0 to 4.3 ms.  The multiply-adds bound it, then the shared-memory
-// loads beside them.  Few rows: smaller tiles, so that less is multiplied for
-// nothing, and longer steps for more bytes in flight (64 experts of 16 rows
-// 410 us, in tiles of 64 rows 605; of 40 rows 615).
+// or not, 4.0 to 4.3 ms.  The multiply-adds bound it (55 % of their 74.4
+// TFLOP/s), then the shared-memory loads beside them.  Few rows: smaller tiles,
+// so that less is multiplied for nothing, and longer steps for more bytes in
+// flight (64 experts of 16 rows 410 us, in tiles of 64 rows 605; of 40 rows
+// 615).  The weights' bytes would take 82 of the 410: with one row of sums to a
+// thread every weight that it reads from shared memory goes into a single
+// multiply-add.  The gradient of the weights, 8 x 8 sums to a thread whatever
+// the rows: 32 experts of 1024 rows, 1024 x 2048, 3.3 ms, 41 TFLOP/s; 64 experts
+// of 16, 40 and 64 rows 305, 494 and 604 us (writing 537 MB).
 template <int U, int K, bool RAGGED_K, bool B_ALONG>
 __global__ void __launch_bounds__(kThreads, Shape<U, K>::kCtas)
     float_products_kernel(const __grid_constant__ FloatArgs a) {
@@ -68,7 +73,8 @@ __global__ void __launch_bounds__(kThreads, Shape<U, K>::kCtas)
   const Segments s{s_segments, s_segments + experts, s_segments + 2 * experts};
   dev::wait_for_previous();
   const int m_tiles = (a.m + kM - 1) / kM, n_tiles = (a.n + kN - 1) / kN;
-  load_segments<kThreads>(a.segments, s, sums, a.most, [&](int count) { return RAGGED_K ? m_tiles : (count + kM - 1) / kM; });
+  load_segments<kThreads>(a.segments, s, sums, a.most,
+                          [&](int count) { return RAGGED_K ? m_tiles : (count + kM - 1) / kM; });
   const uint32_t tiles = (uint32_t)s.tiles[experts] * n_tiles;
   if (!RAGGED_K)
     clear_other_rows(reinterpret_cast<uint16_t*>(a.c), 2 * (int64_t)a.n, a.segments, s,
@@ -158,8 +164,9 @@ cudaError_t run(FloatArgs a, cudaStream_t stream) {
   constexpr size_t kMost = sizeof(Shape<U, K>) + 4 * (3 * kMaxExperts + 1);
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMost);
   if (e) return e;
-  return launch_after_previous(kernel, std::max<int64_t>(1, std::min<int64_t>(Shape<U, K>::kCtas * kSms, tiles)), kThreads,
-                               sizeof(Shape<U, K>) + 4 * (3 * (size_t)a.segments.experts + 1), a, stream);
+  const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(Shape<U, K>::kCtas * kSms, tiles));
+  return launch_after_previous(kernel, grid, kThreads, sizeof(Shape<U, K>) + 4 * (3 * (size_t)a.segments.experts + 1), a,
+                               stream);
 }
 
 // Rows an expert on average up to which tiles have 16 and 64 rows.  64 experts,

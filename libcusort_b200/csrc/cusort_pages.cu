@@ -43,7 +43,8 @@ struct PagesArgs {
   uint8_t* served;
   // workspace
   int32_t* tile_counts;    // [kTiles] blocks that a tile of the pool adds to the list; and the blocks taken
-  int32_t *holders, *map;  // compact: [num_blocks] tables that hold a block, less one; the move that a block takes part in
+  // compact: [num_blocks] tables that hold a block, less one; the move that a block takes part in
+  int32_t *holders, *map;
   int phase;               // of the form with a launch for each
   int row_lanes, row_parts;  // see for_rows
 };
@@ -539,8 +540,10 @@ extern "C" cudaError_t cusort_page_fork(void* d_temp_storage, size_t* temp_stora
       d_num_free == nullptr || d_num_free_out == nullptr)
     return cudaErrorInvalidValue;
   // what is read by every CTA, whenever it comes to run, must not be written meanwhile
-  if (d_num_free == d_num_free_out || (num_blocks > 0 && (d_free_blocks == d_free_blocks_out || d_shares == d_shares_out)) ||
-      (tables && d_block_tables == d_block_tables_out) || (num_children > 0 && num_requests > 0 && d_lens == d_lens_out))
+  if (d_num_free == d_num_free_out ||
+      (num_blocks > 0 && (d_free_blocks == d_free_blocks_out || d_shares == d_shares_out)) ||
+      (tables && d_block_tables == d_block_tables_out) ||
+      (num_children > 0 && num_requests > 0 && d_lens == d_lens_out))
     return cudaErrorInvalidValue;
   PagesArgs a{};
   a.tables = d_block_tables;
@@ -664,7 +667,8 @@ extern "C" cudaError_t cusort_page_copy(void* const* d_caches, const int64_t* bl
         if (pieces == 0) return cudaErrorInvalidValue;
         break;
       }
-      a.caches[a.num_caches++] = {static_cast<char*>(d_caches[c]), block_strides[c], (int64_t)block_bytes[c], (int)pieces};
+      a.caches[a.num_caches++] = {static_cast<char*>(d_caches[c]), block_strides[c], (int64_t)block_bytes[c],
+                                  (int)pieces};
       pieces += of;
       bits |= reinterpret_cast<uintptr_t>(d_caches[c]) | (uintptr_t)block_strides[c] | (uintptr_t)block_bytes[c];
     }
@@ -675,11 +679,12 @@ extern "C" cudaError_t cusort_page_copy(void* const* d_caches, const int64_t* bl
     a.groups = (int)std::min<int64_t>(num_pairs, kCtas);
     a.parts = (int)std::min<int64_t>(pieces, std::max<int64_t>(1, kCtas / a.groups));
     const int64_t grid = (int64_t)a.groups * a.parts;
-    const cudaError_t e = (bits & 15) == 0  ? launch_after_previous(copy_kernel<uint4>, grid, kCopyThreads, 0, a, stream)
-                          : (bits & 7) == 0 ? launch_after_previous(copy_kernel<uint2>, grid, kCopyThreads, 0, a, stream)
-                          : (bits & 3) == 0 ? launch_after_previous(copy_kernel<uint32_t>, grid, kCopyThreads, 0, a, stream)
-                          : (bits & 1) == 0 ? launch_after_previous(copy_kernel<uint16_t>, grid, kCopyThreads, 0, a, stream)
-                                            : launch_after_previous(copy_kernel<uint8_t>, grid, kCopyThreads, 0, a, stream);
+    const auto copy = [&](auto kernel) { return launch_after_previous(kernel, grid, kCopyThreads, 0, a, stream); };
+    const cudaError_t e = (bits & 15) == 0  ? copy(copy_kernel<uint4>)
+                          : (bits & 7) == 0 ? copy(copy_kernel<uint2>)
+                          : (bits & 3) == 0 ? copy(copy_kernel<uint32_t>)
+                          : (bits & 1) == 0 ? copy(copy_kernel<uint16_t>)
+                                            : copy(copy_kernel<uint8_t>);
     if (e) return e;
   }
   return cudaSuccess;

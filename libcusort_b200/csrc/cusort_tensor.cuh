@@ -13,8 +13,9 @@ namespace cusort_b200 {
 namespace dev {
 
 // 64 16-bit elements along the contiguous dimension: the width of every box
-// that the tiled copies bring, whose 16-byte pieces they permute within each 8
-// rows (128-byte swizzle).
+// that the tiled copies load, whose 16-byte pieces they permute within each 8
+// rows (128-byte swizzle).  Boxes that are stored are half as wide, with the
+// 64-byte swizzle.
 constexpr int kBoxRowBytes = 128;
 
 // A box into this CTA's shared memory, counted on the barrier `bar` (PAIR: of either CTA of a cluster of two).

@@ -38,12 +38,12 @@ outside every segment keep their input.
 
 The routing operators are those of ``libcusort_b200.routing`` (its docstrings have the details), with
 gradients through autograd: ``route`` to the logits, ``dispatch`` to the rows (float32, float16 or bfloat16
-ones), ``combine`` to the rows, the weights and the residual.  ``expert_products`` is that of ``libcusort_b200.experts``,
-with gradients to the rows and the weights.  ``page_plan`` (with a free list) and the other page operators are those of
-``libcusort_b200.paging``.
+ones), ``combine`` to the rows, the weights and the residual.  ``expert_products`` is that of
+``libcusort_b200.experts``, with gradients to the rows and the weights.  ``page_plan`` (with a free list) and the
+other page operators are those of ``libcusort_b200.paging``.
 
-All of them are stable, allocate fresh outputs (the inputs are never written, except ``page_plan``'s block tables and ``page_copy``'s caches), run on torch's current
-CUDA stream through the C ABI (``cusort_sort_keys``, ``cusort_sort_pairs``, ``cusort_route`` and so on) and have
+All of them are stable, allocate fresh outputs (the inputs are never written, except ``page_plan``'s block tables and
+``page_copy``'s caches), run on torch's current CUDA stream through the C ABI (``cusort_sort_keys``, ``cusort_sort_pairs``, ``cusort_route`` and so on) and have
 fake (meta) implementations, so they trace under ``torch.compile`` / ``torch.export`` as opaque
 calls.  ``end_bit = -1`` means all key bits.  There is no CPU implementation: a CPU tensor raises.
 Floating-point keys follow the radix (IEEE total) order of the reference: -0.0 sorts before +0.0

@@ -50,8 +50,8 @@ def page_plan(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_tables: t
     be planned again; its caller goes on with the returned ``num_free``.  Without a free list the
     tables hold all blocks already.  ``num_tokens``: the length of the slot map, which may be more
     or less than there are new tokens; blocks that begin beyond it are written one after the other,
-    so a map that leaves out most of a long prompt makes the call slow.  The plan's tensors are parts of one allocation, unless
-    ``separate``."""
+    so a map that leaves out most of a long prompt makes the call slow.  The plan's tensors are parts
+    of one allocation, unless ``separate``."""
     return PagePlan._make(_capi.native().page_plan(cached_lens, new_lens, block_tables, block_size, num_tokens,
                                                    free_blocks, num_free, separate))
 
@@ -98,8 +98,8 @@ def page_fork(block_tables: torch.Tensor, lens: torch.Tensor, parents: torch.Ten
     served, and empty.  ``shares`` (int32 [num_blocks]) is the number of tables that hold each
     block beyond the first, zeros at the start.  Blocks that no table holds any more join the free
     list, ascending; the copy may read from one of them, so it comes before the next step's writes.
-    ``free_blocks`` is as long as ``shares``.  The results are parts of one allocation, unless
-    ``separate``."""
+    ``free_blocks`` is as long as ``shares``; tables are at most 2^30 blocks wide.  The results are
+    parts of one allocation, unless ``separate``."""
     return PageFork._make(_capi.native().page_fork(block_tables, lens, parents, block_size, free_blocks, num_free,
                                                    shares, separate))
 

@@ -13,14 +13,14 @@ F32, F16, BF16 = 0, 1, 2
 
 def _products(kind, rows=P, weights=P, temp=None):
     room = C.c_size_t(BIG)
-    return _capi.load().cusort_expert_products(temp, C.byref(room), kind, rows, 64, weights, 64 * 72, 72, 1, P, P, P, 10,
-                                               64, 72, 3, None)
+    return _capi.load().cusort_expert_products(temp, C.byref(room), kind, rows, 64, weights, 64 * 72, 72, 1, P, P, P,
+                                               10, 64, 72, 3, None)
 
 
 def _gradient(kind, rows=P, grad=P, temp=None):
     room = C.c_size_t(BIG)
-    return _capi.load().cusort_expert_products_grad_weights(temp, C.byref(room), kind, rows, 64, grad, 72, P, P, P, 0, 10,
-                                                            64, 72, 3, None)
+    return _capi.load().cusort_expert_products_grad_weights(temp, C.byref(room), kind, rows, 64, grad, 72, P, P, P, 0,
+                                                            10, 64, 72, 3, None)
 
 
 @pytest.mark.parametrize("call", [_products, _gradient])

@@ -1,5 +1,5 @@
-"""The example's layer in 16 bits where every value on the way can be held in 16 bits: results and gradients are those of
-the formula in 64 bits."""
+"""The example's layer in 16 bits where every value on the way can be held in 16 bits: results and gradients are those
+of the formula in 64 bits."""
 from __future__ import annotations
 
 import importlib.util
@@ -28,8 +28,8 @@ def _sparse(gen, each, *shape):
 
 
 def _values(tokens=70, hidden=64, inner=96, experts=12):
-    """A token has the value 4 at two of the first 12 places, which the router makes the logits of: its two experts, with
-    half the weight each."""
+    """A token has the value 4 at two of the first 12 places, which the router makes the logits of: its two experts,
+    with half the weight each."""
     gen = torch.Generator().manual_seed(6)
     x = _sparse(gen, 6, tokens, hidden)
     x[:, :experts] = 0
@@ -52,9 +52,9 @@ def _formula(x, router, up, down):
 
 
 def test_the_example_in_16_bits():
-    """To the bit, but for what the router's gradient goes into: a logit's is worked out in 32 bits from values up to 12,
-    in 8 operations at most (8 * 12 * 2^-24), and the router's adds up those of 70 tokens times 4 (below 2^-9 together);
-    what is off so before it is rounded may be rounded the other way (2^-8 of it)."""
+    """To the bit, but for what the router's gradient goes into: a logit's is worked out in 32 bits from values up to
+    12, in 8 operations at most (8 * 12 * 2^-24), and the router's adds up those of 70 tokens times 4 (below 2^-9
+    together); what is off so before it is rounded may be rounded the other way (2^-8 of it)."""
     *values, g = _values()
     wide = [v.cuda().double().requires_grad_() for v in values]
     want = _formula(*wide)

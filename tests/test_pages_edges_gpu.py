@@ -32,7 +32,8 @@ def test_every_used_block_moves(blocks):
     lens = np.full(8, tables.shape[1] * 4)
     got = paging.page_compact(dev(tables), dev(lens), 4, blocks)
     same(got, ref.compact(tables, lens, 4, blocks))
-    assert got.sources.tolist() == list(range(blocks // 2, blocks)) and got.destinations.tolist() == list(range(blocks // 2))
+    assert got.sources.tolist() == list(range(blocks // 2, blocks))
+    assert got.destinations.tolist() == list(range(blocks // 2))
 
 
 def test_copying_the_moves_of_a_pool():

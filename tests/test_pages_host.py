@@ -23,7 +23,8 @@ def _i(*shape):
 def test_width_of_tables(width, match):
     pool = dict(free_blocks=_i(9), num_free=_i(1), shares=_i(9))
     for call in (lambda t: paging.page_fork(t, _i(1), _i(2), 16, **pool),
-                 lambda t: paging.page_free(t, _i(1), _i(1), 16, **pool), lambda t: paging.page_compact(t, _i(1), 16, 9)):
+                 lambda t: paging.page_free(t, _i(1), _i(1), 16, **pool),
+                 lambda t: paging.page_compact(t, _i(1), 16, 9)):
         with pytest.raises(ValueError, match=match):
             call(_i(1, width))
 
