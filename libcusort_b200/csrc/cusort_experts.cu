@@ -131,19 +131,6 @@ __device__ __forceinline__ void init_pipe(Pipe<STAGES, PAIR>& p, uint32_t column
   dev::tmem_fence_after();
 }
 
-// The end of every warp's work: tensor memory is given back.
-template <int STAGES, bool PAIR>
-__device__ __forceinline__ void close_pipe(Pipe<STAGES, PAIR>& p, uint32_t columns) {
-  dev::tmem_fence_before();
-  if (PAIR) dev::cluster_sync();
-  else __syncthreads();
-  if (threadIdx.x == 0 && p.gave_up) atomicOr(&g_product_status, 1u);
-  if (threadIdx.x / 32 == 1) {
-    dev::tmem_fence_after();
-    dev::tmem_free<PAIR>(p.tmem, columns);
-  }
-}
-
 // The producer's place in the ring of stages.
 template <int STAGES> struct Ring {
   int stage = 0;
@@ -153,12 +140,25 @@ template <int STAGES> struct Ring {
   }
 };
 
-// After a wait ran out: copies in flight, which take microseconds, are given a
-// millisecond before the CTA ends.
-__device__ __forceinline__ void settle(const dev::WaitLimit& limit) {
-  if (!*limit.gave_up) return;
-  const uint64_t t0 = dev::globaltimer_ns();
-  while (dev::globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
+// The end of every warp's work: tensor memory is given back.  Where a wait ran
+// out, whoever's it was, copies and products may be under way that nobody waited
+// for; they take microseconds and are given a millisecond.  (Where none ran out
+// in one CTA of a pair, its sums were whole, so that the other one's products
+// are done too.)
+template <int STAGES, bool PAIR>
+__device__ __forceinline__ void close_pipe(Pipe<STAGES, PAIR>& p, uint32_t columns) {
+  dev::tmem_fence_before();
+  __syncthreads();
+  if (p.gave_up) {
+    if (threadIdx.x == 0) atomicOr(&g_product_status, 1u);
+    const uint64_t t0 = dev::globaltimer_ns();
+    while (dev::globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
+  }
+  if (PAIR) dev::cluster_sync();
+  if (threadIdx.x / 32 == 1) {
+    dev::tmem_fence_after();
+    dev::tmem_free<PAIR>(p.tmem, columns);
+  }
 }
 
 // What stands in the results in the place of two sums that a wait in vain has
@@ -322,7 +322,6 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
           }
         }
       }
-      settle(limit);
     }
   } else if (warp == 1 && rank == 0) {
     if (dev::elect_one()) {
@@ -353,7 +352,6 @@ __global__ void __launch_bounds__(kThreads, 1) product_kernel(const __grid_const
         }
         if (!lost) dev::mma_commit<PAIR>(at.sum_full(sums.stage));
       }
-      settle(limit);
     }
   } else if (warp == 3) {
     clear_other_rows(static_cast<uint16_t*>(a.out), a.width, a.segments, s, blockIdx.x, gridDim.x);
@@ -542,7 +540,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      settle(limit);
     }
   } else if (warp == 1 && rank == 0) {
     if (dev::elect_one()) {
@@ -588,7 +585,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!lost) dev::mma_commit<true>(at.sum_full(sums.stage));
         sums.next();
       }
-      settle(limit);
     }
   } else if (warp == 3) {
     // What came with the ends of segments is cleared.  With the ends in the stages, among the steps, this took about a

@@ -63,3 +63,23 @@ def test_what_is_lost_is_nan(name, skip):
     if skip <= 3:
         assert told == 1
     assert torch.equal(call(), right) and X.product_status() == 0
+
+
+@pytest.mark.parametrize("limit", [1, 2000, 20000])
+@pytest.mark.parametrize("name", CASES)
+def test_waits_that_get_hardly_any_time(name, limit):
+    """Any wait may run out here, in any role: every result is right or NaN, and NaN is told."""
+    call, mask, _ = CASES[name]()
+    assert X.product_status() == 0
+    lib, right = _capi.load(), call()
+    for _ in range(5):
+        before = lib.cusort_set_wait_limit_ns(limit)
+        try:
+            got = call()
+        finally:
+            lib.cusort_set_wait_limit_ns(before)
+        told, nan = X.product_status(), torch.isnan(got)
+        assert (nan | (got == right)).all()
+        assert told == 1 or not nan.any()
+        assert not nan[~mask].any()
+    assert torch.equal(call(), right) and X.product_status() == 0
