@@ -71,8 +71,9 @@ constexpr int kSms = 148;
 constexpr uint32_t kBoxBytes = kBlockK * dev::kBoxRowBytes;  // 64 rows of 64 elements
 constexpr uint32_t kAll = 0xffffffffu;
 
-// Products that gave up waiting (a bounded wait ran out): 1.
-__device__ uint32_t g_product_status;
+// CTAs that gave up waiting (a bounded wait ran out), and how many of them were
+// told: what comes between a reader's look and its answer stays for the next one.
+__device__ uint32_t g_lost[2];
 
 constexpr int kEnds = 4;  // buffers for the ends of segments, in the gradient of the weights
 
@@ -150,7 +151,7 @@ __device__ __forceinline__ void close_pipe(Pipe<STAGES, PAIR>& p, uint32_t colum
   dev::tmem_fence_before();
   __syncthreads();
   if (p.gave_up) {
-    if (threadIdx.x == 0) atomicOr(&g_product_status, 1u);
+    if (threadIdx.x == 0) atomicAdd(&g_lost[0], 1u);
     const uint64_t t0 = dev::globaltimer_ns();
     while (dev::globaltimer_ns() - t0 < 1000000) __nanosleep(1000);
   }
@@ -953,9 +954,14 @@ extern "C" cudaError_t cusort_expert_products_grad_weights(
 
 extern "C" cudaError_t cusort_read_product_status(uint32_t* status, cudaStream_t stream) {
   if (status == nullptr) return cudaErrorInvalidValue;
-  void* word = nullptr;
-  cudaError_t e = cudaGetSymbolAddress(&word, g_product_status);
-  if (!e) e = cudaMemcpyAsync(status, word, sizeof(uint32_t), cudaMemcpyDeviceToHost, stream);
-  if (!e) e = cudaMemsetAsync(word, 0, sizeof(uint32_t), stream);
+  void* words = nullptr;
+  uint32_t lost[2] = {};
+  cudaError_t e = cudaGetSymbolAddress(&words, g_lost);
+  if (!e) e = cudaMemcpyAsync(lost, words, sizeof(lost), cudaMemcpyDeviceToHost, stream);
+  if (!e) e = cudaStreamSynchronize(stream);
+  if (e) return e;
+  *status = lost[0] != lost[1];
+  if (*status == 0) return cudaSuccess;
+  e = cudaMemcpyAsync(static_cast<uint32_t*>(words) + 1, lost, sizeof(uint32_t), cudaMemcpyHostToDevice, stream);
   return e ? e : cudaStreamSynchronize(stream);
 }

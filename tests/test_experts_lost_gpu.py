@@ -83,3 +83,30 @@ def test_waits_that_get_hardly_any_time(name, limit):
         assert told == 1 or not nan.any()
         assert not nan[~mask].any()
     assert torch.equal(call(), right) and X.product_status() == 0
+
+
+def test_a_status_set_while_it_is_read_is_told():
+    """One CTA gives up in each call while another stream's status is read without a pause: every call is told by a read
+    that began before the next call, whichever."""
+    c, o, capacity, there = plan([4])
+    x, w = matrix(capacity, 64, torch.bfloat16, there), weights_of(1, 64, 64, torch.bfloat16, "in_out")
+    lib, stream, reader = _capi.load(), torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    assert X.product_status() == 0
+    before, missed = lib.cusort_set_wait_limit_ns(1000), 0
+    lib.cusort_debug_set_skip_tile(0)
+    try:
+        for _ in range(300):
+            with torch.cuda.stream(stream):
+                X.expert_products(x, w, c, o)
+                done = stream.record_event()
+            told, over = 0, False
+            while not over:
+                over = done.query()
+                with torch.cuda.stream(reader):
+                    told += X.product_status()
+            missed += told != 1
+    finally:
+        lib.cusort_debug_set_skip_tile(-1)
+        lib.cusort_set_wait_limit_ns(before)
+    assert missed == 0
